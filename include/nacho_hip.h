@@ -347,6 +347,118 @@ int nacho_gpu_spgemm64_f32(const nacho_csr *a, const nacho_csr *b, nacho_csr64 *
                            int32_t num_blocks, int32_t threads_per_block, void *stream,
                            const nacho_allocator *alloc);
 
+/* ---- dense rows through computed structure -------------------------------------------
+ * Attention over blocks of keys that a score selects for each query, and tokens sorted by
+ * expert and back.  The structure is found at run time: queries x key blocks, or experts x
+ * tokens; these entry points find it and move or multiply dense rows through it.  No
+ * counterpart in the reference.
+ *
+ * Dense operands are float32, float16 or bfloat16 (NACHO_F32 ...), all of one call's alike;
+ * sums, softmax statistics and scores are float32, and results are rounded to the operands'
+ * type once.  Results go into the caller's buffers; scratch comes from `alloc` (or the
+ * library's allocator).  All calls are asynchronous on `stream`, read nothing back, and may be
+ * captured into a graph when `alloc` may be called in a capture.  A result depends on nothing
+ * but the operands: sums have a fixed order. */
+#define NACHO_F32 0
+#define NACHO_F16 1
+#define NACHO_BF16 2
+
+/* A dense operand [batch][row][head][head_dim]: strides in elements, the last dimension
+ * contiguous.  `data` and every stride are multiples of 16 bytes. */
+typedef struct nacho_heads {
+    void *data;
+    int64_t batch_stride;
+    int64_t row_stride;
+    int64_t head_stride;
+} nacho_heads;
+
+/* Operands of the block attention.  Query t of sequence b stands at place
+ * p = length[b] - queries + t of its cache and sees, of the keys in its blocks, those at places
+ * <= p (causal) or < length[b]; a query at a place < 0 sees nothing.  Head h of q uses key head
+ * h / (q_heads / kv_heads), and all heads of such a group share the block ids. */
+typedef struct nacho_block_attention_args {
+    int32_t dtype;
+    int32_t batch, queries, keys;        /* keys: rows of k and v                           */
+    int32_t q_heads, kv_heads, head_dim; /* head_dim: a multiple of 8, at most 128          */
+    int32_t block;                       /* keys of a block: 32, 64 or 128                  */
+    int32_t count;                       /* ids per query and key head                      */
+    int32_t causal;                      /* 0 or 1                                          */
+    float scale;                         /* factor of q . k, finite                         */
+    const int32_t *lengths;              /* [batch], in [0, keys]; NULL: keys for all        */
+    const int32_t *blocks;               /* [batch][queries][kv_heads][count], in any order; an
+                                            id outside the sequence is no block, a repeated one
+                                            counts once                                     */
+    nacho_heads q, k, v;                 /* operands                                        */
+    nacho_heads out;                     /* [batch][queries][q_heads][head_dim]; 0 for a query
+                                            that sees nothing                               */
+    float *lse;                          /* [batch][queries][q_heads]: log of the sum of
+                                            exp(scale q . k), -inf for such a query.  May be
+                                            NULL in the forward pass                        */
+    nacho_heads dout, dq, dk, dv;        /* the backward pass only: gradients of out, q, k, v */
+} nacho_block_attention_args;
+
+/* out and lse from q, k, v and blocks. */
+int nacho_block_attention(const nacho_block_attention_args *args, void *stream,
+                          const nacho_allocator *alloc);
+
+/* dq, dk and dv from dout and the forward pass's operands and results. */
+int nacho_block_attention_backward(const nacho_block_attention_args *args, void *stream,
+                                   const nacho_allocator *alloc);
+
+/* means[batch][blocks][kv_heads][head_dim] (float32, blocks = ceil(keys / block)): the mean of
+ * each block's keys that are within the sequence's length, 0 for a block without. */
+int nacho_block_means(int32_t dtype, int32_t batch, int32_t keys, int32_t kv_heads,
+                      int32_t head_dim, int32_t block, const nacho_heads *k,
+                      const int32_t *lengths, float *means, void *stream);
+
+/* scores[batch][queries][kv_heads][blocks] (float32): scale times the sum of the group's query
+ * heads, times the block's mean key; -inf for a block that starts after the query's place
+ * (causal) or at the sequence's length or later. */
+int nacho_block_scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block,
+                       int32_t causal, float scale, const nacho_heads *q, const float *means,
+                       const int32_t *lengths, float *scores, void *stream);
+
+/* ids[rows = batch * queries * kv_heads][count] from scores[rows][blocks]: each query's `local`
+ * latest blocks up to its own place and its first `sink` blocks (taken in this order, latest
+ * and earliest first, while there is room), then the blocks of the highest scores, equal ones
+ * lowest id first.  A block with a score of -inf or NaN is taken only as one of the former.  Not
+ * causal: a query's latest block is its sequence's.  Ids ascend; -1 fills the row. */
+int nacho_block_select(int32_t batch, int32_t queries, int32_t kv_heads, int32_t keys,
+                       int32_t block, int32_t count, int32_t sink, int32_t local,
+                       int32_t causal, const float *scores, const int32_t *lengths,
+                       int32_t *ids, void *stream);
+
+/* Entries e = token * per_token + i of experts[tokens][per_token] (ids of `id_bytes` = 4 or 8
+ * bytes) sorted by expert, in order of e within one: pos[n_experts + 1] are the experts'
+ * offsets, order[place] is the entry at a place and slot[e] the place of an entry.  Entries
+ * with an id outside [0, n_experts) are dropped: slot -1, and their order follows at the end.
+ * At most NACHO_MAX_EXPERTS experts. */
+#define NACHO_MAX_EXPERTS 2048
+int nacho_route(const void *experts, int32_t id_bytes, int64_t tokens, int32_t per_token,
+                int32_t n_experts, int32_t *pos, int32_t *order, int32_t *slot, void *stream,
+                const nacho_allocator *alloc);
+
+/* rows[place][width] = x[order[place] / per_token][width], 0 past the last expert's entries.
+ * x_stride: elements between x's rows; rows are contiguous. */
+int nacho_dispatch(int32_t dtype, int64_t tokens, int32_t per_token, int32_t n_experts,
+                   int64_t width, const void *x, int64_t x_stride, const int32_t *pos,
+                   const int32_t *slot, void *rows, void *stream);
+
+/* out[token][width] = sum over i of weights[token][i] * rows[slot[token][i]][width], dropped
+ * entries left out; weights NULL: 1 (the gradient of a dispatch). */
+int nacho_combine(int32_t dtype, int64_t tokens, int32_t per_token, int64_t width,
+                  const void *rows, int64_t row_stride, const float *weights,
+                  const int32_t *slot, void *out, void *stream);
+
+/* The gradients of nacho_combine: drows[place] = weight * dout[token] (0 past the last expert's
+ * entries), dweights[token][i] = dout[token] . rows[slot[token][i]] (0 for a dropped one). */
+int nacho_combine_backward(int32_t dtype, int64_t tokens, int32_t per_token, int32_t n_experts,
+                           int64_t width, const void *rows, int64_t row_stride,
+                           const float *weights, const int32_t *pos, const int32_t *slot,
+                           const void *dout, int64_t dout_stride, void *drows, float *dweights,
+                           void *stream);
+
 /* ---- input validation ------------------------------------------------------------
  * The entry points trust operand contents, as the reference's generated code does.  This
  * checks a CSR operand against the input contract on the device: pos[0] == 0, pos

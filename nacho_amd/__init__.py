@@ -5,8 +5,18 @@ target: the tensor classes, the `gpu_<kernel>_f32` entry points, the converters 
 Matrix Market / FROSTT readers.  Every `gpu_` entry point runs hand-written HIP kernels from
 libnacho_hip.so through its C ABI (include/nacho_hip.h); nothing here computes on the CPU
 except the file readers (host C++ in the same library).
+
+Beside the reference's surface: products of dense rows with structure that scores decide at run
+time, attention over selected blocks of keys (blocks.py) and tokens sorted by expert (routing.py).
 """
 
+from .blocks import (  # noqa: F401
+    gpu_block_attention,
+    gpu_block_attention_backward,
+    gpu_block_means,
+    gpu_block_scores,
+    gpu_block_select,
+)
 from .convert import to_coo, to_coo3, to_csf3, to_csr, to_dcsr  # noqa: F401
 from .ops import (  # noqa: F401
     cached_bytes,
@@ -35,6 +45,7 @@ from .ops import (  # noqa: F401
 )
 from ._device import record_stream  # noqa: F401
 from .io import COO2D, COO3D_parsed, parse2D, parse3D_i32_f32  # noqa: F401
+from .routing import Route, gpu_combine, gpu_dispatch, gpu_route  # noqa: F401
 from .tensors import (  # noqa: F401
     COO3_gpu, COO_gpu, CSF3_gpu, CSR64_gpu, CSR_gpu, DCSR_gpu, Scalar_gpu)
 

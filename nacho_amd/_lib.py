@@ -132,6 +132,35 @@ class Coo3dHost(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class BlockAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_int32) for name in
+          ("dtype", "batch", "queries", "keys", "q_heads", "kv_heads", "head_dim", "block",
+           "count", "causal")),
+        ("scale", ctypes.c_float),
+        ("lengths", ctypes.c_void_p),
+        ("blocks", ctypes.c_void_p),
+        ("q", Heads),
+        ("k", Heads),
+        ("v", Heads),
+        ("out", Heads),
+        ("lse", ctypes.c_void_p),
+        ("dout", Heads),
+        ("dq", Heads),
+        ("dk", Heads),
+        ("dv", Heads),
+    ]
+
+
 class Allocator(ctypes.Structure):
     _fields_ = [
         ("ctx", ctypes.c_void_p),
@@ -173,6 +202,23 @@ ENTRY_POINTS_3 = {
 # passes the result buffers in z
 ENTRY_POINTS_NOALLOC = {
     "nacho_gpu_csr_add_f32_noalloc": (CsrDesc, CsrDesc),
+}
+
+_I32, _I64, _PTR = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+_HEADS, _ALLOC = ctypes.POINTER(Heads), ctypes.POINTER(Allocator)
+
+# dense rows through computed structure: name -> arguments
+ENTRY_POINTS_DENSE = {
+    "nacho_block_attention": (ctypes.POINTER(BlockAttentionArgs), _PTR, _ALLOC),
+    "nacho_block_attention_backward": (ctypes.POINTER(BlockAttentionArgs), _PTR, _ALLOC),
+    "nacho_block_means": (*[_I32] * 6, _HEADS, _PTR, _PTR, _PTR),
+    "nacho_block_scores": (*[_I32] * 9, ctypes.c_float, _HEADS, _PTR, _PTR, _PTR, _PTR),
+    "nacho_block_select": (*[_I32] * 9, _PTR, _PTR, _PTR, _PTR),
+    "nacho_route": (_PTR, _I32, _I64, _I32, _I32, _PTR, _PTR, _PTR, _PTR, _ALLOC),
+    "nacho_dispatch": (_I32, _I64, _I32, _I32, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR),
+    "nacho_combine": (_I32, _I64, _I32, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR),
+    "nacho_combine_backward": (_I32, _I64, _I32, _I32, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR,
+                               _I64, _PTR, _PTR, _PTR),
 }
 
 _lib = None
@@ -217,6 +263,10 @@ def load() -> ctypes.CDLL:
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(operand), ctypes.POINTER(operand), ctypes.POINTER(result),
                        ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
+    for name, arguments in ENTRY_POINTS_DENSE.items():
+        fn = getattr(lib, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = list(arguments)
     lib.nacho_parse2d.restype = ctypes.c_int
     lib.nacho_parse2d.argtypes = [ctypes.c_char_p, ctypes.POINTER(Coo2dHost)]
     lib.nacho_parse3d.restype = ctypes.c_int
@@ -255,16 +305,22 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_bridge_module = None
+
+
 def load_bridge():
     """The call path between the Python classes and the library (_bridge.so, built with it);
     raises if it has not been built."""
-    try:
-        from . import _bridge
-    except ImportError as e:
-        raise RuntimeError(f"_bridge.so does not load ({e}); "
-                           "run `python -m nacho_amd.build`") from e
-    _bridge.set_free(ctypes.cast(load().nacho_free, ctypes.c_void_p).value)
-    return _bridge
+    global _bridge_module
+    if _bridge_module is None:
+        try:
+            from . import _bridge
+        except ImportError as e:
+            raise RuntimeError(f"_bridge.so does not load ({e}); "
+                               "run `python -m nacho_amd.build`") from e
+        _bridge.set_free(ctypes.cast(load().nacho_free, ctypes.c_void_p).value)
+        _bridge_module = _bridge
+    return _bridge_module
 
 
 def error_string(code: int) -> str:

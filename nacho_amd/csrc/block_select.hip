@@ -1,0 +1,422 @@
+// Which blocks of keys a query attends to: each block's mean key, every query's scores against
+// the means, and the blocks of the highest scores.
+//
+// means: bound by reading k once.  A workgroup per (sequence, block, head): 16 lanes read a key
+// (16 bytes or 32 each), 16 keys at a time; float32 sums.
+//
+// scores: scale (sum of the group's heads of q) . mean, in float32 throughout: they are compared
+// with each other, and the product is small (one row per group and one column per block of keys),
+// so it runs on the float32 matrix instruction.  A workgroup sums 64 queries' heads into LDS and
+// goes over the blocks 64 at a time, 16 to a wavefront.
+//
+// select: a wavefront per query and key head.  Scores become unsigned numbers of the same order,
+// and the count-th largest is found bit by bit with ballots; no sort, and ties are counted off
+// from the lowest id.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <new>
+
+#include "dense_tiles.hpp"
+#include "runtime.hpp"
+
+namespace nacho {
+namespace select {
+
+using namespace dense;
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ int length_of(const int *lengths, int b, int keys) {
+    return lengths ? min(max(lengths[b], 0), keys) : keys;
+}
+
+// ---- means ----------------------------------------------------------------------------
+
+struct MeansArgs {
+    int keys, heads, dim, block, blocks;
+    int64_t batch_stride, row_stride, head_stride;
+    const int *lengths;
+    float *means;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void means_kernel(MeansArgs a, const T *__restrict__ k) {
+    constexpr int kSlices = kThreads / 16;
+    __shared__ float s_sum[kSlices][128 + 1];
+    const int h = static_cast<int>(blockIdx.x % a.heads);
+    const int64_t bj = blockIdx.x / a.heads;
+    const int j = static_cast<int>(bj % a.blocks), b = static_cast<int>(bj / a.blocks);
+    const int piece = static_cast<int>(threadIdx.x) % 16, slice = static_cast<int>(threadIdx.x) / 16;
+    const int first = j * a.block;
+    const int there = min(max(length_of(a.lengths, b, a.keys) - first, 0), a.block);
+    float sum[8] = {};
+    if (8 * piece < a.dim) {
+        const T *p = k + b * a.batch_stride + first * a.row_stride + h * a.head_stride + 8 * piece;
+#pragma unroll 4
+        for (int key = slice; key < there; key += kSlices) {
+            const Frag<T> f = row_frag<T>(p + key * a.row_stride);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += static_cast<float>(f[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_sum[slice][8 * piece + i] = sum[i];
+    __syncthreads();
+    const int col = static_cast<int>(threadIdx.x);
+    if (col < a.dim) {
+        float total = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kSlices; ++x) total += s_sum[x][col];
+        a.means[(bj * a.heads + h) * a.dim + col] =
+            there > 0 ? total / static_cast<float>(there) : 0.0f;
+    }
+}
+
+// ---- scores ---------------------------------------------------------------------------
+
+struct ScoresArgs {
+    int queries, keys, heads, group, dim, block, blocks, causal;
+    float scale;
+    int64_t batch_stride, row_stride, head_stride;
+    const float *means;
+    const int *lengths;
+    float *scores;
+    int tiles;     // of 64 queries
+    int per_part;  // steps of 64 blocks that a workgroup takes
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T *__restrict__ q,
+                                                          int sequences) {
+    constexpr int kRow = kTileRow<float, DP>;
+    __shared__ __align__(16) float s_q[64 * kRow];
+    const int heads = sequences * a.heads;
+    const int bh = static_cast<int>(blockIdx.x) % heads;
+    const int rest = static_cast<int>(blockIdx.x) / heads;
+    const int tile = rest % a.tiles, part = rest / a.tiles;
+    const int b = bh / a.heads, h = bh % a.heads;
+    const int t0 = 64 * tile, tokens = min(64, a.queries - t0);
+    const int length = length_of(a.lengths, b, a.keys);
+    const int place0 = length - a.queries + t0;
+    const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
+    const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    // the group's heads, summed
+    constexpr int kPieces = DP / 8;
+    for (int x = threadIdx.x; x < 64 * kPieces; x += kThreads) {
+        const int r = x / kPieces, col = x % kPieces * 8;
+        float sum[8] = {};
+        if (r < tokens && col < a.dim) {
+            const T *p = q + b * a.batch_stride + (t0 + r) * a.row_stride +
+                         static_cast<int64_t>(h) * a.group * a.head_stride + col;
+#pragma unroll 4
+            for (int i = 0; i < a.group; ++i) {
+                const Frag<T> f = row_frag<T>(p + i * a.head_stride);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += static_cast<float>(f[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s_q[r * kRow + col + j] = sum[j] * a.scale;
+    }
+    __syncthreads();
+    const int row_tiles = (tokens + 15) / 16;
+    // the last block that some query of the tile may see
+    const int last_place = place0 + tokens - 1;
+    const int last = last_place < 0 ? -1 : (a.causal ? last_place : length - 1);
+    const int steps = (a.blocks + 63) / 64;
+    const int end = min(steps, (part + 1) * a.per_part);
+    for (int step = part * a.per_part; step < end; ++step) {
+        const int j = 64 * step + 16 * wave + c;
+        if (64 * step + 16 * wave >= a.blocks) continue;
+        f32x4 acc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (static_cast<int64_t>(64 * step + 16 * wave) * a.block <= last) {  // uniform
+            f32x8 m[DP / 32];
+            const float *p = j < a.blocks
+                                 ? a.means + ((static_cast<int64_t>(b) * a.blocks + j) * a.heads + h) *
+                                                 a.dim
+                                 : nullptr;
+            load_row_frags<float, DP>(p, a.dim, g, m);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (t < row_tiles) {
+#pragma unroll
+                    for (int kk = 0; kk < DP / 32; ++kk) {
+                        acc[t] = mma(row_frag<float>(s_q + (16 * t + c) * kRow + 32 * kk + 8 * g),
+                                     m[kk], acc[t]);
+                    }
+                }
+            }
+        }
+        if (j >= a.blocks) continue;
+        const int64_t first_key = static_cast<int64_t>(j) * a.block;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * t + 4 * g + i;
+                if (r >= tokens) continue;
+                const int place = place0 + r;
+                const int seen = place < 0 ? -1 : (a.causal ? place : length - 1);
+                const int64_t row = (static_cast<int64_t>(b) * a.queries + t0 + r) * a.heads + h;
+                a.scores[row * a.blocks + j] = first_key <= seen ? acc[t][i] : kNegInf;
+            }
+        }
+    }
+}
+
+// ---- selection ------------------------------------------------------------------------
+
+struct SelectArgs {
+    int64_t rows;
+    int queries, heads, keys, block, blocks, count, sink, local, causal;
+    const float *scores;
+    const int *lengths;
+    int *ids;
+};
+
+constexpr int kMaxForced = 1 << 20;  // of sink and of local: fits above the infinity's number
+
+// A number that orders like the score: 0 for a block that is not to be taken, the forced blocks'
+// above every score's, in the order in which they are taken.
+__device__ __forceinline__ unsigned order_of(const SelectArgs &a, float score, int j, int own) {
+    if (j > own) return 0u;
+    if (own - j < a.local) return UINT_MAX - static_cast<unsigned>(own - j);
+    if (j < a.sink) return UINT_MAX - static_cast<unsigned>(a.local) - static_cast<unsigned>(j);
+    if (!(score > kNegInf)) return 0u;                     // (NaN too)
+    const unsigned u = __float_as_uint(score + 0.0f);      // -0 as 0
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+// NR registers a lane hold the row (64 NR blocks); NR = 0 reads it again each time.
+template <int NR>
+__global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
+    const int64_t row = blockIdx.x * static_cast<int64_t>(kThreads / dev::kWave) +
+                        threadIdx.x / dev::kWave;
+    if (row >= a.rows) return;
+    const int lane = dev::lane();
+    const int64_t bt = row / a.heads;
+    const int t = static_cast<int>(bt % a.queries), b = static_cast<int>(bt / a.queries);
+    const int length = length_of(a.lengths, b, a.keys);
+    const int place = length - a.queries + t;
+    const int own = place < 0 ? -1 : (a.causal ? place : length - 1) / a.block;
+    const float *scores = a.scores + row * a.blocks;
+    const int chunks = NR ? NR : (a.blocks + dev::kWave - 1) / dev::kWave;
+    auto fetch = [&](int r) {
+        const int j = r * dev::kWave + lane;
+        return j < a.blocks && j <= own ? order_of(a, scores[j], j, own) : 0u;
+    };
+    unsigned held[NR ? NR : 1];
+    if constexpr (NR > 0) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) held[r] = fetch(r);
+    }
+    auto key = [&](int r) { return NR ? held[NR ? r : 0] : fetch(r); };
+    auto at_least = [&](unsigned x) {
+        int n = 0;
+#pragma unroll(NR ? NR : 1)
+        for (int r = 0; r < chunks; ++r) n += __popcll(__ballot(key(r) >= x));
+        return n;
+    };
+    // the largest threshold that `count` numbers reach (0: fewer than that many are not 0)
+    unsigned threshold = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned x = threshold | 1u << bit;
+        const int n = at_least(x);
+        if (n >= a.count) threshold = x;
+        if (n == a.count) break;
+    }
+    const bool all = threshold == 0u;
+    int ties = 0;  // how many of those equal to the threshold
+    if (!all) {
+        int above = 0;
+#pragma unroll(NR ? NR : 1)
+        for (int r = 0; r < chunks; ++r) above += __popcll(__ballot(key(r) > threshold));
+        ties = a.count - above;
+    }
+    int *ids = a.ids + row * a.count;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    int at = 0;
+#pragma unroll(NR ? NR : 1)
+    for (int r = 0; r < chunks; ++r) {
+        const unsigned x = key(r);
+        const unsigned long long equal = __ballot(!all && x == threshold);
+        const bool take = all ? x > 0u
+                              : x > threshold ||
+                                    (x == threshold && __popcll(equal & before) < ties);
+        const unsigned long long taken = __ballot(take);
+        if (take) ids[at + __popcll(taken & before)] = r * dev::kWave + lane;
+        at += __popcll(taken);
+        ties -= min(ties, static_cast<int>(__popcll(equal)));
+    }
+    for (int i = at + lane; i < a.count; i += dev::kWave) ids[i] = -1;
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+bool aligned(const nacho_heads *h, int dtype, bool optional) {
+    if (!h) return false;
+    if (!h->data) return optional;
+    const int64_t per = dtype == NACHO_F32 ? 4 : 8;
+    return reinterpret_cast<uintptr_t>(h->data) % 16 == 0 && h->batch_stride % per == 0 &&
+           h->row_stride % per == 0 && h->head_stride % per == 0;
+}
+
+bool good_dim(int32_t dim) { return dim >= 8 && dim <= 128 && dim % 8 == 0; }
+bool good_block(int32_t block) { return block == 32 || block == 64 || block == 128; }
+bool good_type(int32_t dtype) { return dtype >= NACHO_F32 && dtype <= NACHO_BF16; }
+
+int means(int32_t dtype, int32_t batch, int32_t keys, int32_t heads, int32_t dim, int32_t block,
+          const nacho_heads *k, const int32_t *lengths, float *out, void *stream) {
+    const bool empty = batch == 0 || keys == 0;
+    if (!good_type(dtype) || batch < 0 || keys < 0 || heads < 1 || !good_dim(dim) ||
+        !good_block(block) || !aligned(k, dtype, empty) || (!out && !empty)) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if (empty) return NACHO_OK;
+    const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
+    const int64_t grid = blocks * batch * heads;
+    if (grid > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
+    const MeansArgs a{keys,
+                      heads,
+                      dim,
+                      block,
+                      static_cast<int>(blocks),
+                      k->batch_stride,
+                      k->row_stride,
+                      k->head_stride,
+                      lengths,
+                      out};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned n = static_cast<unsigned>(grid);
+    if (dtype == NACHO_F32) {
+        means_kernel<float><<<n, kThreads, 0, s>>>(a, static_cast<const float *>(k->data));
+    } else if (dtype == NACHO_F16) {
+        means_kernel<_Float16><<<n, kThreads, 0, s>>>(a, static_cast<const _Float16 *>(k->data));
+    } else {
+        means_kernel<__bf16><<<n, kThreads, 0, s>>>(a, static_cast<const __bf16 *>(k->data));
+    }
+    NACHO_TRY_HIP(hipGetLastError());
+    return NACHO_OK;
+}
+
+template <typename T>
+int launch_scores(const ScoresArgs &a, const void *q, int batch, unsigned grid, hipStream_t s) {
+    const T *data = static_cast<const T *>(q);
+    if (a.dim <= 64) {
+        scores_kernel<T, 64><<<grid, kThreads, 0, s>>>(a, data, batch);
+    } else {
+        scores_kernel<T, 128><<<grid, kThreads, 0, s>>>(a, data, batch);
+    }
+    NACHO_TRY_HIP(hipGetLastError());
+    return NACHO_OK;
+}
+
+int scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys, int32_t q_heads,
+           int32_t kv_heads, int32_t dim, int32_t block, int32_t causal, float scale,
+           const nacho_heads *q, const float *mean, const int32_t *lengths, float *out,
+           void *stream) {
+    const bool empty = batch == 0 || queries == 0 || keys == 0;
+    if (!good_type(dtype) || batch < 0 || queries < 0 || keys < 0 || q_heads < 1 || kv_heads < 1 ||
+        q_heads % kv_heads != 0 || !good_dim(dim) || !good_block(block) ||
+        (causal != 0 && causal != 1) || !std::isfinite(scale) || !aligned(q, dtype, empty) ||
+        reinterpret_cast<uintptr_t>(mean) % 16 != 0 || ((!mean || !out) && !empty)) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if (empty) return NACHO_OK;
+    const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
+    const int64_t tiles = (static_cast<int64_t>(queries) + 63) / 64;
+    const int64_t groups = tiles * batch * kv_heads;
+    const int64_t steps = (blocks + 63) / 64;
+    if (groups * steps > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
+    // enough workgroups for every CU to have two, while each sums its queries' heads once
+    int64_t parts = (512 + groups - 1) / groups;
+    if (parts > steps) parts = steps;
+    const int64_t per_part = (steps + parts - 1) / parts;
+    const ScoresArgs a{queries,
+                       keys,
+                       kv_heads,
+                       q_heads / kv_heads,
+                       dim,
+                       block,
+                       static_cast<int>(blocks),
+                       causal,
+                       scale,
+                       q->batch_stride,
+                       q->row_stride,
+                       q->head_stride,
+                       mean,
+                       lengths,
+                       out,
+                       static_cast<int>(tiles),
+                       static_cast<int>(per_part)};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned grid = static_cast<unsigned>(groups * parts);
+    switch (dtype) {
+        case NACHO_F32: return launch_scores<float>(a, q->data, batch, grid, s);
+        case NACHO_F16: return launch_scores<_Float16>(a, q->data, batch, grid, s);
+        default: return launch_scores<__bf16>(a, q->data, batch, grid, s);
+    }
+}
+
+int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t block,
+           int32_t count, int32_t sink, int32_t local, int32_t causal, const float *score,
+           const int32_t *lengths, int32_t *ids, void *stream) {
+    if (batch < 0 || queries < 0 || heads < 1 || keys < 0 || !good_block(block) || count < 0 ||
+        sink < 0 || local < 0 || sink > kMaxForced || local > kMaxForced ||
+        (causal != 0 && causal != 1)) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    const int64_t rows = static_cast<int64_t>(batch) * queries * heads;
+    if (rows == 0 || count == 0) return NACHO_OK;
+    if (!ids || (!score && keys > 0)) return NACHO_ERR_INVALID_ARGUMENT;
+    const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
+    const int64_t grid = (rows + 3) / 4;
+    if (grid > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
+    const SelectArgs a{rows,  queries, heads, keys,   block, static_cast<int>(blocks), count, sink,
+                       local, causal,  score, lengths, ids};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned n = static_cast<unsigned>(grid);
+    if (blocks <= 2 * dev::kWave) {
+        select_kernel<2><<<n, kThreads, 0, s>>>(a);
+    } else if (blocks <= 8 * dev::kWave) {
+        select_kernel<8><<<n, kThreads, 0, s>>>(a);
+    } else if (blocks <= 32 * dev::kWave) {
+        select_kernel<32><<<n, kThreads, 0, s>>>(a);
+    } else {
+        select_kernel<0><<<n, kThreads, 0, s>>>(a);
+    }
+    NACHO_TRY_HIP(hipGetLastError());
+    return NACHO_OK;
+}
+
+}  // namespace select
+}  // namespace nacho
+
+extern "C" int nacho_block_means(int32_t dtype, int32_t batch, int32_t keys, int32_t kv_heads,
+                                 int32_t head_dim, int32_t block, const nacho_heads *k,
+                                 const int32_t *lengths, float *means, void *stream) {
+    return nacho::select::means(dtype, batch, keys, kv_heads, head_dim, block, k, lengths, means,
+                                stream);
+}
+
+extern "C" int nacho_block_scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys,
+                                  int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                  int32_t block, int32_t causal, float scale,
+                                  const nacho_heads *q, const float *means,
+                                  const int32_t *lengths, float *scores, void *stream) {
+    return nacho::select::scores(dtype, batch, queries, keys, q_heads, kv_heads, head_dim, block,
+                                 causal, scale, q, means, lengths, scores, stream);
+}
+
+extern "C" int nacho_block_select(int32_t batch, int32_t queries, int32_t kv_heads, int32_t keys,
+                                  int32_t block, int32_t count, int32_t sink, int32_t local,
+                                  int32_t causal, const float *scores, const int32_t *lengths,
+                                  int32_t *ids, void *stream) {
+    return nacho::select::select(batch, queries, kv_heads, keys, block, count, sink, local, causal,
+                                 scores, lengths, ids, stream);
+}

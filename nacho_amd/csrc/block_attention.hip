@@ -27,6 +27,7 @@
 
 #include "dense_tiles.hpp"
 #include "runtime.hpp"
+#include "scan.hpp"
 
 namespace nacho {
 namespace attention {
@@ -88,13 +89,13 @@ __host__ __device__ inline Tiling tiling(const Shape &s, int rows) {
 }
 
 template <int R>
-struct Tile {
+struct RowTile {
     int b, h, t0, head0, tokens;  // tokens: those that exist
     int length, place0;           // place of token t0
 
     // heads: sequences x key heads; the fastest index, so that workgroups that follow each
     // other, which go to different XCDs, read different heads' keys.
-    __device__ __forceinline__ Tile(const Shape &s, const int *lengths, int index) {
+    __device__ __forceinline__ RowTile(const Shape &s, const int *lengths, int index) {
         const Tiling tl = tiling(s, R);
         const int heads = s.batch * s.kv_heads;
         const int bh = index % heads;
@@ -126,19 +127,26 @@ struct Tile {
     }
 };
 
-// The union of the tile's blocks within [first, first + kWindow): mask[] by block of the
-// window, and the numbers of the blocks with a token, ascending, in ids[0 .. returned).
+// The union of the tile's blocks within [first, first + kWindow): a mask of tokens by block of
+// the window, and the numbers of the blocks with a token, ascending, in ids[0 .. returned).
+template <int R>
 struct Lists {
-    unsigned long long mask[kWindow];
+    static constexpr int kWords = (R + 63) / 64;
+    unsigned long long mask[kWindow][kWords];
     unsigned short ids[kWindow];
     int sums[kWaves];
+
+    __device__ __forceinline__ bool has(int nth, int token) const {
+        return mask[ids[nth]][token / 64] >> (token % 64) & 1ull;
+    }
 };
 
 template <int R>
-__device__ int window_lists(const Shape &s, const int *__restrict__ ids, const Tile<R> &tile,
-                            int first, Lists &lists) {
+__device__ int window_lists(const Shape &s, const int *__restrict__ ids, const RowTile<R> &tile,
+                            int first, Lists<R> &lists) {
+    constexpr int kWords = Lists<R>::kWords;
     __syncthreads();  // (the lists of the window before are done with)
-    for (int i = threadIdx.x; i < kWindow; i += kThreads) lists.mask[i] = 0ull;
+    for (int i = threadIdx.x; i < kWindow * kWords; i += kThreads) (&lists.mask[0][0])[i] = 0ull;
     __syncthreads();
     for (int i = threadIdx.x; i < tile.tokens * s.count; i += kThreads) {
         const int token = i / s.count, x = i - token * s.count;
@@ -149,66 +157,131 @@ __device__ int window_lists(const Shape &s, const int *__restrict__ ids, const T
         // (unsigned: an id < 0 is past the last one)
         if (last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block) &&
             id >= first && id < first + kWindow) {
-            atomicOr(&lists.mask[id - first], 1ull << token);
+            atomicOr(&lists.mask[id - first][token / 64], 1ull << (token % 64));
         }
     }
     __syncthreads();
     constexpr int kPer = kWindow / kThreads;
+    auto filled = [&](int i) {
+        unsigned long long any = lists.mask[i][0];
+#pragma unroll
+        for (int w = 1; w < kWords; ++w) any |= lists.mask[i][w];
+        return any != 0ull;
+    };
     int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) mine += lists.mask[threadIdx.x * kPer + j] != 0ull;
+    for (int j = 0; j < kPer; ++j) mine += filled(threadIdx.x * kPer + j);
     int total = 0;
     int at = dev::block_exclusive_sum<kThreads>(mine, lists.sums, total);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         const int i = threadIdx.x * kPer + j;
-        if (lists.mask[i] != 0ull) lists.ids[at++] = static_cast<unsigned short>(i);
+        if (filled(i)) lists.ids[at++] = static_cast<unsigned short>(i);
     }
     __syncthreads();
     return total;
 }
 
-// ---- forward, tiles of 64 rows --------------------------------------------------------
+// Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
+// rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
+// sequence's end hold its last key's.  Every wavefront calls it; `use` has no barrier.
+template <typename T, int DP, int BN, int R>
+struct KeySteps {
+    using Lds = Tile<T, DP, BN, kThreads>;
+    T *k[2], *v[2];
+    Lists<R> &lists;
 
-// One online-softmax step for a row (a lane's column) over 16 N keys: s are the products, at
-// most the first `limit` keys from the step's first (this lane's g included) are seen.  Updates
-// the running maximum and sum and returns the factor for what was summed before.
+    template <typename Use>
+    __device__ __forceinline__ void run(const Args<T> &a, const RowTile<R> &tile, Use use) {
+        const Shape &s = a.s;
+        const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
+        const int end = tile.last_key(s, tile.tokens - 1) + 1;  // keys that some row sees
+        const int steps_of = s.block / BN;
+        for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
+            const int steps = window_lists(s, a.ids, tile, first, lists) * steps_of;
+            auto first_key = [&](int step) {
+                return (first + __builtin_amdgcn_readfirstlane(lists.ids[step / steps_of])) *
+                           s.block +
+                       step % steps_of * BN;
+            };
+            auto load = [&](int step, T *to_k, T *to_v) {
+                const int key = first_key(step);
+                const int most = tile.length - 1 - key;
+                const T *from_k = k_base + key * a.k.row_stride;
+                const T *from_v = v_base + key * a.v.row_stride;
+                Lds::load(to_k, threadIdx.x, s.dim,
+                          [&](int r) { return from_k + min(r, most) * a.k.row_stride; });
+                Lds::load(to_v, threadIdx.x, s.dim,
+                          [&](int r) { return from_v + min(r, most) * a.v.row_stride; });
+            };
+            if (steps > 0) load(0, k[0], v[0]);
+            __syncthreads();
+            for (int step = 0; step < steps; step += 2) {
+                if (step + 1 < steps) load(step + 1, k[1], v[1]);
+                use(k[0], v[0], step / steps_of, first_key(step));
+                __syncthreads();
+                if (step + 1 >= steps) break;
+                if (step + 2 < steps) load(step + 2, k[0], v[0]);
+                use(k[1], v[1], (step + 1) / steps_of, first_key(step + 1));
+                __syncthreads();
+            }
+        }
+    }
+};
+
+// ---- forward, tiles of 64 or 128 rows -------------------------------------------------
+
+// The factor of q . k for base-2 exponentials.  It is not negative (operands are negated for a
+// negative scale), so that the largest product is the largest score, and not 0, so that a masked
+// score of -inf stays one.
+__device__ __forceinline__ float base2_scale(float scale) {
+    return fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f);
+}
+
+constexpr float kSlack = 8.0f;  // the running maximum follows a row's when it is 2^8 behind
+
+// One online-softmax step for a row (a lane's column) over 16 N keys: s are the products, the
+// first `limit` keys from the step's first (this lane's 4 g included) are seen.  s become the
+// probabilities against the running maximum m, which may stay up to kSlack below the row's own
+// (they are at most 2^kSlack then): sums are brought to a new one only when some row of the
+// wavefront needs it.  Returns whether they were, by `factor`.
 template <int N>
-__device__ __forceinline__ float softmax_step(f32x4 (&s)[N], float scale2, int limit, float &m,
-                                              float &l) {
+__device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, float &m,
+                                             float &l, float &factor) {
     if (!__all(limit >= 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[t][i] = 16 * t + i < limit ? s[t][i] * scale2 : kNegInf;
-            }
+            for (int i = 0; i < 4; ++i) s[t][i] = 16 * t + i < limit ? s[t][i] : kNegInf;
         }
-    } else {
-#pragma unroll
-        for (int t = 0; t < N; ++t) s[t] *= scale2;
     }
-    float top = kNegInf;
+    float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
     }
-    const float now = fmaxf(m, column_max(top));
-    const float base = now == kNegInf ? 0.0f : now;
-    const float factor = exp2_fast(m - base);
-    m = now;
+    top = column_max(top) * scale2;
+    const bool moved = __any(top > m + kSlack);
+    factor = 1.0f;
+    if (moved) {
+        const float now = fmaxf(m, top);
+        factor = now == kNegInf ? 1.0f : exp2_fast(m - now);
+        m = now;
+        l *= factor;
+    }
+    const float base = m == kNegInf ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[t][i] = exp2_fast(s[t][i] - base);
+            s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], scale2, -base));
             sum += s[t][i];
         }
     }
-    l = l * factor + sum;
-    return factor;
+    l += sum;
+    return moved;
 }
 
 // The keys of a step that a row sees, as softmax_step's limit.
@@ -216,92 +289,96 @@ __device__ __forceinline__ int step_limit(bool selected, int last_key, int first
     return selected ? last_key + 1 - first_key - 4 * g : 0;
 }
 
-template <typename T, int DP, int BN>
-__global__ __launch_bounds__(kThreads) void tile_kernel(Args<T> a) {
-    constexpr int kRow = kTileRow<T, DP>;
-    __shared__ __align__(16) T s_k[BN * kRow];
-    __shared__ __align__(16) T s_v[BN * kRow];
-    __shared__ Lists s_lists;
-    const Shape &s = a.s;
-    const Tile<64> tile(s, a.lengths, static_cast<int>(blockIdx.x));
-    const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
-    const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
-    int token, head;
-    const bool exists = tile.row(s, 16 * wave + c, token, head);
-    const int last_key = exists ? tile.last_key(s, token) : -1;
-    Frag<T> q[DP / 32];
-    load_row_frags<T, DP>(exists ? a.q.row(tile.b, tile.t0 + token, head) : nullptr, s.dim, g, q);
-    f32x4 o[DP / 16];
+// A lane's rows of a tile: COLS of them, 16 apart.
+template <int COLS>
+struct LaneRows {
+    int token[COLS], head[COLS], last_key[COLS];
+    bool exists[COLS];
+
+    __device__ __forceinline__ LaneRows(const Shape &s, const RowTile<64 * COLS> &tile, int wave,
+                                        int c) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kNegInf, l = 0.0f;
-    const float scale2 = s.scale * kLog2e;
-    const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
-    const int end = tile.last_key(s, tile.tokens - 1) + 1;  // keys that some row sees
-    const int steps_of = s.block / BN;
-    TileLoad<T, DP, BN, kThreads> k_next, v_next;
-    for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
-        const int steps = window_lists(s, a.ids, tile, first, s_lists) * steps_of;
-        auto first_key = [&](int step) {
-            return (first + s_lists.ids[step / steps_of]) * s.block + step % steps_of * BN;
-        };
-        auto load = [&](int step) {
-            const int key = first_key(step);
-            k_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                return key + r < tile.length ? k_base + (key + r) * a.k.row_stride : nullptr;
-            });
-            v_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                return key + r < tile.length ? v_base + (key + r) * a.v.row_stride : nullptr;
-            });
-        };
-        if (steps > 0) load(0);
-        for (int step = 0; step < steps; ++step) {
-            __syncthreads();
-            k_next.store(threadIdx.x, s_k);
-            v_next.store(threadIdx.x, s_v);
-            __syncthreads();
-            if (step + 1 < steps) load(step + 1);
-            const unsigned long long tokens = s_lists.mask[s_lists.ids[step / steps_of]];
-            const bool selected = exists && (tokens >> token & 1ull);
-            const int limit = step_limit(selected, last_key, first_key(step), g);
-            if (!__any(limit > 0)) continue;
-            f32x4 p[BN / 16];
-#pragma unroll
-            for (int t = 0; t < BN / 16; ++t) {
-                p[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    p[t] = mma(row_frag<T>(s_k + (16 * t + c) * kRow + 32 * kk + 8 * g), q[kk],
-                               p[t]);
-                }
-            }
-            const float factor = softmax_step<BN / 16>(p, scale2, limit, m, l);
-            if (!__all(factor == 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) o[i] *= factor;
-            }
-#pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                const Frag<T> pf = result_frag<T>(p[2 * u], p[2 * u + 1]);
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    o[i] = mma(column_frag<kRow>(s_v + 32 * u * kRow, 16 * i, g, c), pf, o[i]);
-                }
-            }
+        for (int x = 0; x < COLS; ++x) {
+            exists[x] = tile.row(s, 16 * (COLS * wave + x) + c, token[x], head[x]);
+            if (!exists[x]) token[x] = 0;
+            last_key[x] = exists[x] ? tile.last_key(s, token[x]) : -1;
         }
     }
-    l = column_sum(l);
-    if (!exists) return;
-    const float inverse = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // (NaN stays)
-    T *out = a.out.row(tile.b, tile.t0 + token, head);
+    // softmax_step's limits; whether some row of the wavefront sees a key
+    __device__ __forceinline__ bool limits(const Lists<64 * COLS> &lists, int nth, int first_key,
+                                           int g, int (&limit)[COLS]) const {
+        bool any = false;
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-        const int col = 16 * i + 4 * g;
-        if (col < s.dim) store4<T>(out + col, o[i] * inverse);
+        for (int x = 0; x < COLS; ++x) {
+            const bool selected = exists[x] && lists.has(nth, token[x]);
+            limit[x] = step_limit(selected, last_key[x], first_key, g);
+            any = any || limit[x] > 0;
+        }
+        return __any(any);
     }
-    if (a.lse && g == 0) {
-        a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + token) * s.q_heads + head] =
-            l == 0.0f ? kNegInf : (m + log2_fast(l)) * kLn2;
+};
+
+template <typename T, int DP, int BN, int COLS>
+__global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args<T> a) {
+    using Lds = Tile<T, DP, BN, kThreads>;
+    constexpr int kRowsOf = 64 * COLS;
+    __shared__ __align__(16) T s_k0[Lds::kElements];
+    __shared__ __align__(16) T s_v0[Lds::kElements];
+    __shared__ __align__(16) T s_k1[Lds::kElements];
+    __shared__ __align__(16) T s_v1[Lds::kElements];
+    __shared__ Lists<kRowsOf> s_lists;
+    const Shape &s = a.s;
+    const RowTile<kRowsOf> tile(s, a.lengths, static_cast<int>(blockIdx.x));
+    const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
+    const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const LaneRows<COLS> rows(s, tile, wave, c);
+    Frag<T> q[COLS][DP / 32];
+    f32x4 o[COLS][DP / 16];
+    float m[COLS], l[COLS];
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) {
+        load_row_frags<T, DP>(
+            rows.exists[x] ? a.q.row(tile.b, tile.t0 + rows.token[x], rows.head[x]) : nullptr,
+            s.dim, g, q[x]);
+        if (s.scale < 0.0f) negate<T, DP>(q[x]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[x] = kNegInf;
+        l[x] = 0.0f;
+    }
+    const float scale2 = base2_scale(s.scale);
+    KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
+    steps.run(a, tile, [&](const T *s_k, const T *s_v, int nth, int first_key) {
+        int limit[COLS];
+        if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
+        f32x4 p[COLS][BN / 16];
+        row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+            float factor;
+            if (softmax_step<BN / 16>(p[x], scale2, limit[x], m[x], l[x], factor)) {
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
+            }
+        }
+        column_products<Lds, T, DP, COLS, BN / 16>(s_v, p, g, c, o);
+    });
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) {
+        const float sum = column_sum(l[x]);
+        if (!rows.exists[x]) continue;
+        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (NaN stays)
+        const int t = tile.t0 + rows.token[x], head = rows.head[x];
+        T *out = a.out.row(tile.b, t, head);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int col = 16 * i + 4 * g;
+            if (col < s.dim) store4<T>(out + col, o[x][i] * inverse);
+        }
+        if (a.lse && g == 0) {
+            a.lse[(static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head] =
+                sum == 0.0f ? kNegInf : (m[x] + log2_fast(sum)) * kLn2;
+        }
     }
 }
 
@@ -317,36 +394,39 @@ constexpr int kSplitKeys = 32;  // keys of a step
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, Partials part) {
-    constexpr int kRow = kTileRow<T, DP>;
+    using Stage = TileStage<T, DP, kSplitKeys>;
     constexpr int kJoin = DP + 4;  // floats of a row of o in LDS
-    constexpr int kTileBytes = kSplitKeys * kRow * static_cast<int>(sizeof(T));
+    constexpr int kTileBytes = Stage::Lds::kElements * static_cast<int>(sizeof(T));
     constexpr int kJoinBytes = 16 * kJoin * 4;
     constexpr int kWaveBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
     __shared__ __align__(16) unsigned char s_wave[kWaves][kWaveBytes];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-    __shared__ Lists s_lists;
+    __shared__ Lists<16> s_lists;
     const Shape &s = a.s;
     const int split = static_cast<int>(blockIdx.x) % splits;
     const int index = static_cast<int>(blockIdx.x) / splits;
-    const Tile<16> tile(s, a.lengths, index);
+    const RowTile<16> tile(s, a.lengths, index);
     const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
     const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
     T *s_v = reinterpret_cast<T *>(s_wave[wave]);
     int token, head;
     const bool exists = tile.row(s, c, token, head);
+    if (!exists) token = 0;
     const int last_key = exists ? tile.last_key(s, token) : -1;
-    Frag<T> q[DP / 32];
-    load_row_frags<T, DP>(exists ? a.q.row(tile.b, tile.t0 + token, head) : nullptr, s.dim, g, q);
-    f32x4 o[DP / 16];
+    Frag<T> q[1][DP / 32];
+    load_row_frags<T, DP>(exists ? a.q.row(tile.b, tile.t0 + token, head) : nullptr, s.dim, g,
+                          q[0]);
+    if (s.scale < 0.0f) negate<T, DP>(q[0]);
+    f32x4 o[1][DP / 16];
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < DP / 16; ++i) o[0][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = kNegInf, l = 0.0f;
-    const float scale2 = s.scale * kLog2e;
+    const float scale2 = base2_scale(s.scale);
     const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
     const int end = tile.last_key(s, tile.tokens - 1) + 1;
     const int steps_of = s.block / kSplitKeys;
     const int stride = splits * kWaves;
-    TileLoad<T, DP, kSplitKeys, dev::kWave> v_next;
+    Stage v_next;
     Frag<T> k_next[2][DP / 32];
     for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
         const int steps = window_lists(s, a.ids, tile, first, s_lists) * steps_of;
@@ -368,29 +448,28 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
         int step = split * kWaves + wave;
         if (step < steps) load(step);
         for (; step < steps; step += stride) {  // the wavefront's own
-            const unsigned long long tokens = s_lists.mask[s_lists.ids[step / steps_of]];
-            const bool selected = exists && (tokens >> token & 1ull);
+            const bool selected = exists && s_lists.has(step / steps_of, token);
             const int limit = step_limit(selected, last_key, first_key(step), g);
-            f32x4 p[2];
+            f32x4 p[1][2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                p[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                p[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) p[t] = mma(k_next[t][kk], q[kk], p[t]);
+                for (int kk = 0; kk < DP / 32; ++kk) {
+                    p[0][t] = mma(k_next[t][kk], q[0][kk], p[0][t]);
+                }
             }
             dev::wave_sync();  // the reads of the step before
             v_next.store(lane, s_v);
             dev::wave_sync();
             if (step + stride < steps) load(step + stride);
             if (!__any(limit > 0)) continue;
-            const float factor = softmax_step<2>(p, scale2, limit, m, l);
+            float factor;
+            if (softmax_step<2>(p[0], scale2, limit, m, l, factor)) {
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) o[i] *= factor;
-            const Frag<T> pf = result_frag<T>(p[0], p[1]);
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                o[i] = mma(column_frag<kRow>(s_v, 16 * i, g, c), pf, o[i]);
+                for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
             }
+            column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
         }
     }
     l = column_sum(l);
@@ -399,7 +478,7 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
     float *s_o = reinterpret_cast<float *>(s_wave[wave]);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-        *reinterpret_cast<f32x4 *>(s_o + c * kJoin + 16 * i + 4 * g) = o[i];
+        *reinterpret_cast<f32x4 *>(s_o + c * kJoin + 16 * i + 4 * g) = o[0][i];
     }
     if (g == 0) {
         s_m[wave][c] = m;
@@ -446,7 +525,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(DP) void join_kernel(Args<T> a, int splits, Partials part) {
     const Shape &s = a.s;
     const int index = static_cast<int>(blockIdx.x) / 16, r = static_cast<int>(blockIdx.x) % 16;
-    const Tile<16> tile(s, a.lengths, index);
+    const RowTile<16> tile(s, a.lengths, index);
     int t, hd;
     if (!tile.row(s, r, t, hd)) return;
     const int64_t at = static_cast<int64_t>(index) * splits * 16 + r;
@@ -496,261 +575,393 @@ __global__ __launch_bounds__(kThreads) void delta_kernel(Args<T> a, float *__res
 }
 
 // bits[b][h][block][token / 32]: the tokens that see something of the block through their ids.
+// A workgroup has 128 tokens of a head (four words of each block), gathered in LDS for
+// kMarkWindow blocks at a time: with a word per block and tokens of 32 each, atomics on the
+// words in memory took 29 us, five times this, for 2 x 4096 tokens with 12 ids of 4 heads.
+constexpr int kMarkWords = 4;
+constexpr int kMarkWindow = 1024;
+
 __global__ __launch_bounds__(kThreads) void mark_kernel(Shape s, const int *__restrict__ lengths,
                                                         const int *__restrict__ ids, int words,
                                                         unsigned *__restrict__ bits) {
-    const int64_t n = static_cast<int64_t>(s.batch) * s.queries * s.kv_heads * s.count;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int id = ids[i];
-        const int64_t row = i / s.count;
-        const int h = static_cast<int>(row % s.kv_heads);
-        const int64_t bt = row / s.kv_heads;
-        const int t = static_cast<int>(bt % s.queries), b = static_cast<int>(bt / s.queries);
-        const int length = length_of(s, lengths, b);
-        const int place = length - s.queries + t;
-        const int last = place < 0 ? -1 : s.causal ? place : length - 1;
-        if (last < 0 || static_cast<unsigned>(id) > static_cast<unsigned>(last / s.block)) continue;
-        const int64_t at = (static_cast<int64_t>(b) * s.kv_heads + h) * s.blocks + id;
-        atomicOr(&bits[at * words + t / 32], 1u << (t % 32));
+    __shared__ __align__(16) unsigned s_bits[kMarkWindow][kMarkWords];
+    const int heads = s.batch * s.kv_heads;
+    const int bh = static_cast<int>(blockIdx.x) % heads;
+    const int w0 = static_cast<int>(blockIdx.x) / heads * kMarkWords;
+    const int b = bh / s.kv_heads, h = bh % s.kv_heads;
+    const int length = length_of(s, lengths, b);
+    const int t0 = 32 * w0;
+    const int n = min(32 * kMarkWords, s.queries - t0) * s.count;
+    for (int first = 0; first < s.blocks; first += kMarkWindow) {  // uniform
+        for (int i = threadIdx.x; i < kMarkWindow * kMarkWords; i += kThreads) {
+            (&s_bits[0][0])[i] = 0u;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const int t = i / s.count, x = i - t * s.count;
+            const int place = length - s.queries + t0 + t;
+            const int last = place < 0 ? -1 : s.causal ? place : length - 1;
+            const int64_t row = (static_cast<int64_t>(b) * s.queries + t0 + t) * s.kv_heads + h;
+            const int id = ids[row * s.count + x];
+            if (last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block) &&
+                id >= first && id < first + kMarkWindow) {
+                atomicOr(&s_bits[id - first][t / 32], 1u << (t % 32));
+            }
+        }
+        __syncthreads();
+        const int there = min(kMarkWindow, s.blocks - first);
+        for (int i = threadIdx.x; i < there; i += kThreads) {
+            const int64_t row = static_cast<int64_t>(bh) * s.blocks + first + i;
+            *reinterpret_cast<u32x4 *>(bits + row * words + w0) =
+                *reinterpret_cast<const u32x4 *>(s_bits[i]);
+        }
+        __syncthreads();
     }
 }
 
-__global__ __launch_bounds__(kThreads) void clear_kernel(unsigned *__restrict__ words, int64_t n) {
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        words[i] = 0u;
-    }
+// items[row]: parts of at most `per_item` tokens that the row (a block of a head) is worked on
+// in, one at least.  A wavefront per row.
+__global__ __launch_bounds__(kThreads) void items_kernel(int64_t rows, int words, int per_item,
+                                                         const unsigned *__restrict__ bits,
+                                                         int64_t *__restrict__ items) {
+    const int64_t row =
+        blockIdx.x * static_cast<int64_t>(kWaves) + threadIdx.x / dev::kWave;
+    if (row >= rows) return;
+    int n = 0;
+    for (int w = dev::lane(); w < words; w += dev::kWave) n += __popc(bits[row * words + w]);
+    n = dev::wave_sum(n);
+    if (dev::lane() == 0) items[row] = n > per_item ? (n + per_item - 1) / per_item : 1;
 }
 
-// Gradient of the scores from the products s = q . k and dp = dout . v of 16 N keys: ds (without
-// the scale) replaces dp, and the probabilities s.
+// From the products s = q . k and dp = dout . v of 16 N keys with a row: s become probabilities
+// and dp the scores' gradients (without the scale).
 template <int N>
 __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], float scale2,
                                                float lse2, float delta, int limit) {
+    const bool whole = __all(limit >= 16 * N);
 #pragma unroll
     for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool seen = 16 * t + i < limit;
-            s[t][i] = seen ? exp2_fast(s[t][i] * scale2 - lse2) : 0.0f;
-            dp[t][i] = seen ? s[t][i] * (dp[t][i] - delta) : 0.0f;
+            const float p = exp2_fast(__builtin_fmaf(s[t][i], scale2, -lse2));
+            const float ds = p * (dp[t][i] - delta);
+            const bool seen = whole || 16 * t + i < limit;
+            s[t][i] = seen ? p : 0.0f;
+            dp[t][i] = seen ? ds : 0.0f;
         }
     }
 }
 
-template <typename T, int DP, int BN>
-__global__ __launch_bounds__(kThreads) void dq_kernel(Args<T> a, const float *__restrict__ delta) {
-    constexpr int kRow = kTileRow<T, DP>;
-    __shared__ __align__(16) T s_k[BN * kRow];
-    __shared__ __align__(16) T s_v[BN * kRow];
-    __shared__ Lists s_lists;
+template <typename T, int DP, int BN, int COLS>
+__global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a,
+                                                         const float *__restrict__ delta) {
+    using Lds = Tile<T, DP, BN, kThreads>;
+    constexpr int kRowsOf = 64 * COLS;
+    __shared__ __align__(16) T s_k0[Lds::kElements];
+    __shared__ __align__(16) T s_v0[Lds::kElements];
+    __shared__ __align__(16) T s_k1[Lds::kElements];
+    __shared__ __align__(16) T s_v1[Lds::kElements];
+    __shared__ Lists<kRowsOf> s_lists;
     const Shape &s = a.s;
-    const Tile<64> tile(s, a.lengths, static_cast<int>(blockIdx.x));
+    const RowTile<kRowsOf> tile(s, a.lengths, static_cast<int>(blockIdx.x));
     const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
     const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
-    int token, head;
-    const bool exists = tile.row(s, 16 * wave + c, token, head);
-    const int last_key = exists ? tile.last_key(s, token) : -1;
-    Frag<T> q[DP / 32], dout[DP / 32];
-    load_row_frags<T, DP>(exists ? a.q.row(tile.b, tile.t0 + token, head) : nullptr, s.dim, g, q);
-    load_row_frags<T, DP>(exists ? a.dout.row(tile.b, tile.t0 + token, head) : nullptr, s.dim, g,
-                          dout);
-    const int64_t at =
-        (static_cast<int64_t>(tile.b) * s.queries + tile.t0 + token) * s.q_heads + head;
-    const float lse = exists ? a.lse[at] : 0.0f;
-    const float lse2 = lse == kNegInf ? 0.0f : lse * kLog2e;
-    const float row_delta = exists ? delta[at] : 0.0f;
-    f32x4 o[DP / 16];
+    const LaneRows<COLS> rows(s, tile, wave, c);
+    Frag<T> q[COLS][DP / 32], dout[COLS][DP / 32];
+    f32x4 o[COLS][DP / 16];
+    float lse2[COLS], row_delta[COLS];
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const float scale2 = s.scale * kLog2e;
-    const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
-    const int end = tile.last_key(s, tile.tokens - 1) + 1;
-    const int steps_of = s.block / BN;
-    TileLoad<T, DP, BN, kThreads> k_next, v_next;
-    for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
-        const int steps = window_lists(s, a.ids, tile, first, s_lists) * steps_of;
-        auto first_key = [&](int step) {
-            return (first + s_lists.ids[step / steps_of]) * s.block + step % steps_of * BN;
-        };
-        auto load = [&](int step) {
-            const int key = first_key(step);
-            k_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                return key + r < tile.length ? k_base + (key + r) * a.k.row_stride : nullptr;
-            });
-            v_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                return key + r < tile.length ? v_base + (key + r) * a.v.row_stride : nullptr;
-            });
-        };
-        if (steps > 0) load(0);
-        for (int step = 0; step < steps; ++step) {
-            __syncthreads();
-            k_next.store(threadIdx.x, s_k);
-            v_next.store(threadIdx.x, s_v);
-            __syncthreads();
-            if (step + 1 < steps) load(step + 1);
-            const unsigned long long tokens = s_lists.mask[s_lists.ids[step / steps_of]];
-            const bool selected = exists && (tokens >> token & 1ull);
-            const int limit = step_limit(selected, last_key, first_key(step), g);
-            if (!__any(limit > 0)) continue;
-            f32x4 p[BN / 16], dp[BN / 16];
+    for (int x = 0; x < COLS; ++x) {
+        const bool exists = rows.exists[x];
+        const int t = tile.t0 + rows.token[x], head = rows.head[x];
+        load_row_frags<T, DP>(exists ? a.q.row(tile.b, t, head) : nullptr, s.dim, g, q[x]);
+        load_row_frags<T, DP>(exists ? a.dout.row(tile.b, t, head) : nullptr, s.dim, g, dout[x]);
+        if (s.scale < 0.0f) negate<T, DP>(q[x]);
+        const int64_t at = (static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head;
+        const float lse = exists ? a.lse[at] : 0.0f;
+        lse2[x] = lse == kNegInf ? 0.0f : lse * kLog2e;
+        row_delta[x] = exists ? delta[at] : 0.0f;
 #pragma unroll
-            for (int t = 0; t < BN / 16; ++t) {
-                p[t] = dp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    const int x = (16 * t + c) * kRow + 32 * kk + 8 * g;
-                    p[t] = mma(row_frag<T>(s_k + x), q[kk], p[t]);
-                    dp[t] = mma(row_frag<T>(s_v + x), dout[kk], dp[t]);
-                }
-            }
-            score_gradient<BN / 16>(p, dp, scale2, lse2, row_delta, limit);
-#pragma unroll
-            for (int u = 0; u < BN / 32; ++u) {
-                const Frag<T> ds = result_frag<T>(dp[2 * u], dp[2 * u + 1]);
-#pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    o[i] = mma(column_frag<kRow>(s_k + 32 * u * kRow, 16 * i, g, c), ds, o[i]);
-                }
-            }
-        }
+        for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (!exists) return;
-    T *dq = a.dq.row(tile.b, tile.t0 + token, head);
+    const float scale2 = base2_scale(s.scale);
+    KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
+    steps.run(a, tile, [&](const T *s_k, const T *s_v, int nth, int first_key) {
+        int limit[COLS];
+        if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
+        f32x4 p[COLS][BN / 16], dp[COLS][BN / 16];
+        row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
+        row_products<Lds, T, DP, COLS, BN / 16>(s_v, dout, g, c, dp);
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-        const int col = 16 * i + 4 * g;
-        if (col < s.dim) store4<T>(dq + col, o[i] * s.scale);
+        for (int x = 0; x < COLS; ++x) {
+            score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x]);
+        }
+        column_products<Lds, T, DP, COLS, BN / 16>(s_k, dp, g, c, o);
+    });
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) {
+        if (!rows.exists[x]) continue;
+        T *dq = a.dq.row(tile.b, tile.t0 + rows.token[x], rows.head[x]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int col = 16 * i + 4 * g;
+            if (col < s.dim) store4<T>(dq + col, o[x][i] * s.scale);
+        }
     }
 }
 
-constexpr int kTokenWords = 64;  // words of a block's bits that are listed at a time
-constexpr int kRows = 32;        // (token, head) rows of a step
+constexpr int kItemTokens = 2048;  // tokens of an item, at most (their numbers are in LDS)
+constexpr int kStepRows = 32;      // (token, head) rows of a wavefront's step
+constexpr int kMaxGroup = 1024;    // heads of a group: what the division below holds for
 
-// dk and dv of 16 x WAVES keys of a block: each wavefront has 16 keys' columns, and all go over
-// the rows of the tokens that selected the block.
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES *dev::kWave) void dkv_kernel(
-    Args<T> a, const float *__restrict__ delta, int words, const unsigned *__restrict__ bits) {
-    constexpr int kBlock = WAVES * dev::kWave;
-    constexpr int kRow = kTileRow<T, DP>;
-    __shared__ __align__(16) T s_q[kRows * kRow];
-    __shared__ __align__(16) T s_do[kRows * kRow];
-    __shared__ __align__(16) float s_lse[kRows], s_delta[kRows];
-    __shared__ __align__(16) int s_last[kRows];
-    __shared__ unsigned short s_tokens[kTokenWords * 32];
-    __shared__ int s_sums[WAVES];
+// Work on dk and dv: the rows (blocks of heads) in items of at most per_item tokens, so that a
+// block that every query selects is not one workgroup's.  start[row] are the rows' first items.
+struct Items {
+    const int64_t *start;
+    int64_t rows;
+    int per_item, words;
+    const unsigned *bits;
+    float *partial;  // [item][key of the block][2][DP]: dk and dv of an item of several
+};
+
+// dk and dv of 16 COLS LANES keys of a block.  Each of LANES wavefronts has 16 COLS of the keys;
+// with LANES = 2 the four wavefronts are two such sets, which take 32 rows of the item's tokens
+// in turn and add their sums at the end.
+template <typename T, int DP, int COLS, int LANES>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(Args<T> a, const float *__restrict__ delta,
+                                                       Items items, unsigned group_inverse) {
+    constexpr int kSets = kWaves / LANES;
+    constexpr int kStep = kSets * kStepRows;
+    using Lds = Tile<T, DP, kStep, kThreads>;
+    constexpr int kKeys = 16 * COLS * LANES;
+    // two buffers of q and dout, and later the sums of the second set
+    __shared__ __align__(16) T s_q0[Lds::kElements];
+    __shared__ __align__(16) T s_do0[Lds::kElements];
+    __shared__ __align__(16) T s_q1[Lds::kElements];
+    __shared__ __align__(16) T s_do1[Lds::kElements];
+    __shared__ __align__(16) float s_lse[2][kStep], s_delta[2][kStep];
+    __shared__ __align__(16) int s_last[2][kStep];
+    __shared__ int s_tokens[kItemTokens];
+    __shared__ int s_sums[kWaves];
     const Shape &s = a.s;
-    const int heads = s.batch * s.kv_heads;
-    const int parts = s.block / (16 * WAVES);
-    const int bh = static_cast<int>(blockIdx.x) % heads;
-    const int part = static_cast<int>(blockIdx.x) / heads;
-    const int id = part / parts;
+    const int parts = s.block / kKeys;
+    // Workgroups go to the 8 XCDs in turn: each XCD takes a stretch of items, so that the rows
+    // of few heads are in its L2.
+    const int64_t all = items.start[items.rows] * parts;
+    const int64_t stretch = (all + 7) / 8;
+    const int64_t index = blockIdx.x % 8 * stretch + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= stretch || index >= all) return;
+    const int64_t item = index / parts;
+    const int part = static_cast<int>(index % parts);
+    const int64_t row = dev::last_le(items.start, 0, items.rows - 1, item);
+    const int64_t nth = item - items.start[row];
+    const bool whole = items.start[row + 1] - items.start[row] == 1;
+    const int bh = static_cast<int>(row / s.blocks), id = static_cast<int>(row % s.blocks);
     const int b = bh / s.kv_heads, h = bh % s.kv_heads;
     const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
     const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const int part_of = wave % LANES, set = wave / LANES;  // of the keys, of the rows
     const int length = length_of(s, a.lengths, b);
-    const int key = id * s.block + part % parts * 16 * WAVES + 16 * wave + c;
-    const bool exists = key < length;
-    Frag<T> k[DP / 32], v[DP / 32];
-    load_row_frags<T, DP>(exists ? a.k.row(b, key, h) : nullptr, s.dim, g, k);
-    load_row_frags<T, DP>(exists ? a.v.row(b, key, h) : nullptr, s.dim, g, v);
-    f32x4 dk[DP / 16], dv[DP / 16];
+    const int in_block = part * kKeys + 16 * COLS * part_of + c;  // + 16 x
+    const int first_key = id * s.block + in_block;
+    Frag<T> k[COLS][DP / 32], v[COLS][DP / 32];
+    f32x4 dk[COLS][DP / 16], dv[COLS][DP / 16];
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) dk[i] = dv[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const float scale2 = s.scale * kLog2e;
+    for (int x = 0; x < COLS; ++x) {
+        const int key = first_key + 16 * x;
+        const bool exists = key < length;
+        load_row_frags<T, DP>(exists ? a.k.row(b, key, h) : nullptr, s.dim, g, k[x]);
+        load_row_frags<T, DP>(exists ? a.v.row(b, key, h) : nullptr, s.dim, g, v[x]);
+        if (s.scale < 0.0f) negate<T, DP>(k[x]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) dk[x][i] = dv[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const float scale2 = base2_scale(s.scale);
     const int place0 = length - s.queries;
-    const unsigned *row_bits = bits + (static_cast<int64_t>(bh) * s.blocks + id) * words;
-    TileLoad<T, DP, kRows, kBlock> q_next, do_next;
-    for (int w0 = 0; w0 < words; w0 += kTokenWords) {  // uniform
-        // the tokens of these words, ascending
-        __syncthreads();
-        const int w = static_cast<int>(threadIdx.x);
-        unsigned mine = w < kTokenWords && w0 + w < words ? row_bits[w0 + w] : 0u;
+
+    // The item's tokens, ascending: those of the row's set bits from the nth * per_item-th on.
+    const unsigned *row_bits = items.bits + row * items.words;
+    const int64_t from = nth * items.per_item;
+    int64_t seen = 0;
+    for (int w0 = 0; w0 < items.words; w0 += kThreads) {  // uniform
+        const int w = w0 + static_cast<int>(threadIdx.x);
+        unsigned mine = w < items.words ? row_bits[w] : 0u;
         int total = 0;
-        int at = dev::block_exclusive_sum<kBlock>(static_cast<int>(__popc(mine)), s_sums,
-                                                   total);
-        for (; mine; mine &= mine - 1u) {
-            s_tokens[at++] = static_cast<unsigned short>(32 * w + __ffs(mine) - 1);
+        const int before = dev::block_exclusive_sum<kThreads>(static_cast<int>(__popc(mine)),
+                                                              s_sums, total);
+        int64_t at = seen + before - from;
+        for (; mine; mine &= mine - 1u, ++at) {
+            if (at >= 0 && at < items.per_item) {
+                s_tokens[at] = 32 * w + __ffs(static_cast<int>(mine)) - 1;
+            }
         }
-        __syncthreads();
-        const int rows = total * s.group;
-        auto token_of = [&](int r) { return 32 * w0 + s_tokens[r / s.group]; };
-        auto load = [&](int r0) {
-            q_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                const int x = r0 + r;
-                return x < rows ? a.q.row(b, token_of(x), h * s.group + x % s.group) : nullptr;
-            });
-            do_next.load(threadIdx.x, s.dim, [&](int r) -> const T * {
-                const int x = r0 + r;
-                return x < rows ? a.dout.row(b, token_of(x), h * s.group + x % s.group) : nullptr;
-            });
+        seen += total;
+        if (seen >= from + items.per_item) break;
+    }
+    __syncthreads();
+    const int64_t left = seen - from;
+    const int rows = static_cast<int>(left < items.per_item ? (left < 0 ? 0 : left)
+                                                            : items.per_item) * s.group;
+    // x / group (exact: x < 2^11 group, and group^2 2^11 < 2^32)
+    auto token_at = [&](int x) {
+        return s.group == 1 ? x
+                            : static_cast<int>(__umulhi(static_cast<unsigned>(x), group_inverse));
+    };
+    auto load = [&](int r0, T *to_q, T *to_do) {
+        auto place = [&](int r, int &t, int &head) {
+            const int x = min(r0 + r, rows - 1);
+            const int at = token_at(x);
+            t = s_tokens[at];
+            head = h * s.group + x - at * s.group;
         };
-        if (rows > 0) load(0);
-        for (int r0 = 0; r0 < rows; r0 += kRows) {
-            __syncthreads();
-            q_next.store(threadIdx.x, s_q);
-            do_next.store(threadIdx.x, s_do);
-            if (threadIdx.x < kRows) {
-                const int x = r0 + static_cast<int>(threadIdx.x);
-                float lse = 0.0f, d = 0.0f;
-                int last = -1;
-                if (x < rows) {
-                    const int t = token_of(x);
-                    const int64_t i = (static_cast<int64_t>(b) * s.queries + t) * s.q_heads +
-                                      h * s.group + x % s.group;
-                    lse = a.lse[i];
-                    lse = lse == kNegInf ? 0.0f : lse * kLog2e;
-                    d = delta[i];
-                    last = s.causal ? place0 + t : length - 1;
+        Lds::load(to_q, threadIdx.x, s.dim, [&](int r) -> const T * {
+            int t, head;
+            place(r, t, head);
+            return a.q.row(b, t, head);
+        });
+        Lds::load(to_do, threadIdx.x, s.dim, [&](int r) -> const T * {
+            int t, head;
+            place(r, t, head);
+            return a.dout.row(b, t, head);
+        });
+    };
+    // lse, delta and last key of row r0 + thread, for the first kStep threads
+    auto info = [&](int r0, int buffer) {
+        const int x = r0 + static_cast<int>(threadIdx.x);
+        float lse = 0.0f, d = 0.0f;
+        int last = -1;
+        if (x < rows) {
+            const int at = token_at(x), t = s_tokens[at];
+            const int64_t i = (static_cast<int64_t>(b) * s.queries + t) * s.q_heads +
+                              h * s.group + x - at * s.group;
+            lse = a.lse[i];
+            lse = lse == kNegInf ? 0.0f : lse * kLog2e;
+            d = delta[i];
+            last = s.causal ? place0 + t : length - 1;
+        }
+        s_lse[buffer][threadIdx.x] = lse;
+        s_delta[buffer][threadIdx.x] = d;
+        s_last[buffer][threadIdx.x] = last;
+    };
+    auto use = [&](const T *s_q, const T *s_do, int buffer) {
+        const T *my_q = s_q + set * kStepRows * DP, *my_do = s_do + set * kStepRows * DP;
+        constexpr int kN = kStepRows / 16;
+        f32x4 p[COLS][kN], dp[COLS][kN];
+        row_products<Lds, T, DP, COLS, kN>(my_q, k, g, c, p);
+        row_products<Lds, T, DP, COLS, kN>(my_do, v, g, c, dp);
+#pragma unroll
+        for (int t = 0; t < kN; ++t) {
+            // this lane's rows 16 t + 4 g + i, its keys in each
+            const int r = set * kStepRows + 16 * t + 4 * g;
+            const f32x4 lse = *reinterpret_cast<const f32x4 *>(&s_lse[buffer][r]);
+            const f32x4 d = *reinterpret_cast<const f32x4 *>(&s_delta[buffer][r]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int last = s_last[buffer][r + i];
+#pragma unroll
+                for (int x = 0; x < COLS; ++x) {
+                    const float e = exp2_fast(__builtin_fmaf(p[x][t][i], scale2, -lse[i]));
+                    const float ds = e * (dp[x][t][i] - d[i]);
+                    const bool sees = first_key + 16 * x <= last;
+                    p[x][t][i] = sees ? e : 0.0f;
+                    dp[x][t][i] = sees ? ds : 0.0f;
                 }
-                s_lse[threadIdx.x] = lse;
-                s_delta[threadIdx.x] = d;
-                s_last[threadIdx.x] = last;
             }
-            __syncthreads();
-            if (r0 + kRows < rows) load(r0 + kRows);
-            f32x4 p[kRows / 16], dp[kRows / 16];
+        }
+        column_products<Lds, T, DP, COLS, kN>(my_do, p, g, c, dv);
+        column_products<Lds, T, DP, COLS, kN>(my_q, dp, g, c, dk);
+    };
+    const bool informs = threadIdx.x < kStep;
+    if (rows > 0) {
+        load(0, s_q0, s_do0);
+        if (informs) info(0, 0);
+    }
+    __syncthreads();
+    for (int r0 = 0; r0 < rows; r0 += 2 * kStep) {
+        if (r0 + kStep < rows) {
+            load(r0 + kStep, s_q1, s_do1);
+            if (informs) info(r0 + kStep, 1);
+        }
+        use(s_q0, s_do0, 0);
+        __syncthreads();
+        if (r0 + kStep >= rows) break;
+        if (r0 + 2 * kStep < rows) {
+            load(r0 + 2 * kStep, s_q0, s_do0);
+            if (informs) info(r0 + 2 * kStep, 0);
+        }
+        use(s_q1, s_do1, 1);
+        __syncthreads();
+    }
+    if constexpr (kSets == 2) {
+        // The second set's sums are added to the first's, dk's through the buffers of q and dv's
+        // through those of dout.
+        static_assert(16 * COLS * DP * 4 <= Lds::kElements * static_cast<int>(sizeof(T)),
+                      "a wavefront's sums fit a buffer");
+        float *sum_k = reinterpret_cast<float *>(part_of ? s_q1 : s_q0);
+        float *sum_v = reinterpret_cast<float *>(part_of ? s_do1 : s_do0);
+        auto each = [&](auto f) {
 #pragma unroll
-            for (int t = 0; t < kRows / 16; ++t) {
-                p[t] = dp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    const int x = (16 * t + c) * kRow + 32 * kk + 8 * g;
-                    p[t] = mma(row_frag<T>(s_q + x), k[kk], p[t]);
-                    dp[t] = mma(row_frag<T>(s_do + x), v[kk], dp[t]);
-                }
-                // this lane's rows 16 t + 4 g + i, its key in each
-                const f32x4 lse = *reinterpret_cast<const f32x4 *>(s_lse + 16 * t + 4 * g);
-                const f32x4 d = *reinterpret_cast<const f32x4 *>(s_delta + 16 * t + 4 * g);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool seen = key <= s_last[16 * t + 4 * g + i];
-                    p[t][i] = seen ? exp2_fast(p[t][i] * scale2 - lse[i]) : 0.0f;
-                    dp[t][i] = seen ? p[t][i] * (dp[t][i] - d[i]) : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kRows / 32; ++u) {
-                const Frag<T> pf = result_frag<T>(p[2 * u], p[2 * u + 1]);
-                const Frag<T> ds = result_frag<T>(dp[2 * u], dp[2 * u + 1]);
+            for (int x = 0; x < COLS; ++x) {
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) {
-                    dv[i] = mma(column_frag<kRow>(s_do + 32 * u * kRow, 16 * i, g, c), pf, dv[i]);
-                    dk[i] = mma(column_frag<kRow>(s_q + 32 * u * kRow, 16 * i, g, c), ds, dk[i]);
+                    const int at = ((x * (DP / 16) + i) * dev::kWave + lane) * 4;
+                    f(*reinterpret_cast<f32x4 *>(sum_k + at), dk[x][i]);
+                    f(*reinterpret_cast<f32x4 *>(sum_v + at), dv[x][i]);
                 }
+            }
+        };
+        if (set == 1) each([](f32x4 &there, const f32x4 &mine) { there = mine; });
+        __syncthreads();
+        if (set == 1) return;
+        each([](const f32x4 &there, f32x4 &mine) { mine += there; });
+    }
+#pragma unroll
+    for (int x = 0; x < COLS; ++x) {
+        const int key = first_key + 16 * x;
+        float *part_out = items.partial + (item * s.block + in_block + 16 * x) * (2 * DP);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const f32x4 sk = dk[x][i], sv = dv[x][i];
+            const int col = 16 * i + 4 * g;
+            if (!whole) {
+                *reinterpret_cast<f32x4 *>(part_out + col) = sk;
+                *reinterpret_cast<f32x4 *>(part_out + DP + col) = sv;
+            } else if (key < s.keys && col < s.dim) {  // (past the length: zeros)
+                store4<T>(a.dk.row(b, key, h) + col, sk * s.scale);
+                store4<T>(a.dv.row(b, key, h) + col, sv);
             }
         }
     }
-    if (key >= s.keys) return;  // (keys past the length have gradients: zeros)
-    T *out_k = a.dk.row(b, key, h), *out_v = a.dv.row(b, key, h);
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-        const int col = 16 * i + 4 * g;
-        if (col < s.dim) {
-            store4<T>(out_k + col, dk[i] * s.scale);
-            store4<T>(out_v + col, dv[i]);
+}
+
+// Adds up the items of a row that has several, in their order: a workgroup per 16 keys.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void dkv_join_kernel(Args<T> a, Items items) {
+    const Shape &s = a.s;
+    const int parts = s.block / 16;
+    const int64_t row = blockIdx.x / parts;
+    const int part = static_cast<int>(blockIdx.x % parts);
+    const int64_t from = items.start[row], to = items.start[row + 1];
+    if (to - from <= 1) return;
+    const int bh = static_cast<int>(row / s.blocks), id = static_cast<int>(row % s.blocks);
+    const int b = bh / s.kv_heads, h = bh % s.kv_heads;
+    constexpr int kPieces = 2 * DP / 4;  // of a key: four columns of dk or dv
+    for (int x = threadIdx.x; x < 16 * kPieces; x += kThreads) {
+        const int in_block = 16 * part + x / kPieces, piece = x % kPieces;
+        const int key = id * s.block + in_block;
+        const bool is_v = piece >= kPieces / 2;
+        const int col = 4 * (is_v ? piece - kPieces / 2 : piece);
+        if (key >= s.keys || col >= s.dim) continue;
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int64_t i = from; i < to; ++i) {
+            sum += *reinterpret_cast<const f32x4 *>(
+                items.partial + (i * s.block + in_block) * (2 * DP) + 4 * piece);
+        }
+        if (is_v) {
+            store4<T>(a.dv.row(b, key, h) + col, sum);
+        } else {
+            store4<T>(a.dk.row(b, key, h) + col, sum * s.scale);
         }
     }
 }
@@ -767,7 +978,7 @@ bool aligned(const nacho_heads &h, int item, bool optional = false) {
 int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
     if (!p || p->dtype < NACHO_F32 || p->dtype > NACHO_BF16) return NACHO_ERR_INVALID_ARGUMENT;
     if (p->batch < 0 || p->queries < 0 || p->keys < 0 || p->q_heads < 1 || p->kv_heads < 1 ||
-        p->q_heads % p->kv_heads != 0 || p->head_dim < 8 || p->head_dim > 128 ||
+        p->q_heads % p->kv_heads != 0 || p->q_heads / p->kv_heads > kMaxGroup || p->head_dim < 8 || p->head_dim > 128 ||
         p->head_dim % 8 != 0 || (p->block != 32 && p->block != 64 && p->block != 128) ||
         p->count < 0 || (p->causal != 0 && p->causal != 1) || !std::isfinite(p->scale)) {
         return NACHO_ERR_INVALID_ARGUMENT;
@@ -813,17 +1024,39 @@ Args<T> args_of(const nacho_block_attention_args &p, const Shape &s) {
                    p.lse};
 }
 
-// Calls f with the keys of a step: 64, or 32 where the block or float32's tiles (twice as large:
-// 32 keys keep two workgroups on a CU) want it.
+constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
+
+// Calls f with the keys of a step, 64, or 32 where the block or float32's tiles (twice as large)
+// want it, and the column tiles of a wavefront: two share what each reads of LDS, one where that
+// leaves CUs without a workgroup.
 template <typename T, typename F>
-void with_step(const Shape &s, F f) {
+int with_tiles(const Shape &s, F f) {
+    const int heads = s.batch * s.kv_heads;
+    const int64_t large = static_cast<int64_t>(tiling(s, 128).per_head) * heads;
+    auto columns = [&](auto keys) {
+        if (sizeof(T) == 2 && large >= kFullGrid) {
+            f(keys, std::integral_constant<int, sizeof(T) == 2 ? 2 : 1>{},
+              static_cast<unsigned>(large));
+        } else {
+            f(keys, std::integral_constant<int, 1>{},
+              static_cast<unsigned>(tiling(s, 64).per_head * heads));
+        }
+    };
     if constexpr (sizeof(T) == 2) {
-        if (s.block % 64 == 0) return f(std::integral_constant<int, 64>{});
+        if (s.block % 64 == 0) {
+            columns(std::integral_constant<int, 64>{});
+        } else {
+            columns(std::integral_constant<int, 32>{});
+        }
+    } else {
+        columns(std::integral_constant<int, 32>{});
     }
-    f(std::integral_constant<int, 32>{});
+    NACHO_TRY_HIP(hipGetLastError());
+    return NACHO_OK;
 }
 
-constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
+constexpr int64_t kItemTarget = 1536;
+constexpr int64_t kItemLeast = 128;
 
 template <typename T, int DP>
 int forward(Call &call, const Args<T> &a) {
@@ -832,11 +1065,9 @@ int forward(Call &call, const Args<T> &a) {
     const int heads = s.batch * s.kv_heads;
     const int tiles = tiling(s, 64).per_head * heads;
     if (tiles >= kFullGrid) {
-        with_step<T>(s, [&](auto keys) {
-            tile_kernel<T, DP, keys()><<<static_cast<unsigned>(tiles), kThreads, 0, stream>>>(a);
+        return with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
+            tile_kernel<T, DP, keys(), columns()><<<grid, kThreads, 0, stream>>>(a);
         });
-        NACHO_TRY_HIP(hipGetLastError());
-        return NACHO_OK;
     }
     const Tiling small = tiling(s, 16);
     const int64_t few = static_cast<int64_t>(small.per_head) * heads;
@@ -863,48 +1094,72 @@ int forward(Call &call, const Args<T> &a) {
     return NACHO_OK;
 }
 
-unsigned grid_for(int64_t n, int per) {
-    const int64_t want = (n + per - 1) / per;
-    return static_cast<unsigned>(want < 1 ? 1 : want > 65536 ? 65536 : want);
-}
-
 template <typename T, int DP>
 int backward(Call &call, const Args<T> &a) {
     const Shape &s = a.s;
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
-    const int64_t rows = static_cast<int64_t>(s.batch) * s.queries * s.q_heads;
-    const int words = (s.queries + 31) / 32;
-    const int64_t all_words = static_cast<int64_t>(heads) * s.blocks * words;
+    const int64_t queries = static_cast<int64_t>(s.batch) * s.queries * s.q_heads;
     float *delta = nullptr;
-    unsigned *bits = nullptr;
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(rows), &delta));
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(all_words), &bits));
-    if (rows > 0) {
-        delta_kernel<T><<<static_cast<unsigned>((rows + 15) / 16), kThreads, 0, stream>>>(a, delta);
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(queries), &delta));
+    if (queries > 0) {
+        delta_kernel<T><<<ceil_div(static_cast<size_t>(queries), 16), kThreads, 0, stream>>>(
+            a, delta);
         NACHO_TRY_HIP(hipGetLastError());
-        const unsigned tiles = static_cast<unsigned>(tiling(s, 64).per_head * heads);
-        with_step<T>(s, [&](auto keys) {
-            dq_kernel<T, DP, keys()><<<tiles, kThreads, 0, stream>>>(a, delta);
-        });
+        NACHO_TRY(with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
+            // (two column tiles of 128 have registers for 32 keys of q . k and dout . v)
+            constexpr int kKeys = DP == 128 && columns() == 2 ? 32 : keys();
+            dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(a, delta);
+        }));
+    }
+    Items items{};
+    items.rows = static_cast<int64_t>(heads) * s.blocks;
+    if (items.rows == 0) return NACHO_OK;
+    const int groups = (s.queries + 32 * kMarkWords - 1) / (32 * kMarkWords);
+    items.words = groups * kMarkWords;
+    const int64_t listed = queries / s.group * s.count;
+    // About kItemTarget items of equal size, but none so short that its sums cost more to store
+    // than to compute.
+    const int64_t per_item = (listed + kItemTarget - 1) / kItemTarget;
+    items.per_item = static_cast<int>(
+        per_item < kItemLeast ? kItemLeast : per_item > kItemTokens ? kItemTokens : per_item);
+    const int64_t most = items.rows + listed / items.per_item;
+    const bool wide = sizeof(T) == 2 && s.block % 64 == 0;  // 64 keys to a workgroup
+    const int parts = s.block / (wide ? 64 : 32);
+    if (most * parts > INT32_MAX - 8 || items.rows * (s.block / 16) > INT32_MAX) {
+        return NACHO_ERR_INDEX_OVERFLOW;
+    }
+    unsigned *bits = nullptr;
+    int64_t *counts = nullptr, *start = nullptr;
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows) * items.words, &bits));
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows), &counts));
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows) + 1, &start));
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(most) * s.block * 2 * DP, &items.partial));
+    items.bits = bits;
+    items.start = start;
+    if (groups > 0) {
+        mark_kernel<<<static_cast<unsigned>(groups * heads), kThreads, 0, stream>>>(
+            s, a.lengths, a.ids, items.words, bits);
         NACHO_TRY_HIP(hipGetLastError());
     }
-    if (heads * static_cast<int64_t>(s.blocks) > 0) {
-        if (all_words > 0) {
-            clear_kernel<<<grid_for(all_words, kThreads), kThreads, 0, stream>>>(bits, all_words);
-            NACHO_TRY_HIP(hipGetLastError());
-            const int64_t n = rows / s.group * s.count;
-            mark_kernel<<<grid_for(n, kThreads), kThreads, 0, stream>>>(s, a.lengths, a.ids, words,
-                                                                        bits);
-            NACHO_TRY_HIP(hipGetLastError());
-        }
-        if (s.block % 64 == 0) {
-            const unsigned grid = static_cast<unsigned>(heads * s.blocks * (s.block / 64));
-            dkv_kernel<T, DP, 4><<<grid, 4 * dev::kWave, 0, stream>>>(a, delta, words, bits);
-        } else {
-            const unsigned grid = static_cast<unsigned>(heads * s.blocks * (s.block / 32));
-            dkv_kernel<T, DP, 2><<<grid, 2 * dev::kWave, 0, stream>>>(a, delta, words, bits);
-        }
+    items_kernel<<<ceil_div(static_cast<size_t>(items.rows), kWaves), kThreads, 0, stream>>>(
+        items.rows, items.words, items.per_item, bits, counts);
+    NACHO_TRY_HIP(hipGetLastError());
+    NACHO_TRY(scan::exclusive_scan_i64(call, counts, items.rows, start));
+    const unsigned grid = static_cast<unsigned>((most * parts + 7) / 8 * 8);
+    const unsigned inverse =
+        s.group == 1 ? 0u : static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(s.group)) + 1u;
+    if (!wide) {
+        dkv_kernel<T, DP, 1, 2><<<grid, kThreads, 0, stream>>>(a, delta, items, inverse);
+    } else if constexpr (sizeof(T) == 2) {
+        // (two column tiles of 128 do not fit the registers)
+        dkv_kernel<T, DP, DP == 64 ? 2 : 1, DP == 64 ? 2 : 4>
+            <<<grid, kThreads, 0, stream>>>(a, delta, items, inverse);
+    }
+    NACHO_TRY_HIP(hipGetLastError());
+    if (listed > items.per_item) {  // else no row has several
+        dkv_join_kernel<T, DP><<<static_cast<unsigned>(items.rows * (s.block / 16)), kThreads, 0,
+                                 stream>>>(a, items);
         NACHO_TRY_HIP(hipGetLastError());
     }
     return NACHO_OK;

@@ -76,12 +76,7 @@ __device__ __forceinline__ Frag<T> result_frag(f32x4 lo, f32x4 hi) {
     return f;
 }
 
-// Elements of a row of a tile of DP columns in LDS: 16 bytes more than the data, so that the 16
-// rows that a fragment's lanes read lie in different banks.
-template <typename T, int DP>
-constexpr int kTileRow = DP + 16 / static_cast<int>(sizeof(T));
-
-// Eight consecutive elements (16-byte aligned).
+// Eight consecutive elements in memory (16-byte aligned).
 template <typename T>
 __device__ __forceinline__ Frag<T> row_frag(const T *p) {
     return *reinterpret_cast<const Frag<T> *>(p);
@@ -93,62 +88,152 @@ __device__ __forceinline__ Frag<float> row_frag<float>(const float *p) {
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Column `col0 + c` of rows 4 g + j and 16 + 4 g + j (j < 4) of the 32 rows at `tile` (rows of
-// ROW elements).  16-bit types use the transposing LDS read: the 16 lanes of a group name four
-// rows of 16 elements, four lanes a row, and lane c receives column c of the four rows.
-template <int ROW>
-__device__ __forceinline__ f32x8 column_frag(const float *tile, int col0, int g, int c) {
-    f32x8 f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        f[j] = tile[(4 * g + j) * ROW + col0 + c];
-        f[4 + j] = tile[(16 + 4 * g + j) * ROW + col0 + c];
-    }
-    return f;
-}
-template <int ROW, typename T>
-__device__ __forceinline__ Frag<T> column_frag(const T *tile, int col0, int g, int c) {
-    using Shared = __attribute__((address_space(3))) s16x4 *;
-    const T *p = tile + (4 * g + (c >> 2)) * ROW + col0 + 4 * (c & 3);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (Shared)(reinterpret_cast<const s16x4 *>(p)));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (Shared)(reinterpret_cast<const s16x4 *>(p + 16 * ROW)));
-    const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(Frag<T>, both);
-}
+// Elements of a padded row of DP elements in LDS: 16 bytes more than the data, so that the 16 rows
+// that a fragment's lanes read lie in different banks.
+template <typename T, int DP>
+constexpr int kTileRow = DP + 16 / static_cast<int>(sizeof(T));
 
-// Rows of a [rows][D] operand on their way to a tile of ROWS x DP in LDS: each of THREADS
-// threads carries N 16-byte pieces.  Pieces at or past column D are zero.
+// Rows of DP elements in LDS, filled straight from memory: a wavefront's load names a source per
+// lane and writes 64 consecutive 16-byte pieces.  Rows are not padded (they cannot be); instead
+// piece p of row r lies at place p ^ swizzle(r), which the loads' sources take care of, so that
+// the 16 rows that a fragment reads lie in different banks, and so do the rows of a column.
 template <typename T, int DP, int ROWS, int THREADS>
-struct TileLoad {
-    static constexpr int kPer = 16 / sizeof(T);       // elements of a piece
-    static constexpr int kPieces = DP / kPer;         // pieces of a row
-    static constexpr int kN = ROWS * kPieces / THREADS;
+struct Tile {
+    static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a piece
+    static constexpr int kPieces = DP / kPer;                      // pieces of a row
+    static constexpr int kLoads = ROWS * kPieces / THREADS;
+    static constexpr int kElements = ROWS * DP;
     static_assert(ROWS * kPieces % THREADS == 0, "whole pieces per thread");
-    u32x4 piece[kN];
 
-    // row_of(r): the row's first element, or null for a row of zeros.
+    __device__ __forceinline__ static int swizzle(int row) {
+        return kPieces >= 16 ? row & 15 : (row >> 1) & 7;
+    }
+
+    // row_of(r): row r of the source, r < ROWS; every one has to be there (rows that are masked
+    // name another's).  Pieces at or past column D repeat the row's first.  Complete after the
+    // next __syncthreads.
     template <typename RowOf>
-    __device__ __forceinline__ void load(int thread, int D, RowOf row_of) {
+    __device__ __forceinline__ static void load(T *tile, int thread, int D, RowOf row_of) {
+        using Global = const __attribute__((address_space(1))) void *;
+        using Shared = __attribute__((address_space(3))) void *;
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
+        for (int i = 0; i < kLoads; ++i) {
             const int at = thread + i * THREADS;
-            const int r = at / kPieces, col = at % kPieces * kPer;
-            const T *row = row_of(r);
+            const int r = at / kPieces;
+            const int piece = (at % kPieces) ^ swizzle(r);
+            const T *from = row_of(r) + (piece * kPer < D ? piece * kPer : 0);
+            T *to = tile + (i * THREADS + (thread & ~(dev::kWave - 1))) * kPer;
+            __builtin_amdgcn_global_load_lds((Global)from, (Shared)to, 16, 0, 0);
+        }
+    }
+
+    // Columns 32 kk + 8 g .. + 8 of row 16 t + c.
+    __device__ __forceinline__ static Frag<T> row(const T *tile, int t, int kk, int g, int c) {
+        const T *p = tile + (16 * t + c) * DP;
+        const int x = swizzle(c);  // (of row 16 t + c as well)
+        if constexpr (sizeof(T) == 4) {
+            const int piece = 8 * kk + 2 * g;
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(p + (piece ^ x) * kPer);
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(p + ((piece + 1) ^ x) * kPer);
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const Frag<T> *>(p + ((4 * kk + g) ^ x) * kPer);
+        }
+    }
+
+    // Column 16 i + c of rows 32 u + 4 g + j and 32 u + 16 + 4 g + j (j < 4).  16-bit types use
+    // the transposing LDS read: the 16 lanes of a group name four rows of 16 elements, four lanes
+    // a row, and lane c receives column c of the four rows.
+    __device__ __forceinline__ static Frag<T> column(const T *tile, int u, int i, int g, int c) {
+        if constexpr (sizeof(T) == 4) {
+            Frag<T> f;
+            const int piece = 4 * i + (c >> 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 4 * g + j;
+                const T *p = tile + (32 * u + r) * DP + (piece ^ swizzle(r)) * kPer + (c & 3);
+                f[j] = p[0];
+                f[4 + j] = p[16 * DP];
+            }
+            return f;
+        } else {
+            using Shared = __attribute__((address_space(3))) s16x4 *;
+            const int r = 4 * g + (c >> 2);
+            const T *p = tile + (32 * u + r) * DP +
+                         ((2 * i + ((c >> 1) & 1)) ^ swizzle(r)) * kPer + 4 * (c & 1);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(p)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(p + 16 * DP)));
+            const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(Frag<T>, both);
+        }
+    }
+};
+
+// A Tile's rows on their way through registers, for a tile that one wavefront fills and reads by
+// itself: pieces at or past column D, and rows that are not there, are zeros.
+template <typename T, int DP, int ROWS>
+struct TileStage {
+    using Lds = Tile<T, DP, ROWS, dev::kWave>;
+    u32x4 piece[Lds::kLoads];
+
+    // row_of(r): the row's first element, or null.
+    template <typename RowOf>
+    __device__ __forceinline__ void load(int lane, int D, RowOf row_of) {
+#pragma unroll
+        for (int i = 0; i < Lds::kLoads; ++i) {
+            const int at = lane + i * dev::kWave;
+            const int col = at % Lds::kPieces * Lds::kPer;
+            const T *row = row_of(at / Lds::kPieces);
             piece[i] = u32x4{0u, 0u, 0u, 0u};
             if (row && col < D) piece[i] = *reinterpret_cast<const u32x4 *>(row + col);
         }
     }
-    __device__ __forceinline__ void store(int thread, T *tile) const {
+    __device__ __forceinline__ void store(int lane, T *tile) const {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int at = thread + i * THREADS;
-            const int r = at / kPieces, col = at % kPieces * kPer;
-            *reinterpret_cast<u32x4 *>(tile + r * kTileRow<T, DP> + col) = piece[i];
+        for (int i = 0; i < Lds::kLoads; ++i) {
+            const int at = lane + i * dev::kWave;
+            const int r = at / Lds::kPieces, p = (at % Lds::kPieces) ^ Lds::swizzle(r);
+            *reinterpret_cast<u32x4 *>(tile + r * DP + p * Lds::kPer) = piece[i];
         }
     }
 };
+
+// products[x][t] = rows 16 t .. of the tile times column tile x of the operand.
+template <typename Lds, typename T, int DP, int COLS, int N>
+__device__ __forceinline__ void row_products(const T *tile, const Frag<T> (&operand)[COLS][DP / 32],
+                                             int g, int c, f32x4 (&products)[COLS][N]) {
+#pragma unroll
+    for (int t = 0; t < N; ++t) {
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) products[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; ++kk) {
+            const Frag<T> f = Lds::row(tile, t, kk, g, c);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) products[x][t] = mma(f, operand[x][kk], products[x][t]);
+        }
+    }
+}
+
+// sums[x] += the tile's columns times p[x], the products' rows rounded to T.
+template <typename Lds, typename T, int DP, int COLS, int N>
+__device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[COLS][N], int g,
+                                                int c, f32x4 (&sums)[COLS][DP / 16]) {
+#pragma unroll
+    for (int u = 0; u < N / 2; ++u) {
+        Frag<T> f[COLS];
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const Frag<T> v = Lds::column(tile, u, i, g, c);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) sums[x][i] = mma(v, f[x], sums[x][i]);
+        }
+    }
+}
 
 // A row of D elements as operand fragments (k = 32 kk + 8 g + j); null gives zeros.
 template <typename T, int DP>
@@ -158,6 +243,12 @@ __device__ __forceinline__ void load_row_frags(const T *row, int D, int g, Frag<
         const int col = 32 * kk + 8 * g;
         f[kk] = (row && col < D) ? row_frag<T>(row + col) : zero_frag<T>();
     }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void negate(Frag<T> (&f)[DP / 32]) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 32; ++kk) f[kk] = -f[kk];
 }
 
 // Four consecutive results rounded to T and stored together.
@@ -170,14 +261,21 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {
     *reinterpret_cast<t4 *>(p) = o;
 }
 
-// Maximum and sum over the four lanes of a column (lanes c, 16 + c, 32 + c, 48 + c).
+// Maximum and sum over the four lanes of a column (lanes c, 16 + c, 32 + c, 48 + c): exchanges of
+// rows of 16 and of 32 lanes between two registers, which hold the same value here.
 __device__ __forceinline__ float column_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, dev::kWave));
-    return fmaxf(v, __shfl_xor(v, 32, dev::kWave));
+    const unsigned x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const unsigned y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float column_sum(float v) {
-    v += __shfl_xor(v, 16, dev::kWave);
-    return v + __shfl_xor(v, 32, dev::kWave);
+    const unsigned x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const unsigned y = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

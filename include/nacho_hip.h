@@ -364,7 +364,9 @@ int nacho_gpu_spgemm64_f32(const nacho_csr *a, const nacho_csr *b, nacho_csr64 *
 #define NACHO_BF16 2
 
 /* A dense operand [batch][row][head][head_dim]: strides in elements, the last dimension
- * contiguous.  `data` and every stride are multiples of 16 bytes. */
+ * contiguous.  `data` and every stride are multiples of 16 bytes, and rows are at most
+ * NACHO_MAX_ROW_BYTES apart. */
+#define NACHO_MAX_ROW_BYTES ((int64_t)1 << 26)
 typedef struct nacho_heads {
     void *data;
     int64_t batch_stride;

@@ -334,6 +334,7 @@ nacho_heads heads(at::Tensor &t) {
     bool ok = (t.stride(3) == 1 || t.size(3) == 1) &&
               reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % per == 0);
+    ok = ok && (t.size(1) <= 1 || t.stride(1) * t.element_size() <= NACHO_MAX_ROW_BYTES);
     if (!ok) t = t.clone(at::MemoryFormat::Contiguous);
     auto stride = [&](int i) { return t.size(i) <= 1 ? int64_t{0} : t.stride(i); };
     return nacho_heads{t.numel() > 0 ? t.data_ptr() : nullptr, stride(0), stride(1), stride(2)};

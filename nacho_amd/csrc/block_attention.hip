@@ -184,7 +184,7 @@ __device__ int window_lists(const Shape &s, const int *__restrict__ ids, const R
 
 // Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
 // rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
-// sequence's end hold its last key's.  Every wavefront calls it; `use` has no barrier.
+// sequence's end are zeros.  Every wavefront calls it; `use` has no barrier.
 template <typename T, int DP, int BN, int R>
 struct KeySteps {
     using Lds = Tile<T, DP, BN, kThreads>;
@@ -196,33 +196,30 @@ struct KeySteps {
         const Shape &s = a.s;
         const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
         const int end = tile.last_key(s, tile.tokens - 1) + 1;  // keys that some row sees
-        const int steps_of = s.block / BN;
+        const int shift = s.block / BN == 1 ? 0 : s.block / BN == 2 ? 1 : 2;  // steps of a block
+        const typename Lds::Source k_source(threadIdx.x, s.dim, a.k.row_stride);
+        const typename Lds::Source v_source(threadIdx.x, s.dim, a.v.row_stride);
         for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
-            const int steps = window_lists(s, a.ids, tile, first, lists) * steps_of;
+            const int steps = window_lists(s, a.ids, tile, first, lists) << shift;
             auto first_key = [&](int step) {
-                return (first + __builtin_amdgcn_readfirstlane(lists.ids[step / steps_of])) *
+                return (first + __builtin_amdgcn_readfirstlane(lists.ids[step >> shift])) *
                            s.block +
-                       step % steps_of * BN;
+                       (step & ((1 << shift) - 1)) * BN;
             };
             auto load = [&](int step, T *to_k, T *to_v) {
-                const int key = first_key(step);
-                const int most = tile.length - 1 - key;
-                const T *from_k = k_base + key * a.k.row_stride;
-                const T *from_v = v_base + key * a.v.row_stride;
-                Lds::load(to_k, threadIdx.x, s.dim,
-                          [&](int r) { return from_k + min(r, most) * a.k.row_stride; });
-                Lds::load(to_v, threadIdx.x, s.dim,
-                          [&](int r) { return from_v + min(r, most) * a.v.row_stride; });
+                const int key = first_key(step), there = tile.length - key;
+                Lds::load(to_k, threadIdx.x, k_source, k_base + key * a.k.row_stride, there);
+                Lds::load(to_v, threadIdx.x, v_source, v_base + key * a.v.row_stride, there);
             };
             if (steps > 0) load(0, k[0], v[0]);
             __syncthreads();
             for (int step = 0; step < steps; step += 2) {
                 if (step + 1 < steps) load(step + 1, k[1], v[1]);
-                use(k[0], v[0], step / steps_of, first_key(step));
+                use(k[0], v[0], step >> shift, first_key(step));
                 __syncthreads();
                 if (step + 1 >= steps) break;
                 if (step + 2 < steps) load(step + 2, k[0], v[0]);
-                use(k[1], v[1], (step + 1) / steps_of, first_key(step + 1));
+                use(k[1], v[1], (step + 1) >> shift, first_key(step + 1));
                 __syncthreads();
             }
         }
@@ -245,10 +242,14 @@ constexpr float kSlack = 8.0f;  // the running maximum follows a row's when it i
 // probabilities against the running maximum m, which may stay up to kSlack below the row's own
 // (they are at most 2^kSlack then): sums are brought to a new one only when some row of the
 // wavefront needs it.  Returns whether they were, by `factor`.
+//
+// Most steps are seen whole or not at all: a row that sees nothing of a step takes a maximum of
+// infinity there, and only steps that some row sees in part are masked key by key.
 template <int N>
 __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, float &m,
                                              float &l, float &factor) {
-    if (!__all(limit >= 16 * N)) {
+    const bool none = limit <= 0;
+    if (__any(!none && limit < 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
@@ -261,7 +262,7 @@ __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int li
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
     }
-    top = column_max(top) * scale2;
+    top = column_max(none ? kNegInf : top) * scale2;
     const bool moved = __any(top > m + kSlack);
     factor = 1.0f;
     if (moved) {
@@ -270,7 +271,7 @@ __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int li
         m = now;
         l *= factor;
     }
-    const float base = m == kNegInf ? 0.0f : m;
+    const float base = none ? -kNegInf : m == kNegInf ? 0.0f : m;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
@@ -638,16 +639,21 @@ __global__ __launch_bounds__(kThreads) void items_kernel(int64_t rows, int words
 template <int N>
 __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], float scale2,
                                                float lse2, float delta, int limit) {
-    const bool whole = __all(limit >= 16 * N);
+    const bool none = limit <= 0;
+    const float base = none ? -kNegInf : lse2;  // (as in softmax_step)
 #pragma unroll
     for (int t = 0; t < N; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float p = exp2_fast(__builtin_fmaf(s[t][i], scale2, -lse2));
-            const float ds = p * (dp[t][i] - delta);
-            const bool seen = whole || 16 * t + i < limit;
-            s[t][i] = seen ? p : 0.0f;
-            dp[t][i] = seen ? ds : 0.0f;
+            s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], scale2, -base));
+            dp[t][i] = s[t][i] * (dp[t][i] - delta);
+        }
+    }
+    if (__any(!none && limit < 16 * N)) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[t][i] = 16 * t + i < limit ? dp[t][i] : 0.0f;
         }
     }
 }
@@ -741,6 +747,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
     __shared__ __align__(16) T s_do1[Lds::kElements];
     __shared__ __align__(16) float s_lse[2][kStep], s_delta[2][kStep];
     __shared__ __align__(16) int s_last[2][kStep];
+    __shared__ bool s_partial[2];
     __shared__ int s_tokens[kItemTokens];
     __shared__ int s_sums[kWaves];
     const Shape &s = a.s;
@@ -825,11 +832,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
             return a.dout.row(b, t, head);
         });
     };
-    // lse, delta and last key of row r0 + thread, for the first kStep threads
+    // lse, delta and last key of row r0 + thread, for the first kStep threads (part of the first
+    // wavefront); infinity for a row that is not there makes its probabilities 0.
+    const int block_end = (id + 1) * s.block - 1;
     auto info = [&](int r0, int buffer) {
         const int x = r0 + static_cast<int>(threadIdx.x);
-        float lse = 0.0f, d = 0.0f;
-        int last = -1;
+        float lse = -kNegInf, d = 0.0f;
+        int last = block_end;
         if (x < rows) {
             const int at = token_at(x), t = s_tokens[at];
             const int64_t i = (static_cast<int64_t>(b) * s.queries + t) * s.q_heads +
@@ -842,6 +851,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
         s_lse[buffer][threadIdx.x] = lse;
         s_delta[buffer][threadIdx.x] = d;
         s_last[buffer][threadIdx.x] = last;
+        // whether some row sees a part of the block only
+        const bool partial = __any(last < block_end);
+        if (threadIdx.x == 0) s_partial[buffer] = partial;
     };
     auto use = [&](const T *s_q, const T *s_do, int buffer) {
         const T *my_q = s_q + set * kStepRows * DP, *my_do = s_do + set * kStepRows * DP;
@@ -856,15 +868,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
             const f32x4 lse = *reinterpret_cast<const f32x4 *>(&s_lse[buffer][r]);
             const f32x4 d = *reinterpret_cast<const f32x4 *>(&s_delta[buffer][r]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int last = s_last[buffer][r + i];
+            for (int x = 0; x < COLS; ++x) {
 #pragma unroll
-                for (int x = 0; x < COLS; ++x) {
-                    const float e = exp2_fast(__builtin_fmaf(p[x][t][i], scale2, -lse[i]));
-                    const float ds = e * (dp[x][t][i] - d[i]);
-                    const bool sees = first_key + 16 * x <= last;
-                    p[x][t][i] = sees ? e : 0.0f;
-                    dp[x][t][i] = sees ? ds : 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    p[x][t][i] = exp2_fast(__builtin_fmaf(p[x][t][i], scale2, -lse[i]));
+                    dp[x][t][i] = p[x][t][i] * (dp[x][t][i] - d[i]);
+                }
+            }
+        }
+        if (s_partial[buffer]) {
+#pragma unroll
+            for (int t = 0; t < kN; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int last = s_last[buffer][set * kStepRows + 16 * t + 4 * g + i];
+#pragma unroll
+                    for (int x = 0; x < COLS; ++x) {
+                        const bool sees = first_key + 16 * x <= last;
+                        p[x][t][i] = sees ? p[x][t][i] : 0.0f;
+                        dp[x][t][i] = sees ? dp[x][t][i] : 0.0f;
+                    }
                 }
             }
         }
@@ -972,7 +995,8 @@ bool aligned(const nacho_heads &h, int item, bool optional = false) {
     if (!h.data) return optional;
     const int64_t per = 16 / item;
     return reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && h.batch_stride % per == 0 &&
-           h.row_stride % per == 0 && h.head_stride % per == 0;
+           h.row_stride % per == 0 && h.head_stride % per == 0 && h.row_stride >= 0 &&
+           h.row_stride <= NACHO_MAX_ROW_BYTES / item;
 }
 
 int check(const nacho_block_attention_args *p, bool backward, Shape *s) {

@@ -116,15 +116,55 @@ struct Tile {
     __device__ __forceinline__ static void load(T *tile, int thread, int D, RowOf row_of) {
         using Global = const __attribute__((address_space(1))) void *;
         using Shared = __attribute__((address_space(3))) void *;
+        const int wave_first = __builtin_amdgcn_readfirstlane(thread & ~(dev::kWave - 1));
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int at = thread + i * THREADS;
             const int r = at / kPieces;
             const int piece = (at % kPieces) ^ swizzle(r);
             const T *from = row_of(r) + (piece * kPer < D ? piece * kPer : 0);
-            T *to = tile + (i * THREADS + (thread & ~(dev::kWave - 1))) * kPer;
+            T *to = tile + (i * THREADS + wave_first) * kPer;
             __builtin_amdgcn_global_load_lds((Global)from, (Shared)to, 16, 0, 0);
         }
+    }
+
+    // The same for rows `stride` bytes apart from a step to the next: what a thread reads of the
+    // step's first row on, in bytes, is worked out once.  Rows from `there` on and pieces at or
+    // past column D are past the buffer's end, where loads give zeros.
+    struct Source {
+        unsigned offset[kLoads];
+        unsigned stride, bytes;  // of a row, of its data
+
+        __device__ __forceinline__ Source(int thread, int D, int64_t row_stride)
+            : stride(static_cast<unsigned>(row_stride * static_cast<int>(sizeof(T)))),
+              bytes(static_cast<unsigned>(D * static_cast<int>(sizeof(T)))) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = thread + i * THREADS;
+                const int r = at / kPieces;
+                const unsigned piece = static_cast<unsigned>((at % kPieces) ^ swizzle(r));
+                offset[i] = 16u * piece < bytes ? static_cast<unsigned>(r) * stride + 16u * piece
+                                                : 0xffffff00u;
+            }
+        }
+    };
+
+    __device__ __forceinline__ static void load(T *tile, int thread, const Source &from,
+                                                const T *first, int there) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass does not know buffer descriptors)
+        using Shared = __attribute__((address_space(3))) void *;
+        const int wave_first = __builtin_amdgcn_readfirstlane(thread & ~(dev::kWave - 1));
+        const unsigned end =
+            there > 0 ? static_cast<unsigned>(min(there, ROWS) - 1) * from.stride + from.bytes : 0u;
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<T *>(first), 0, end, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            T *to = tile + (i * THREADS + wave_first) * kPer;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (Shared)to, 16,
+                                                     static_cast<int>(from.offset[i]), 0, 0, 0);
+        }
+#endif
     }
 
     // Columns 32 kk + 8 g .. + 8 of row 16 t + c.

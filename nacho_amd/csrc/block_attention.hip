@@ -27,7 +27,6 @@
 
 #include "dense_tiles.hpp"
 #include "runtime.hpp"
-#include "scan.hpp"
 
 namespace nacho {
 namespace attention {
@@ -217,9 +216,8 @@ struct KeySteps {
                 if (step + 1 < steps) load(step + 1, k[1], v[1]);
                 use(k[0], v[0], step >> shift, first_key(step));
                 __syncthreads();
-                if (step + 1 >= steps) break;
                 if (step + 2 < steps) load(step + 2, k[0], v[0]);
-                use(k[1], v[1], (step + 1) >> shift, first_key(step + 1));
+                if (step + 1 < steps) use(k[1], v[1], (step + 1) >> shift, first_key(step + 1));
                 __syncthreads();
             }
         }
@@ -531,10 +529,12 @@ __global__ __launch_bounds__(DP) void join_kernel(Args<T> a, int splits, Partial
     if (!tile.row(s, r, t, hd)) return;
     const int64_t at = static_cast<int64_t>(index) * splits * 16 + r;
     float top = kNegInf;
+#pragma unroll 8
     for (int i = 0; i < splits; ++i) top = fmaxf(top, part.ml[2 * (at + 16 * i)]);
     const float base = top == kNegInf ? 0.0f : top;
     float sum = 0.0f, v = 0.0f;
     const int col = static_cast<int>(threadIdx.x);
+#pragma unroll 8
     for (int i = 0; i < splits; ++i) {
         const int64_t x = at + 16 * i;
         const float f = exp2_fast(part.ml[2 * x] - base);
@@ -551,30 +551,6 @@ __global__ __launch_bounds__(DP) void join_kernel(Args<T> a, int splits, Partial
 
 // ---- backward -------------------------------------------------------------------------
 
-// delta[b][t][head] = dout . out: 16 lanes per row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void delta_kernel(Args<T> a, float *__restrict__ delta) {
-    const Shape &s = a.s;
-    const int64_t rows = static_cast<int64_t>(s.batch) * s.queries * s.q_heads;
-    const int64_t r = blockIdx.x * static_cast<int64_t>(kThreads / 16) + threadIdx.x / 16;
-    const int c = threadIdx.x % 16;
-    float v = 0.0f;
-    if (r < rows) {
-        const int head = static_cast<int>(r % s.q_heads);
-        const int64_t bt = r / s.q_heads;
-        const int t = static_cast<int>(bt % s.queries), b = static_cast<int>(bt / s.queries);
-        const T *x = a.dout.row(b, t, head), *y = a.out.row(b, t, head);
-        for (int col = 8 * c; col < s.dim; col += 128) {
-            const Frag<T> fx = row_frag<T>(x + col), fy = row_frag<T>(y + col);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v += static_cast<float>(fx[j]) * static_cast<float>(fy[j]);
-        }
-    }
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) v += __shfl_xor(v, off, dev::kWave);
-    if (r < rows && c == 0) delta[r] = v;
-}
-
 // bits[b][h][block][token / 32]: the tokens that see something of the block through their ids.
 // A workgroup has 128 tokens of a head (four words of each block), gathered in LDS for
 // kMarkWindow blocks at a time: with a word per block and tokens of 32 each, atomics on the
@@ -582,9 +558,11 @@ __global__ __launch_bounds__(kThreads) void delta_kernel(Args<T> a, float *__res
 constexpr int kMarkWords = 4;
 constexpr int kMarkWindow = 1024;
 
+// counts[b][h][block], 0 before, become the numbers of tokens.
 __global__ __launch_bounds__(kThreads) void mark_kernel(Shape s, const int *__restrict__ lengths,
                                                         const int *__restrict__ ids, int words,
-                                                        unsigned *__restrict__ bits) {
+                                                        unsigned *__restrict__ bits,
+                                                        int *__restrict__ counts) {
     __shared__ __align__(16) unsigned s_bits[kMarkWindow][kMarkWords];
     const int heads = s.batch * s.kv_heads;
     const int bh = static_cast<int>(blockIdx.x) % heads;
@@ -613,25 +591,34 @@ __global__ __launch_bounds__(kThreads) void mark_kernel(Shape s, const int *__re
         const int there = min(kMarkWindow, s.blocks - first);
         for (int i = threadIdx.x; i < there; i += kThreads) {
             const int64_t row = static_cast<int64_t>(bh) * s.blocks + first + i;
-            *reinterpret_cast<u32x4 *>(bits + row * words + w0) =
-                *reinterpret_cast<const u32x4 *>(s_bits[i]);
+            const u32x4 mine = *reinterpret_cast<const u32x4 *>(s_bits[i]);
+            *reinterpret_cast<u32x4 *>(bits + row * words + w0) = mine;
+            const int n = __popc(mine[0]) + __popc(mine[1]) + __popc(mine[2]) + __popc(mine[3]);
+            if (n > 0) atomicAdd(&counts[row], n);
         }
         __syncthreads();
     }
 }
 
-// items[row]: parts of at most `per_item` tokens that the row (a block of a head) is worked on
-// in, one at least.  A wavefront per row.
-__global__ __launch_bounds__(kThreads) void items_kernel(int64_t rows, int words, int per_item,
-                                                         const unsigned *__restrict__ bits,
-                                                         int64_t *__restrict__ items) {
-    const int64_t row =
-        blockIdx.x * static_cast<int64_t>(kWaves) + threadIdx.x / dev::kWave;
-    if (row >= rows) return;
-    int n = 0;
-    for (int w = dev::lane(); w < words; w += dev::kWave) n += __popc(bits[row * words + w]);
-    n = dev::wave_sum(n);
-    if (dev::lane() == 0) items[row] = n > per_item ? (n + per_item - 1) / per_item : 1;
+// start[row]: the items before the row's, each of at most per_item of its tokens, one at least;
+// start[rows] is their number.  One workgroup: the rows are the blocks of the key heads.
+constexpr int kStartBlock = 1024;
+
+__global__ __launch_bounds__(kStartBlock) void start_kernel(int64_t rows, int per_item,
+                                                            const int *__restrict__ counts,
+                                                            int *__restrict__ start) {
+    __shared__ int s_sums[kStartBlock / dev::kWave];
+    int carry = 0;
+    for (int64_t first = 0; first < rows; first += kStartBlock) {  // uniform
+        const int64_t row = first + threadIdx.x;
+        const int n = row < rows && counts ? counts[row] : 0;
+        const int items = row < rows ? max(1, (n + per_item - 1) / per_item) : 0;
+        int total = 0;
+        const int at = carry + dev::block_exclusive_sum<kStartBlock>(items, s_sums, total);
+        if (row < rows) start[row] = at;
+        carry += total;
+    }
+    if (threadIdx.x == 0) start[rows] = carry;
 }
 
 // From the products s = q . k and dp = dout . v of 16 N keys with a row: s become probabilities
@@ -658,9 +645,11 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
     }
 }
 
+// dq, and delta and zeroed counts for the launches that follow.
 template <typename T, int DP, int BN, int COLS>
-__global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a,
-                                                         const float *__restrict__ delta) {
+__global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a, float *__restrict__ delta,
+                                                         int64_t rows_of_blocks,
+                                                         int *__restrict__ counts) {
     using Lds = Tile<T, DP, BN, kThreads>;
     constexpr int kRowsOf = 64 * COLS;
     __shared__ __align__(16) T s_k0[Lds::kElements];
@@ -672,6 +661,10 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a,
     const RowTile<kRowsOf> tile(s, a.lengths, static_cast<int>(blockIdx.x));
     const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
     const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < rows_of_blocks;
+         i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        counts[i] = 0;  // for the launch that counts
+    }
     const LaneRows<COLS> rows(s, tile, wave, c);
     Frag<T> q[COLS][DP / 32], dout[COLS][DP / 32];
     f32x4 o[COLS][DP / 16];
@@ -686,7 +679,19 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a,
         const int64_t at = (static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head;
         const float lse = exists ? a.lse[at] : 0.0f;
         lse2[x] = lse == kNegInf ? 0.0f : lse * kLog2e;
-        row_delta[x] = exists ? delta[at] : 0.0f;
+        Frag<T> out[DP / 32];
+        load_row_frags<T, DP>(exists ? a.out.row(tile.b, t, head) : nullptr, s.dim, g, out);
+        float sum = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; ++kk) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum = __builtin_fmaf(static_cast<float>(dout[x][kk][j]),
+                                     static_cast<float>(out[kk][j]), sum);
+            }
+        }
+        row_delta[x] = column_sum(sum);
+        if (exists && g == 0) delta[at] = row_delta[x];
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -723,7 +728,7 @@ constexpr int kMaxGroup = 1024;    // heads of a group: what the division below 
 // Work on dk and dv: the rows (blocks of heads) in items of at most per_item tokens, so that a
 // block that every query selects is not one workgroup's.  start[row] are the rows' first items.
 struct Items {
-    const int64_t *start;
+    const int *start;
     int64_t rows;
     int per_item, words;
     const unsigned *bits;
@@ -734,7 +739,7 @@ struct Items {
 // with LANES = 2 the four wavefronts are two such sets, which take 32 rows of the item's tokens
 // in turn and add their sums at the end.
 template <typename T, int DP, int COLS, int LANES>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(Args<T> a, const float *__restrict__ delta,
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(Args<T> a, const float *__restrict__ delta,
                                                        Items items, unsigned group_inverse) {
     constexpr int kSets = kWaves / LANES;
     constexpr int kStep = kSets * kStepRows;
@@ -745,16 +750,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
     __shared__ __align__(16) T s_do0[Lds::kElements];
     __shared__ __align__(16) T s_q1[Lds::kElements];
     __shared__ __align__(16) T s_do1[Lds::kElements];
-    __shared__ __align__(16) float s_lse[2][kStep], s_delta[2][kStep];
-    __shared__ __align__(16) int s_last[2][kStep];
-    __shared__ bool s_partial[2];
+    // of the rows of four steps: where they are, and what their products need
+    __shared__ int64_t s_at_q[4][kStep], s_at_do[4][kStep];
+    __shared__ __align__(16) float s_lse[4][kStep], s_delta[4][kStep];
+    __shared__ __align__(16) int s_last[4][kStep];
+    __shared__ bool s_partial[4];
     __shared__ int s_tokens[kItemTokens];
     __shared__ int s_sums[kWaves];
     const Shape &s = a.s;
     const int parts = s.block / kKeys;
     // Workgroups go to the 8 XCDs in turn: each XCD takes a stretch of items, so that the rows
     // of few heads are in its L2.
-    const int64_t all = items.start[items.rows] * parts;
+    const int64_t all = static_cast<int64_t>(items.start[items.rows]) * parts;
     const int64_t stretch = (all + 7) / 8;
     const int64_t index = blockIdx.x % 8 * stretch + blockIdx.x / 8;
     if (blockIdx.x / 8 >= stretch || index >= all) return;
@@ -814,49 +821,45 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
         return s.group == 1 ? x
                             : static_cast<int>(__umulhi(static_cast<unsigned>(x), group_inverse));
     };
-    auto load = [&](int r0, T *to_q, T *to_do) {
-        auto place = [&](int r, int &t, int &head) {
-            const int x = min(r0 + r, rows - 1);
-            const int at = token_at(x);
-            t = s_tokens[at];
-            head = h * s.group + x - at * s.group;
-        };
-        Lds::load(to_q, threadIdx.x, s.dim, [&](int r) -> const T * {
-            int t, head;
-            place(r, t, head);
-            return a.q.row(b, t, head);
-        });
-        Lds::load(to_do, threadIdx.x, s.dim, [&](int r) -> const T * {
-            int t, head;
-            place(r, t, head);
-            return a.dout.row(b, t, head);
-        });
+    const T *q_base = a.q.row(b, 0, h * s.group), *do_base = a.dout.row(b, 0, h * s.group);
+    auto load = [&](int step, T *to_q, T *to_do) {
+        const int ring = step & 3;
+        Lds::load(to_q, threadIdx.x, s.dim, [&](int r) { return q_base + s_at_q[ring][r]; });
+        Lds::load(to_do, threadIdx.x, s.dim, [&](int r) { return do_base + s_at_do[ring][r]; });
     };
-    // lse, delta and last key of row r0 + thread, for the first kStep threads (part of the first
-    // wavefront); infinity for a row that is not there makes its probabilities 0.
+    // The first kStep threads (part of the first wavefront) work out the rows of a step: `begin`
+    // two steps ahead, and `end` once lse and delta are there.  Steps past the last row repeat
+    // it, with an infinity for lse, which makes its probabilities 0.
     const int block_end = (id + 1) * s.block - 1;
-    auto info = [&](int r0, int buffer) {
-        const int x = r0 + static_cast<int>(threadIdx.x);
-        float lse = -kNegInf, d = 0.0f;
-        int last = block_end;
-        if (x < rows) {
-            const int at = token_at(x), t = s_tokens[at];
-            const int64_t i = (static_cast<int64_t>(b) * s.queries + t) * s.q_heads +
-                              h * s.group + x - at * s.group;
-            lse = a.lse[i];
-            lse = lse == kNegInf ? 0.0f : lse * kLog2e;
-            d = delta[i];
-            last = s.causal ? place0 + t : length - 1;
-        }
-        s_lse[buffer][threadIdx.x] = lse;
-        s_delta[buffer][threadIdx.x] = d;
-        s_last[buffer][threadIdx.x] = last;
+    const bool informs = threadIdx.x < kStep;
+    float next_lse = 0.0f, next_delta = 0.0f;
+    int next_last = 0;
+    auto begin = [&](int step) {
+        const int x = min(step * kStep + static_cast<int>(threadIdx.x), rows - 1);
+        const int at = token_at(x), t = s_tokens[at], head = x - at * s.group;
+        s_at_q[step & 3][threadIdx.x] = t * a.q.row_stride + head * a.q.head_stride;
+        s_at_do[step & 3][threadIdx.x] = t * a.dout.row_stride + head * a.dout.head_stride;
+        const int64_t i =
+            (static_cast<int64_t>(b) * s.queries + t) * s.q_heads + h * s.group + head;
+        next_lse = a.lse[i];
+        next_delta = delta[i];
+        next_last = s.causal ? place0 + t : length - 1;
+    };
+    auto end = [&](int step) {
+        const bool there = step * kStep + static_cast<int>(threadIdx.x) < rows;
+        const int last = there ? next_last : block_end;
+        s_lse[step & 3][threadIdx.x] =
+            there ? (next_lse == kNegInf ? 0.0f : next_lse * kLog2e) : -kNegInf;
+        s_delta[step & 3][threadIdx.x] = next_delta;
+        s_last[step & 3][threadIdx.x] = last;
         // whether some row sees a part of the block only
         const bool partial = __any(last < block_end);
-        if (threadIdx.x == 0) s_partial[buffer] = partial;
+        if (threadIdx.x == 0) s_partial[step & 3] = partial;
     };
-    auto use = [&](const T *s_q, const T *s_do, int buffer) {
-        const T *my_q = s_q + set * kStepRows * DP, *my_do = s_do + set * kStepRows * DP;
+    auto use = [&](const T *s_q, const T *s_do, int step) {
+        const int buffer = step & 3;
+        const T *my_q = s_q + set * kStepRows * Lds::kRow,
+                *my_do = s_do + set * kStepRows * Lds::kRow;
         constexpr int kN = kStepRows / 16;
         f32x4 p[COLS][kN], dp[COLS][kN];
         row_products<Lds, T, DP, COLS, kN>(my_q, k, g, c, p);
@@ -894,26 +897,31 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void dkv_kernel(A
         column_products<Lds, T, DP, COLS, kN>(my_do, p, g, c, dv);
         column_products<Lds, T, DP, COLS, kN>(my_q, dp, g, c, dk);
     };
-    const bool informs = threadIdx.x < kStep;
-    if (rows > 0) {
+    if (rows > 0) {  // uniform
+        if (informs) {
+            begin(0);
+            end(0);
+            begin(1);
+            end(1);
+        }
+        __syncthreads();
         load(0, s_q0, s_do0);
-        if (informs) info(0, 0);
-    }
-    __syncthreads();
-    for (int r0 = 0; r0 < rows; r0 += 2 * kStep) {
-        if (r0 + kStep < rows) {
-            load(r0 + kStep, s_q1, s_do1);
-            if (informs) info(r0 + kStep, 1);
-        }
-        use(s_q0, s_do0, 0);
         __syncthreads();
-        if (r0 + kStep >= rows) break;
-        if (r0 + 2 * kStep < rows) {
-            load(r0 + 2 * kStep, s_q0, s_do0);
-            if (informs) info(r0 + 2 * kStep, 0);
+        // (A last step without rows takes probabilities of 0: a branch around it costs a second
+        // copy of the sums' registers.)
+        const int steps = (rows + kStep - 1) / kStep;
+        for (int step = 0; step < steps; step += 2) {
+            load(step + 1, s_q1, s_do1);
+            if (informs) begin(step + 2);
+            use(s_q0, s_do0, step);
+            if (informs) end(step + 2);
+            __syncthreads();
+            load(step + 2, s_q0, s_do0);
+            if (informs) begin(step + 3);
+            use(s_q1, s_do1, step + 1);
+            if (informs) end(step + 3);
+            __syncthreads();
         }
-        use(s_q1, s_do1, 1);
-        __syncthreads();
     }
     if constexpr (kSets == 2) {
         // The second set's sums are added to the first's, dk's through the buffers of q and dv's
@@ -964,7 +972,7 @@ __global__ __launch_bounds__(kThreads) void dkv_join_kernel(Args<T> a, Items ite
     const int parts = s.block / 16;
     const int64_t row = blockIdx.x / parts;
     const int part = static_cast<int>(blockIdx.x % parts);
-    const int64_t from = items.start[row], to = items.start[row + 1];
+    const int from = items.start[row], to = items.start[row + 1];
     if (to - from <= 1) return;
     const int bh = static_cast<int>(row / s.blocks), id = static_cast<int>(row % s.blocks);
     const int b = bh / s.kv_heads, h = bh % s.kv_heads;
@@ -1079,7 +1087,7 @@ int with_tiles(const Shape &s, F f) {
     return NACHO_OK;
 }
 
-constexpr int64_t kItemTarget = 1536;
+constexpr int64_t kItemTarget = 768;
 constexpr int64_t kItemLeast = 128;
 
 template <typename T, int DP>
@@ -1087,25 +1095,28 @@ int forward(Call &call, const Args<T> &a) {
     const Shape &s = a.s;
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
-    const int tiles = tiling(s, 64).per_head * heads;
-    if (tiles >= kFullGrid) {
+    if (static_cast<int64_t>(tiling(s, 64).per_head) * heads >= kFullGrid) {
         return with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
             tile_kernel<T, DP, keys(), columns()><<<grid, kThreads, 0, stream>>>(a);
         });
     }
+    // Fewer tiles than CUs: tiles of 16 rows, whose wavefronts share the steps.  Joining splits
+    // costs about as much as three steps (5 us), so a wavefront keeps two steps at least, and
+    // there are no more workgroups than CUs.  One query of 32 heads over 16 blocks of 64: 20 us
+    // in one split, 14 in four; over 8 blocks of 32 (16 heads of 64) 7.8 in one, 12.4 in two.
     const Tiling small = tiling(s, 16);
     const int64_t few = static_cast<int64_t>(small.per_head) * heads;
     const int64_t listed = static_cast<int64_t>(small.tokens) * s.count;
     const int64_t steps = (listed < s.blocks ? listed : s.blocks) * (s.block / kSplitKeys);
-    int64_t splits = (2 * kFullGrid + few - 1) / few;
-    const int64_t most = (steps + kWaves - 1) / kWaves;
+    int64_t splits = kFullGrid / few;
+    const int64_t most = (steps + 2 * kWaves - 1) / (2 * kWaves);
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     Partials part{};
     if (splits > 1) {
         const size_t rows = static_cast<size_t>(few) * static_cast<size_t>(splits) * 16;
-        NACHO_TRY(call.scratch_n(2 * rows, &part.ml));
-        NACHO_TRY(call.scratch_n(rows * DP, &part.o));
+        NACHO_TRY(call.scratch_n(rows * (DP + 2), &part.o));
+        part.ml = part.o + rows * DP;
     }
     split_kernel<T, DP><<<static_cast<unsigned>(few * splits), kThreads, 0, stream>>>(
         a, static_cast<int>(splits), part);
@@ -1124,21 +1135,8 @@ int backward(Call &call, const Args<T> &a) {
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
     const int64_t queries = static_cast<int64_t>(s.batch) * s.queries * s.q_heads;
-    float *delta = nullptr;
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(queries), &delta));
-    if (queries > 0) {
-        delta_kernel<T><<<ceil_div(static_cast<size_t>(queries), 16), kThreads, 0, stream>>>(
-            a, delta);
-        NACHO_TRY_HIP(hipGetLastError());
-        NACHO_TRY(with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
-            // (two column tiles of 128 have registers for 32 keys of q . k and dout . v)
-            constexpr int kKeys = DP == 128 && columns() == 2 ? 32 : keys();
-            dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(a, delta);
-        }));
-    }
     Items items{};
     items.rows = static_cast<int64_t>(heads) * s.blocks;
-    if (items.rows == 0) return NACHO_OK;
     const int groups = (s.queries + 32 * kMarkWords - 1) / (32 * kMarkWords);
     items.words = groups * kMarkWords;
     const int64_t listed = queries / s.group * s.count;
@@ -1153,23 +1151,41 @@ int backward(Call &call, const Args<T> &a) {
     if (most * parts > INT32_MAX - 8 || items.rows * (s.block / 16) > INT32_MAX) {
         return NACHO_ERR_INDEX_OVERFLOW;
     }
-    unsigned *bits = nullptr;
-    int64_t *counts = nullptr, *start = nullptr;
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows) * items.words, &bits));
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows), &counts));
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(items.rows) + 1, &start));
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(most) * s.block * 2 * DP, &items.partial));
+    const bool several = listed > items.per_item;  // else no row has several items
+    // One piece of scratch: an allocation costs about as much as a small kernel.
+    const size_t sizes[] = {static_cast<size_t>(queries) * 4,
+                            static_cast<size_t>(items.rows) * items.words * 4,
+                            static_cast<size_t>(items.rows) * 4,
+                            static_cast<size_t>(items.rows + 1) * 4,
+                            several ? static_cast<size_t>(most) * s.block * 2 * DP * 4 : 0};
+    size_t at[6] = {0};
+    for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + (sizes[i] + 255) / 256 * 256;
+    unsigned char *scratch = nullptr;
+    NACHO_TRY(call.scratch_n(at[5], &scratch));
+    float *delta = reinterpret_cast<float *>(scratch + at[0]);
+    unsigned *bits = reinterpret_cast<unsigned *>(scratch + at[1]);
+    int *counts = reinterpret_cast<int *>(scratch + at[2]);
+    int *start = reinterpret_cast<int *>(scratch + at[3]);
+    items.partial = reinterpret_cast<float *>(scratch + at[4]);
     items.bits = bits;
     items.start = start;
-    if (groups > 0) {
+    if (queries > 0) {
+        NACHO_TRY(with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
+            // (two column tiles of 96 or 128 leave registers for 32 keys of q . k and dout . v)
+            constexpr int kKeys = DP > 64 && columns() == 2 ? 32 : keys();
+            dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(
+                a, delta, items.rows, counts);
+        }));
+    }
+    if (items.rows == 0) return NACHO_OK;
+    if (queries > 0) {
         mark_kernel<<<static_cast<unsigned>(groups * heads), kThreads, 0, stream>>>(
-            s, a.lengths, a.ids, items.words, bits);
+            s, a.lengths, a.ids, items.words, bits, counts);
         NACHO_TRY_HIP(hipGetLastError());
     }
-    items_kernel<<<ceil_div(static_cast<size_t>(items.rows), kWaves), kThreads, 0, stream>>>(
-        items.rows, items.words, items.per_item, bits, counts);
+    start_kernel<<<1, kStartBlock, 0, stream>>>(items.rows, items.per_item,
+                                                queries > 0 ? counts : nullptr, start);
     NACHO_TRY_HIP(hipGetLastError());
-    NACHO_TRY(scan::exclusive_scan_i64(call, counts, items.rows, start));
     const unsigned grid = static_cast<unsigned>((most * parts + 7) / 8 * 8);
     const unsigned inverse =
         s.group == 1 ? 0u : static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(s.group)) + 1u;
@@ -1181,7 +1197,7 @@ int backward(Call &call, const Args<T> &a) {
             <<<grid, kThreads, 0, stream>>>(a, delta, items, inverse);
     }
     NACHO_TRY_HIP(hipGetLastError());
-    if (listed > items.per_item) {  // else no row has several
+    if (several) {
         dkv_join_kernel<T, DP><<<static_cast<unsigned>(items.rows * (s.block / 16)), kThreads, 0,
                                  stream>>>(a, items);
         NACHO_TRY_HIP(hipGetLastError());
@@ -1193,6 +1209,7 @@ template <typename T>
 int run(const nacho_block_attention_args &p, const Shape &s, Call &call, bool back) {
     const Args<T> a = args_of<T>(p, s);
     if (s.dim <= 64) return back ? backward<T, 64>(call, a) : forward<T, 64>(call, a);
+    if (s.dim <= 96) return back ? backward<T, 96>(call, a) : forward<T, 96>(call, a);
     return back ? backward<T, 128>(call, a) : forward<T, 128>(call, a);
 }
 

@@ -93,16 +93,18 @@ __device__ __forceinline__ Frag<float> row_frag<float>(const float *p) {
 template <typename T, int DP>
 constexpr int kTileRow = DP + 16 / static_cast<int>(sizeof(T));
 
-// Rows of DP elements in LDS, filled straight from memory: a wavefront's load names a source per
+// Rows in LDS, filled straight from memory: a wavefront's load names a source per
 // lane and writes 64 consecutive 16-byte pieces.  Rows are not padded (they cannot be); instead
 // piece p of row r lies at place p ^ swizzle(r), which the loads' sources take care of, so that
 // the 16 rows that a fragment reads lie in different banks, and so do the rows of a column.
+// Products use the first DP columns; a row in LDS has the next power of two.
 template <typename T, int DP, int ROWS, int THREADS>
 struct Tile {
+    static constexpr int kRow = DP <= 64 ? 64 : 128;
     static constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // elements of a piece
-    static constexpr int kPieces = DP / kPer;                      // pieces of a row
+    static constexpr int kPieces = kRow / kPer;                    // pieces of a row
     static constexpr int kLoads = ROWS * kPieces / THREADS;
-    static constexpr int kElements = ROWS * DP;
+    static constexpr int kElements = ROWS * kRow;
     static_assert(ROWS * kPieces % THREADS == 0, "whole pieces per thread");
 
     __device__ __forceinline__ static int swizzle(int row) {
@@ -169,7 +171,7 @@ struct Tile {
 
     // Columns 32 kk + 8 g .. + 8 of row 16 t + c.
     __device__ __forceinline__ static Frag<T> row(const T *tile, int t, int kk, int g, int c) {
-        const T *p = tile + (16 * t + c) * DP;
+        const T *p = tile + (16 * t + c) * kRow;
         const int x = swizzle(c);  // (of row 16 t + c as well)
         if constexpr (sizeof(T) == 4) {
             const int piece = 8 * kk + 2 * g;
@@ -191,20 +193,19 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = 4 * g + j;
-                const T *p = tile + (32 * u + r) * DP + (piece ^ swizzle(r)) * kPer + (c & 3);
+                const T *p = tile + (32 * u + r) * kRow + (piece ^ swizzle(r)) * kPer + (c & 3);
                 f[j] = p[0];
-                f[4 + j] = p[16 * DP];
+                f[4 + j] = p[16 * kRow];
             }
             return f;
         } else {
             using Shared = __attribute__((address_space(3))) s16x4 *;
             const int r = 4 * g + (c >> 2);
-            const T *p = tile + (32 * u + r) * DP +
-                         ((2 * i + ((c >> 1) & 1)) ^ swizzle(r)) * kPer + 4 * (c & 1);
+            const int at = r * kRow + ((2 * i + ((c >> 1) & 1)) ^ swizzle(r)) * kPer + 4 * (c & 1);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (Shared)(reinterpret_cast<const s16x4 *>(p)));
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + (32 * u * kRow + at))));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (Shared)(reinterpret_cast<const s16x4 *>(p + 16 * DP)));
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + (32 * u * kRow + 16 * kRow + at))));
             const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             return __builtin_bit_cast(Frag<T>, both);
         }
@@ -235,7 +236,7 @@ struct TileStage {
         for (int i = 0; i < Lds::kLoads; ++i) {
             const int at = lane + i * dev::kWave;
             const int r = at / Lds::kPieces, p = (at % Lds::kPieces) ^ Lds::swizzle(r);
-            *reinterpret_cast<u32x4 *>(tile + r * DP + p * Lds::kPer) = piece[i];
+            *reinterpret_cast<u32x4 *>(tile + r * Lds::kRow + p * Lds::kPer) = piece[i];
         }
     }
 };

@@ -18,6 +18,7 @@ graph.  There is no CPU fallback.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -28,12 +29,24 @@ from .ops import _entry
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
+_BOUND: dict = {}
+
+
+def _bind(name):
+    fn = _BOUND[name] = functools.partial(getattr(_lib.load_bridge(), name),
+                                          _entry("nacho_" + name))
+    return fn
+
+
 def _call(name, device, *args):
     """The bridge's call of entry point nacho_<name>; None for refused operands."""
-    address = _entry("nacho_" + name)
-    with _device.on_device(device):
-        got = getattr(_lib.load_bridge(), name)(address, _device.current_stream(device),
-                                                device.index, *args)
+    fn = _BOUND.get(name) or _bind(name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        got = fn(torch._C._cuda_getCurrentRawStream(index), index, *args)
+    else:
+        with _device.on_device(device):
+            got = fn(torch._C._cuda_getCurrentRawStream(index), index, *args)
     if type(got) is int:
         _lib.check(got, "nacho_" + name)
     return got

@@ -391,7 +391,8 @@ struct Partials {
 
 constexpr int kSplitKeys = 32;  // keys of a step
 
-template <typename T, int DP>
+// AHEAD: steps whose operands are on their way.  Two need the registers of a CU to itself.
+template <typename T, int DP, int AHEAD>
 __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, Partials part) {
     using Stage = TileStage<T, DP, kSplitKeys>;
     constexpr int kJoin = DP + 4;  // floats of a row of o in LDS
@@ -401,6 +402,7 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
     __shared__ __align__(16) unsigned char s_wave[kWaves][kWaveBytes];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16];
     __shared__ Lists<16> s_lists;
+    __shared__ int s_few[kWaves][dev::kWave];
     const Shape &s = a.s;
     const int split = static_cast<int>(blockIdx.x) % splits;
     const int index = static_cast<int>(blockIdx.x) / splits;
@@ -423,52 +425,91 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
     const float scale2 = base2_scale(s.scale);
     const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
     const int end = tile.last_key(s, tile.tokens - 1) + 1;
-    const int steps_of = s.block / kSplitKeys;
+    const int shift = s.block == 32 ? 0 : s.block == 64 ? 1 : 2;  // steps of a block
     const int stride = splits * kWaves;
-    Stage v_next;
-    Frag<T> k_next[2][DP / 32];
-    for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
-        const int steps = window_lists(s, a.ids, tile, first, s_lists) * steps_of;
+    Stage v_next[AHEAD];
+    Frag<T> k_next[AHEAD][2][DP / 32];
+    // The wavefront's own of `steps` steps; block_of(n): the n-th block, selected(n): whether
+    // the lane's row selected it.
+    auto work = [&](int steps, auto block_of, auto selected) {
         auto first_key = [&](int step) {
-            return (first + s_lists.ids[step / steps_of]) * s.block + step % steps_of * kSplitKeys;
+            return block_of(step >> shift) * s.block + (step & ((1 << shift) - 1)) * kSplitKeys;
         };
-        auto load = [&](int step) {
+        auto load = [&](int step, Frag<T> (&k)[2][DP / 32], Stage &v) {
             const int key = first_key(step);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r = key + 16 * t + c;
                 load_row_frags<T, DP>(r < tile.length ? k_base + r * a.k.row_stride : nullptr,
-                                      s.dim, g, k_next[t]);
+                                      s.dim, g, k[t]);
             }
-            v_next.load(lane, s.dim, [&](int r) -> const T * {
+            v.load(lane, s.dim, [&](int r) -> const T * {
                 return key + r < tile.length ? v_base + (key + r) * a.v.row_stride : nullptr;
             });
         };
-        int step = split * kWaves + wave;
-        if (step < steps) load(step);
-        for (; step < steps; step += stride) {  // the wavefront's own
-            const bool selected = exists && s_lists.has(step / steps_of, token);
-            const int limit = step_limit(selected, last_key, first_key(step), g);
-            f32x4 p[1][2];
+        const int from = split * kWaves + wave;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                p[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < AHEAD; ++d) {
+            if (from + d * stride < steps) load(from + d * stride, k_next[d], v_next[d]);
+        }
+        for (int step0 = from; step0 < steps; step0 += AHEAD * stride) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    p[0][t] = mma(k_next[t][kk], q[0][kk], p[0][t]);
+            for (int d = 0; d < AHEAD; ++d) {
+                const int step = step0 + d * stride;
+                if (step >= steps) break;
+                const int limit = step_limit(exists && selected(step >> shift), last_key,
+                                             first_key(step), g);
+                f32x4 p[1][2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    p[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int kk = 0; kk < DP / 32; ++kk) {
+                        p[0][t] = mma(k_next[d][t][kk], q[0][kk], p[0][t]);
+                    }
                 }
-            }
-            dev::wave_sync();  // the reads of the step before
-            v_next.store(lane, s_v);
-            dev::wave_sync();
-            if (step + stride < steps) load(step + stride);
-            if (!__any(limit > 0)) continue;
-            float factor;
-            if (softmax_step<2>(p[0], scale2, limit, m, l, factor)) {
+                dev::wave_sync();  // the reads of the step before
+                v_next[d].store(lane, s_v);
+                dev::wave_sync();
+                if (step + AHEAD * stride < steps) {
+                    load(step + AHEAD * stride, k_next[d], v_next[d]);
+                }
+                if (!__any(limit > 0)) continue;
+                float factor;
+                if (softmax_step<2>(p[0], scale2, limit, m, l, factor)) {
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
+                    for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
+                }
+                column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
             }
-            column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
+        }
+    };
+    if (tile.tokens == 1 && s.count <= dev::kWave) {
+        // One token: its ids are the list, once each.  Every wavefront makes its own copy.
+        const int last = tile.last_key(s, 0);
+        const int64_t row =
+            (static_cast<int64_t>(tile.b) * s.queries + tile.t0) * s.kv_heads + tile.h;
+        const int id = lane < s.count ? a.ids[row * s.count + lane] : -1;
+        bool first = last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block);
+        for (int j = 0; j + 1 < s.count; ++j) {
+            const int other = __builtin_amdgcn_readlane(id, j);
+            first = first && !(j < lane && other == id);
+        }
+        const unsigned long long listed = __ballot(first);
+        int *list = s_few[wave];
+        if (first) list[__popcll(listed & ((1ull << lane) - 1ull))] = id;
+        dev::wave_sync();
+        work(static_cast<int>(__popcll(listed)) << shift,
+             [&](int n) { return __builtin_amdgcn_readfirstlane(list[n]); },
+             [](int) { return true; });
+    } else {
+        for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
+            const int blocks = window_lists(s, a.ids, tile, first, s_lists);
+            work(blocks << shift,
+                 [&](int n) {
+                     return first + __builtin_amdgcn_readfirstlane(s_lists.ids[n]);
+                 },
+                 [&](int n) { return s_lists.has(n, token); });
         }
     }
     l = column_sum(l);
@@ -1118,8 +1159,13 @@ int forward(Call &call, const Args<T> &a) {
         NACHO_TRY(call.scratch_n(rows * (DP + 2), &part.o));
         part.ml = part.o + rows * DP;
     }
-    split_kernel<T, DP><<<static_cast<unsigned>(few * splits), kThreads, 0, stream>>>(
-        a, static_cast<int>(splits), part);
+    const unsigned grid = static_cast<unsigned>(few * splits);
+    if (sizeof(T) == 2 && grid <= kFullGrid) {
+        split_kernel<T, DP, sizeof(T) == 2 ? 2 : 1>
+            <<<grid, kThreads, 0, stream>>>(a, static_cast<int>(splits), part);
+    } else {
+        split_kernel<T, DP, 1><<<grid, kThreads, 0, stream>>>(a, static_cast<int>(splits), part);
+    }
     NACHO_TRY_HIP(hipGetLastError());
     if (splits > 1) {
         join_kernel<T, DP><<<static_cast<unsigned>(few * 16), DP, 0, stream>>>(

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
 
 struct SelectArgs {
     int64_t rows;
-    int queries, heads, keys, block, blocks, count, sink, local, causal;
+    int queries, heads, keys, shift, blocks, count, sink, local, causal;  // block = 2^shift
     const float *scores;
     const int *lengths;
     int *ids;
@@ -182,78 +182,147 @@ struct SelectArgs {
 constexpr int kMaxForced = 1 << 20;  // of sink and of local: fits above the infinity's number
 
 // A number that orders like the score: 0 for a block that is not to be taken, the forced blocks'
-// above every score's, in the order in which they are taken.
+// above every score's, in the order in which they are taken.  (Selects, not branches.)
+constexpr unsigned kHighestScore = 0xff800000u;  // of an infinity
+
 __device__ __forceinline__ unsigned order_of(const SelectArgs &a, float score, int j, int own) {
-    if (j > own) return 0u;
-    if (own - j < a.local) return UINT_MAX - static_cast<unsigned>(own - j);
-    if (j < a.sink) return UINT_MAX - static_cast<unsigned>(a.local) - static_cast<unsigned>(j);
-    if (!(score > kNegInf)) return 0u;                     // (NaN too)
-    const unsigned u = __float_as_uint(score + 0.0f);      // -0 as 0
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const unsigned u = __float_as_uint(score + 0.0f);  // -0 as 0
+    unsigned x = u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
+    x = score > kNegInf ? x : 0u;  // (NaN too)
+    x = j < a.sink ? UINT_MAX - static_cast<unsigned>(a.local) - static_cast<unsigned>(j) : x;
+    x = own - j < a.local ? UINT_MAX - static_cast<unsigned>(own - j) : x;
+    return j > own ? 0u : x;
 }
 
-// NR registers a lane hold the row (64 NR blocks); NR = 0 reads it again each time.
+// Selects for one row, whose scores are in `held_score` (NR > 0) or read again each time.
 template <int NR>
-__global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
-    const int64_t row = blockIdx.x * static_cast<int64_t>(kThreads / dev::kWave) +
-                        threadIdx.x / dev::kWave;
-    if (row >= a.rows) return;
+__device__ __forceinline__ void select_row(const SelectArgs &a, unsigned row32, const float *scores,
+                                           const float (&held_score)[NR ? NR : 1]) {
     const int lane = dev::lane();
-    const int64_t bt = row / a.heads;
-    const int t = static_cast<int>(bt % a.queries), b = static_cast<int>(bt / a.queries);
+    const int chunks = NR ? NR : (a.blocks + dev::kWave - 1) / dev::kWave;
+    const int64_t row = row32;
+    const unsigned bt = row32 / static_cast<unsigned>(a.heads);
+    const int t = static_cast<int>(bt % static_cast<unsigned>(a.queries));
+    const int b = static_cast<int>(bt / static_cast<unsigned>(a.queries));
     const int length = length_of(a.lengths, b, a.keys);
     const int place = length - a.queries + t;
-    const int own = place < 0 ? -1 : (a.causal ? place : length - 1) / a.block;
-    const float *scores = a.scores + row * a.blocks;
-    const int chunks = NR ? NR : (a.blocks + dev::kWave - 1) / dev::kWave;
-    auto fetch = [&](int r) {
-        const int j = r * dev::kWave + lane;
-        return j < a.blocks && j <= own ? order_of(a, scores[j], j, own) : 0u;
-    };
+    const int own = place < 0 ? -1 : (a.causal ? place : length - 1) >> a.shift;
     unsigned held[NR ? NR : 1];
     if constexpr (NR > 0) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) held[r] = fetch(r);
+        for (int r = 0; r < NR; ++r) {
+            held[r] = order_of(a, held_score[r], r * dev::kWave + lane, own);
+        }
     }
-    auto key = [&](int r) { return NR ? held[NR ? r : 0] : fetch(r); };
+    auto key = [&](int r) {
+        if constexpr (NR > 0) {
+            return held[r];
+        } else {
+            const int j = r * dev::kWave + lane;
+            return j < a.blocks ? order_of(a, scores[j], j, own) : 0u;
+        }
+    };
     auto at_least = [&](unsigned x) {
         int n = 0;
-#pragma unroll(NR ? NR : 1)
+#pragma unroll NR ? NR : 1
         for (int r = 0; r < chunks; ++r) n += __popcll(__ballot(key(r) >= x));
         return n;
     };
-    // the largest threshold that `count` numbers reach (0: fewer than that many are not 0)
+    // The largest threshold that `count` numbers reach, or 0 where no more than `count` are to be
+    // had: between lo, which that many reach, and hi, which they do not.  A float's number falls
+    // by 2^23 when it is halved, so lo is a step or two of that below the highest score's, and
+    // half of what is between them is where the count is met, most often after a few halvings.
     unsigned threshold = 0u;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned x = threshold | 1u << bit;
-        const int n = at_least(x);
-        if (n >= a.count) threshold = x;
-        if (n == a.count) break;
+    int above = 0;  // how many are over the threshold
+    if (at_least(1u) > a.count) {
+        unsigned top = 0u;
+#pragma unroll NR ? NR : 1
+        for (int r = 0; r < chunks; ++r) {
+            const unsigned x = key(r);
+            top = max(top, x <= kHighestScore ? x : 0u);
+        }
+        top = __builtin_amdgcn_readlane(dev::wave_inclusive_umax_dpp(top), dev::kWave - 1);
+        unsigned lo = 0u, hi = top + 1u;
+        int n = at_least(hi);
+        above = n;
+        if (n >= a.count) {  // forced blocks alone
+            lo = hi;
+            hi = UINT_MAX;
+            above = at_least(hi);
+            if (above >= a.count) {  // (count = 1: the latest block's number is the highest)
+                lo = hi;
+                n = above;
+            }
+        } else {
+            for (unsigned width = 1u << 23;; width *= 2u) {
+                lo = hi > width ? hi - width : 1u;
+                n = at_least(lo);
+                if (n >= a.count || width > UINT_MAX / 2u) break;
+                above = n;
+                hi = lo;
+            }
+        }
+        while (n != a.count && hi - lo > 1u) {
+            const unsigned mid = lo + (hi - lo) / 2u;
+            const int m = at_least(mid);
+            if (m >= a.count) {
+                lo = mid;
+                n = m;
+            } else {
+                hi = mid;
+                above = m;
+            }
+        }
+        threshold = lo;
+        if (n == a.count) above = -1;  // no ties to break
     }
-    const bool all = threshold == 0u;
-    int ties = 0;  // how many of those equal to the threshold
-    if (!all) {
-        int above = 0;
-#pragma unroll(NR ? NR : 1)
-        for (int r = 0; r < chunks; ++r) above += __popcll(__ballot(key(r) > threshold));
-        ties = a.count - above;
-    }
+    // those over the threshold, and of those at it the lowest ids that there is room for
+    int ties = above < 0 || threshold == 0u ? INT_MAX : a.count - above;
+    const unsigned least = max(threshold, 1u);
     int *ids = a.ids + row * a.count;
     const unsigned long long before = (1ull << lane) - 1ull;
     int at = 0;
-#pragma unroll(NR ? NR : 1)
+#pragma unroll NR ? NR : 1
     for (int r = 0; r < chunks; ++r) {
         const unsigned x = key(r);
-        const unsigned long long equal = __ballot(!all && x == threshold);
-        const bool take = all ? x > 0u
-                              : x > threshold ||
-                                    (x == threshold && __popcll(equal & before) < ties);
-        const unsigned long long taken = __ballot(take);
-        if (take) ids[at + __popcll(taken & before)] = r * dev::kWave + lane;
+        unsigned long long taken = __ballot(x >= least);
+        if (ties != INT_MAX) {  // uniform
+            const unsigned long long equal = __ballot(x == least);
+            const bool extra = x == least && static_cast<int>(__popcll(equal & before)) >= ties;
+            taken &= ~__ballot(extra);
+            ties -= min(ties, static_cast<int>(__popcll(equal)));
+        }
+        if (taken >> lane & 1ull) ids[at + __popcll(taken & before)] = r * dev::kWave + lane;
         at += __popcll(taken);
-        ties -= min(ties, static_cast<int>(__popcll(equal)));
     }
     for (int i = at + lane; i < a.count; i += dev::kWave) ids[i] = -1;
+}
+
+// NR registers a lane hold a row (64 NR blocks); NR = 0 reads it again each time.  A wavefront
+// has ROWS rows: many rows of few blocks are otherwise bound by the start of wavefronts (65,536
+// rows of 128 blocks: 29 us with one each).
+template <int NR, int ROWS>
+__global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
+    // (a wavefront's number in scalar registers: the divisions are a few scalar instructions)
+    const unsigned first = ROWS * __builtin_amdgcn_readfirstlane(
+        blockIdx.x * (kThreads / dev::kWave) + threadIdx.x / dev::kWave);
+    const unsigned rows = static_cast<unsigned>(a.rows);
+    float held[ROWS][NR ? NR : 1];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {  // all loads at once
+        const float *scores = a.scores + static_cast<int64_t>(first + i) * a.blocks;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int j = r * dev::kWave + dev::lane();
+            held[i][r] = first + i < rows && j < a.blocks ? scores[j] : kNegInf;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (first + i >= rows) return;
+        select_row<NR>(a, first + i, a.scores + static_cast<int64_t>(first + i) * a.blocks,
+                       held[i]);
+    }
 }
 
 // ---- host -----------------------------------------------------------------------------
@@ -363,6 +432,8 @@ int scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys, int32_t 
     }
 }
 
+constexpr int64_t kManyRows = 16384;  // of which one to a wavefront is two rounds of the device
+
 int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t block,
            int32_t count, int32_t sink, int32_t local, int32_t causal, const float *score,
            const int32_t *lengths, int32_t *ids, void *stream) {
@@ -376,19 +447,22 @@ int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t 
     if (!ids || (!score && keys > 0)) return NACHO_ERR_INVALID_ARGUMENT;
     const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
     const int64_t grid = (rows + 3) / 4;
-    if (grid > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
-    const SelectArgs a{rows,  queries, heads, keys,   block, static_cast<int>(blocks), count, sink,
+    if (rows > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
+    const int shift = block == 32 ? 5 : block == 64 ? 6 : 7;
+    const SelectArgs a{rows,  queries, heads, keys,   shift, static_cast<int>(blocks), count, sink,
                        local, causal,  score, lengths, ids};
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned n = static_cast<unsigned>(grid);
-    if (blocks <= 2 * dev::kWave) {
-        select_kernel<2><<<n, kThreads, 0, s>>>(a);
+    if (blocks <= 2 * dev::kWave && rows >= kManyRows) {
+        select_kernel<2, 4><<<(n + 3) / 4, kThreads, 0, s>>>(a);
+    } else if (blocks <= 2 * dev::kWave) {
+        select_kernel<2, 1><<<n, kThreads, 0, s>>>(a);
     } else if (blocks <= 8 * dev::kWave) {
-        select_kernel<8><<<n, kThreads, 0, s>>>(a);
+        select_kernel<8, 1><<<n, kThreads, 0, s>>>(a);
     } else if (blocks <= 32 * dev::kWave) {
-        select_kernel<32><<<n, kThreads, 0, s>>>(a);
+        select_kernel<32, 1><<<n, kThreads, 0, s>>>(a);
     } else {
-        select_kernel<0><<<n, kThreads, 0, s>>>(a);
+        select_kernel<0, 1><<<n, kThreads, 0, s>>>(a);
     }
     NACHO_TRY_HIP(hipGetLastError());
     return NACHO_OK;

@@ -88,24 +88,24 @@ struct ScoresArgs {
     int per_part;  // steps of 64 blocks that a workgroup takes
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int TOKENS>
 __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T *__restrict__ q,
                                                           int sequences) {
     constexpr int kRow = kTileRow<float, DP>;
-    __shared__ __align__(16) float s_q[64 * kRow];
+    __shared__ __align__(16) float s_q[TOKENS * kRow];
     const int heads = sequences * a.heads;
     const int bh = static_cast<int>(blockIdx.x) % heads;
     const int rest = static_cast<int>(blockIdx.x) / heads;
     const int tile = rest % a.tiles, part = rest / a.tiles;
     const int b = bh / a.heads, h = bh % a.heads;
-    const int t0 = 64 * tile, tokens = min(64, a.queries - t0);
+    const int t0 = TOKENS * tile, tokens = min(TOKENS, a.queries - t0);
     const int length = length_of(a.lengths, b, a.keys);
     const int place0 = length - a.queries + t0;
     const int wave = static_cast<int>(threadIdx.x) / dev::kWave;
     const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
     // the group's heads, summed
     constexpr int kPieces = DP / 8;
-    for (int x = threadIdx.x; x < 64 * kPieces; x += kThreads) {
+    for (int x = threadIdx.x; x < TOKENS * kPieces; x += kThreads) {
         const int r = x / kPieces, col = x % kPieces * 8;
         float sum[8] = {};
         if (r < tokens && col < a.dim) {
@@ -131,9 +131,9 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
     for (int step = part * a.per_part; step < end; ++step) {
         const int j = 64 * step + 16 * wave + c;
         if (64 * step + 16 * wave >= a.blocks) continue;
-        f32x4 acc[4];
+        f32x4 acc[TOKENS / 16];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < TOKENS / 16; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (static_cast<int64_t>(64 * step + 16 * wave) * a.block <= last) {  // uniform
             f32x8 m[DP / 32];
             const float *p = j < a.blocks
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
                                  : nullptr;
             load_row_frags<float, DP>(p, a.dim, g, m);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < TOKENS / 16; ++t) {
                 if (t < row_tiles) {
 #pragma unroll
                     for (int kk = 0; kk < DP / 32; ++kk) {
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
         if (j >= a.blocks) continue;
         const int64_t first_key = static_cast<int64_t>(j) * a.block;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < TOKENS / 16; ++t) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * t + 4 * g + i;
@@ -373,13 +373,15 @@ int means(int32_t dtype, int32_t batch, int32_t keys, int32_t heads, int32_t dim
     return NACHO_OK;
 }
 
+constexpr int kScoreTokens = 16;
+
 template <typename T>
 int launch_scores(const ScoresArgs &a, const void *q, int batch, unsigned grid, hipStream_t s) {
     const T *data = static_cast<const T *>(q);
     if (a.dim <= 64) {
-        scores_kernel<T, 64><<<grid, kThreads, 0, s>>>(a, data, batch);
+        scores_kernel<T, 64, kScoreTokens><<<grid, kThreads, 0, s>>>(a, data, batch);
     } else {
-        scores_kernel<T, 128><<<grid, kThreads, 0, s>>>(a, data, batch);
+        scores_kernel<T, 128, kScoreTokens><<<grid, kThreads, 0, s>>>(a, data, batch);
     }
     NACHO_TRY_HIP(hipGetLastError());
     return NACHO_OK;
@@ -398,7 +400,7 @@ int scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys, int32_t 
     }
     if (empty) return NACHO_OK;
     const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
-    const int64_t tiles = (static_cast<int64_t>(queries) + 63) / 64;
+    const int64_t tiles = (static_cast<int64_t>(queries) + kScoreTokens - 1) / kScoreTokens;
     const int64_t groups = tiles * batch * kv_heads;
     const int64_t steps = (blocks + 63) / 64;
     if (groups * steps > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;

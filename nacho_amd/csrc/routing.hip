@@ -234,14 +234,20 @@ __device__ void clear_behind(const Rows &a, T *__restrict__ rows) {
     }
 }
 
+// A token of the workgroup, in scalar registers (LANES is a multiple of a wavefront).
+template <int LANES>
+__device__ __forceinline__ int64_t token_of() {
+    return blockIdx.x * static_cast<int64_t>(kThreads / LANES) +
+           __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+}
+
 // LANES threads per token.
 template <typename T, int N, int LANES>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(Rows a, const T *__restrict__ x,
                                                             int64_t x_stride,
                                                             T *__restrict__ rows) {
     if (blockIdx.x >= a.token_groups) return clear_behind<T, N>(a, rows);
-    const int64_t token =
-        blockIdx.x * static_cast<int64_t>(kThreads / LANES) + threadIdx.x / LANES;
+    const int64_t token = token_of<LANES>();
     if (token >= a.tokens) return;
     const int *slots = a.slot + token * a.per_token;
     for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
@@ -254,28 +260,40 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(Rows a, const T *__r
     }
 }
 
+// The rows of STEP experts are on their way together; a dropped entry's stand-in is row 0, whose
+// values are passed over.
 template <typename T, int N, int LANES>
 __global__ __launch_bounds__(kThreads) void combine_kernel(Rows a, const T *__restrict__ rows,
                                                            int64_t row_stride,
                                                            const float *__restrict__ weights,
                                                            T *__restrict__ out) {
-    const int64_t token =
-        blockIdx.x * static_cast<int64_t>(kThreads / LANES) + threadIdx.x / LANES;
+    constexpr int kStep = 4;
+    const int64_t token = token_of<LANES>();
     if (token >= a.tokens) return;
-    const int *slots = a.slot + token * a.per_token;
+    const int64_t e = token * a.per_token;
     for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
          col += LANES * N) {
         float sum[N] = {};
-#pragma unroll 4
-        for (int i = 0; i < a.per_token; ++i) {
-            const int64_t at = slots[i];
-            if (at < 0) continue;
-            const float w = weights ? weights[token * a.per_token + i] : 1.0f;
-            const auto piece =
-                *reinterpret_cast<const Piece<T, N> *>(rows + at * row_stride + col);
+        for (int i0 = 0; i0 < a.per_token; i0 += kStep) {
+            Piece<T, N> piece[kStep];
+            float w[kStep];
+            bool there[kStep];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                sum[j] = __builtin_fmaf(w, static_cast<float>(piece.v[j]), sum[j]);
+            for (int i = 0; i < kStep; ++i) {
+                const bool listed = i0 + i < a.per_token;
+                const int64_t at = listed ? a.slot[e + i0 + i] : -1;
+                there[i] = at >= 0;
+                w[i] = weights && listed ? weights[e + i0 + i] : 1.0f;
+                piece[i] = *reinterpret_cast<const Piece<T, N> *>(
+                    rows + (there[i] ? at : 0) * row_stride + col);
+            }
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float x = static_cast<float>(piece[i].v[j]);
+                    sum[j] = there[i] ? __builtin_fmaf(w[i], x, sum[j]) : sum[j];
+                }
             }
         }
         Piece<T, N> o;
@@ -293,8 +311,7 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(
     if (blockIdx.x >= a.token_groups) return clear_behind<T, N>(a, drows);
     constexpr int kWavesPer = LANES / dev::kWave;
     __shared__ float s_sum[kThreads / dev::kWave];
-    const int64_t token =
-        blockIdx.x * static_cast<int64_t>(kThreads / LANES) + threadIdx.x / LANES;
+    const int64_t token = token_of<LANES>();
     if (LANES < kThreads && token >= a.tokens) return;  // (no barrier below for whole wavefronts)
     for (int i = 0; i < a.per_token; ++i) {
         const int64_t e = token * a.per_token + i;

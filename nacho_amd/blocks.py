@@ -188,14 +188,17 @@ class _BlockAttention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, blocks, lengths, out, lse)
         ctx.how = block, causal, scale
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)  # (lse's would be a launch that fills zeros)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
         q, k, v, blocks, lengths, out, lse = ctx.saved_tensors
-        grads = gpu_block_attention_backward(dout, q, k, v, blocks, ctx.how[0], out, lse, lengths,
-                                             *ctx.how[1:])
+        grads = None, None, None
+        if dout is not None:
+            grads = _call("block_attention_backward", q.device, q, k, v, blocks, lengths, *ctx.how,
+                          dout, out, lse)
         return (*grads, None, None, None, None, None)
 
 

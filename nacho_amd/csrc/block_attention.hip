@@ -17,6 +17,11 @@
 // dq = scale ds K goes tile by tile as the forward pass; dk = scale ds^T Q and dv = p^T dout go
 // block by block over the tokens that selected the block, found from a bit matrix [block][token],
 // the transpose of the lists; so no sum depends on an order of atomics.
+//
+// A key that a row does not see must not reach it, whatever its values: keys past the sequence's
+// end are read as zeros, but a block's other rows are there for the tile's other tokens, and 0
+// times infinity is no number.  So a tile whose result is not finite is done again with masks key
+// by key and with the values that are not finite taken out (Pass); nothing else pays for that.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -184,14 +189,30 @@ __device__ int window_lists(const Shape &s, const int *__restrict__ ids, const R
 // Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
 // rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
 // sequence's end are zeros.  Every wavefront calls it; `use` has no barrier.
+// How a tile is worked on: as it is; where that is not finite, once more for which results see
+// something that is not (these keep what they have), and once with what is not finite left out of
+// the products over keys, for the others.
+enum Pass { kPlain = 0, kMarks, kFinite };
+
+// A result of a pass after kPlain's, at a place that holds those of the passes before.
+template <typename T>
+__device__ __forceinline__ void store_again(T *p, float v, int pass) {
+    const float there = static_cast<float>(*p);
+    if (pass == kMarks ? v == 0.0f : there - there == 0.0f) {
+        *p = static_cast<T>(pass == kMarks ? 0.0f : v);
+    }
+}
+
 template <typename T, int DP, int BN, int R>
 struct KeySteps {
     using Lds = Tile<T, DP, BN, kThreads>;
     T *k[2], *v[2];
     Lists<R> &lists;
 
+    // masked[]: the operand whose products over keys the pass concerns (k or v).
     template <typename Use>
-    __device__ __forceinline__ void run(const Args<T> &a, const RowTile<R> &tile, Use use) {
+    __device__ __forceinline__ void run(const Args<T> &a, const RowTile<R> &tile, int pass,
+                                        T *const (&masked)[2], Use use) {
         const Shape &s = a.s;
         const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
         const int end = tile.last_key(s, tile.tokens - 1) + 1;  // keys that some row sees
@@ -210,15 +231,22 @@ struct KeySteps {
                 Lds::load(to_k, threadIdx.x, k_source, k_base + key * a.k.row_stride, there);
                 Lds::load(to_v, threadIdx.x, v_source, v_base + key * a.v.row_stride, there);
             };
+            auto arrived = [&](T *tile_of) {
+                __syncthreads();
+                if (pass != kPlain) {  // uniform
+                    Lds::make_finite(tile_of, threadIdx.x, pass == kMarks);
+                    __syncthreads();
+                }
+            };
             if (steps > 0) load(0, k[0], v[0]);
-            __syncthreads();
+            arrived(masked[0]);
             for (int step = 0; step < steps; step += 2) {
                 if (step + 1 < steps) load(step + 1, k[1], v[1]);
                 use(k[0], v[0], step >> shift, first_key(step));
-                __syncthreads();
+                arrived(masked[1]);
                 if (step + 2 < steps) load(step + 2, k[0], v[0]);
                 if (step + 1 < steps) use(k[1], v[1], (step + 1) >> shift, first_key(step + 1));
-                __syncthreads();
+                arrived(masked[0]);
             }
         }
     }
@@ -242,12 +270,12 @@ constexpr float kSlack = 8.0f;  // the running maximum follows a row's when it i
 // wavefront needs it.  Returns whether they were, by `factor`.
 //
 // Most steps are seen whole or not at all: a row that sees nothing of a step takes a maximum of
-// infinity there, and only steps that some row sees in part are masked key by key.
+// infinity there, and only steps that some row sees in part, or `every` one, are masked key by key.
 template <int N>
-__device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, float &m,
-                                             float &l, float &factor) {
+__device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, bool every,
+                                             float &m, float &l, float &factor) {
     const bool none = limit <= 0;
-    if (__any(!none && limit < 16 * N)) {
+    if (every || __any(!none && limit < 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
@@ -340,44 +368,60 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args<T> a) {
             rows.exists[x] ? a.q.row(tile.b, tile.t0 + rows.token[x], rows.head[x]) : nullptr,
             s.dim, g, q[x]);
         if (s.scale < 0.0f) negate<T, DP>(q[x]);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m[x] = kNegInf;
-        l[x] = 0.0f;
     }
     const float scale2 = base2_scale(s.scale);
     KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
-    steps.run(a, tile, [&](const T *s_k, const T *s_v, int nth, int first_key) {
-        int limit[COLS];
-        if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
-        f32x4 p[COLS][BN / 16];
-        row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
+    for (int pass = kPlain; pass <= kFinite; ++pass) {  // uniform
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
-            float factor;
-            if (softmax_step<BN / 16>(p[x], scale2, limit[x], m[x], l[x], factor)) {
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
+            for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m[x] = kNegInf;
+            l[x] = 0.0f;
+        }
+        steps.run(a, tile, pass, {s_v0, s_v1}, [&](const T *s_k, const T *s_v, int nth,
+                                                   int first_key) {
+            int limit[COLS];
+            if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
+            f32x4 p[COLS][BN / 16];
+            row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) {
+                float factor;
+                if (softmax_step<BN / 16>(p[x], scale2, limit[x], pass != kPlain, m[x], l[x],
+                                          factor)) {
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
+                }
+            }
+            column_products<Lds, T, DP, COLS, BN / 16>(s_v, p, g, c, o);
+        });
+        float wrong = 0.0f;
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+            wrong += not_finite<DP / 16>(o[x]) + l[x] * 0.0f;
+            const float sum = column_sum(l[x]);
+            if (!rows.exists[x]) continue;
+            const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            const int t = tile.t0 + rows.token[x], head = rows.head[x];
+            T *out = a.out.row(tile.b, t, head);
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const int col = 16 * i + 4 * g;
+                if (col >= s.dim) continue;
+                if (pass == kPlain) {
+                    store4<T>(out + col, o[x][i] * inverse);
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) store_again(out + col + j, o[x][i][j] * inverse, pass);
+            }
+            if (a.lse && g == 0) {
+                a.lse[(static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head] =
+                    sum == 0.0f ? kNegInf : (m[x] + log2_fast(sum)) * kLn2;
             }
         }
-        column_products<Lds, T, DP, COLS, BN / 16>(s_v, p, g, c, o);
-    });
-#pragma unroll
-    for (int x = 0; x < COLS; ++x) {
-        const float sum = column_sum(l[x]);
-        if (!rows.exists[x]) continue;
-        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (NaN stays)
-        const int t = tile.t0 + rows.token[x], head = rows.head[x];
-        T *out = a.out.row(tile.b, t, head);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const int col = 16 * i + 4 * g;
-            if (col < s.dim) store4<T>(out + col, o[x][i] * inverse);
-        }
-        if (a.lse && g == 0) {
-            a.lse[(static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head] =
-                sum == 0.0f ? kNegInf : (m[x] + log2_fast(sum)) * kLn2;
-        }
+        if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;
     }
 }
 
@@ -392,8 +436,10 @@ struct Partials {
 constexpr int kSplitKeys = 32;  // keys of a step
 
 // AHEAD: steps whose operands are on their way.  Two need the registers of a CU to itself.
-template <typename T, int DP, int AHEAD>
-__global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, Partials part) {
+// ONE: a tile is one token (of at most 64 ids): its ids are the list, and its rows see the same
+// keys, so that nothing is masked but what is read as zeros.
+template <typename T, int DP, int AHEAD, bool ONE>
+__global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) void split_kernel(Args<T> a, int splits, Partials part) {
     using Stage = TileStage<T, DP, kSplitKeys>;
     constexpr int kJoin = DP + 4;  // floats of a row of o in LDS
     constexpr int kTileBytes = Stage::Lds::kElements * static_cast<int>(sizeof(T));
@@ -401,8 +447,7 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
     constexpr int kWaveBytes = kTileBytes > kJoinBytes ? kTileBytes : kJoinBytes;
     __shared__ __align__(16) unsigned char s_wave[kWaves][kWaveBytes];
     __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-    __shared__ Lists<16> s_lists;
-    __shared__ int s_few[kWaves][dev::kWave];
+    __shared__ std::conditional_t<ONE, int[kWaves][dev::kWave], Lists<16>> s_lists;
     const Shape &s = a.s;
     const int split = static_cast<int>(blockIdx.x) % splits;
     const int index = static_cast<int>(blockIdx.x) / splits;
@@ -419,9 +464,8 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
                           q[0]);
     if (s.scale < 0.0f) negate<T, DP>(q[0]);
     f32x4 o[1][DP / 16];
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) o[0][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kNegInf, l = 0.0f;
+    float m, l;
+    int pass = kPlain;
     const float scale2 = base2_scale(s.scale);
     const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
     const int end = tile.last_key(s, tile.tokens - 1) + 1;
@@ -469,6 +513,7 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
                     }
                 }
                 dev::wave_sync();  // the reads of the step before
+                if (pass != kPlain) v_next[d].make_finite(pass == kMarks);
                 v_next[d].store(lane, s_v);
                 dev::wave_sync();
                 if (step + AHEAD * stride < steps) {
@@ -476,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
                 }
                 if (!__any(limit > 0)) continue;
                 float factor;
-                if (softmax_step<2>(p[0], scale2, limit, m, l, factor)) {
+                if (softmax_step<2>(p[0], scale2, limit, pass != kPlain, m, l, factor)) {
 #pragma unroll
                     for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
                 }
@@ -484,79 +529,93 @@ __global__ __launch_bounds__(kThreads) void split_kernel(Args<T> a, int splits, 
             }
         }
     };
-    if (tile.tokens == 1 && s.count <= dev::kWave) {
-        // One token: its ids are the list, once each.  Every wavefront makes its own copy.
-        const int last = tile.last_key(s, 0);
-        const int64_t row =
-            (static_cast<int64_t>(tile.b) * s.queries + tile.t0) * s.kv_heads + tile.h;
-        const int id = lane < s.count ? a.ids[row * s.count + lane] : -1;
-        bool first = last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block);
-        for (int j = 0; j + 1 < s.count; ++j) {
-            const int other = __builtin_amdgcn_readlane(id, j);
-            first = first && !(j < lane && other == id);
-        }
-        const unsigned long long listed = __ballot(first);
-        int *list = s_few[wave];
-        if (first) list[__popcll(listed & ((1ull << lane) - 1ull))] = id;
-        dev::wave_sync();
-        work(static_cast<int>(__popcll(listed)) << shift,
-             [&](int n) { return __builtin_amdgcn_readfirstlane(list[n]); },
-             [](int) { return true; });
-    } else {
-        for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
-            const int blocks = window_lists(s, a.ids, tile, first, s_lists);
-            work(blocks << shift,
-                 [&](int n) {
-                     return first + __builtin_amdgcn_readfirstlane(s_lists.ids[n]);
-                 },
-                 [&](int n) { return s_lists.has(n, token); });
-        }
-    }
-    l = column_sum(l);
-    // Join the wavefronts: each row's sums are brought to the largest maximum.
-    dev::wave_sync();
-    float *s_o = reinterpret_cast<float *>(s_wave[wave]);
+    for (;; ++pass) {  // uniform
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-        *reinterpret_cast<f32x4 *>(s_o + c * kJoin + 16 * i + 4 * g) = o[0][i];
-    }
-    if (g == 0) {
-        s_m[wave][c] = m;
-        s_l[wave][c] = l;
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < 16 * DP; x += kThreads) {
-        const int r = x / DP, col = x % DP;
-        int t, hd;
-        if (!tile.row(s, r, t, hd)) continue;
-        float top = kNegInf;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_m[w][r]);
-        const float base = top == kNegInf ? 0.0f : top;
-        float sum = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = exp2_fast(s_m[w][r] - base);
-            sum += f * s_l[w][r];
-            v += f * reinterpret_cast<const float *>(s_wave[w])[r * kJoin + col];
-        }
-        if (splits > 1) {
-            const int64_t at = (static_cast<int64_t>(index) * splits + split) * 16 + r;
-            part.o[at * DP + col] = v;
-            if (col == 0) {
-                part.ml[2 * at] = top;
-                part.ml[2 * at + 1] = sum;
+        for (int i = 0; i < DP / 16; ++i) o[0][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m = kNegInf;
+        l = 0.0f;
+        if constexpr (ONE) {
+            // The valid ids, once each.  Every wavefront makes its own copy.
+            const int last = tile.last_key(s, 0);
+            const int64_t row =
+                (static_cast<int64_t>(tile.b) * s.queries + tile.t0) * s.kv_heads + tile.h;
+            const int id = lane < s.count ? a.ids[row * s.count + lane] : -1;
+            bool first = last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block);
+            for (int j = 0; j + 1 < s.count; ++j) {
+                const int other = __builtin_amdgcn_readlane(id, j);
+                first = first && !(j < lane && other == id);
             }
-            continue;
+            const unsigned long long listed = __ballot(first);
+            int *list = s_lists[wave];
+            if (first) list[__popcll(listed & ((1ull << lane) - 1ull))] = id;
+            dev::wave_sync();
+            work(static_cast<int>(__popcll(listed)) << shift,
+                 [&](int n) { return __builtin_amdgcn_readfirstlane(list[n]); },
+                 [](int) { return true; });
+        } else {
+            for (int first = 0; first * s.block < end; first += kWindow) {  // uniform
+                const int blocks = window_lists(s, a.ids, tile, first, s_lists);
+                work(blocks << shift,
+                     [&](int n) {
+                         return first + __builtin_amdgcn_readfirstlane(s_lists.ids[n]);
+                     },
+                     [&](int n) { return s_lists.has(n, token); });
+            }
         }
-        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-        if (col < s.dim) {
-            a.out.row(tile.b, tile.t0 + t, hd)[col] = static_cast<T>(v * inverse);
+        l = column_sum(l);
+        // Join the wavefronts: each row's sums are brought to the largest maximum.
+        dev::wave_sync();
+        float *s_o = reinterpret_cast<float *>(s_wave[wave]);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            *reinterpret_cast<f32x4 *>(s_o + c * kJoin + 16 * i + 4 * g) = o[0][i];
         }
-        if (col == 0 && a.lse) {
-            a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + t) * s.q_heads + hd] =
-                sum == 0.0f ? kNegInf : (top + log2_fast(sum)) * kLn2;
+        if (g == 0) {
+            s_m[wave][c] = m;
+            s_l[wave][c] = l;
         }
+        __syncthreads();
+        bool wrong = false;
+        for (int x = threadIdx.x; x < 16 * DP; x += kThreads) {
+            const int r = x / DP, col = x % DP;
+            int t, hd;
+            if (!tile.row(s, r, t, hd)) continue;
+            float top = kNegInf;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_m[w][r]);
+            const float base = top == kNegInf ? 0.0f : top;
+            float sum = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = exp2_fast(s_m[w][r] - base);
+                sum += f * s_l[w][r];
+                v += f * reinterpret_cast<const float *>(s_wave[w])[r * kJoin + col];
+            }
+            wrong = wrong || !(v - v == 0.0f) || !(sum - sum == 0.0f);
+            if (splits > 1) {
+                const int64_t at = (static_cast<int64_t>(index) * splits + split) * 16 + r;
+                if (pass == kPlain) {
+                    part.o[at * DP + col] = v;
+                } else {
+                    store_again(&part.o[at * DP + col], v, pass);
+                }
+                if (col == 0) {
+                    part.ml[2 * at] = top;
+                    part.ml[2 * at + 1] = sum;
+                }
+                continue;
+            }
+            const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            T *out = a.out.row(tile.b, tile.t0 + t, hd) + col;
+            if (col < s.dim && pass == kPlain) *out = static_cast<T>(v * inverse);
+            if (col < s.dim && pass != kPlain) store_again(out, v * inverse, pass);
+            if (col == 0 && a.lse) {
+                a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + t) * s.q_heads + hd] =
+                    sum == 0.0f ? kNegInf : (top + log2_fast(sum)) * kLn2;
+            }
+        }
+        if (ONE || pass == kFinite) break;
+        if (!__syncthreads_or(wrong) && pass == kPlain) break;
     }
 }
 
@@ -666,7 +725,7 @@ __global__ __launch_bounds__(kStartBlock) void start_kernel(int64_t rows, int pe
 // and dp the scores' gradients (without the scale).
 template <int N>
 __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], float scale2,
-                                               float lse2, float delta, int limit) {
+                                               float lse2, float delta, int limit, bool every) {
     const bool none = limit <= 0;
     const float base = none ? -kNegInf : lse2;  // (as in softmax_step)
 #pragma unroll
@@ -677,7 +736,7 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
             dp[t][i] = s[t][i] * (dp[t][i] - delta);
         }
     }
-    if (__any(!none && limit < 16 * N)) {
+    if (every || __any(!none && limit < 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
@@ -733,32 +792,43 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a, float *__res
         }
         row_delta[x] = column_sum(sum);
         if (exists && g == 0) delta[at] = row_delta[x];
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const float scale2 = base2_scale(s.scale);
     KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
-    steps.run(a, tile, [&](const T *s_k, const T *s_v, int nth, int first_key) {
-        int limit[COLS];
-        if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
-        f32x4 p[COLS][BN / 16], dp[COLS][BN / 16];
-        row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
-        row_products<Lds, T, DP, COLS, BN / 16>(s_v, dout, g, c, dp);
+    // (No marks: what a row sees that is not finite is in its lse or delta.)
+    for (int pass = kPlain; pass <= kFinite; pass += kFinite) {  // uniform
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
-            score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x]);
-        }
-        column_products<Lds, T, DP, COLS, BN / 16>(s_k, dp, g, c, o);
-    });
 #pragma unroll
-    for (int x = 0; x < COLS; ++x) {
-        if (!rows.exists[x]) continue;
-        T *dq = a.dq.row(tile.b, tile.t0 + rows.token[x], rows.head[x]);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            const int col = 16 * i + 4 * g;
-            if (col < s.dim) store4<T>(dq + col, o[x][i] * s.scale);
+            for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        steps.run(a, tile, pass, {s_k0, s_k1}, [&](const T *s_k, const T *s_v, int nth,
+                                                   int first_key) {
+            int limit[COLS];
+            if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
+            f32x4 p[COLS][BN / 16], dp[COLS][BN / 16];
+            row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
+            row_products<Lds, T, DP, COLS, BN / 16>(s_v, dout, g, c, dp);
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) {
+                score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x],
+                                        pass != kPlain);
+            }
+            column_products<Lds, T, DP, COLS, BN / 16>(s_k, dp, g, c, o);
+        });
+        float wrong = 0.0f;
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+            wrong += not_finite<DP / 16>(o[x]);
+            if (!rows.exists[x]) continue;
+            T *dq = a.dq.row(tile.b, tile.t0 + rows.token[x], rows.head[x]);
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const int col = 16 * i + 4 * g;
+                if (col < s.dim) store4<T>(dq + col, o[x][i] * s.scale);
+            }
+        }
+        if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;
     }
 }
 
@@ -1160,11 +1230,17 @@ int forward(Call &call, const Args<T> &a) {
         part.ml = part.o + rows * DP;
     }
     const unsigned grid = static_cast<unsigned>(few * splits);
-    if (sizeof(T) == 2 && grid <= kFullGrid) {
-        split_kernel<T, DP, sizeof(T) == 2 ? 2 : 1>
+    auto launch = [&](auto ahead, auto one) {
+        split_kernel<T, DP, ahead(), one()>
             <<<grid, kThreads, 0, stream>>>(a, static_cast<int>(splits), part);
+    };
+    constexpr std::integral_constant<int, sizeof(T) == 2 ? 2 : 1> two;
+    constexpr std::integral_constant<int, 1> one;
+    const bool token = (small.tokens == 1 || s.queries == 1) && s.count <= dev::kWave;
+    if (grid <= kFullGrid) {
+        token ? launch(two, std::true_type{}) : launch(two, std::false_type{});
     } else {
-        split_kernel<T, DP, 1><<<grid, kThreads, 0, stream>>>(a, static_cast<int>(splits), part);
+        token ? launch(one, std::true_type{}) : launch(one, std::false_type{});
     }
     NACHO_TRY_HIP(hipGetLastError());
     if (splits > 1) {

@@ -93,6 +93,22 @@ __device__ __forceinline__ Frag<float> row_frag<float>(const float *p) {
 template <typename T, int DP>
 constexpr int kTileRow = DP + 16 / static_cast<int>(sizeof(T));
 
+// What a product with masked operands needs where some are not finite (0 times infinity is no
+// number): each element that is not becomes 0, or with `marks` 1, and the others 0.
+template <typename T>
+__device__ __forceinline__ u32x4 finite_piece(u32x4 bits, bool marks) {
+    constexpr int kN = 16 / static_cast<int>(sizeof(T));
+    typedef T piece_t __attribute__((ext_vector_type(kN)));
+    piece_t v = __builtin_bit_cast(piece_t, bits);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const float x = static_cast<float>(v[j]);
+        const bool finite = x - x == 0.0f;
+        v[j] = marks ? static_cast<T>(finite ? 0.0f : 1.0f) : finite ? v[j] : static_cast<T>(0.0f);
+    }
+    return __builtin_bit_cast(u32x4, v);
+}
+
 // Rows in LDS, filled straight from memory: a wavefront's load names a source per
 // lane and writes 64 consecutive 16-byte pieces.  Rows are not padded (they cannot be); instead
 // piece p of row r lies at place p ^ swizzle(r), which the loads' sources take care of, so that
@@ -169,6 +185,13 @@ struct Tile {
 #endif
     }
 
+    __device__ static void make_finite(T *tile, int thread, bool marks) {
+        for (int i = 0; i < kLoads; ++i) {
+            u32x4 *p = reinterpret_cast<u32x4 *>(tile + (thread + i * THREADS) * kPer);
+            *p = finite_piece<T>(*p, marks);
+        }
+    }
+
     // Columns 32 kk + 8 g .. + 8 of row 16 t + c.
     __device__ __forceinline__ static Frag<T> row(const T *tile, int t, int kk, int g, int c) {
         const T *p = tile + (16 * t + c) * kRow;
@@ -230,6 +253,10 @@ struct TileStage {
             piece[i] = u32x4{0u, 0u, 0u, 0u};
             if (row && col < D) piece[i] = *reinterpret_cast<const u32x4 *>(row + col);
         }
+    }
+    __device__ __forceinline__ void make_finite(bool marks) {
+#pragma unroll
+        for (int i = 0; i < Lds::kLoads; ++i) piece[i] = finite_piece<T>(piece[i], marks);
     }
     __device__ __forceinline__ void store(int lane, T *tile) const {
 #pragma unroll
@@ -317,6 +344,18 @@ __device__ __forceinline__ float column_sum(float v) {
     const unsigned y = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
     const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// 0, or no number where some sum is not finite.
+template <int N>
+__device__ __forceinline__ float not_finite(const f32x4 (&v)[N]) {
+    float x = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x = __builtin_fmaf(v[n][i], 0.0f, x);
+    }
+    return x;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -123,6 +123,54 @@ def test_rows_without_blocks(gpu, sizes):
     _check(gpu, q, k, v, ids[..., :0], dout, sizes[6])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [(2, 300, 300, 32, 8, 64, 64, 2), (1, 64, 200, 4, 2, 128, 32, 2),
+                                   (1, 3, 200, 4, 2, 72, 64, 1), (2, 1, 200, 4, 2, 72, 64, 2)],
+                         ids=str)
+def test_not_finite_in_masked_places(gpu, sizes, dtype):
+    """Keys and values that are not finite reach the queries that see them, and no others: not
+    those that other queries of their tile selected, nor later keys of a query's own block."""
+    q, k, v, ids, dout = _operands(17, dtype, *sizes)
+    block, (batch, keys, kv_heads, dim) = sizes[6], k.shape
+    group = q.shape[2] // kv_heads
+    bad_k, bad_v = k.clone(), v.clone()
+    for b in range(batch):
+        for h in range(kv_heads):
+            bad_v[b, keys - 40 + h, h, 3] = math.inf
+            bad_v[b, 17 + h, h, dim - 1] = math.nan
+            bad_k[b, keys - 1, h] = math.nan  # seen by the last query alone
+            bad_k[b, keys // 2, h, 1] = -math.inf
+    hurt = ~(torch.isfinite(bad_k).all(-1) & torch.isfinite(bad_v).all(-1))  # [b, keys, h]
+    see = ref.visible(ids, q.shape[1], keys, block, None, True)
+    sees = (see & hurt.transpose(1, 2)[:, :, None]).any(-1).transpose(1, 2)  # [b, queries, h]
+    sees = sees.repeat_interleave(group, -1)
+    assert sizes[1] == 1 or (sees.any() and not sees.all())
+    sees_v = torch.stack([(see & ~torch.isfinite(bad_v[..., c]).transpose(1, 2)[:, :, None])
+                          .any(-1).transpose(1, 2) for c in range(dim)], -1)
+    sees_v = sees_v.repeat_interleave(group, 2)
+    sees_k = (see & ~torch.isfinite(bad_k).all(-1).transpose(1, 2)[:, :, None]).any(-1)
+    sees_k = sees_k.transpose(1, 2).repeat_interleave(group, -1)
+
+    good = torch.nan_to_num(bad_k, 0.0, 0.0, 0.0), torch.nan_to_num(bad_v, 0.0, 0.0, 0.0)
+    want = ref.Attention(q, *good, ids, block, dout=dout)
+    dev = [x.to(gpu).requires_grad_() for x in (q, bad_k, bad_v)]
+    out, lse = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), block, return_lse=True)
+    dq, = torch.autograd.grad(out, dev[:1], dout.to(gpu))
+    out, lse, dq = out.detach().cpu(), lse.cpu(), dq.cpu()
+    clean = ~sees_k[..., None] & ~sees_v
+    none = torch.zeros((), dtype=torch.float64)
+
+    def check(got, name, where):
+        ref.near(torch.where(where, got.double(), none),
+                 torch.where(where, getattr(want, name), none),
+                 getattr(want, name + "_off"), name)
+
+    check(out, "out", clean)
+    check(lse, "lse", ~sees_k)
+    check(dq, "dq", ~sees[..., None].expand_as(dq))
+    assert not torch.isfinite(out[sees_v & ~sees_k[..., None]]).any()
+
+
 @pytest.mark.parametrize("batch,queries,keys", [(0, 4, 40), (2, 0, 40), (2, 4, 0)])
 def test_empty_operands(gpu, batch, queries, keys):
     q, k, v, _, dout = _operands(6, torch.bfloat16, batch, queries, keys, 4, 2, 32, 32, 1)

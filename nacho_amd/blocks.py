@@ -39,7 +39,8 @@ def _bind(name):
 
 
 def _call(name, device, *args):
-    """The bridge's call of entry point nacho_<name>; None for refused operands."""
+    """The bridge's call of entry point nacho_<name>; None for operands that it or the entry point
+    refuses: the caller then names what is wrong."""
     fn = _BOUND.get(name) or _bind(name)
     index = device.index
     if torch._C._cuda_getDevice() == index:
@@ -48,16 +49,18 @@ def _call(name, device, *args):
         with _device.on_device(device):
             got = fn(torch._C._cuda_getCurrentRawStream(index), index, *args)
     if type(got) is int:
+        if got == -1:  # NACHO_ERR_INVALID_ARGUMENT
+            return None
         _lib.check(got, "nacho_" + name)
     return got
 
 
 def _device_of(t, name):
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return t.device
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
-        raise ValueError(f"{name}: expected a GPU tensor, got device {t.device}")
-    return t.device
+    raise ValueError(f"{name}: expected a GPU tensor, got device {t.device}")
 
 
 # ---- what is wrong with refused operands ----------------------------------------------
@@ -91,11 +94,12 @@ def _check_block(block):
         raise ValueError(f"block must be 32, 64 or 128, got {block}")
 
 
-def _refuse_attention(q, k, v, blocks, lengths):
+def _refuse_attention(q, k, v, blocks, lengths, block):
     device = q.device
     _check_tensor(q, "q", device, 4, _TYPES)
     for t, name in ((k, "k"), (v, "v")):
         _check_tensor(t, name, device, 4, (q.dtype,))
+    _check_heads(q.shape[2], k.shape[2], q.shape[3], block)
     if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"shapes of q {tuple(q.shape)}, k {tuple(k.shape)} and v "
                          f"{tuple(v.shape)} do not fit")
@@ -104,14 +108,16 @@ def _refuse_attention(q, k, v, blocks, lengths):
     if tuple(blocks.shape[:3]) != want:
         raise ValueError(f"blocks: expected shape {want} + (count,), got {tuple(blocks.shape)}")
     _check_lengths(lengths, device, q.shape[0])
-    raise ValueError("gpu_block_attention: an operand has more than 2^31 - 1 rows")
+    raise ValueError("gpu_block_attention: refused operands (more than 2^31 - 1 rows, or more "
+                     "than 1024 heads of q to a key head)")
 
 
-def _scale(scale, head_dim):
-    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+def _scale(scale, shape):
+    if scale is None:
+        return (shape[-1] or 1) ** -0.5 if shape else 1.0
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    return scale
+    return float(scale)
 
 
 # ---- means, scores, selection ---------------------------------------------------------
@@ -121,11 +127,10 @@ def gpu_block_means(k: torch.Tensor, block: int,
     """Mean key of each block, float32 [batch, ceil(keys / block), kv_heads, head_dim], over the
     keys within the sequence's length; 0 for a block without any.  No gradient."""
     device = _device_of(k, "k")
-    if k.dim() == 4:
-        _check_heads(1, 1, k.shape[3], block)
     got = _call("block_means", device, k, lengths, block)
     if got is None:
         _check_tensor(k, "k", device, 4, _TYPES)
+        _check_heads(1, 1, k.shape[3], block)
         _check_lengths(lengths, device, k.shape[0])
         raise ValueError("gpu_block_means: refused operands")
     return got
@@ -140,14 +145,13 @@ def gpu_block_scores(q: torch.Tensor, means: torch.Tensor, block: int, keys: int
     starts after the query's place, or not causal, at the sequence's end.  `keys`: rows of the
     cache.  No gradient."""
     device = _device_of(q, "q")
-    if q.dim() == 4 and isinstance(means, torch.Tensor) and means.dim() == 4:
-        _check_heads(q.shape[2], means.shape[2], q.shape[3], block)
-        scale = _scale(scale, q.shape[3])
-        got = _call("block_scores", device, q, means, lengths, block, keys, bool(causal), scale)
-        if got is not None:
-            return got
+    got = _call("block_scores", device, q, means, lengths, block, keys, bool(causal),
+                _scale(scale, q.shape))
+    if got is not None:
+        return got
     _check_tensor(q, "q", device, 4, _TYPES)
     _check_tensor(means, "means", device, 4, (torch.float32,))
+    _check_heads(q.shape[2], means.shape[2], q.shape[3], block)
     _check_lengths(lengths, device, q.shape[0])
     raise ValueError(f"means: expected [{q.shape[0]}, ceil({keys} / {block}), kv_heads, "
                      f"{q.shape[3]}], got {tuple(means.shape)}")
@@ -161,7 +165,6 @@ def gpu_block_select(scores: torch.Tensor, count: int, block: int, keys: int,
     whatever their scores, then those of the highest scores, equal ones lowest id first.  A block
     with a score of -inf or NaN is taken only as one of the former."""
     device = _device_of(scores, "scores")
-    _check_block(block)
     if count < 0 or not 0 <= sink <= 1 << 20 or not 0 <= local <= 1 << 20:
         raise ValueError(f"count, sink and local must be >= 0 (sink and local <= 2^20), got "
                          f"{count}, {sink} and {local}")
@@ -169,6 +172,7 @@ def gpu_block_select(scores: torch.Tensor, count: int, block: int, keys: int,
                 local)
     if got is None:
         _check_tensor(scores, "scores", device, 4, (torch.float32,))
+        _check_block(block)
         _check_lengths(lengths, device, scores.shape[0])
         raise ValueError(f"scores: expected ceil({keys} / {block}) blocks, got "
                          f"{tuple(scores.shape)}")
@@ -183,7 +187,7 @@ class _BlockAttention(torch.autograd.Function):
         got = _call("block_attention", q.device, q, k, v, blocks, lengths, block, causal, scale,
                     True)
         if got is None:
-            _refuse_attention(q, k, v, blocks, lengths)
+            _refuse_attention(q, k, v, blocks, lengths, block)
         out, lse = got
         ctx.save_for_backward(q, k, v, blocks, lengths, out, lse)
         ctx.how = block, causal, scale
@@ -214,20 +218,16 @@ def gpu_block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block
     float32 [batch, queries, q_heads] (-inf for such a query; no gradient), with which results
     over disjoint sets of keys can be joined.  Differentiable in q, k and v."""
     device = _device_of(q, "q")
-    if q.dim() == 4 and isinstance(k, torch.Tensor) and k.dim() == 4:
-        _check_heads(q.shape[2], k.shape[2], q.shape[3], block)
-        scale = _scale(scale, q.shape[3])
-    else:
-        _refuse_attention(q, k, v, blocks, lengths)
+    scale = _scale(scale, q.shape)
     causal = bool(causal)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+    if torch.is_grad_enabled() and (q.requires_grad or getattr(k, "requires_grad", False) or
                                     getattr(v, "requires_grad", False)):
         out, lse = _BlockAttention.apply(q, k, v, blocks, lengths, block, causal, scale)
         return (out, lse) if return_lse else out
     got = _call("block_attention", device, q, k, v, blocks, lengths, block, causal, scale,
                 return_lse)
     if got is None:
-        _refuse_attention(q, k, v, blocks, lengths)
+        _refuse_attention(q, k, v, blocks, lengths, block)
     return got if return_lse else got[0]
 
 
@@ -239,13 +239,8 @@ def gpu_block_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.T
     """(dq, dk, dv) of gpu_block_attention from its output's gradient, its operands and its
     results, for callers that keep their own record of a step.  Deterministic."""
     device = _device_of(q, "q")
-    if q.dim() == 4 and isinstance(k, torch.Tensor) and k.dim() == 4:
-        _check_heads(q.shape[2], k.shape[2], q.shape[3], block)
-        scale = _scale(scale, q.shape[3])
-    else:
-        _refuse_attention(q, k, v, blocks, lengths)
     got = _call("block_attention_backward", device, q, k, v, blocks, lengths, block, bool(causal),
-                scale, dout, out, lse)
+                _scale(scale, q.shape), dout, out, lse)
     if got is None:
         for t, name in ((dout, "dout"), (out, "out")):
             _check_tensor(t, name, device, 4, (q.dtype,))
@@ -254,5 +249,5 @@ def gpu_block_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.T
         _check_tensor(lse, "lse", device, 3, (torch.float32,))
         if lse.shape != q.shape[:3]:
             raise ValueError(f"lse: expected shape {tuple(q.shape[:3])}, got {tuple(lse.shape)}")
-        _refuse_attention(q, k, v, blocks, lengths)
+        _refuse_attention(q, k, v, blocks, lengths, block)
     return got

@@ -64,12 +64,17 @@ Heads<T> heads(const nacho_heads &h) {
 }
 
 template <typename T>
-struct Args {
+struct Forward {
     Shape s;
-    Heads<T> q, k, v, out, dout, dq, dk, dv;
+    Heads<T> q, k, v, out;
     const int *lengths;
     const int *ids;
     float *lse;
+};
+
+template <typename T>
+struct Backward : Forward<T> {
+    Heads<T> dout, dq, dk, dv;
 };
 
 __device__ __forceinline__ int length_of(const Shape &s, const int *lengths, int b) {
@@ -211,7 +216,7 @@ struct KeySteps {
 
     // masked[]: the operand whose products over keys the pass concerns (k or v).
     template <typename Use>
-    __device__ __forceinline__ void run(const Args<T> &a, const RowTile<R> &tile, int pass,
+    __device__ __forceinline__ void run(const Forward<T> &a, const RowTile<R> &tile, int pass,
                                         T *const (&masked)[2], Use use) {
         const Shape &s = a.s;
         const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
@@ -346,7 +351,7 @@ struct LaneRows {
 };
 
 template <typename T, int DP, int BN, int COLS>
-__global__ __launch_bounds__(kThreads, 2) void tile_kernel(Args<T> a) {
+__global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
     using Lds = Tile<T, DP, BN, kThreads>;
     constexpr int kRowsOf = 64 * COLS;
     __shared__ __align__(16) T s_k0[Lds::kElements];
@@ -439,7 +444,7 @@ constexpr int kSplitKeys = 32;  // keys of a step
 // ONE: a tile is one token (of at most 64 ids): its ids are the list, and its rows see the same
 // keys, so that nothing is masked but what is read as zeros.
 template <typename T, int DP, int AHEAD, bool ONE>
-__global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) void split_kernel(Args<T> a, int splits, Partials part) {
+__global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) void split_kernel(Forward<T> a, int splits, Partials part) {
     using Stage = TileStage<T, DP, kSplitKeys>;
     constexpr int kJoin = DP + 4;  // floats of a row of o in LDS
     constexpr int kTileBytes = Stage::Lds::kElements * static_cast<int>(sizeof(T));
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) voi
 
 // Joins the splits of a row: a workgroup of DP threads per row of a tile.
 template <typename T, int DP>
-__global__ __launch_bounds__(DP) void join_kernel(Args<T> a, int splits, Partials part) {
+__global__ __launch_bounds__(DP) void join_kernel(Forward<T> a, int splits, Partials part) {
     const Shape &s = a.s;
     const int index = static_cast<int>(blockIdx.x) / 16, r = static_cast<int>(blockIdx.x) % 16;
     const RowTile<16> tile(s, a.lengths, index);
@@ -747,7 +752,7 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
 
 // dq, and delta and zeroed counts for the launches that follow.
 template <typename T, int DP, int BN, int COLS>
-__global__ __launch_bounds__(kThreads, 2) void dq_kernel(Args<T> a, float *__restrict__ delta,
+__global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *__restrict__ delta,
                                                          int64_t rows_of_blocks,
                                                          int *__restrict__ counts) {
     using Lds = Tile<T, DP, BN, kThreads>;
@@ -850,7 +855,7 @@ struct Items {
 // with LANES = 2 the four wavefronts are two such sets, which take 32 rows of the item's tokens
 // in turn and add their sums at the end.
 template <typename T, int DP, int COLS, int LANES>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(Args<T> a, const float *__restrict__ delta,
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(Backward<T> a, const float *__restrict__ delta,
                                                        Items items, unsigned group_inverse) {
     constexpr int kSets = kWaves / LANES;
     constexpr int kStep = kSets * kStepRows;
@@ -1078,7 +1083,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(A
 
 // Adds up the items of a row that has several, in their order: a workgroup per 16 keys.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void dkv_join_kernel(Args<T> a, Items items) {
+__global__ __launch_bounds__(kThreads) void dkv_join_kernel(Backward<T> a, Items items) {
     const Shape &s = a.s;
     const int parts = s.block / 16;
     const int64_t row = blockIdx.x / parts;
@@ -1152,19 +1157,21 @@ int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
 }
 
 template <typename T>
-Args<T> args_of(const nacho_block_attention_args &p, const Shape &s) {
-    return Args<T>{s,
-                   heads<T>(p.q),
-                   heads<T>(p.k),
-                   heads<T>(p.v),
-                   heads<T>(p.out),
-                   heads<T>(p.dout),
-                   heads<T>(p.dq),
-                   heads<T>(p.dk),
-                   heads<T>(p.dv),
-                   p.lengths,
-                   p.blocks,
-                   p.lse};
+Backward<T> args_of(const nacho_block_attention_args &p, const Shape &s) {
+    Backward<T> a;
+    static_cast<Forward<T> &>(a) = Forward<T>{s,
+                                              heads<T>(p.q),
+                                              heads<T>(p.k),
+                                              heads<T>(p.v),
+                                              heads<T>(p.out),
+                                              p.lengths,
+                                              p.blocks,
+                                              p.lse};
+    a.dout = heads<T>(p.dout);
+    a.dq = heads<T>(p.dq);
+    a.dk = heads<T>(p.dk);
+    a.dv = heads<T>(p.dv);
+    return a;
 }
 
 constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
@@ -1202,7 +1209,7 @@ constexpr int64_t kItemTarget = 768;
 constexpr int64_t kItemLeast = 128;
 
 template <typename T, int DP>
-int forward(Call &call, const Args<T> &a) {
+int forward(Call &call, const Forward<T> &a) {
     const Shape &s = a.s;
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
@@ -1211,17 +1218,22 @@ int forward(Call &call, const Args<T> &a) {
             tile_kernel<T, DP, keys(), columns()><<<grid, kThreads, 0, stream>>>(a);
         });
     }
-    // Fewer tiles than CUs: tiles of 16 rows, whose wavefronts share the steps.  Joining splits
-    // costs about as much as three steps (5 us), so a wavefront keeps two steps at least, and
-    // there are no more workgroups than CUs.  One query of 32 heads over 16 blocks of 64: 20 us
-    // in one split, 14 in four; over 8 blocks of 32 (16 heads of 64) 7.8 in one, 12.4 in two.
+    // Fewer tiles than CUs: tiles of 16 rows, whose wavefronts share the steps.  What a step waits
+    // for is its operands (2 to 3 us from memory that nothing read lately), so there are as many
+    // workgroups as find a CU, down to less than a step for each wavefront; past 16 splits the
+    // join costs more than they save, and up to 8 steps one split is done before it would begin.
+    // One query of 32 heads of 128, in us by splits (1, 2, 4, 8, 16, 32): over 4 blocks of 64
+    // 8.6 10.3 11.1 10.1 10.9 12.6, over 16 blocks 18 15 13 10.8 11.8 13, over 64 blocks
+    // 64 40 27 18.4 16.1 16.8; 16 sequences over 16 blocks 23.2 20.8 21.4 24.7 38 66.
     const Tiling small = tiling(s, 16);
     const int64_t few = static_cast<int64_t>(small.per_head) * heads;
-    const int64_t listed = static_cast<int64_t>(small.tokens) * s.count;
+    const int64_t listed =
+        static_cast<int64_t>(small.tokens < s.queries ? small.tokens : s.queries) * s.count;
     const int64_t steps = (listed < s.blocks ? listed : s.blocks) * (s.block / kSplitKeys);
     int64_t splits = kFullGrid / few;
-    const int64_t most = (steps + 2 * kWaves - 1) / (2 * kWaves);
+    const int64_t most = steps <= 2 * kWaves ? 1 : (steps + 2) / 3;
     if (splits > most) splits = most;
+    if (splits > 16) splits = 16;
     if (splits < 1) splits = 1;
     Partials part{};
     if (splits > 1) {
@@ -1252,7 +1264,7 @@ int forward(Call &call, const Args<T> &a) {
 }
 
 template <typename T, int DP>
-int backward(Call &call, const Args<T> &a) {
+int backward(Call &call, const Backward<T> &a) {
     const Shape &s = a.s;
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
@@ -1329,7 +1341,7 @@ int backward(Call &call, const Args<T> &a) {
 
 template <typename T>
 int run(const nacho_block_attention_args &p, const Shape &s, Call &call, bool back) {
-    const Args<T> a = args_of<T>(p, s);
+    const Backward<T> a = args_of<T>(p, s);
     if (s.dim <= 64) return back ? backward<T, 64>(call, a) : forward<T, 64>(call, a);
     if (s.dim <= 96) return back ? backward<T, 96>(call, a) : forward<T, 96>(call, a);
     return back ? backward<T, 128>(call, a) : forward<T, 128>(call, a);

@@ -123,8 +123,15 @@ struct Tile {
     static constexpr int kElements = ROWS * kRow;
     static_assert(ROWS * kPieces % THREADS == 0, "whole pieces per thread");
 
+    // A different number for each of the 16 rows of a fragment (of 8 rows in each half of the
+    // banks, where a row is half of them), and for the rows of a column read, which takes two
+    // neighbouring pieces of eight rows at a time, one that differs in more than its last bit.
     __device__ __forceinline__ static int swizzle(int row) {
-        return kPieces >= 16 ? row & 15 : (row >> 1) & 7;
+        if constexpr (kPieces >= 16) {
+            return ((row << 1) & 14) | ((row >> 3) & 1);
+        } else {
+            return (row & 6) | ((row >> 3) & 1);
+        }
     }
 
     // row_of(r): row r of the source, r < ROWS; every one has to be there (rows that are masked

@@ -1134,7 +1134,7 @@ int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
     const int64_t rows = static_cast<int64_t>(p->batch) * p->queries * p->q_heads;
     const int64_t blocks = (static_cast<int64_t>(p->keys) + p->block - 1) / p->block;
     const int64_t parts = blocks * (p->block / 32) * p->batch * p->kv_heads;
-    if (rows > INT32_MAX / 16 || parts > INT32_MAX || p->keys > INT32_MAX - 256 ||
+    if (rows > INT32_MAX / 16 || parts > INT32_MAX || p->keys > INT32_MAX - (1 << 17) ||
         p->count > INT32_MAX / 64) {
         return NACHO_ERR_INDEX_OVERFLOW;
     }

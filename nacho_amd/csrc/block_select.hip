@@ -128,6 +128,7 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
     const int last = last_place < 0 ? -1 : (a.causal ? last_place : length - 1);
     const int steps = (a.blocks + 63) / 64;
     const int end = min(steps, (part + 1) * a.per_part);
+    const int64_t next_row = static_cast<int64_t>(a.heads) * a.blocks;
     for (int step = part * a.per_part; step < end; ++step) {
         const int j = 64 * step + 16 * wave + c;
         if (64 * step + 16 * wave >= a.blocks) continue;
@@ -153,17 +154,18 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
             }
         }
         if (j >= a.blocks) continue;
-        const int64_t first_key = static_cast<int64_t>(j) * a.block;
+        float *p = a.scores + ((static_cast<int64_t>(b) * a.queries + t0 + 4 * g) * a.heads + h) *
+                                  a.blocks + j;
+        // (queries whose place is before the block's first key do not see it)
+        const int64_t unseen = static_cast<int64_t>(j) * a.block - place0;
 #pragma unroll
         for (int t = 0; t < TOKENS / 16; ++t) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * t + 4 * g + i;
-                if (r >= tokens) continue;
-                const int place = place0 + r;
-                const int seen = place < 0 ? -1 : (a.causal ? place : length - 1);
-                const int64_t row = (static_cast<int64_t>(b) * a.queries + t0 + r) * a.heads + h;
-                a.scores[row * a.blocks + j] = first_key <= seen ? acc[t][i] : kNegInf;
+                const bool sees = a.causal ? r >= unseen
+                                           : place0 + r >= 0 && unseen < length - place0;
+                if (r < tokens) p[(16 * t + i) * next_row] = sees ? acc[t][i] : kNegInf;
             }
         }
     }

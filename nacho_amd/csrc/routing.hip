@@ -212,6 +212,26 @@ struct alignas(N * sizeof(T)) Piece {
     T v[N];
 };
 
+// Rows are too many to be read again from a cache by what comes next: they go past it.
+template <typename T, int N>
+__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
+    if constexpr (N * sizeof(T) == 16) {
+        return __builtin_bit_cast(Piece<T, N>, __builtin_nontemporal_load(
+                                                   reinterpret_cast<const dense::u32x4 *>(p)));
+    } else {
+        return *reinterpret_cast<const Piece<T, N> *>(p);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
+    if constexpr (N * sizeof(T) == 16) {
+        __builtin_nontemporal_store(__builtin_bit_cast(dense::u32x4, v),
+                                    reinterpret_cast<dense::u32x4 *>(p));
+    } else {
+        *reinterpret_cast<Piece<T, N> *>(p) = v;
+    }
+}
+
 struct Rows {
     int64_t tokens, width;
     int per_token, n_experts;
@@ -255,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(Rows a, const T *__r
         const auto piece = *reinterpret_cast<const Piece<T, N> *>(x + token * x_stride + col);
         for (int i = 0; i < a.per_token; ++i) {
             const int64_t at = slots[i];
-            if (at >= 0) *reinterpret_cast<Piece<T, N> *>(rows + at * a.width + col) = piece;
+            if (at >= 0) store_piece<T, N>(rows + at * a.width + col, piece);
         }
     }
 }
@@ -284,8 +304,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Rows a, const T *__re
                 const int64_t at = listed ? a.slot[e + i0 + i] : -1;
                 there[i] = at >= 0;
                 w[i] = weights && listed ? weights[e + i0 + i] : 1.0f;
-                piece[i] = *reinterpret_cast<const Piece<T, N> *>(
-                    rows + (there[i] ? at : 0) * row_stride + col);
+                piece[i] = load_piece<T, N>(rows + (there[i] ? at : 0) * row_stride + col);
             }
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
@@ -323,7 +342,7 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(
                  col += LANES * N) {
                 const auto d =
                     *reinterpret_cast<const Piece<T, N> *>(dout + token * dout_stride + col);
-                const auto y = *reinterpret_cast<const Piece<T, N> *>(rows + at * row_stride + col);
+                const auto y = load_piece<T, N>(rows + at * row_stride + col);
                 Piece<T, N> o;
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
@@ -331,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(
                     dot = __builtin_fmaf(x, static_cast<float>(y.v[j]), dot);
                     o.v[j] = static_cast<T>(w * x);
                 }
-                *reinterpret_cast<Piece<T, N> *>(drows + at * a.width + col) = o;
+                store_piece<T, N>(drows + at * a.width + col, o);
             }
         }
         dot = dev::wave_sum(dot);

@@ -191,9 +191,6 @@ __device__ int window_lists(const Shape &s, const int *__restrict__ ids, const R
     return total;
 }
 
-// Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
-// rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
-// sequence's end are zeros.  Every wavefront calls it; `use` has no barrier.
 // How a tile is worked on: as it is; where that is not finite, once more for which results see
 // something that is not (these keep what they have), and once with what is not finite left out of
 // the products over keys, for the others.
@@ -208,6 +205,11 @@ __device__ __forceinline__ void store_again(T *p, float v, int pass) {
     }
 }
 
+// Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
+// rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
+// sequence's end are zeros.  Every wavefront calls it; `use` has no barrier.
+//
+// Loads go from memory to LDS without registers, into one of two buffers while the other is used.
 template <typename T, int DP, int BN, int R>
 struct KeySteps {
     using Lds = Tile<T, DP, BN, kThreads>;
@@ -350,6 +352,17 @@ struct LaneRows {
     }
 };
 
+// 64 COLS rows of a key head, four wavefronts.  Each has COLS column tiles of 16 rows, which share
+// what it reads of LDS: with one, LDS takes as long as the matrix products and the softmax each.
+//
+// 8192 queries of 32 heads of 128 (8 key heads, bfloat16), 16 of 128 blocks: 306 us.  The union of
+// a wavefront's rows is 27 blocks where each selects 15, so 233 GFLOP are done for 125 that are
+// asked for, at 760 TFLOP/s; a large matrix product of the library reaches 1250 here.  Matrix
+// products are 32% of a CU's time and the vector unit 42%, and with two wavefronts to a SIMD (254
+// registers) these overlap only in part: that is the bound.  64 single tokens of caches of 16384
+// keys, with the same heads and blocks: 50 us for 270 MB, 5.4 TB/s, near a large copy's 5.7.
+// Three sequences of up to 777 queries of 12 heads of 80 in float32, 9 blocks of 32: 55 to 70 us
+// by their lengths, half of it float32 matrix products.
 template <typename T, int DP, int BN, int COLS>
 __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
     using Lds = Tile<T, DP, BN, kThreads>;
@@ -440,11 +453,19 @@ struct Partials {
 
 constexpr int kSplitKeys = 32;  // keys of a step
 
-// AHEAD: steps whose operands are on their way.  Two need the registers of a CU to itself.
 // ONE: a tile is one token (of at most 64 ids): its ids are the list, and its rows see the same
 // keys, so that nothing is masked but what is read as zeros.
-template <typename T, int DP, int AHEAD, bool ONE>
-__global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) void split_kernel(Forward<T> a, int splits, Partials part) {
+//
+// Keys go from memory into operand registers, since no other wavefront reads them; values pass
+// through the wavefront's own LDS for the transposed read.  One step is on its way while the last
+// is worked on; with two, which take the registers of a CU, a call is 0.7 us longer.
+// Bound by the time that operands take to arrive, while there is less than one workgroup to a
+// CU: one token of 16 heads of 64 over 8 blocks of 32 takes 6.0 us a call, one of 32 heads of
+// 128 over 16 blocks of 64 11.5 with the launch that joins its splits (12.9 without ONE), 32
+// such tokens 33 us for 134 MB.
+template <typename T, int DP, bool ONE>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel(
+    Forward<T> a, int splits, Partials part) {
     using Stage = TileStage<T, DP, kSplitKeys>;
     constexpr int kJoin = DP + 4;  // floats of a row of o in LDS
     constexpr int kTileBytes = Stage::Lds::kElements * static_cast<int>(sizeof(T));
@@ -476,62 +497,52 @@ __global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) voi
     const int end = tile.last_key(s, tile.tokens - 1) + 1;
     const int shift = s.block == 32 ? 0 : s.block == 64 ? 1 : 2;  // steps of a block
     const int stride = splits * kWaves;
-    Stage v_next[AHEAD];
-    Frag<T> k_next[AHEAD][2][DP / 32];
+    Stage v_next;
+    Frag<T> k_next[2][DP / 32];
     // The wavefront's own of `steps` steps; block_of(n): the n-th block, selected(n): whether
     // the lane's row selected it.
     auto work = [&](int steps, auto block_of, auto selected) {
         auto first_key = [&](int step) {
             return block_of(step >> shift) * s.block + (step & ((1 << shift) - 1)) * kSplitKeys;
         };
-        auto load = [&](int step, Frag<T> (&k)[2][DP / 32], Stage &v) {
+        auto load = [&](int step) {
             const int key = first_key(step);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r = key + 16 * t + c;
                 load_row_frags<T, DP>(r < tile.length ? k_base + r * a.k.row_stride : nullptr,
-                                      s.dim, g, k[t]);
+                                      s.dim, g, k_next[t]);
             }
-            v.load(lane, s.dim, [&](int r) -> const T * {
+            v_next.load(lane, s.dim, [&](int r) -> const T * {
                 return key + r < tile.length ? v_base + (key + r) * a.v.row_stride : nullptr;
             });
         };
         const int from = split * kWaves + wave;
+        if (from < steps) load(from);
+        for (int step = from; step < steps; step += stride) {
+            const int limit =
+                step_limit(exists && selected(step >> shift), last_key, first_key(step), g);
+            f32x4 p[1][2];
 #pragma unroll
-        for (int d = 0; d < AHEAD; ++d) {
-            if (from + d * stride < steps) load(from + d * stride, k_next[d], v_next[d]);
-        }
-        for (int step0 = from; step0 < steps; step0 += AHEAD * stride) {
+            for (int t = 0; t < 2; ++t) {
+                p[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int d = 0; d < AHEAD; ++d) {
-                const int step = step0 + d * stride;
-                if (step >= steps) break;
-                const int limit = step_limit(exists && selected(step >> shift), last_key,
-                                             first_key(step), g);
-                f32x4 p[1][2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    p[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int kk = 0; kk < DP / 32; ++kk) {
-                        p[0][t] = mma(k_next[d][t][kk], q[0][kk], p[0][t]);
-                    }
+                for (int kk = 0; kk < DP / 32; ++kk) {
+                    p[0][t] = mma(k_next[t][kk], q[0][kk], p[0][t]);
                 }
-                dev::wave_sync();  // the reads of the step before
-                if (pass != kPlain) v_next[d].make_finite(pass == kMarks);
-                v_next[d].store(lane, s_v);
-                dev::wave_sync();
-                if (step + AHEAD * stride < steps) {
-                    load(step + AHEAD * stride, k_next[d], v_next[d]);
-                }
-                if (!__any(limit > 0)) continue;
-                float factor;
-                if (softmax_step<2>(p[0], scale2, limit, pass != kPlain, m, l, factor)) {
-#pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
-                }
-                column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
             }
+            dev::wave_sync();  // the reads of the step before
+            if (pass != kPlain) v_next.make_finite(pass == kMarks);
+            v_next.store(lane, s_v);
+            dev::wave_sync();
+            if (step + stride < steps) load(step + stride);
+            if (!__any(limit > 0)) continue;
+            float factor;
+            if (softmax_step<2>(p[0], scale2, limit, pass != kPlain, m, l, factor)) {
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
+            }
+            column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
         }
     };
     for (;; ++pass) {  // uniform
@@ -545,7 +556,8 @@ __global__ __launch_bounds__(kThreads, AHEAD == 2 || sizeof(T) == 4 ? 1 : 2) voi
             const int64_t row =
                 (static_cast<int64_t>(tile.b) * s.queries + tile.t0) * s.kv_heads + tile.h;
             const int id = lane < s.count ? a.ids[row * s.count + lane] : -1;
-            bool first = last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block);
+            bool first =
+                last >= 0 && static_cast<unsigned>(id) <= static_cast<unsigned>(last / s.block);
             for (int j = 0; j + 1 < s.count; ++j) {
                 const int other = __builtin_amdgcn_readlane(id, j);
                 first = first && !(j < lane && other == id);
@@ -659,7 +671,7 @@ __global__ __launch_bounds__(DP) void join_kernel(Forward<T> a, int splits, Part
 // bits[b][h][block][token / 32]: the tokens that see something of the block through their ids.
 // A workgroup has 128 tokens of a head (four words of each block), gathered in LDS for
 // kMarkWindow blocks at a time: with a word per block and tokens of 32 each, atomics on the
-// words in memory took 29 us, five times this, for 2 x 4096 tokens with 12 ids of 4 heads.
+// words in memory took 29 us, this 6, for 2 x 4096 tokens with 12 ids of 4 heads.
 constexpr int kMarkWords = 4;
 constexpr int kMarkWindow = 1024;
 
@@ -750,7 +762,14 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
     }
 }
 
-// dq, and delta and zeroed counts for the launches that follow.
+// dq, and delta and zeroed counts for the launches that follow.  Three products to the forward
+// pass's two, and 32 keys a step where two column tiles of q and dout fill the registers.
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 172 us, 68 GFLOP that are asked for and
+// 1.6 times that with the union's.
+//
+// ds is rounded to the operands' type for its product, and delta is of the rounded out: with
+// bfloat16 and keys that lean one way these put dq 0.0018 and 0.0006 off, the final rounding
+// 0.0017, relative to its norm.
 template <typename T, int DP, int BN, int COLS>
 __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *__restrict__ delta,
                                                          int64_t rows_of_blocks,
@@ -854,9 +873,16 @@ struct Items {
 // dk and dv of 16 COLS LANES keys of a block.  Each of LANES wavefronts has 16 COLS of the keys;
 // with LANES = 2 the four wavefronts are two such sets, which take 32 rows of the item's tokens
 // in turn and add their sums at the end.
+//
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 203 us for 90 GFLOP (rows that did not
+// select the block take no part); with one workgroup per block instead of items 1146 us.  LDS is
+// the bound, 45% of a CU's time and waits for it: a wavefront's 16 keys use each fragment once.
+// Two column tiles use it twice; for heads of 64 training steps take 247 us with them and 280
+// without, for 128 they leave one wavefront to a SIMD and the kernel takes 276 us.  32 keys to a
+// workgroup instead of 64: training steps 506 us instead of 481, heads of 64 267 instead of 247.
 template <typename T, int DP, int COLS, int LANES>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(Backward<T> a, const float *__restrict__ delta,
-                                                       Items items, unsigned group_inverse) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
+    Backward<T> a, const float *__restrict__ delta, Items items, unsigned group_inverse) {
     constexpr int kSets = kWaves / LANES;
     constexpr int kStep = kSets * kStepRows;
     using Lds = Tile<T, DP, kStep, kThreads>;
@@ -1081,7 +1107,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(B
     }
 }
 
-// Adds up the items of a row that has several, in their order: a workgroup per 16 keys.
+// Adds up the items of a row that has several, in their order: a workgroup per 16 keys.  16 us
+// after the items above, bound by reading them.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void dkv_join_kernel(Backward<T> a, Items items) {
     const Shape &s = a.s;
@@ -1126,8 +1153,9 @@ bool aligned(const nacho_heads &h, int item, bool optional = false) {
 int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
     if (!p || p->dtype < NACHO_F32 || p->dtype > NACHO_BF16) return NACHO_ERR_INVALID_ARGUMENT;
     if (p->batch < 0 || p->queries < 0 || p->keys < 0 || p->q_heads < 1 || p->kv_heads < 1 ||
-        p->q_heads % p->kv_heads != 0 || p->q_heads / p->kv_heads > kMaxGroup || p->head_dim < 8 || p->head_dim > 128 ||
-        p->head_dim % 8 != 0 || (p->block != 32 && p->block != 64 && p->block != 128) ||
+        p->q_heads % p->kv_heads != 0 || p->q_heads / p->kv_heads > kMaxGroup ||
+        p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0 ||
+        (p->block != 32 && p->block != 64 && p->block != 128) ||
         p->count < 0 || (p->causal != 0 && p->causal != 1) || !std::isfinite(p->scale)) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
@@ -1176,21 +1204,40 @@ Backward<T> args_of(const nacho_block_attention_args &p, const Shape &s) {
 
 constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
 
+// Two column tiles per wavefront share what each reads of LDS, but are half as many workgroups
+// with twice the work. Us with two and with one, by tiles of 128 rows: heads of 128 192: 114
+// 72, 320: 112 112, 512: 116 123 and 107 103, 768: 171 163, 1024: 183 202, 2048: 308 361 and
+// 276 320; training steps 512: 253 240, 896: 425 434, 1024: 481 497; of heads of 96 512: 192
+// 178, 1024: 339 344. Heads of 64, whose registers leave room for more wavefronts with one:
+// 512: 81 57, 1024: 127 97, 2048: 158 145; training 1024: 322 276.
+constexpr int64_t kTwoColumns = 4 * kFullGrid;
+template <typename T, int DP>
+constexpr bool kMayShare = sizeof(T) == 2 && DP > 64;
+
+// Tiles of 16 rows up to which their kernel is faster than that of tiles of 64; us of the one
+// and the other by their number: bfloat16 heads of 128 256: 41 62, 512: 49 63, 544: 64 53, 640:
+// 79 64; float16 of 64 512: 27 37, 640: 33 38; float32 of 128 256: 81 211, 512: 152 219, 768:
+// 219 215, 1024: 288 226; of 64 768: 106 137. Where there are as many tiles of 64 as CUs
+// (single tokens of many sequences make as many of either) these are at least as fast: 64 x 4
+// tokens 93 with them, 100 with 16.
+template <typename T>
+constexpr int64_t kFewTiles = (sizeof(T) == 2 ? 2 : 3) * kFullGrid;
+
 // Calls f with the keys of a step, 64, or 32 where the block or float32's tiles (twice as large)
-// want it, and the column tiles of a wavefront: two share what each reads of LDS, one where that
-// leaves CUs without a workgroup.
-template <typename T, typename F>
+// want it (attention of 8192 queries of 32 heads of 128: 308 us with 64, 398 with 32), and the
+// column tiles of a wavefront.
+template <typename T, int DP, typename F>
 int with_tiles(const Shape &s, F f) {
     const int heads = s.batch * s.kv_heads;
     const int64_t large = static_cast<int64_t>(tiling(s, 128).per_head) * heads;
     auto columns = [&](auto keys) {
-        if (sizeof(T) == 2 && large >= kFullGrid) {
-            f(keys, std::integral_constant<int, sizeof(T) == 2 ? 2 : 1>{},
-              static_cast<unsigned>(large));
-        } else {
-            f(keys, std::integral_constant<int, 1>{},
-              static_cast<unsigned>(tiling(s, 64).per_head * heads));
+        if constexpr (kMayShare<T, DP>) {
+            if (large >= kTwoColumns) {
+                return f(keys, std::integral_constant<int, 2>{}, static_cast<unsigned>(large));
+            }
         }
+        f(keys, std::integral_constant<int, 1>{},
+          static_cast<unsigned>(tiling(s, 64).per_head * heads));
     };
     if constexpr (sizeof(T) == 2) {
         if (s.block % 64 == 0) {
@@ -1205,28 +1252,32 @@ int with_tiles(const Shape &s, F f) {
     return NACHO_OK;
 }
 
+// Training steps of 16 heads of 128, 4 key heads, in us by the target (384, 512, 768, 1024, 1536):
+// 2 x 4096 queries 543 524 481 494 491; 2 x 2048 (512, 768, 1024) 270 253 243; by the least (128,
+// 192, 256, 384): 2 x 1024 131 118 127 133, 1 x 1024 of half the heads 98 104 112 127.
 constexpr int64_t kItemTarget = 768;
-constexpr int64_t kItemLeast = 128;
+constexpr int64_t kItemLeast = 128;  // tokens
 
 template <typename T, int DP>
 int forward(Call &call, const Forward<T> &a) {
     const Shape &s = a.s;
     const hipStream_t stream = call.stream();
     const int heads = s.batch * s.kv_heads;
-    if (static_cast<int64_t>(tiling(s, 64).per_head) * heads >= kFullGrid) {
-        return with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
+    const Tiling small = tiling(s, 16);
+    const int64_t few = static_cast<int64_t>(small.per_head) * heads;
+    const int64_t tiles = static_cast<int64_t>(tiling(s, 64).per_head) * heads;
+    if (few > kFewTiles<T> || tiles >= kFullGrid) {
+        return with_tiles<T, DP>(s, [&](auto keys, auto columns, unsigned grid) {
             tile_kernel<T, DP, keys(), columns()><<<grid, kThreads, 0, stream>>>(a);
         });
     }
-    // Fewer tiles than CUs: tiles of 16 rows, whose wavefronts share the steps.  What a step waits
+    // Few rows: tiles of 16 of them, whose wavefronts share the steps.  What a step waits
     // for is its operands (2 to 3 us from memory that nothing read lately), so there are as many
     // workgroups as find a CU, down to less than a step for each wavefront; past 16 splits the
     // join costs more than they save, and up to 8 steps one split is done before it would begin.
     // One query of 32 heads of 128, in us by splits (1, 2, 4, 8, 16, 32): over 4 blocks of 64
     // 8.6 10.3 11.1 10.1 10.9 12.6, over 16 blocks 18 15 13 10.8 11.8 13, over 64 blocks
     // 64 40 27 18.4 16.1 16.8; 16 sequences over 16 blocks 23.2 20.8 21.4 24.7 38 66.
-    const Tiling small = tiling(s, 16);
-    const int64_t few = static_cast<int64_t>(small.per_head) * heads;
     const int64_t listed =
         static_cast<int64_t>(small.tokens < s.queries ? small.tokens : s.queries) * s.count;
     const int64_t steps = (listed < s.blocks ? listed : s.blocks) * (s.block / kSplitKeys);
@@ -1242,22 +1293,15 @@ int forward(Call &call, const Forward<T> &a) {
         part.ml = part.o + rows * DP;
     }
     const unsigned grid = static_cast<unsigned>(few * splits);
-    auto launch = [&](auto ahead, auto one) {
-        split_kernel<T, DP, ahead(), one()>
-            <<<grid, kThreads, 0, stream>>>(a, static_cast<int>(splits), part);
-    };
-    constexpr std::integral_constant<int, sizeof(T) == 2 ? 2 : 1> two;
-    constexpr std::integral_constant<int, 1> one;
-    const bool token = (small.tokens == 1 || s.queries == 1) && s.count <= dev::kWave;
-    if (grid <= kFullGrid) {
-        token ? launch(two, std::true_type{}) : launch(two, std::false_type{});
+    const int n = static_cast<int>(splits);
+    if ((small.tokens == 1 || s.queries == 1) && s.count <= dev::kWave) {
+        split_kernel<T, DP, true><<<grid, kThreads, 0, stream>>>(a, n, part);
     } else {
-        token ? launch(one, std::true_type{}) : launch(one, std::false_type{});
+        split_kernel<T, DP, false><<<grid, kThreads, 0, stream>>>(a, n, part);
     }
     NACHO_TRY_HIP(hipGetLastError());
     if (splits > 1) {
-        join_kernel<T, DP><<<static_cast<unsigned>(few * 16), DP, 0, stream>>>(
-            a, static_cast<int>(splits), part);
+        join_kernel<T, DP><<<static_cast<unsigned>(few * 16), DP, 0, stream>>>(a, n, part);
         NACHO_TRY_HIP(hipGetLastError());
     }
     return NACHO_OK;
@@ -1304,12 +1348,13 @@ int backward(Call &call, const Backward<T> &a) {
     items.bits = bits;
     items.start = start;
     if (queries > 0) {
-        NACHO_TRY(with_tiles<T>(s, [&](auto keys, auto columns, unsigned grid) {
-            // (two column tiles of 96 or 128 leave registers for 32 keys of q . k and dout . v)
-            constexpr int kKeys = DP > 64 && columns() == 2 ? 32 : keys();
+        const int launched = with_tiles<T, DP>(s, [&](auto keys, auto columns, unsigned grid) {
+            // (two column tiles leave registers for 32 keys of q . k and dout . v)
+            constexpr int kKeys = columns() == 2 ? 32 : keys();
             dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(
                 a, delta, items.rows, counts);
-        }));
+        });
+        NACHO_TRY(launched);
     }
     if (items.rows == 0) return NACHO_OK;
     if (queries > 0) {
@@ -1321,8 +1366,8 @@ int backward(Call &call, const Backward<T> &a) {
                                                 queries > 0 ? counts : nullptr, start);
     NACHO_TRY_HIP(hipGetLastError());
     const unsigned grid = static_cast<unsigned>((most * parts + 7) / 8 * 8);
-    const unsigned inverse =
-        s.group == 1 ? 0u : static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(s.group)) + 1u;
+    const unsigned group = static_cast<unsigned>(s.group);
+    const unsigned inverse = group == 1 ? 0u : static_cast<unsigned>((1ull << 32) / group) + 1u;
     if (!wide) {
         dkv_kernel<T, DP, 1, 2><<<grid, kThreads, 0, stream>>>(a, delta, items, inverse);
     } else if constexpr (sizeof(T) == 2) {

@@ -2,21 +2,27 @@
 // the means, and the blocks of the highest scores.
 //
 // means: bound by reading k once.  A workgroup per (sequence, block, head): 16 lanes read a key
-// (16 bytes or 32 each), 16 keys at a time; float32 sums.
+// (16 bytes or 32 each), 16 keys at a time; float32 sums.  8192 keys of 8 heads of 128 in bfloat16
+// (17 MB): 5 us, a launch and 3 us of reads.
 //
-// scores: scale (sum of the group's heads of q) . mean, in float32 throughout: they are compared
-// with each other, and the product is small (one row per group and one column per block of keys),
-// so it runs on the float32 matrix instruction.  A workgroup sums 64 queries' heads into LDS and
-// goes over the blocks 64 at a time, 16 to a wavefront.
+// scores: scale (sum of the group's heads of q) . mean, in float32 throughout: they are
+// compared with each other, and the product is small (one row per group and one column per
+// block of keys), so it runs on the float32 matrix instruction. A workgroup sums 16 queries'
+// heads into LDS and goes over the blocks 64 at a time, 16 to a wavefront. 8192 queries of 32
+// heads of 128 against 128 blocks: 30 us, where reading q and writing the scores would take 18.
+// 48 sequences' tokens against 512 blocks each (101 MB of means): 16 us, a copy's rate; 32 or
+// 64 queries to a workgroup are no faster for many queries and 1.3 us slower there.
 //
-// select: a wavefront per query and key head.  Scores become unsigned numbers of the same order,
-// and the count-th largest is found bit by bit with ballots; no sort, and ties are counted off
-// from the lowest id.
+// select: a wavefront per query and key head. Scores become unsigned numbers of the same order,
+// and a threshold that the wanted number of them reaches is found with ballots: no sort, and
+// ties are counted off from the lowest id. 65,536 rows of 128 blocks: 28 us, bound by
+// instructions, about ten counts a row; reading the scores would take 7.
 #include <hip/hip_runtime.h>
 
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 #include <new>
 
 #include "dense_tiles.hpp"
@@ -49,7 +55,8 @@ __global__ __launch_bounds__(kThreads) void means_kernel(MeansArgs a, const T *_
     const int h = static_cast<int>(blockIdx.x % a.heads);
     const int64_t bj = blockIdx.x / a.heads;
     const int j = static_cast<int>(bj % a.blocks), b = static_cast<int>(bj / a.blocks);
-    const int piece = static_cast<int>(threadIdx.x) % 16, slice = static_cast<int>(threadIdx.x) / 16;
+    const int thread = static_cast<int>(threadIdx.x);
+    const int piece = thread % 16, slice = thread / 16;
     const int first = j * a.block;
     const int there = min(max(length_of(a.lengths, b, a.keys) - first, 0), a.block);
     float sum[8] = {};
@@ -84,7 +91,7 @@ struct ScoresArgs {
     const float *means;
     const int *lengths;
     float *scores;
-    int tiles;     // of 64 queries
+    int tiles;     // of TOKENS queries
     int per_part;  // steps of 64 blocks that a workgroup takes
 };
 
@@ -137,11 +144,8 @@ __global__ __launch_bounds__(kThreads) void scores_kernel(ScoresArgs a, const T 
         for (int t = 0; t < TOKENS / 16; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (static_cast<int64_t>(64 * step + 16 * wave) * a.block <= last) {  // uniform
             f32x8 m[DP / 32];
-            const float *p = j < a.blocks
-                                 ? a.means + ((static_cast<int64_t>(b) * a.blocks + j) * a.heads + h) *
-                                                 a.dim
-                                 : nullptr;
-            load_row_frags<float, DP>(p, a.dim, g, m);
+            const int64_t row = (static_cast<int64_t>(b) * a.blocks + j) * a.heads + h;
+            load_row_frags<float, DP>(j < a.blocks ? a.means + row * a.dim : nullptr, a.dim, g, m);
 #pragma unroll
             for (int t = 0; t < TOKENS / 16; ++t) {
                 if (t < row_tiles) {
@@ -300,31 +304,25 @@ __device__ __forceinline__ void select_row(const SelectArgs &a, unsigned row32, 
     for (int i = at + lane; i < a.count; i += dev::kWave) ids[i] = -1;
 }
 
-// NR registers a lane hold a row (64 NR blocks); NR = 0 reads it again each time.  A wavefront
-// has ROWS rows: many rows of few blocks are otherwise bound by the start of wavefronts (65,536
-// rows of 128 blocks: 29 us with one each).
-template <int NR, int ROWS>
+// A wavefront per row (four rows each, so that their loads are on the way together, took 30 us
+// instead of 28 for 65,536 rows of 128 blocks). NR registers a lane hold a row of 64 NR blocks;
+// NR = 0, for longer ones, reads it again each time. Empty registers cost as much as full ones:
+// 32,768 rows of 64 blocks 13 us with one, 15 with two, 19 with four, 26 with eight; 384 rows
+// of 1024 blocks 8 with 16, 14 with 32, 53 with none.
+template <int NR>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
     // (a wavefront's number in scalar registers: the divisions are a few scalar instructions)
-    const unsigned first = ROWS * __builtin_amdgcn_readfirstlane(
+    const unsigned row = __builtin_amdgcn_readfirstlane(
         blockIdx.x * (kThreads / dev::kWave) + threadIdx.x / dev::kWave);
-    const unsigned rows = static_cast<unsigned>(a.rows);
-    float held[ROWS][NR ? NR : 1];
+    if (row >= static_cast<unsigned>(a.rows)) return;
+    const float *scores = a.scores + static_cast<int64_t>(row) * a.blocks;
+    float held[NR ? NR : 1];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {  // all loads at once
-        const float *scores = a.scores + static_cast<int64_t>(first + i) * a.blocks;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int j = r * dev::kWave + dev::lane();
-            held[i][r] = first + i < rows && j < a.blocks ? scores[j] : kNegInf;
-        }
+    for (int r = 0; r < NR; ++r) {
+        const int j = r * dev::kWave + dev::lane();
+        held[r] = j < a.blocks ? scores[j] : kNegInf;
     }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        if (first + i >= rows) return;
-        select_row<NR>(a, first + i, a.scores + static_cast<int64_t>(first + i) * a.blocks,
-                       held[i]);
-    }
+    select_row<NR>(a, row, scores, held);
 }
 
 // ---- host -----------------------------------------------------------------------------
@@ -406,8 +404,10 @@ int scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys, int32_t 
     const int64_t groups = tiles * batch * kv_heads;
     const int64_t steps = (blocks + 63) / 64;
     if (groups * steps > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
-    // enough workgroups for every CU to have two, while each sums its queries' heads once
-    int64_t parts = (512 + groups - 1) / groups;
+    // Enough workgroups for every CU to have four, while each sums its queries' heads once.  48
+    // tokens of 8 key heads against 512 blocks, in us by the workgroups aimed at (256, 512, 1024,
+    // 2048): 21.3 17.9 16.2 17.7.
+    int64_t parts = (1024 + groups - 1) / groups;
     if (parts > steps) parts = steps;
     const int64_t per_part = (steps + parts - 1) / parts;
     const ScoresArgs a{queries,
@@ -436,8 +436,6 @@ int scores(int32_t dtype, int32_t batch, int32_t queries, int32_t keys, int32_t 
     }
 }
 
-constexpr int64_t kManyRows = 16384;  // of which one to a wavefront is two rounds of the device
-
 int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t block,
            int32_t count, int32_t sink, int32_t local, int32_t causal, const float *score,
            const int32_t *lengths, int32_t *ids, void *stream) {
@@ -457,16 +455,21 @@ int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t 
                        local, causal,  score, lengths, ids};
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned n = static_cast<unsigned>(grid);
-    if (blocks <= 2 * dev::kWave && rows >= kManyRows) {
-        select_kernel<2, 4><<<(n + 3) / 4, kThreads, 0, s>>>(a);
+    auto launch = [&](auto nr) { select_kernel<nr()><<<n, kThreads, 0, s>>>(a); };
+    if (blocks <= dev::kWave) {
+        launch(std::integral_constant<int, 1>{});
     } else if (blocks <= 2 * dev::kWave) {
-        select_kernel<2, 1><<<n, kThreads, 0, s>>>(a);
+        launch(std::integral_constant<int, 2>{});
+    } else if (blocks <= 4 * dev::kWave) {
+        launch(std::integral_constant<int, 4>{});
     } else if (blocks <= 8 * dev::kWave) {
-        select_kernel<8, 1><<<n, kThreads, 0, s>>>(a);
+        launch(std::integral_constant<int, 8>{});
+    } else if (blocks <= 16 * dev::kWave) {
+        launch(std::integral_constant<int, 16>{});
     } else if (blocks <= 32 * dev::kWave) {
-        select_kernel<32, 1><<<n, kThreads, 0, s>>>(a);
+        launch(std::integral_constant<int, 32>{});
     } else {
-        select_kernel<0, 1><<<n, kThreads, 0, s>>>(a);
+        launch(std::integral_constant<int, 0>{});
     }
     NACHO_TRY_HIP(hipGetLastError());
     return NACHO_OK;

@@ -434,3 +434,40 @@ def test_refusals(gpu):
         nacho_amd.gpu_block_select(torch.zeros(1, 1, 1, 3, device=gpu), 2, 32, 32)
     with pytest.raises(ValueError, match="count"):
         nacho_amd.gpu_block_select(torch.zeros(1, 1, 1, 1, device=gpu), -2, 32, 32)
+
+
+# 1024 tiles of 128 rows: a wavefront has two column tiles (heads of more than 64, 16 bits).
+WIDE = [(8, 70, 200, 128, 64, 128, 64, 2), (8, 65, 140, 128, 64, 96, 32, 3)]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+@pytest.mark.parametrize("sizes", WIDE, ids=str)
+def test_two_column_tiles(gpu, sizes, dtype):
+    _check(gpu, *_operands(21, dtype, *sizes), sizes[6])
+
+
+def test_two_column_tiles_of_ragged_lengths(gpu):
+    q, k, v, ids, dout = _operands(22, torch.bfloat16, *WIDE[0])
+    ids[:, ::3] = -1
+    lengths = torch.tensor([0, 1, 69, 70, 71, 128, 199, 200], dtype=torch.int32)
+    for b, length in enumerate(lengths.tolist()):
+        k[b, length:], v[b, length:] = float("nan"), float("inf")
+    _check(gpu, q, k, v, ids, dout, 64, lengths)
+
+
+def test_two_column_tiles_and_not_finite_values(gpu):
+    test_not_finite_in_masked_places(gpu, (16, 40, 200, 128, 32, 72, 64, 2), torch.bfloat16)
+
+
+@pytest.mark.parametrize("blocks", (3, 64, 65, 129, 256, 300, 513, 1030, 2048, 2060))
+def test_select_of_any_width(gpu, blocks):
+    """A row's scores are held in 1 to 32 registers of a wavefront, or read again: every form."""
+    g = torch.Generator().manual_seed(blocks)
+    keys, count = 32 * blocks - 5, 40
+    score = torch.randn(2, 3, 2, blocks, generator=g)
+    score[1] = (score[1] * 2).round()  # many equal ones
+    score[:, 1, :, ::3] = -math.inf
+    lengths = torch.tensor([keys, max(3, keys // 2)], dtype=torch.int32)
+    want = ref.select(score, count, 32, keys, lengths)
+    got = nacho_amd.gpu_block_select(score.to(gpu), count, 32, keys, lengths.to(gpu))
+    assert torch.equal(got.cpu(), want)

@@ -762,14 +762,15 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
     }
 }
 
-// dq, and delta and zeroed counts for the launches that follow.  Three products to the forward
-// pass's two, and 32 keys a step where two column tiles of q and dout fill the registers.
-// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 172 us, 68 GFLOP that are asked for and
-// 1.6 times that with the union's.
+// dq, and delta and zeroed counts for the launches that follow.  32 keys a step where two column
+// tiles of q and dout fill the registers.
 //
-// ds is rounded to the operands' type for its product, and delta is of the rounded out: with
-// bfloat16 and keys that lean one way these put dq 0.0018 and 0.0006 off, the final rounding
-// 0.0017, relative to its norm.
+// ds is rounded to the operands' type for its product, and what that takes is a second product with
+// the same columns (16-bit types): dq then is 0.0019 of its norm off with bfloat16 instead of
+// 0.0026, where its own rounding makes 0.0017 and delta, which is of the rounded out, 0.0006.
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 199 us (172 without the second product), 68
+// GFLOP that are asked for and 1.6 times that with the union's.  Matrix products 38%, vector unit
+// 41% of a CU's time.
 template <typename T, int DP, int BN, int COLS>
 __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *__restrict__ delta,
                                                          int64_t rows_of_blocks,
@@ -838,7 +839,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
                 score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x],
                                         pass != kPlain);
             }
-            column_products<Lds, T, DP, COLS, BN / 16>(s_k, dp, g, c, o);
+            column_products<Lds, T, DP, COLS, BN / 16, sizeof(T) == 2>(s_k, dp, g, c, o);
         });
         float wrong = 0.0f;
 #pragma unroll

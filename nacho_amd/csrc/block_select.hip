@@ -22,8 +22,8 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
-#include <type_traits>
 #include <new>
+#include <type_traits>
 
 #include "dense_tiles.hpp"
 #include "runtime.hpp"

@@ -292,20 +292,34 @@ __device__ __forceinline__ void row_products(const T *tile, const Frag<T> (&oper
     }
 }
 
-// sums[x] += the tile's columns times p[x], the products' rows rounded to T.
-template <typename Lds, typename T, int DP, int COLS, int N>
+// sums[x] += the tile's columns times p[x], the products' rows rounded to T; with REST what the
+// rounding took is a second product with the same columns.
+template <typename Lds, typename T, int DP, int COLS, int N, bool REST = false>
 __device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[COLS][N], int g,
                                                 int c, f32x4 (&sums)[COLS][DP / 16]) {
 #pragma unroll
     for (int u = 0; u < N / 2; ++u) {
-        Frag<T> f[COLS];
+        Frag<T> f[COLS], rest[COLS];
 #pragma unroll
-        for (int x = 0; x < COLS; ++x) f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
+        for (int x = 0; x < COLS; ++x) {
+            f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
+            if constexpr (REST) {
+                f32x4 low[2];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    low[i / 4][i % 4] = p[x][2 * u + i / 4][i % 4] - static_cast<float>(f[x][i]);
+                }
+                rest[x] = result_frag<T>(low[0], low[1]);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
             const Frag<T> v = Lds::column(tile, u, i, g, c);
 #pragma unroll
-            for (int x = 0; x < COLS; ++x) sums[x][i] = mma(v, f[x], sums[x][i]);
+            for (int x = 0; x < COLS; ++x) {
+                sums[x][i] = mma(v, f[x], sums[x][i]);
+                if constexpr (REST) sums[x][i] = mma(v, rest[x], sums[x][i]);
+            }
         }
     }
 }

@@ -878,9 +878,9 @@ struct Items {
 // 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 203 us for 90 GFLOP (rows that did not
 // select the block take no part); with one workgroup per block instead of items 1146 us.  LDS is
 // the bound, 45% of a CU's time and waits for it: a wavefront's 16 keys use each fragment once.
-// Two column tiles use it twice; for heads of 64 training steps take 247 us with them and 280
-// without, for 128 they leave one wavefront to a SIMD and the kernel takes 276 us.  32 keys to a
-// workgroup instead of 64: training steps 506 us instead of 481, heads of 64 267 instead of 247.
+// Two column tiles use it twice: for heads of 64 training steps are 32 us of 330 shorter with them;
+// for 128 they leave one wavefront to a SIMD, and the kernel takes 276 us.  32 keys to a workgroup
+// instead of 64: training steps 531 us instead of 507, heads of 64 317 instead of 298.
 template <typename T, int DP, int COLS, int LANES>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
     Backward<T> a, const float *__restrict__ delta, Items items, unsigned group_inverse) {
@@ -1206,11 +1206,11 @@ Backward<T> args_of(const nacho_block_attention_args &p, const Shape &s) {
 constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
 
 // Two column tiles per wavefront share what each reads of LDS, but are half as many workgroups
-// with twice the work. Us with two and with one, by tiles of 128 rows: heads of 128 192: 114
-// 72, 320: 112 112, 512: 116 123 and 107 103, 768: 171 163, 1024: 183 202, 2048: 308 361 and
-// 276 320; training steps 512: 253 240, 896: 425 434, 1024: 481 497; of heads of 96 512: 192
-// 178, 1024: 339 344. Heads of 64, whose registers leave room for more wavefronts with one:
-// 512: 81 57, 1024: 127 97, 2048: 158 145; training 1024: 322 276.
+// with twice the work.  us with two and with one, by tiles of 128 rows; attention of heads of 128:
+// 192: 114 72, 320: 112 112, 512: 116 123 and 107 103, 768: 171 163, 1024: 183 202, 2048: 308 361
+// and 276 320; its training steps: 512: 265 249, 896: 450 450, 1024: 508 516, 2048: 1113 1161; of
+// heads of 96: 512: 200 184, 1024: 359 359.  Heads of 64, whose registers leave room for more
+// wavefronts with one: 512: 81 57, 1024: 127 97, 2048: 158 145; training 1024: 331 288.
 constexpr int64_t kTwoColumns = 4 * kFullGrid;
 template <typename T, int DP>
 constexpr bool kMayShare = sizeof(T) == 2 && DP > 64;
@@ -1254,10 +1254,10 @@ int with_tiles(const Shape &s, F f) {
 }
 
 // Training steps of 16 heads of 128, 4 key heads, in us by the target (384, 512, 768, 1024, 1536):
-// 2 x 4096 queries 543 524 481 494 491; 2 x 2048 (512, 768, 1024) 270 253 243; by the least (128,
-// 192, 256, 384): 2 x 1024 131 118 127 133, 1 x 1024 of half the heads 98 104 112 127.
+// 2 x 4096 queries 570 550 507 520 518; 2 x 2048 (512, 768, 1024) 265 249 239; by the least (128,
+// 192, 256, 384): 2 x 1024 134 121 130 136, 1 x 1024 of half the heads 107 107 115 131.
 constexpr int64_t kItemTarget = 768;
-constexpr int64_t kItemLeast = 128;  // tokens
+constexpr int64_t kItemLeast = 192;  // tokens
 
 template <typename T, int DP>
 int forward(Call &call, const Forward<T> &a) {

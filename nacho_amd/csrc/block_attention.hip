@@ -239,7 +239,7 @@ struct KeySteps {
                 Lds::load(to_v, threadIdx.x, v_source, v_base + key * a.v.row_stride, there);
             };
             auto arrived = [&](T *tile_of) {
-                __syncthreads();
+                rows_arrived();
                 if (pass != kPlain) {  // uniform
                     Lds::make_finite(tile_of, threadIdx.x, pass == kMarks);
                     __syncthreads();
@@ -494,6 +494,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
     int pass = kPlain;
     const float scale2 = base2_scale(s.scale);
     const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
+    // Keys that some row sees; past them zeros are read.  (Not the sequence's end: a later
+    // token's keys may lie in the last one's block, and with ONE nothing else masks values.)
     const int end = tile.last_key(s, tile.tokens - 1) + 1;
     const int shift = s.block == 32 ? 0 : s.block == 64 ? 1 : 2;  // steps of a block
     const int stride = splits * kWaves;
@@ -510,11 +512,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r = key + 16 * t + c;
-                load_row_frags<T, DP>(r < tile.length ? k_base + r * a.k.row_stride : nullptr,
-                                      s.dim, g, k_next[t]);
+                load_row_frags<T, DP>(r < end ? k_base + r * a.k.row_stride : nullptr, s.dim, g,
+                                      k_next[t]);
             }
             v_next.load(lane, s.dim, [&](int r) -> const T * {
-                return key + r < tile.length ? v_base + (key + r) * a.v.row_stride : nullptr;
+                return key + r < end ? v_base + (key + r) * a.v.row_stride : nullptr;
             });
         };
         const int from = split * kWaves + wave;
@@ -1049,7 +1051,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
         }
         __syncthreads();
         load(0, s_q0, s_do0);
-        __syncthreads();
+        rows_arrived();
         // (A last step without rows takes probabilities of 0: a branch around it costs a second
         // copy of the sums' registers.)
         const int steps = (rows + kStep - 1) / kStep;
@@ -1058,12 +1060,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
             if (informs) begin(step + 2);
             use(s_q0, s_do0, step);
             if (informs) end(step + 2);
-            __syncthreads();
+            rows_arrived();
             load(step + 2, s_q0, s_do0);
             if (informs) begin(step + 3);
             use(s_q1, s_do1, step + 1);
             if (informs) end(step + 3);
-            __syncthreads();
+            rows_arrived();
         }
     }
     if constexpr (kSets == 2) {

@@ -109,6 +109,13 @@ __device__ __forceinline__ u32x4 finite_piece(u32x4 bits, bool marks) {
     return __builtin_bit_cast(u32x4, v);
 }
 
+// A barrier after which every wavefront's loads from memory to LDS are complete.  (Each waits for
+// its own: a barrier alone orders accesses to LDS, and these loads count as memory's.)
+__device__ __forceinline__ void rows_arrived() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+}
+
 // Rows in LDS, filled straight from memory: a wavefront's load names a source per
 // lane and writes 64 consecutive 16-byte pieces.  Rows are not padded (they cannot be); instead
 // piece p of row r lies at place p ^ swizzle(r), which the loads' sources take care of, so that
@@ -136,7 +143,7 @@ struct Tile {
 
     // row_of(r): row r of the source, r < ROWS; every one has to be there (rows that are masked
     // name another's).  Pieces at or past column D repeat the row's first.  Complete after the
-    // next __syncthreads.
+    // next rows_arrived.
     template <typename RowOf>
     __device__ __forceinline__ static void load(T *tile, int thread, int D, RowOf row_of) {
         using Global = const __attribute__((address_space(1))) void *;

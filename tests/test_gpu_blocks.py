@@ -471,3 +471,30 @@ def test_select_of_any_width(gpu, blocks):
     want = ref.select(score, count, 32, keys, lengths)
     got = nacho_amd.gpu_block_select(score.to(gpu), count, 32, keys, lengths.to(gpu))
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [(1, 3, 200, 16, 1, 72, 64, 1), (2, 4, 2100, 32, 2, 128, 64, 9),
+                                   (1, 2, 130, 20, 1, 64, 32, 2), (2, 4, 95, 4, 2, 64, 32, 2)],
+                         ids=str)
+def test_later_keys_of_the_own_block(gpu, sizes, dtype):
+    """A few new tokens: the last one's key and value, which lie in the block of those before it,
+    reach none of these, also where a tile of rows is the heads of one token."""
+    q, k, v, ids, dout = _operands(31, dtype, *sizes)
+    queries, keys, block = sizes[1], sizes[2], sizes[6]
+    ids[..., 0] = (keys - 1) // block
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[:, -1], bad_v[:, -1] = math.nan, math.inf
+    k[:, -1], v[:, -1] = 0.0, 0.0
+    want = ref.Attention(q, k, v, ids, block, dout=dout)
+    dev = [x.to(gpu).requires_grad_() for x in (q, bad_k, bad_v)]
+    out, lse = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), block, return_lse=True)
+    dq, = torch.autograd.grad(out, dev[:1], dout.to(gpu))
+    before = (torch.arange(queries) < queries - 1)[None, :, None]
+    none = torch.zeros((), dtype=torch.float64)
+    for got, name in ((out, "out"), (lse, "lse"), (dq, "dq")):
+        where = before.expand(lse.shape) if name == "lse" else before[..., None].expand(q.shape)
+        ref.near(torch.where(where, got.detach().cpu().double(), none),
+                 torch.where(where, getattr(want, name), none), getattr(want, name + "_off"),
+                 name)
+    assert not torch.isfinite(out[:, -1]).any()

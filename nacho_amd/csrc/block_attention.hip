@@ -10,8 +10,12 @@
 //
 // Products are transposed: S^T = K Q^T puts a row's keys into the four lanes of its column, so
 // the row's maximum is two lane exchanges, and P^T already lies as the operand of
-// O^T = V^T P^T (dense_tiles.hpp).  Probabilities are rounded to the operands' type for that
-// product, as its operand has to be; their sum l is of the unrounded ones in float32.
+// O^T = V^T P^T (dense_tiles.hpp).  An operand of a product has to have the rows' type.  Where a
+// sequence has few rows, bound by their keys' bytes, 16-bit types take a probability in two parts,
+// so that out is what rounding it once makes it: 0.0017 of its norm off with bfloat16, 0.0002 with
+// float16.  Where it has many, bound by products, one rounded part is taken: out is 0.0021 and
+// 0.00026 off for two thirds of the time (kPartsRows).  The sum l is of the unrounded ones in
+// float32 either way.
 //
 // Backward, with delta = dout . out and p from the stored lse: ds = p (dout . v - delta),
 // dq = scale ds K goes tile by tile as the forward pass; dk = scale ds^T Q and dv = p^T dout go
@@ -323,6 +327,12 @@ __device__ __forceinline__ int step_limit(bool selected, int last_key, int first
     return selected ? last_key + 1 - first_key - 4 * g : 0;
 }
 
+// What a row's sum of p v is to be multiplied by: `sum` is that of p.
+template <typename T, bool PARTS>
+__device__ __forceinline__ float row_factor(float sum) {
+    return sum > 0.0f ? (PARTS ? kPartsScale<T> : 1.0f) / sum : sum == 0.0f ? 0.0f : sum;
+}
+
 // A lane's rows of a tile: COLS of them, 16 apart.
 template <int COLS>
 struct LaneRows {
@@ -363,7 +373,7 @@ struct LaneRows {
 // keys, with the same heads and blocks: 50 us for 270 MB, 5.4 TB/s, near a large copy's 5.7.
 // Three sequences of up to 777 queries of 12 heads of 80 in float32, 9 blocks of 32: 55 to 70 us
 // by their lengths, half of it float32 matrix products.
-template <typename T, int DP, int BN, int COLS>
+template <typename T, int DP, int BN, int COLS, bool PARTS>
 __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
     using Lds = Tile<T, DP, BN, kThreads>;
     constexpr int kRowsOf = 64 * COLS;
@@ -412,7 +422,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
                     for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
                 }
             }
-            column_products<Lds, T, DP, COLS, BN / 16>(s_v, p, g, c, o);
+            column_products<Lds, T, DP, COLS, BN / 16, PARTS>(s_v, p, g, c, o);
         });
         float wrong = 0.0f;
 #pragma unroll
@@ -420,7 +430,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
             wrong += not_finite<DP / 16>(o[x]) + l[x] * 0.0f;
             const float sum = column_sum(l[x]);
             if (!rows.exists[x]) continue;
-            const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            const float inverse = row_factor<T, PARTS>(sum);
             const int t = tile.t0 + rows.token[x], head = rows.head[x];
             T *out = a.out.row(tile.b, t, head);
 #pragma unroll
@@ -544,7 +554,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
             }
-            column_products<typename Stage::Lds, T, DP, 1, 2>(s_v, p, g, c, o);
+            column_products<typename Stage::Lds, T, DP, 1, 2, true>(s_v, p, g, c, o);
         }
     };
     for (;; ++pass) {  // uniform
@@ -624,7 +634,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
                 }
                 continue;
             }
-            const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+            const float inverse = row_factor<T, true>(sum);
             T *out = a.out.row(tile.b, tile.t0 + t, hd) + col;
             if (col < s.dim && pass == kPlain) *out = static_cast<T>(v * inverse);
             if (col < s.dim && pass != kPlain) store_again(out, v * inverse, pass);
@@ -660,7 +670,7 @@ __global__ __launch_bounds__(DP) void join_kernel(Forward<T> a, int splits, Part
         sum += f * part.ml[2 * x + 1];
         v += f * part.o[x * DP + col];
     }
-    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    const float inverse = row_factor<T, true>(sum);
     if (col < s.dim) a.out.row(tile.b, tile.t0 + t, hd)[col] = static_cast<T>(v * inverse);
     if (col == 0 && a.lse) {
         a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + t) * s.q_heads + hd] =
@@ -767,9 +777,9 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
 // dq, and delta and zeroed counts for the launches that follow.  32 keys a step where two column
 // tiles of q and dout fill the registers.
 //
-// ds is rounded to the operands' type for its product, and what that takes is a second product with
-// the same columns (16-bit types): dq then is 0.0019 of its norm off with bfloat16 instead of
-// 0.0026, where its own rounding makes 0.0017 and delta, which is of the rounded out, 0.0006.
+// ds is in two parts of the operands' type for its product (16-bit types): dq then is 0.0019 of its
+// norm off with bfloat16 instead of 0.0026, where its own rounding makes 0.0017 and delta, which is
+// of the rounded out, 0.0006.
 // 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 199 us (172 without the second product), 68
 // GFLOP that are asked for and 1.6 times that with the union's.  Matrix products 38%, vector unit
 // 41% of a CU's time.
@@ -841,7 +851,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
                 score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x],
                                         pass != kPlain);
             }
-            column_products<Lds, T, DP, COLS, BN / 16, sizeof(T) == 2>(s_k, dp, g, c, o);
+            column_products<Lds, T, DP, COLS, BN / 16, true>(s_k, dp, g, c, o);
         });
         float wrong = 0.0f;
 #pragma unroll
@@ -852,7 +862,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const int col = 16 * i + 4 * g;
-                if (col < s.dim) store4<T>(dq + col, o[x][i] * s.scale);
+                if (col < s.dim) store4<T>(dq + col, o[x][i] * (s.scale * kPartsScale<T>));
             }
         }
         if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;
@@ -1039,8 +1049,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
                 }
             }
         }
-        column_products<Lds, T, DP, COLS, kN>(my_do, p, g, c, dv);
-        column_products<Lds, T, DP, COLS, kN>(my_q, dp, g, c, dk);
+        column_products<Lds, T, DP, COLS, kN, false>(my_do, p, g, c, dv);
+        column_products<Lds, T, DP, COLS, kN, false>(my_q, dp, g, c, dk);
     };
     if (rows > 0) {  // uniform
         if (informs) {
@@ -1226,16 +1236,22 @@ constexpr bool kMayShare = sizeof(T) == 2 && DP > 64;
 template <typename T>
 constexpr int64_t kFewTiles = (sizeof(T) == 2 ? 2 : 3) * kFullGrid;
 
+// A sequence's rows up to which a probability reaches its product in two parts of the operands' type:
+// one tile then has all of a key head's rows, and its keys' bytes take longer than their products.
+// 64 single tokens of 32 heads of 128: 51.1 us either way; 8192 queries: 307 us with one part, 416
+// with two.
+constexpr int64_t kPartsRows = 64;
+
 // Calls f with the keys of a step, 64, or 32 where the block or float32's tiles (twice as large)
 // want it (attention of 8192 queries of 32 heads of 128: 308 us with 64, 398 with 32), and the
-// column tiles of a wavefront.
+// column tiles of a wavefront (`one_column`: one, however many tiles there are).
 template <typename T, int DP, typename F>
-int with_tiles(const Shape &s, F f) {
+int with_tiles(const Shape &s, bool one_column, F f) {
     const int heads = s.batch * s.kv_heads;
     const int64_t large = static_cast<int64_t>(tiling(s, 128).per_head) * heads;
     auto columns = [&](auto keys) {
         if constexpr (kMayShare<T, DP>) {
-            if (large >= kTwoColumns) {
+            if (!one_column && large >= kTwoColumns) {
                 return f(keys, std::integral_constant<int, 2>{}, static_cast<unsigned>(large));
             }
         }
@@ -1270,8 +1286,15 @@ int forward(Call &call, const Forward<T> &a) {
     const int64_t few = static_cast<int64_t>(small.per_head) * heads;
     const int64_t tiles = static_cast<int64_t>(tiling(s, 64).per_head) * heads;
     if (few > kFewTiles<T> || tiles >= kFullGrid) {
-        return with_tiles<T, DP>(s, [&](auto keys, auto columns, unsigned grid) {
-            tile_kernel<T, DP, keys(), columns()><<<grid, kThreads, 0, stream>>>(a);
+        const bool parts = sizeof(T) == 2 && static_cast<int64_t>(s.queries) * s.group <= kPartsRows;
+        return with_tiles<T, DP>(s, parts, [&](auto keys, auto columns, unsigned grid) {
+            if constexpr (sizeof(T) == 2 && columns() == 1) {
+                if (parts) {
+                    tile_kernel<T, DP, keys(), 1, true><<<grid, kThreads, 0, stream>>>(a);
+                    return;
+                }
+            }
+            tile_kernel<T, DP, keys(), columns(), false><<<grid, kThreads, 0, stream>>>(a);
         });
     }
     // Few rows: tiles of 16 of them, whose wavefronts share the steps.  What a step waits
@@ -1351,7 +1374,7 @@ int backward(Call &call, const Backward<T> &a) {
     items.bits = bits;
     items.start = start;
     if (queries > 0) {
-        const int launched = with_tiles<T, DP>(s, [&](auto keys, auto columns, unsigned grid) {
+        const int launched = with_tiles<T, DP>(s, false, [&](auto keys, auto columns, unsigned grid) {
             // (two column tiles leave registers for 32 keys of q . k and dout . v)
             constexpr int kKeys = columns() == 2 ? 32 : keys();
             dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(

@@ -76,6 +76,42 @@ __device__ __forceinline__ Frag<T> result_frag(f32x4 lo, f32x4 hi) {
     return f;
 }
 
+// Two results of a product as an operand in two parts of T, a 16-bit type, that together hold what
+// one would round away: `head` is x cut off toward 0, `rest` what is left of (1 + 2^-12) x.  The
+// part of 2^-12, which kPartsScale undoes in the sums, gives the rest x's sign and keeps it from
+// being 0 where x is not, so that the products of both with an infinity are the same infinity.
+// (float16: for an x of 2^-12 or more; below, the rest may be 0.)
+template <typename T>
+__device__ __forceinline__ void parts_frag(f32x4 lo, f32x4 hi, Frag<T> &head, Frag<T> &rest) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float x = j < 4 ? lo[j] : hi[j - 4], y = j < 4 ? lo[j + 1] : hi[j - 3];
+        t2 h, r;
+        f2 cut;
+        if constexpr (__is_same(T, __bf16)) {
+            const unsigned a = __float_as_uint(x), b = __float_as_uint(y);
+            h = __builtin_bit_cast(t2, __builtin_amdgcn_perm(b, a, 0x07060302u));
+            cut = f2{__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)};
+        } else {
+            h = __builtin_bit_cast(t2, __builtin_amdgcn_cvt_pkrtz(x, y));
+            cut = f2{static_cast<float>(h[0]), static_cast<float>(h[1])};
+        }
+        constexpr float kMore = 1.0f + 0x1p-12f;
+        const float u = __builtin_fmaf(x, kMore, -cut[0]), v = __builtin_fmaf(y, kMore, -cut[1]);
+        if constexpr (__is_same(T, __bf16)) {
+            r = t2{static_cast<T>(u), static_cast<T>(v)};
+        } else {
+            r = __builtin_bit_cast(t2, __builtin_amdgcn_cvt_pkrtz(u, v));
+        }
+        head[j] = h[0], head[j + 1] = h[1];
+        rest[j] = r[0], rest[j + 1] = r[1];
+    }
+}
+template <typename T>
+constexpr float kPartsScale = sizeof(T) == 2 ? 1.0f / (1.0f + 0x1p-12f) : 1.0f;
+
 // Eight consecutive elements in memory (16-byte aligned).
 template <typename T>
 __device__ __forceinline__ Frag<T> row_frag(const T *p) {
@@ -299,24 +335,22 @@ __device__ __forceinline__ void row_products(const T *tile, const Frag<T> (&oper
     }
 }
 
-// sums[x] += the tile's columns times p[x], the products' rows rounded to T; with REST what the
-// rounding took is a second product with the same columns.
-template <typename Lds, typename T, int DP, int COLS, int N, bool REST = false>
+// sums[x] += the tile's columns times p[x], the products' rows, which 16-bit types take rounded, or
+// with PARTS in two parts: a second product with the same columns, and a sum that is 1 /
+// kPartsScale times as large.
+template <typename Lds, typename T, int DP, int COLS, int N, bool PARTS>
 __device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[COLS][N], int g,
                                                 int c, f32x4 (&sums)[COLS][DP / 16]) {
+    constexpr bool kTwo = PARTS && sizeof(T) == 2;
 #pragma unroll
     for (int u = 0; u < N / 2; ++u) {
         Frag<T> f[COLS], rest[COLS];
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
-            f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
-            if constexpr (REST) {
-                f32x4 low[2];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    low[i / 4][i % 4] = p[x][2 * u + i / 4][i % 4] - static_cast<float>(f[x][i]);
-                }
-                rest[x] = result_frag<T>(low[0], low[1]);
+            if constexpr (kTwo) {
+                parts_frag<T>(p[x][2 * u], p[x][2 * u + 1], f[x], rest[x]);
+            } else {
+                f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
             }
         }
 #pragma unroll
@@ -325,7 +359,7 @@ __device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
                 sums[x][i] = mma(v, f[x], sums[x][i]);
-                if constexpr (REST) sums[x][i] = mma(v, rest[x], sums[x][i]);
+                if constexpr (kTwo) sums[x][i] = mma(v, rest[x], sums[x][i]);
             }
         }
     }

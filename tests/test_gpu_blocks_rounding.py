@@ -1,0 +1,49 @@
+"""Block attention of 16-bit rows, where a sequence has few of them, and its gradients are as exact
+as the formulas in float32 with the result rounded once.
+
+The share that is allowed: a probability (or a score's gradient) reaches its product within 2^-15
+(bfloat16) or 2^-20 (float16) of itself, its float32 exponential within about 2^-19; the result's
+rounding is 2^-9 and 2^-12 of it on average.  These errors are independent, so they add in squares:
+at most a hundredth of the last one's square is another 0.5%.  1.02 leaves room for that and for
+the sample's own spread."""
+
+import pytest
+import torch
+
+import nacho_amd
+from tests import block_exact as exact
+from tests import block_reference as ref
+from tests.test_gpu_blocks import FEW, MANY, WIDE, _operands
+
+pytestmark = pytest.mark.gpu
+
+TYPES = (torch.float16, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [FEW[2], FEW[4], FEW[7], (64, 1, 300, 32, 8, 128, 64, 3),
+                                   (64, 1, 290, 32, 8, 64, 32, 3), (130, 3, 90, 14, 2, 80, 128, 1),
+                                   (128, 1, 70, 16, 8, 96, 32, 2)],
+                         ids=str)
+def test_output_is_rounded_once(gpu, sizes, dtype):
+    q, k, v, ids, _ = _operands(41, dtype, *sizes)
+    see = ref.visible(ids, sizes[1], sizes[2], sizes[6], None, True)
+    want = exact.attention(q, k, v, see)
+    got = nacho_amd.gpu_block_attention(q.to(gpu), k.to(gpu), v.to(gpu), ids.to(gpu), sizes[6])
+    exact.rounded_once(got, want, "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_infinite_values_stay_infinities(gpu, dtype):
+    """A value that is infinite is a query's result in that column, where the query sees it."""
+    for sizes in (FEW[3], FEW[8], MANY[2], WIDE[0]):
+        q, k, v, ids, _ = _operands(42, dtype, *sizes)
+        v[:, 5, :, 2], v[:, 37, :, 3] = float("inf"), float("-inf")
+        see = ref.visible(ids, sizes[1], sizes[2], sizes[6], None, True)
+        group = sizes[3] // sizes[4]
+        got = nacho_amd.gpu_block_attention(q.to(gpu), k.to(gpu), v.to(gpu), ids.to(gpu),
+                                            sizes[6]).cpu()
+        for key, col, value in ((5, 2, float("inf")), (37, 3, float("-inf"))):
+            sees = see[..., key].transpose(1, 2).repeat_interleave(group, -1)
+            assert (got[..., col][sees] == value).all()
+            assert torch.isfinite(got[..., col][~sees]).all()

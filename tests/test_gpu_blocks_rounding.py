@@ -47,3 +47,20 @@ def test_infinite_values_stay_infinities(gpu, dtype):
             sees = see[..., key].transpose(1, 2).repeat_interleave(group, -1)
             assert (got[..., col][sees] == value).all()
             assert torch.isfinite(got[..., col][~sees]).all()
+
+
+def _gradients(gpu, q, k, v, ids, dout, block):
+    """The gradients, and what they are by their formulas (delta of the output that was given)."""
+    dev = [x.to(gpu).requires_grad_() for x in (q, k, v)]
+    out = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), block)
+    grads = torch.autograd.grad(out, dev, dout.to(gpu))
+    see = ref.visible(ids, q.shape[1], k.shape[1], block, None, True)
+    return grads, exact.attention(q, k, v, see, out.detach().cpu(), dout)[1:]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [FEW[6], FEW[7], *MANY[:3], WIDE[1]], ids=str)
+def test_gradients_are_rounded_once(gpu, sizes, dtype):
+    got, want = _gradients(gpu, *_operands(43, dtype, *sizes), sizes[6])
+    for x, y, name in zip(got, want, ("dq", "dk", "dv")):
+        exact.rounded_once(x, y, name)

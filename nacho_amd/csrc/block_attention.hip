@@ -750,6 +750,49 @@ __global__ __launch_bounds__(kStartBlock) void start_kernel(int64_t rows, int pe
     if (threadIdx.x == 0) start[rows] = carry;
 }
 
+// float16 has less range than gradients take that it can hold the sums of: the scores' gradients
+// of a small step fall below 2^-24, those of a scaled loss rise above 65504.  So a column of them
+// is multiplied by a power of two that keeps the largest so far below 2^15, and was at least 2^12
+// when it was chosen; when it has to change, the column's sums follow.
+template <typename T>
+struct Range {
+    static constexpr bool kNeeded = __is_same(T, _Float16);
+    int shift = 100;
+
+    template <int N, int M>
+    __device__ __forceinline__ void bring(f32x4 (&ds)[N], f32x4 (&sums)[M]) {
+        if constexpr (kNeeded) {
+            float top = 0.0f;
+#pragma unroll
+            for (int t = 0; t < N; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(ds[t][i]));
+            }
+            top = column_max(top);
+            const bool over = __builtin_amdgcn_ldexpf(top, shift) > 0x1p15f;
+            if (__any(over)) {
+                // (2^13 is over top 2^now; the exponent of an infinity is 0)
+                const int now = over ? min(shift, 13 - __builtin_amdgcn_frexp_expf(top)) : shift;
+                const float factor = __builtin_amdgcn_ldexpf(1.0f, now - shift);
+#pragma unroll
+                for (int i = 0; i < M; ++i) sums[i] *= factor;
+                shift = now;
+            }
+            const float factor = __builtin_amdgcn_ldexpf(1.0f, shift);
+#pragma unroll
+            for (int t = 0; t < N; ++t) ds[t] *= factor;
+        }
+    }
+    // What undoes it in the sums.
+    __device__ __forceinline__ float inverse() const {
+        return kNeeded ? __builtin_amdgcn_ldexpf(1.0f, -shift) : 1.0f;
+    }
+};
+
+// The same for probabilities, which are at most 1: for dv they are 2^kMore times as large.
+template <typename T>
+constexpr int kMore = Range<T>::kNeeded ? 15 : 0;
+
 // From the products s = q . k and dp = dout . v of 16 N keys with a row: s become probabilities
 // and dp the scores' gradients (without the scale).
 template <int N>
@@ -834,6 +877,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
     KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
     // (No marks: what a row sees that is not finite is in its lse or delta.)
     for (int pass = kPlain; pass <= kFinite; pass += kFinite) {  // uniform
+        Range<T> range[COLS];
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
 #pragma unroll
@@ -850,6 +894,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
             for (int x = 0; x < COLS; ++x) {
                 score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x],
                                         pass != kPlain);
+                range[x].bring(dp[x], o[x]);
             }
             column_products<Lds, T, DP, COLS, BN / 16, true>(s_k, dp, g, c, o);
         });
@@ -859,10 +904,11 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
             wrong += not_finite<DP / 16>(o[x]);
             if (!rows.exists[x]) continue;
             T *dq = a.dq.row(tile.b, tile.t0 + rows.token[x], rows.head[x]);
+            const float undo = range[x].inverse();
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const int col = 16 * i + 4 * g;
-                if (col < s.dim) store4<T>(dq + col, o[x][i] * (s.scale * kPartsScale<T>));
+                if (col < s.dim) store4<T>(dq + col, o[x][i] * undo * (s.scale * kPartsScale<T>));
             }
         }
         if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;
@@ -952,6 +998,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
     }
     const float scale2 = base2_scale(s.scale);
     const int place0 = length - s.queries;
+    Range<T> range[COLS];
 
     // The item's tokens, ascending: those of the row's set bits from the nth * per_item-th on.
     const unsigned *row_bits = items.bits + row * items.words;
@@ -1009,7 +1056,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
         const bool there = step * kStep + static_cast<int>(threadIdx.x) < rows;
         const int last = there ? next_last : block_end;
         s_lse[step & 3][threadIdx.x] =
-            there ? (next_lse == kNegInf ? 0.0f : next_lse * kLog2e) : -kNegInf;
+            there ? (next_lse == kNegInf ? 0.0f : next_lse * kLog2e) - kMore<T> : -kNegInf;
         s_delta[step & 3][threadIdx.x] = next_delta;
         s_last[step & 3][threadIdx.x] = last;
         // whether some row sees a part of the block only
@@ -1054,6 +1101,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
                 }
             }
         }
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) range[x].bring(dp[x], dk[x]);
         column_products<Lds, T, DP, COLS, kN, true>(my_do, p, g, c, dv);
         column_products<Lds, T, DP, COLS, kN, true>(my_q, dp, g, c, dk);
     };
@@ -1081,6 +1130,18 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
             use(s_q1, s_do1, step + 1);
             if (informs) end(step + 3);
             rows_arrived();
+        }
+    }
+    if constexpr (Range<T>::kNeeded) {
+        constexpr float kLess = 1.0f / (1 << kMore<T>);
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+            const float undo = range[x].inverse();
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                dk[x][i] = dk[x][i] * undo * kLess;
+                dv[x][i] *= kLess;
+            }
         }
     }
     if constexpr (kSets == 2) {

@@ -64,3 +64,56 @@ def test_gradients_are_rounded_once(gpu, sizes, dtype):
     got, want = _gradients(gpu, *_operands(43, dtype, *sizes), sizes[6])
     for x, y, name in zip(got, want, ("dq", "dk", "dv")):
         exact.rounded_once(x, y, name)
+
+
+@pytest.mark.parametrize("size", (1e-4, 8e3))
+@pytest.mark.parametrize("sizes", [(1, 65, 130, 6, 2, 128, 64, 2), (2, 90, 333, 4, 4, 64, 32, 5),
+                                   MANY[0]], ids=str)
+def test_float16_gradients_of_small_and_large_steps(gpu, sizes, size):
+    """Gradients of a scaled loss: where float16 holds the results, it does not matter that it
+    would not hold the scores' gradients."""
+    q, k, v, ids, dout = _operands(44, torch.float32, *sizes)
+    q, k = 0.3 * q, 0.3 * k
+    dout = (dout * size).clamp(-60000, 60000)
+    operands = [x.half() if x.is_floating_point() else x for x in (q, k, v, ids, dout)]
+    got, want = _gradients(gpu, *operands, sizes[6])
+    for x, y, name in zip(got, want, ("dq", "dk", "dv")):
+        assert y.abs().max() < 65000, name
+        exact.rounded_once(x, y, name)
+
+
+def test_float16_gradients_of_small_probabilities(gpu):
+    """Queries that see thousands of keys: probabilities down to 2^-20 and below."""
+    q, k, v, _, dout = _operands(45, torch.float16, 1, 40, 4096, 4, 2, 64, 128, 1)
+    ids = torch.arange(32, dtype=torch.int32).expand(1, 40, 2, 32).contiguous()
+    got, want = _gradients(gpu, 1.5 * q, k, v, ids, dout, 128)
+    for x, y, name in zip(got, want, ("dq", "dk", "dv")):
+        exact.rounded_once(x, y, name)
+
+
+SMALL, LARGE = (1e-4, 1.0), (8e3, 8.0)  # of dout and of v
+
+
+@pytest.mark.parametrize("sizes", [(1, 65, 130, 6, 2, 128, 64, 2), (2, 90, 333, 4, 4, 64, 32, 5),
+                                   (1, 70, 140, 3, 3, 72, 128, 1)], ids=str)
+@pytest.mark.parametrize("size", (SMALL, LARGE), ids=str)
+def test_float16_gradients_of_small_and_large_steps(gpu, sizes, size):
+    """Gradients of a scaled loss: where float16 holds the results, it does not matter that it
+    would not hold the scores' gradients."""
+    q, k, v, ids, dout = _operands(44, torch.float32, *sizes)
+    q, k, v = 0.3 * q, 0.3 * k, size[1] * v
+    dout = (dout * size[0]).clamp(-60000, 60000)
+    operands = [x.half() if x.is_floating_point() else x for x in (q, k, v, ids, dout)]
+    got, want = _gradients(gpu, *operands, sizes[6])
+    for x, y, name in zip(got, want, ("dq", "dk", "dv")):
+        assert y.abs().max() < 65000, name
+        exact.rounded_once(x, y, name)
+
+
+def test_float16_gradients_of_small_probabilities(gpu):
+    """Queries that see thousands of keys: probabilities down to 2^-20 and below."""
+    q, k, v, _, dout = _operands(45, torch.float16, 1, 40, 4096, 4, 2, 64, 128, 1)
+    ids = torch.arange(32, dtype=torch.int32).expand(1, 40, 2, 32).contiguous()
+    got, want = _gradients(gpu, 1.5 * q, k, v, ids, dout, 128)
+    for x, y, name in zip(got, want, ("dq", "dk", "dv")):
+        exact.rounded_once(x, y, name)

@@ -211,7 +211,7 @@ __device__ __forceinline__ void store_again(T *p, float v, int pass) {
 
 // Goes over the tile's blocks BN keys at a time: use(k, v, nth, first key) with both operands'
 // rows in LDS, while the next step's are on their way into the other buffer.  Rows past the
-// sequence's end are zeros.  Every wavefront calls it; `use` has no barrier.
+// sequence's end are zeros.  Every wavefront calls it, and every one calls `use` for every step.
 //
 // Loads go from memory to LDS without registers, into one of two buffers while the other is used.
 template <typename T, int DP, int BN, int R>
@@ -220,10 +220,11 @@ struct KeySteps {
     T *k[2], *v[2];
     Lists<R> &lists;
 
-    // masked[]: the operand whose products over keys the pass concerns (k or v).
+    // masked: the operand (k or v) whose products over keys the pass concerns, for passes after
+    // kPlain's to mask when it has arrived; null where `use` does that.
     template <typename Use>
     __device__ __forceinline__ void run(const Forward<T> &a, const RowTile<R> &tile, int pass,
-                                        T *const (&masked)[2], Use use) {
+                                        T *const *masked, Use use) {
         const Shape &s = a.s;
         const T *k_base = a.k.row(tile.b, 0, tile.h), *v_base = a.v.row(tile.b, 0, tile.h);
         const int end = tile.last_key(s, tile.tokens - 1) + 1;  // keys that some row sees
@@ -242,22 +243,22 @@ struct KeySteps {
                 Lds::load(to_k, threadIdx.x, k_source, k_base + key * a.k.row_stride, there);
                 Lds::load(to_v, threadIdx.x, v_source, v_base + key * a.v.row_stride, there);
             };
-            auto arrived = [&](T *tile_of) {
+            auto arrived = [&](int buffer) {
                 rows_arrived();
-                if (pass != kPlain) {  // uniform
-                    Lds::make_finite(tile_of, threadIdx.x, pass == kMarks);
+                if (pass != kPlain && masked) {  // uniform
+                    Lds::make_finite(masked[buffer], threadIdx.x, pass == kMarks);
                     __syncthreads();
                 }
             };
             if (steps > 0) load(0, k[0], v[0]);
-            arrived(masked[0]);
+            arrived(0);
             for (int step = 0; step < steps; step += 2) {
                 if (step + 1 < steps) load(step + 1, k[1], v[1]);
                 use(k[0], v[0], step >> shift, first_key(step));
-                arrived(masked[1]);
+                arrived(1);
                 if (step + 2 < steps) load(step + 2, k[0], v[0]);
                 if (step + 1 < steps) use(k[1], v[1], (step + 1) >> shift, first_key(step + 1));
-                arrived(masked[0]);
+                arrived(0);
             }
         }
     }
@@ -407,8 +408,8 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
             m[x] = kNegInf;
             l[x] = 0.0f;
         }
-        steps.run(a, tile, pass, {s_v0, s_v1}, [&](const T *s_k, const T *s_v, int nth,
-                                                   int first_key) {
+        T *const masked[2] = {s_v0, s_v1};
+        steps.run(a, tile, pass, masked, [&](const T *s_k, const T *s_v, int nth, int first_key) {
             int limit[COLS];
             if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
             f32x4 p[COLS][BN / 16];
@@ -794,10 +795,10 @@ template <typename T>
 constexpr int kMore = Range<T>::kNeeded ? 15 : 0;
 
 // From the products s = q . k and dp = dout . v of 16 N keys with a row: s become probabilities
-// and dp the scores' gradients (without the scale).
+// and dp the scores' gradients (without the scale); with kMarks 1 for each key that the row sees.
 template <int N>
 __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], float scale2,
-                                               float lse2, float delta, int limit, bool every) {
+                                               float lse2, float delta, int limit, int pass) {
     const bool none = limit <= 0;
     const float base = none ? -kNegInf : lse2;  // (as in softmax_step)
 #pragma unroll
@@ -808,11 +809,14 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
             dp[t][i] = s[t][i] * (dp[t][i] - delta);
         }
     }
-    if (every || __any(!none && limit < 16 * N)) {
+    if (pass != kPlain || __any(!none && limit < 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dp[t][i] = 16 * t + i < limit ? dp[t][i] : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const float seen = pass == kMarks ? 1.0f : dp[t][i];
+                dp[t][i] = 16 * t + i < limit ? seen : 0.0f;
+            }
         }
     }
 }
@@ -875,26 +879,29 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
     }
     const float scale2 = base2_scale(s.scale);
     KeySteps<T, DP, BN, kRowsOf> steps{{s_k0, s_k1}, {s_v0, s_v1}, s_lists};
-    // (No marks: what a row sees that is not finite is in its lse or delta.)
-    for (int pass = kPlain; pass <= kFinite; pass += kFinite) {  // uniform
+    for (int pass = kPlain; pass <= kFinite; ++pass) {  // uniform
         Range<T> range[COLS];
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) o[x][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        steps.run(a, tile, pass, {s_k0, s_k1}, [&](const T *s_k, const T *s_v, int nth,
-                                                   int first_key) {
+        steps.run(a, tile, pass, nullptr, [&](T *s_k, const T *s_v, int nth, int first_key) {
             int limit[COLS];
-            if (!rows.limits(s_lists, nth, first_key, g, limit)) return;
+            // (after kPlain's pass every wavefront goes on, to the barriers below)
+            if (!rows.limits(s_lists, nth, first_key, g, limit) && pass == kPlain) return;
             f32x4 p[COLS][BN / 16], dp[COLS][BN / 16];
             row_products<Lds, T, DP, COLS, BN / 16>(s_k, q, g, c, p);
             row_products<Lds, T, DP, COLS, BN / 16>(s_v, dout, g, c, dp);
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
-                score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x],
-                                        pass != kPlain);
+                score_gradient<BN / 16>(p[x], dp[x], scale2, lse2[x], row_delta[x], limit[x], pass);
                 range[x].bring(dp[x], o[x]);
+            }
+            if (pass != kPlain) {  // uniform; the scores are those of the keys as they are
+                __syncthreads();
+                Lds::make_finite(s_k, threadIdx.x, pass == kMarks);
+                __syncthreads();
             }
             column_products<Lds, T, DP, COLS, BN / 16, true>(s_k, dp, g, c, o);
         });
@@ -905,10 +912,18 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
             if (!rows.exists[x]) continue;
             T *dq = a.dq.row(tile.b, tile.t0 + rows.token[x], rows.head[x]);
             const float undo = range[x].inverse();
+            const float factor = pass == kMarks ? 1.0f : s.scale * kPartsScale<T>;
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
                 const int col = 16 * i + 4 * g;
-                if (col < s.dim) store4<T>(dq + col, o[x][i] * undo * (s.scale * kPartsScale<T>));
+                if (col >= s.dim) continue;
+                const f32x4 v = o[x][i] * undo * factor;
+                if (pass == kPlain) {
+                    store4<T>(dq + col, v);
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) store_again(dq + col + j, v[j], pass);
             }
         }
         if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;

@@ -1,0 +1,48 @@
+"""Keys and values that are not finite in places that a query sees, or that nobody sees: results are
+those of the formulas, and no finite number stands where these have none."""
+
+import math
+
+import pytest
+import torch
+
+import nacho_amd
+from tests import block_exact as exact
+from tests import block_reference as ref
+from tests.test_gpu_blocks import FEW, MANY, TYPES, WIDE, _operands
+
+pytestmark = pytest.mark.gpu
+
+# what a finite result may be off, in parts of what rounding it is: these tests look for other values
+NEAR = {torch.float32: 200.0, torch.float16: 2.0, torch.bfloat16: 2.0}
+
+
+def _sees(ids, sizes, key):
+    see = ref.visible(ids, sizes[1], sizes[2], sizes[6], None, True)
+    return see, see[..., key].transpose(1, 2).repeat_interleave(sizes[3] // sizes[4], -1)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [FEW[3], FEW[8], MANY[0], WIDE[0]], ids=str)
+def test_keys_whose_score_is_minus_infinity(gpu, sizes, dtype):
+    """Such a key has probability 0: it is as good as unseen, but dq is 0 times infinity in the
+    column that holds the infinity."""
+    q, k, v, ids, dout = _operands(51, dtype, *sizes)
+    key, col = 3, 1
+    q[..., col] = q[..., col].abs() + 0.25
+    k[:, key, :, col] = -math.inf
+    see, sees = _sees(ids, sizes, key)
+    dev = [x.to(gpu).requires_grad_() for x in (q, k, v)]
+    out = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), sizes[6])
+    grads = [x.cpu() for x in torch.autograd.grad(out, dev, dout.to(gpu))]
+    see = see.clone()
+    see[..., key] = False
+    k[:, key, :, col] = 0.0
+    want = exact.attention(q, k, v, see, out.detach().cpu(), dout)
+    exact.rounded_once(out, want[0], "out", NEAR[dtype])
+    assert sees.any()
+    assert torch.isnan(grads[0][..., col][sees]).all()
+    grads[0][..., col] = torch.where(sees, 0.0, grads[0][..., col])
+    want[1][..., col] = torch.where(sees, 0.0, want[1][..., col])
+    for x, y, name in zip(grads, want[1:], ("dq", "dk", "dv")):
+        exact.rounded_once(x, y, name, NEAR[dtype])

@@ -282,16 +282,21 @@ constexpr float kSlack = 8.0f;  // the running maximum follows a row's when it i
 // wavefront needs it.  Returns whether they were, by `factor`.
 //
 // Most steps are seen whole or not at all: a row that sees nothing of a step takes a maximum of
-// infinity there, and only steps that some row sees in part, or `every` one, are masked key by key.
+// infinity there, and only steps that some row sees in part, or every one after kPlain's pass, are
+// masked key by key.  With kMarks the scores are 0, so that each key that a row sees counts, the
+// ones of the least probabilities too.
 template <int N>
-__device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, bool every,
+__device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, int pass,
                                              float &m, float &l, float &factor) {
     const bool none = limit <= 0;
-    if (every || __any(!none && limit < 16 * N)) {
+    if (pass != kPlain || __any(!none && limit < 16 * N)) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = 16 * t + i < limit ? s[t][i] : kNegInf;
+            for (int i = 0; i < 4; ++i) {
+                const float seen = pass == kMarks ? 0.0f : s[t][i];
+                s[t][i] = 16 * t + i < limit ? seen : kNegInf;
+            }
         }
     }
     float top = s[0][0];
@@ -417,8 +422,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
                 float factor;
-                if (softmax_step<BN / 16>(p[x], scale2, limit[x], pass != kPlain, m[x], l[x],
-                                          factor)) {
+                if (softmax_step<BN / 16>(p[x], scale2, limit[x], pass, m[x], l[x], factor)) {
 #pragma unroll
                     for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
                 }
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
             if (step + stride < steps) load(step + stride);
             if (!__any(limit > 0)) continue;
             float factor;
-            if (softmax_step<2>(p[0], scale2, limit, pass != kPlain, m, l, factor)) {
+            if (softmax_step<2>(p[0], scale2, limit, pass, m, l, factor)) {
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
             }

@@ -46,3 +46,29 @@ def test_keys_whose_score_is_minus_infinity(gpu, sizes, dtype):
     want[1][..., col] = torch.where(sees, 0.0, want[1][..., col])
     for x, y, name in zip(grads, want[1:], ("dq", "dk", "dv")):
         exact.rounded_once(x, y, name, NEAR[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [(2, 1, 200, 4, 2, 72, 64, 4), FEW[3], FEW[8], MANY[0], WIDE[0]],
+                         ids=str)
+def test_infinite_values_of_the_least_probabilities(gpu, sizes, dtype):
+    """An infinity times a probability that is too small for its type is not left out."""
+    q, k, v, ids, _ = _operands(52, dtype, *sizes)
+    key, col = 3, 1
+    q[..., 0] = q[..., 0].abs() + 1.0
+    k[:, key] = 0.0
+    k[:, key, :, 0] = -2000.0  # a score of less than -150
+    v[:, key, :, col] = math.inf
+    see, sees = _sees(ids, sizes, key)
+    got = nacho_amd.gpu_block_attention(q.to(gpu), k.to(gpu), v.to(gpu), ids.to(gpu),
+                                        sizes[6]).cpu()
+    first = torch.zeros(sizes[2], dtype=torch.bool)
+    first[key] = True
+    alone = (see & ~first).any(-1).transpose(1, 2).repeat_interleave(sizes[3] // sizes[4], -1)
+    assert (sees & alone).any()
+    assert not torch.isfinite(got[..., col][sees & alone]).any()
+    v[:, key, :, col] = 0.0
+    want = exact.attention(q, k, v, see)
+    got[..., col] = torch.where(sees, 0.0, got[..., col])
+    want[..., col] = torch.where(sees, 0.0, want[..., col])
+    exact.rounded_once(got, want, "out", NEAR[dtype])

@@ -1055,7 +1055,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
     };
     // The first kStep threads (part of the first wavefront) work out the rows of a step: `begin`
     // two steps ahead, and `end` once lse and delta are there.  Steps past the last row repeat
-    // it, with an infinity for lse, which makes its probabilities 0.
+    // it as one that sees no key.
     const int block_end = (id + 1) * s.block - 1;
     const bool informs = threadIdx.x < kStep;
     float next_lse = 0.0f, next_delta = 0.0f;
@@ -1073,9 +1073,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
     };
     auto end = [&](int step) {
         const bool there = step * kStep + static_cast<int>(threadIdx.x) < rows;
-        const int last = there ? next_last : block_end;
+        const int last = there ? next_last : -1;
         s_lse[step & 3][threadIdx.x] =
-            there ? (next_lse == kNegInf ? 0.0f : next_lse * kLog2e) - kMore<T> : -kNegInf;
+            (next_lse == kNegInf ? 0.0f : next_lse * kLog2e) - kMore<T>;
         s_delta[step & 3][threadIdx.x] = next_delta;
         s_last[step & 3][threadIdx.x] = last;
         // whether some row sees a part of the block only

@@ -72,3 +72,20 @@ def test_infinite_values_of_the_least_probabilities(gpu, sizes, dtype):
     got[..., col] = torch.where(sees, 0.0, got[..., col])
     want[..., col] = torch.where(sees, 0.0, want[..., col])
     exact.rounded_once(got, want, "out", NEAR[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("block", (32, 64, 128))
+@pytest.mark.parametrize("dim", (64, 128))
+def test_gradients_of_keys_that_nobody_sees(gpu, dim, block, dtype):
+    """One query sees an infinite value: its block's later keys and values, infinite ones among
+    them, which it does not see, keep a gradient of 0."""
+    q, k, v, ids, dout = _operands(53, dtype, 1, block, block, 2, 1, dim, block, 1)
+    ids[:] = -1
+    ids[:, 10] = 0
+    v[:, 3], v[:, 20], k[:, 21] = math.inf, -math.inf, math.nan
+    dev = [x.to(gpu).requires_grad_() for x in (q, k, v)]
+    out = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), block)
+    _, dk, dv = torch.autograd.grad(out, dev, dout.to(gpu))
+    assert not torch.isfinite(dk[:, :11]).any()
+    assert not dk[:, 11:].any() and not dv[:, 11:].any()

@@ -22,6 +22,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _device, _lib
 from .ops import _entry
@@ -181,6 +182,16 @@ def gpu_block_select(scores: torch.Tensor, count: int, block: int, keys: int,
 
 # ---- attention ------------------------------------------------------------------------
 
+def _has_derivatives(*tensors):
+    """Whether autograd is to know of a call with these operands.  (A tangent does not show in
+    requires_grad, and the autograd functions, which have none, refuse it.)"""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                return True
+    return forward_ad._current_level >= 0
+
+
 class _BlockAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, blocks, lengths, block, causal, scale):
@@ -216,12 +227,11 @@ def gpu_block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block
     is no block and a repeated one counts once.  Causal: only keys up to the query's place.  A
     query that sees nothing gives 0.  With `return_lse` also the log of the sum of exponentials,
     float32 [batch, queries, q_heads] (-inf for such a query; no gradient), with which results
-    over disjoint sets of keys can be joined.  Differentiable in q, k and v."""
+    over disjoint sets of keys can be joined.  Differentiable in q, k and v (backward mode, once)."""
     device = _device_of(q, "q")
     scale = _scale(scale, q.shape)
     causal = bool(causal)
-    if torch.is_grad_enabled() and (q.requires_grad or getattr(k, "requires_grad", False) or
-                                    getattr(v, "requires_grad", False)):
+    if _has_derivatives(q, k, v):
         out, lse = _BlockAttention.apply(q, k, v, blocks, lengths, block, causal, scale)
         return (out, lse) if return_lse else out
     got = _call("block_attention", device, q, k, v, blocks, lengths, block, causal, scale,

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from .blocks import _TYPES, _call, _check_tensor, _device_of
+from .blocks import _TYPES, _call, _check_tensor, _device_of, _has_derivatives
 from .tensors import CSR_gpu
 
 MAX_EXPERTS = 2048
@@ -125,7 +125,7 @@ def gpu_dispatch(x: torch.Tensor, route: Route) -> torch.Tensor:
     each of its experts, and zeros past the last expert's entries.  Differentiable in x."""
     _device_of(x, "x")
     _check_route(route)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _has_derivatives(x):
         return _Dispatch.apply(x, route)
     return _dispatch(x, route)
 
@@ -139,6 +139,6 @@ def gpu_combine(rows: torch.Tensor, route: Route, weights: torch.Tensor) -> torc
     _device_of(weights, "weights")
     if weights.dtype != torch.float32 and weights.is_floating_point():
         weights = weights.float()
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if _has_derivatives(rows, weights):
         return _Combine.apply(rows, weights, route)
     return _combine(rows, weights, route)

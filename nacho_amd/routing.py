@@ -80,43 +80,47 @@ def _dispatch(x, route):
     return got
 
 
-def _combine(rows, weights, route):
-    got = _call("combine", rows.device, rows, weights, route.slot)
+def _combine(rows, weights, slot):
+    got = _call("combine", rows.device, rows, weights, slot)
     if got is None:
-        device = route.slot.device
-        _refuse_rows(rows, "rows", device, route.tokens * route.per_token)
-        _check_tensor(weights, "weights", device, 2, (torch.float32,))
-        raise ValueError(f"weights: expected shape {tuple(route.slot.shape)}, got "
+        _refuse_rows(rows, "rows", slot.device, slot.numel())
+        _check_tensor(weights, "weights", slot.device, 2, (torch.float32,))
+        raise ValueError(f"weights: expected shape {tuple(slot.shape)}, got "
                          f"{tuple(weights.shape)}")
     return got
+
+
+# The functions save the route's tensors, not the route, so that torch notices when one of them was
+# written again before the backward pass.
+
+def _saved(t):
+    return t.clone() if t.is_inference() else t  # (torch saves none of inference mode)
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, route):
-        ctx.route = route
+        ctx.save_for_backward(_saved(route.slot))
         return _dispatch(x, route)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        return _combine(drows, None, ctx.route), None
+        slot, = ctx.saved_tensors
+        return _combine(drows, None, slot), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, route):
-        ctx.save_for_backward(rows, weights)
-        ctx.route = route
-        return _combine(rows, weights, route)
+        ctx.save_for_backward(rows, weights, _saved(route.pos), _saved(route.slot))
+        return _combine(rows, weights, route.slot)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        rows, weights = ctx.saved_tensors
-        route = ctx.route
-        drows, dweights = _call("combine_backward", rows.device, rows, weights, route.pos,
-                                route.slot, dout)
+        rows, weights, pos, slot = ctx.saved_tensors
+        drows, dweights = _call("combine_backward", rows.device, rows, weights, pos, slot, dout)
         return drows, dweights, None
 
 
@@ -141,4 +145,4 @@ def gpu_combine(rows: torch.Tensor, route: Route, weights: torch.Tensor) -> torc
         weights = weights.float()
     if _has_derivatives(rows, weights):
         return _Combine.apply(rows, weights, route)
-    return _combine(rows, weights, route)
+    return _combine(rows, weights, route.slot)

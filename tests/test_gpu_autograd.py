@@ -39,3 +39,29 @@ def test_routing_refuses_tangents(gpu):
                      (rows, route, forward_ad.make_dual(w.half(), torch.ones_like(w).half()))):
             with pytest.raises(NotImplementedError, match="jvp"):
                 nacho_amd.gpu_combine(*args)
+
+
+@pytest.mark.parametrize("written", ("pos", "slot"))
+def test_a_route_that_is_written_again_is_noticed(gpu, written):
+    route = nacho_amd.gpu_route(torch.tensor([[0, 1], [1, 2]], device=gpu), 3)
+    x, rows, w = (torch.randn(*s, device=gpu).requires_grad_() for s in ((2, 8), (4, 8), (2, 2)))
+    there = nacho_amd.gpu_dispatch(x, route), nacho_amd.gpu_combine(rows, route, w)
+    getattr(route, written).copy_(getattr(route, written).clone())
+    if written == "slot":
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            there[0].sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        there[1].sum().backward()
+
+
+def test_a_route_of_inference_mode(gpu):
+    choices = torch.tensor([[0, 1], [1, 2]], device=gpu)
+    with torch.inference_mode():
+        route = nacho_amd.gpu_route(choices, 3)
+    x, rows, w = (torch.randn(*s, device=gpu).requires_grad_() for s in ((2, 8), (4, 8), (2, 2)))
+    outs = [nacho_amd.gpu_dispatch(x, route), nacho_amd.gpu_combine(rows, route, w)]
+    got = torch.autograd.grad(outs, (x, rows, w), [torch.ones_like(o) for o in outs])
+    route = nacho_amd.gpu_route(choices, 3)
+    outs = [nacho_amd.gpu_dispatch(x, route), nacho_amd.gpu_combine(rows, route, w)]
+    want = torch.autograd.grad(outs, (x, rows, w), [torch.ones_like(o) for o in outs])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

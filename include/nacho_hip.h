@@ -358,7 +358,8 @@ int nacho_gpu_spgemm64_f32(const nacho_csr *a, const nacho_csr *b, nacho_csr64 *
  * type once.  Results go into the caller's buffers; scratch comes from `alloc` (or the
  * library's allocator).  All calls are asynchronous on `stream`, read nothing back, and may be
  * captured into a graph when `alloc` may be called in a capture.  A result depends on nothing
- * but the operands: sums have a fixed order. */
+ * but the operands: sums have a fixed order.  Sizes past what a kernel's counters or a launch's
+ * 2^32 work-items hold are NACHO_ERR_INDEX_OVERFLOW. */
 #define NACHO_F32 0
 #define NACHO_F16 1
 #define NACHO_BF16 2

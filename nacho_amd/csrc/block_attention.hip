@@ -1279,6 +1279,9 @@ int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
     *s = Shape{p->batch,    p->queries,  p->keys,  p->q_heads,
                p->kv_heads, p->head_dim, p->block, p->count,
                p->causal,   p->q_heads / p->kv_heads, static_cast<int>(blocks), p->scale};
+    if (static_cast<int64_t>(tiling(*s, 64).per_head) * p->batch * p->kv_heads > kMostGroups) {
+        return NACHO_ERR_INDEX_OVERFLOW;
+    }
     return NACHO_OK;
 }
 
@@ -1437,7 +1440,8 @@ int backward(Call &call, const Backward<T> &a) {
     const int64_t most = items.rows + listed / items.per_item;
     const bool wide = sizeof(T) == 2 && s.block % 64 == 0;  // 64 keys to a workgroup
     const int parts = s.block / (wide ? 64 : 32);
-    if (most * parts > INT32_MAX - 8 || items.rows * (s.block / 16) > INT32_MAX) {
+    if (most * parts > kMostGroups - 8 || items.rows * (s.block / 16) > kMostGroups ||
+        static_cast<int64_t>(groups) * heads > kMostGroups) {
         return NACHO_ERR_INDEX_OVERFLOW;
     }
     const bool several = listed > items.per_item;  // else no row has several items

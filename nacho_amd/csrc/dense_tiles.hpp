@@ -18,6 +18,10 @@
 namespace nacho {
 namespace dense {
 
+// Workgroups of 256 threads that a launch can have.  A launch of 2^32 work-items or more is no error:
+// it runs what is left of their number modulo 2^32.
+constexpr int64_t kMostGroups = ((int64_t{1} << 32) - 1) / 256;
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -259,11 +259,14 @@ __device__ void clear_behind(const Rows &a, T *__restrict__ rows) {
     }
 }
 
-// A token of the workgroup, in scalar registers (LANES is a multiple of a wavefront).
-template <int LANES>
-__device__ __forceinline__ int64_t token_of() {
-    return blockIdx.x * static_cast<int64_t>(kThreads / LANES) +
-           __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+// Calls f with each token of the threads' own, in scalar registers (LANES is a multiple of a
+// wavefront): one, where a launch can have as many workgroups as that takes.
+template <int LANES, typename F>
+__device__ __forceinline__ void each_token(const Rows &a, F f) {
+    constexpr int kPer = kThreads / LANES;
+    int64_t token = blockIdx.x * static_cast<int64_t>(kPer) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    for (; token < a.tokens; token += a.token_groups * static_cast<int64_t>(kPer)) f(token);
 }
 
 // LANES threads per token.
@@ -272,17 +275,17 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(Rows a, const T *__r
                                                             int64_t x_stride,
                                                             T *__restrict__ rows) {
     if (blockIdx.x >= a.token_groups) return clear_behind<T, N>(a, rows);
-    const int64_t token = token_of<LANES>();
-    if (token >= a.tokens) return;
-    const int *slots = a.slot + token * a.per_token;
-    for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
-         col += LANES * N) {
-        const auto piece = *reinterpret_cast<const Piece<T, N> *>(x + token * x_stride + col);
-        for (int i = 0; i < a.per_token; ++i) {
-            const int64_t at = slots[i];
-            if (at >= 0) store_piece<T, N>(rows + at * a.width + col, piece);
+    each_token<LANES>(a, [&](int64_t token) {
+        const int *slots = a.slot + token * a.per_token;
+        for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
+             col += LANES * N) {
+            const auto piece = *reinterpret_cast<const Piece<T, N> *>(x + token * x_stride + col);
+            for (int i = 0; i < a.per_token; ++i) {
+                const int64_t at = slots[i];
+                if (at >= 0) store_piece<T, N>(rows + at * a.width + col, piece);
+            }
         }
-    }
+    });
 }
 
 // The rows of STEP experts are on their way together; a dropped entry's stand-in is row 0, whose
@@ -293,38 +296,38 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Rows a, const T *__re
                                                            const float *__restrict__ weights,
                                                            T *__restrict__ out) {
     constexpr int kStep = 4;
-    const int64_t token = token_of<LANES>();
-    if (token >= a.tokens) return;
-    const int64_t e = token * a.per_token;
-    for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
-         col += LANES * N) {
-        float sum[N] = {};
-        for (int i0 = 0; i0 < a.per_token; i0 += kStep) {
-            Piece<T, N> piece[kStep];
-            float w[kStep];
-            bool there[kStep];
+    each_token<LANES>(a, [&](int64_t token) {
+        const int64_t e = token * a.per_token;
+        for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
+             col += LANES * N) {
+            float sum[N] = {};
+            for (int i0 = 0; i0 < a.per_token; i0 += kStep) {
+                Piece<T, N> piece[kStep];
+                float w[kStep];
+                bool there[kStep];
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                const bool listed = i0 + i < a.per_token;
-                const int64_t at = listed ? a.slot[e + i0 + i] : -1;
-                there[i] = at >= 0;
-                w[i] = weights && listed ? weights[e + i0 + i] : 1.0f;
-                piece[i] = load_piece<T, N>(rows + (there[i] ? at : 0) * row_stride + col);
-            }
+                for (int i = 0; i < kStep; ++i) {
+                    const bool listed = i0 + i < a.per_token;
+                    const int64_t at = listed ? a.slot[e + i0 + i] : -1;
+                    there[i] = at >= 0;
+                    w[i] = weights && listed ? weights[e + i0 + i] : 1.0f;
+                    piece[i] = load_piece<T, N>(rows + (there[i] ? at : 0) * row_stride + col);
+                }
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {
+                for (int i = 0; i < kStep; ++i) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float x = static_cast<float>(piece[i].v[j]);
-                    sum[j] = there[i] ? __builtin_fmaf(w[i], x, sum[j]) : sum[j];
+                    for (int j = 0; j < N; ++j) {
+                        const float x = static_cast<float>(piece[i].v[j]);
+                        sum[j] = there[i] ? __builtin_fmaf(w[i], x, sum[j]) : sum[j];
+                    }
                 }
             }
-        }
-        Piece<T, N> o;
+            Piece<T, N> o;
 #pragma unroll
-        for (int j = 0; j < N; ++j) o.v[j] = static_cast<T>(sum[j]);
-        *reinterpret_cast<Piece<T, N> *>(out + token * a.width + col) = o;
-    }
+            for (int j = 0; j < N; ++j) o.v[j] = static_cast<T>(sum[j]);
+            *reinterpret_cast<Piece<T, N> *>(out + token * a.width + col) = o;
+        }
+    });
 }
 
 template <typename T, int N, int LANES>
@@ -335,39 +338,40 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(
     if (blockIdx.x >= a.token_groups) return clear_behind<T, N>(a, drows);
     constexpr int kWavesPer = LANES / dev::kWave;
     __shared__ float s_sum[kThreads / dev::kWave];
-    const int64_t token = token_of<LANES>();
-    if (LANES < kThreads && token >= a.tokens) return;  // (no barrier below for whole wavefronts)
-    for (int i = 0; i < a.per_token; ++i) {
-        const int64_t e = token * a.per_token + i;
-        const int64_t at = a.slot[e];
-        float dot = 0.0f;
-        if (at >= 0) {
-            const float w = weights[e];
-            for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
-                 col += LANES * N) {
-                const auto d =
-                    *reinterpret_cast<const Piece<T, N> *>(dout + token * dout_stride + col);
-                const auto y = load_piece<T, N>(rows + at * row_stride + col);
-                Piece<T, N> o;
+    // (with barriers below, a workgroup has one token; else its wavefronts do not wait)
+    each_token<LANES>(a, [&](int64_t token) {
+        for (int i = 0; i < a.per_token; ++i) {
+            const int64_t e = token * a.per_token + i;
+            const int64_t at = a.slot[e];
+            float dot = 0.0f;
+            if (at >= 0) {
+                const float w = weights[e];
+                for (int64_t col = static_cast<int64_t>(threadIdx.x % LANES) * N; col < a.width;
+                     col += LANES * N) {
+                    const auto d =
+                        *reinterpret_cast<const Piece<T, N> *>(dout + token * dout_stride + col);
+                    const auto y = load_piece<T, N>(rows + at * row_stride + col);
+                    Piece<T, N> o;
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float x = static_cast<float>(d.v[j]);
-                    dot = __builtin_fmaf(x, static_cast<float>(y.v[j]), dot);
-                    o.v[j] = static_cast<T>(w * x);
+                    for (int j = 0; j < N; ++j) {
+                        const float x = static_cast<float>(d.v[j]);
+                        dot = __builtin_fmaf(x, static_cast<float>(y.v[j]), dot);
+                        o.v[j] = static_cast<T>(w * x);
+                    }
+                    store_piece<T, N>(drows + at * a.width + col, o);
                 }
-                store_piece<T, N>(drows + at * a.width + col, o);
             }
+            dot = dev::wave_sum(dot);
+            if constexpr (kWavesPer > 1) {
+                if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = dot;
+                __syncthreads();
+                dot = 0.0f;
+                for (int w = 0; w < kWavesPer; ++w) dot += s_sum[w];
+                __syncthreads();
+            }
+            if (threadIdx.x % LANES == 0) dweights[e] = dot;
         }
-        dot = dev::wave_sum(dot);
-        if constexpr (kWavesPer > 1) {
-            if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = dot;
-            __syncthreads();
-            dot = 0.0f;
-            for (int w = 0; w < kWavesPer; ++w) dot += s_sum[w];
-            __syncthreads();
-        }
-        if (threadIdx.x % LANES == 0) dweights[e] = dot;
-    }
+    });
 }
 
 // ---- host -----------------------------------------------------------------------------
@@ -460,14 +464,13 @@ int with_rows(int32_t dtype, int64_t width, bool whole, F f) {
     return typed(__bf16{});
 }
 
-int token_groups(int64_t tokens, int lanes, unsigned *groups) {
-    const int64_t n = (tokens * lanes + kThreads - 1) / kThreads;
-    if (n > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
-    *groups = static_cast<unsigned>(n);
-    return NACHO_OK;
-}
-
 constexpr unsigned kClearGroups = 64;  // workgroups for the rows behind: few in ordinary use
+
+unsigned token_groups(int64_t tokens, int lanes) {
+    const int64_t n = (tokens * lanes + kThreads - 1) / kThreads;
+    const int64_t most = dense::kMostGroups - kClearGroups;
+    return static_cast<unsigned>(n < most ? n : most);
+}
 
 int dispatch(int32_t dtype, int64_t tokens, int32_t per_token, int32_t n_experts, int64_t width,
              const void *x, int64_t x_stride, const int32_t *pos, const int32_t *slot, void *rows,
@@ -482,8 +485,8 @@ int dispatch(int32_t dtype, int64_t tokens, int32_t per_token, int32_t n_experts
     const bool whole = pieces(x, x_stride, width, item) && pieces(rows, width, width, item);
     return with_rows(dtype, width, whole, [&](auto type, auto n, auto lanes) -> int {
         using T = decltype(type);
-        Rows a{tokens, width, per_token, n_experts, pos, slot, 0};
-        NACHO_TRY(token_groups(tokens, lanes(), &a.token_groups));
+        const Rows a{tokens, width, per_token,
+                     n_experts, pos, slot, token_groups(tokens, lanes())};
         dispatch_kernel<T, n(), lanes()>
             <<<a.token_groups + kClearGroups, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                 a, static_cast<const T *>(x), x_stride, static_cast<T *>(rows));
@@ -504,8 +507,7 @@ int combine(int32_t dtype, int64_t tokens, int32_t per_token, int64_t width, con
     const bool whole = pieces(rows, row_stride, width, item) && pieces(out, width, width, item);
     return with_rows(dtype, width, whole, [&](auto type, auto n, auto lanes) -> int {
         using T = decltype(type);
-        Rows a{tokens, width, per_token, 0, nullptr, slot, 0};
-        NACHO_TRY(token_groups(tokens, lanes(), &a.token_groups));
+        const Rows a{tokens, width, per_token, 0, nullptr, slot, token_groups(tokens, lanes())};
         combine_kernel<T, n(), lanes()>
             <<<a.token_groups, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                 a, static_cast<const T *>(rows), row_stride, weights, static_cast<T *>(out));
@@ -531,8 +533,8 @@ int combine_backward(int32_t dtype, int64_t tokens, int32_t per_token, int32_t n
                        pieces(drows, width, width, item);
     return with_rows(dtype, width, whole, [&](auto type, auto n, auto lanes) -> int {
         using T = decltype(type);
-        Rows a{tokens, width, per_token, n_experts, pos, slot, 0};
-        NACHO_TRY(token_groups(tokens, lanes(), &a.token_groups));
+        const Rows a{tokens, width, per_token,
+                     n_experts, pos, slot, token_groups(tokens, lanes())};
         combine_backward_kernel<T, n(), lanes()>
             <<<a.token_groups + kClearGroups, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                 a, static_cast<const T *>(rows), row_stride, weights, static_cast<const T *>(dout),

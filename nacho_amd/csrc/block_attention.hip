@@ -45,6 +45,9 @@ using namespace dense;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / dev::kWave;
 constexpr int kWindow = 512;  // blocks whose masks are in LDS at a time
+// Ids of a query: those of 128 queries, which a tile or a workgroup that marks tokens may have,
+// are counted in 32 bits, kThreads at a time.
+constexpr int kMostIds = (INT_MAX - kThreads) / 128;
 
 struct Shape {
     int batch, queries, keys, q_heads, kv_heads, dim, block, count, causal;
@@ -1261,7 +1264,7 @@ int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
     const int64_t blocks = (static_cast<int64_t>(p->keys) + p->block - 1) / p->block;
     const int64_t parts = blocks * (p->block / 32) * p->batch * p->kv_heads;
     if (rows > INT32_MAX / 16 || parts > INT32_MAX || p->keys > INT32_MAX - (1 << 17) ||
-        p->count > INT32_MAX / 64) {
+        p->count > kMostIds) {
         return NACHO_ERR_INDEX_OVERFLOW;
     }
     const int item = p->dtype == NACHO_F32 ? 4 : 2;

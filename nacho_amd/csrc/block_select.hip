@@ -456,7 +456,8 @@ int select(int32_t batch, int32_t queries, int32_t heads, int32_t keys, int32_t 
     if (!ids || (!score && keys > 0)) return NACHO_ERR_INVALID_ARGUMENT;
     const int64_t blocks = (static_cast<int64_t>(keys) + block - 1) / block;
     const int64_t grid = (rows + 3) / 4;
-    if (rows > INT32_MAX) return NACHO_ERR_INDEX_OVERFLOW;
+    // (a wavefront goes over its row's ids 64 at a time)
+    if (rows > INT32_MAX || count > INT32_MAX - dev::kWave) return NACHO_ERR_INDEX_OVERFLOW;
     const int shift = block == 32 ? 5 : block == 64 ? 6 : 7;
     SelectArgs a{rows,  0,     queries, heads, keys,  shift,   static_cast<int>(blocks), count,
                  sink,  local, causal,  score, lengths, ids};

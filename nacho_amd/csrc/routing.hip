@@ -379,6 +379,8 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(
 // (512 to 4096 entries: 19 us a call, of which most is the host's, and 27 with three launches)
 constexpr int kSmall = kRun * (kSmallBlock / dev::kWave);
 constexpr int kSmallCounters = 8192;  // 32 KB
+// (entries are counted in 32 bits, whole workgroups' runs and a token's by fours)
+constexpr int kMostEntries = INT32_MAX - kRun * kRunWaves;
 
 int route(const void *experts, int32_t id_bytes, int64_t tokens, int32_t per_token,
           int32_t n_experts, int32_t *pos, int32_t *order, int32_t *slot, void *stream,
@@ -387,7 +389,7 @@ int route(const void *experts, int32_t id_bytes, int64_t tokens, int32_t per_tok
         n_experts > NACHO_MAX_EXPERTS || !pos) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
-    if (tokens > (INT32_MAX - kRun * kRunWaves) / per_token) return NACHO_ERR_INDEX_OVERFLOW;
+    if (tokens > kMostEntries / per_token) return NACHO_ERR_INDEX_OVERFLOW;
     const int entries = static_cast<int>(tokens * per_token);
     if (entries > 0 && (!experts || !order || !slot ||
                         reinterpret_cast<uintptr_t>(experts) % static_cast<unsigned>(id_bytes))) {
@@ -423,7 +425,7 @@ int check_rows(int32_t dtype, int64_t tokens, int32_t per_token, int64_t width) 
     if (dtype < NACHO_F32 || dtype > NACHO_BF16 || tokens < 0 || per_token < 1 || width < 0) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
-    if (tokens > INT32_MAX / per_token) return NACHO_ERR_INDEX_OVERFLOW;
+    if (tokens > kMostEntries / per_token) return NACHO_ERR_INDEX_OVERFLOW;
     return NACHO_OK;
 }
 

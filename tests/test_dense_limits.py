@@ -28,3 +28,28 @@ def test_scores_of_more_queries_than_a_launch_has(lib):  # noqa: F811
     h = ctypes.byref(_lib.Heads(0x10000, 1 << 20, 256, 64))
     assert lib.nacho_block_scores(2, 1 << 25, 1, 32, 1, 1, 64, 32, 1, 0.125, h, P(0x1000), None,
                                   P(0x1000), None) == OVERFLOW
+
+
+MOST_IDS = (2 ** 31 - 1 - 256) // 128  # ids of a query: 128 queries of a tile times these are counted
+
+
+def test_attention_of_more_ids_than_a_tile_counts(lib):  # noqa: F811
+    for count in (MOST_IDS + 1, 1 << 24, (2 ** 31 - 1) // 64):
+        a = _args(count=count)
+        assert lib.nacho_block_attention(ctypes.byref(a), None, None) == OVERFLOW
+        assert lib.nacho_block_attention_backward(ctypes.byref(a), None, None) == OVERFLOW
+
+
+def test_selection_of_more_ids_than_a_row_counts(lib):  # noqa: F811
+    for count in (2 ** 31 - 64, 2 ** 31 - 1):
+        assert lib.nacho_block_select(1, 1, 1, 100, 32, count, 1, 1, 1, P(0x1000), None, P(0x1000),
+                                      None) == OVERFLOW
+
+
+def test_rows_of_more_entries_than_are_counted(lib):  # noqa: F811
+    x = P(0x1000)
+    for tokens, per_token in ((1, 2 ** 31 - 1), (1, 2 ** 31 - 1000), (1 << 20, 2048)):
+        assert lib.nacho_dispatch(2, tokens, per_token, 4, 8, x, 8, x, x, x, None) == OVERFLOW
+        assert lib.nacho_combine(2, tokens, per_token, 8, x, 8, None, x, x, None) == OVERFLOW
+        assert lib.nacho_combine_backward(2, tokens, per_token, 4, 8, x, 8, x, x, x, x, 8, x, x,
+                                          None) == OVERFLOW

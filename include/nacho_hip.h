@@ -386,7 +386,7 @@ typedef struct nacho_block_attention_args {
     int32_t block;                       /* keys of a block: 32, 64 or 128                  */
     int32_t count;                       /* ids per query and key head                      */
     int32_t causal;                      /* 0 or 1                                          */
-    float scale;                         /* factor of q . k, finite                         */
+    float scale;                         /* factor of q . k, finite, also times log2(e)     */
     const int32_t *lengths;              /* [batch], in [0, keys]; NULL: keys for all        */
     const int32_t *blocks;               /* [batch][queries][kv_heads][count], in any order; an
                                             id outside the sequence is no block, a repeated one

@@ -28,6 +28,7 @@ from . import _device, _lib
 from .ops import _entry
 
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
+_MOST_SCALE = torch.finfo(torch.float32).max
 
 
 _BOUND: dict = {}
@@ -95,7 +96,7 @@ def _check_block(block):
         raise ValueError(f"block must be 32, 64 or 128, got {block}")
 
 
-def _refuse_attention(q, k, v, blocks, lengths, block):
+def _refuse_attention(q, k, v, blocks, lengths, block, scale):
     device = q.device
     _check_tensor(q, "q", device, 4, _TYPES)
     for t, name in ((k, "k"), (v, "v")):
@@ -109,6 +110,8 @@ def _refuse_attention(q, k, v, blocks, lengths, block):
     if tuple(blocks.shape[:3]) != want:
         raise ValueError(f"blocks: expected shape {want} + (count,), got {tuple(blocks.shape)}")
     _check_lengths(lengths, device, q.shape[0])
+    if abs(scale) > _MOST_SCALE / math.log2(math.e):  # (the exponentials are of base 2)
+        raise ValueError(f"scale must be at most 2.3e38, got {scale}")
     raise ValueError("gpu_block_attention: refused operands (more than 2^31 - 1 rows, or more "
                      "than 1024 heads of q to a key head)")
 
@@ -116,8 +119,8 @@ def _refuse_attention(q, k, v, blocks, lengths, block):
 def _scale(scale, shape):
     if scale is None:
         return (shape[-1] or 1) ** -0.5 if shape else 1.0
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _MOST_SCALE:  # (NaN too)
+        raise ValueError(f"scale must be finite in float32, got {scale}")
     return float(scale)
 
 
@@ -198,7 +201,7 @@ class _BlockAttention(torch.autograd.Function):
         got = _call("block_attention", q.device, q, k, v, blocks, lengths, block, causal, scale,
                     True)
         if got is None:
-            _refuse_attention(q, k, v, blocks, lengths, block)
+            _refuse_attention(q, k, v, blocks, lengths, block, scale)
         out, lse = got
         ctx.save_for_backward(q, k, v, blocks, lengths, out, lse)
         ctx.how = block, causal, scale
@@ -227,7 +230,8 @@ def gpu_block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block
     is no block and a repeated one counts once.  Causal: only keys up to the query's place.  A
     query that sees nothing gives 0.  With `return_lse` also the log of the sum of exponentials,
     float32 [batch, queries, q_heads] (-inf for such a query; no gradient), with which results
-    over disjoint sets of keys can be joined.  Differentiable in q, k and v (backward mode, once)."""
+    over disjoint sets of keys can be joined.  Differentiable in q, k and v (in backward mode,
+    once)."""
     device = _device_of(q, "q")
     scale = _scale(scale, q.shape)
     causal = bool(causal)
@@ -237,7 +241,7 @@ def gpu_block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block
     got = _call("block_attention", device, q, k, v, blocks, lengths, block, causal, scale,
                 return_lse)
     if got is None:
-        _refuse_attention(q, k, v, blocks, lengths, block)
+        _refuse_attention(q, k, v, blocks, lengths, block, scale)
     return got if return_lse else got[0]
 
 
@@ -249,8 +253,9 @@ def gpu_block_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.T
     """(dq, dk, dv) of gpu_block_attention from its output's gradient, its operands and its
     results, for callers that keep their own record of a step.  Deterministic."""
     device = _device_of(q, "q")
+    scale = _scale(scale, q.shape)
     got = _call("block_attention_backward", device, q, k, v, blocks, lengths, block, bool(causal),
-                _scale(scale, q.shape), dout, out, lse)
+                scale, dout, out, lse)
     if got is None:
         for t, name in ((dout, "dout"), (out, "out")):
             _check_tensor(t, name, device, 4, (q.dtype,))
@@ -259,5 +264,5 @@ def gpu_block_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.T
         _check_tensor(lse, "lse", device, 3, (torch.float32,))
         if lse.shape != q.shape[:3]:
             raise ValueError(f"lse: expected shape {tuple(q.shape[:3])}, got {tuple(lse.shape)}")
-        _refuse_attention(q, k, v, blocks, lengths, block)
+        _refuse_attention(q, k, v, blocks, lengths, block, scale)
     return got

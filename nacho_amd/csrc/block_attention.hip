@@ -955,10 +955,10 @@ struct Items {
 // with LANES = 2 the four wavefronts are two such sets, which take 32 rows of the item's tokens
 // in turn and add their sums at the end.
 //
-// p and ds are in two parts of the operands' type for their products (16-bit types), so that dk and
-// dv are what rounding them once makes them, 0.0017 of their norms off with bfloat16 and 0.0002 with
-// float16 (0.0024 and 0.0003 with one rounded part); training steps of 2 x 4096 queries of 16 heads
-// of 128 take 541 us instead of 504 for it.
+// p and ds are in two parts of the operands' type for their products (16-bit types), so that dk
+// and dv are what rounding them once makes them, 0.0017 of their norms off with bfloat16 and 0.0002
+// with float16 (0.0024 and 0.0003 with one rounded part); training steps of 2 x 4096 queries of 16
+// heads of 128 take 541 us instead of 504 for it.
 //
 // 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 203 us for 90 GFLOP (rows that did not
 // select the block take no part); with one workgroup per block instead of items 1146 us.  LDS is
@@ -1257,7 +1257,7 @@ int check(const nacho_block_attention_args *p, bool backward, Shape *s) {
         p->q_heads % p->kv_heads != 0 || p->q_heads / p->kv_heads > kMaxGroup ||
         p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8 != 0 ||
         (p->block != 32 && p->block != 64 && p->block != 128) ||
-        p->count < 0 || (p->causal != 0 && p->causal != 1) || !std::isfinite(p->scale)) {
+        p->count < 0 || (p->causal != 0 && p->causal != 1) || !std::isfinite(p->scale * kLog2e)) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
     const int64_t rows = static_cast<int64_t>(p->batch) * p->queries * p->q_heads;
@@ -1327,8 +1327,9 @@ constexpr bool kMayShare = sizeof(T) == 2 && DP > 64;
 template <typename T>
 constexpr int64_t kFewTiles = (sizeof(T) == 2 ? 2 : 3) * kFullGrid;
 
-// A sequence's rows up to which a probability reaches its product in two parts of the operands' type:
-// one tile then has all of a key head's rows, and its keys' bytes take longer than their products.
+// A sequence's rows up to which a probability reaches its product in two parts of the operands'
+// type: one tile then has all of a key head's rows, and its keys' bytes take longer than their
+// products.
 // 64 single tokens of 32 heads of 128: 51.1 us either way; 8192 queries: 307 us with one part, 416
 // with two.
 constexpr int64_t kPartsRows = 64;
@@ -1377,7 +1378,8 @@ int forward(Call &call, const Forward<T> &a) {
     const int64_t few = static_cast<int64_t>(small.per_head) * heads;
     const int64_t tiles = static_cast<int64_t>(tiling(s, 64).per_head) * heads;
     if (few > kFewTiles<T> || tiles >= kFullGrid) {
-        const bool parts = sizeof(T) == 2 && static_cast<int64_t>(s.queries) * s.group <= kPartsRows;
+        const bool parts =
+            sizeof(T) == 2 && static_cast<int64_t>(s.queries) * s.group <= kPartsRows;
         return with_tiles<T, DP>(s, parts, [&](auto keys, auto columns, unsigned grid) {
             if constexpr (sizeof(T) == 2 && columns() == 1) {
                 if (parts) {
@@ -1466,12 +1468,13 @@ int backward(Call &call, const Backward<T> &a) {
     items.bits = bits;
     items.start = start;
     if (queries > 0) {
-        const int launched = with_tiles<T, DP>(s, false, [&](auto keys, auto columns, unsigned grid) {
+        auto launch = [&](auto keys, auto columns, unsigned grid) {
             // (two column tiles leave registers for 32 keys of q . k and dout . v)
             constexpr int kKeys = columns() == 2 ? 32 : keys();
             dq_kernel<T, DP, kKeys, columns()><<<grid, kThreads, 0, stream>>>(
                 a, delta, items.rows, counts);
-        });
+        };
+        const int launched = with_tiles<T, DP>(s, false, launch);
         NACHO_TRY(launched);
     }
     if (items.rows == 0) return NACHO_OK;

@@ -18,8 +18,8 @@
 namespace nacho {
 namespace dense {
 
-// Workgroups of 256 threads that a launch can have.  A launch of 2^32 work-items or more is no error:
-// it runs what is left of their number modulo 2^32.
+// Workgroups of 256 threads that a launch can have.  A launch of 2^32 work-items or more is no
+// error: it runs what is left of their number modulo 2^32.
 constexpr int64_t kMostGroups = ((int64_t{1} << 32) - 1) / 256;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -84,7 +84,8 @@ __device__ __forceinline__ Frag<T> result_frag(f32x4 lo, f32x4 hi) {
 // one would round away: `head` is x cut off toward 0, `rest` what is left of (1 + 2^-12) x.  The
 // part of 2^-12, which kPartsScale undoes in the sums, gives the rest x's sign and keeps it from
 // being 0 where x is not, so that the products of both with an infinity are the same infinity.
-// (float16: for an x of 2^-12 or more; below, the rest may be 0.)
+// (float16: for an x of 2^-12 or more; below, the rest may be 0.  The rest of an infinity is no
+// number.)
 template <typename T>
 __device__ __forceinline__ void parts_frag(f32x4 lo, f32x4 hi, Frag<T> &head, Frag<T> &rest) {
     typedef T t2 __attribute__((ext_vector_type(2)));

@@ -53,3 +53,26 @@ def test_rows_of_more_entries_than_are_counted(lib):  # noqa: F811
         assert lib.nacho_combine(2, tokens, per_token, 8, x, 8, None, x, x, None) == OVERFLOW
         assert lib.nacho_combine_backward(2, tokens, per_token, 4, 8, x, 8, x, x, x, x, 8, x, x,
                                           None) == OVERFLOW
+
+
+@pytest.mark.parametrize("scale", (2.4e38, -2.4e38, 3.4e38))
+def test_attention_of_a_scale_whose_base_2_factor_is_infinite(lib, scale):  # noqa: F811
+    a = _args(scale=scale)
+    assert lib.nacho_block_attention(ctypes.byref(a), None, None) == INVALID
+    assert lib.nacho_block_attention_backward(ctypes.byref(a), None, None) == INVALID
+
+
+@pytest.mark.parametrize("scale", (1e39, -1e300, 3.5e38, float("inf"), float("nan")))
+def test_a_scale_past_float32_is_named(scale):
+    from nacho_amd import blocks
+
+    with pytest.raises(ValueError, match="scale must be finite"):
+        blocks._scale(scale, (1, 1, 1, 64))
+
+
+def test_scales_in_range_are_kept():
+    from nacho_amd import blocks
+
+    for scale in (0.0, -2.5, 2.3e38, 1e-45):
+        assert blocks._scale(scale, (1, 1, 1, 64)) == scale
+    assert blocks._scale(None, (1, 1, 1, 64)) == 0.125

@@ -89,3 +89,16 @@ def test_gradients_of_keys_that_nobody_sees(gpu, dim, block, dtype):
     _, dk, dv = torch.autograd.grad(out, dev, dout.to(gpu))
     assert not torch.isfinite(dk[:, :11]).any()
     assert not dk[:, 11:].any() and not dv[:, 11:].any()
+
+
+@pytest.mark.parametrize("scale", (2.4e38, -3e38, 1e39, math.nan))
+def test_scales_past_the_range_are_named(gpu, scale):
+    q, k, v, ids, dout = (x.to(gpu) for x in _operands(54, torch.float32, *FEW[3]))
+    f = nacho_amd.gpu_block_attention
+    out, lse = f(q, k, v, ids, 64, return_lse=True)
+    with pytest.raises(ValueError, match="scale must be"):
+        f(q, k, v, ids, 64, scale=scale)
+    with pytest.raises(ValueError, match="scale must be"):
+        f(q.clone().requires_grad_(), k, v, ids, 64, scale=scale)
+    with pytest.raises(ValueError, match="scale must be"):
+        nacho_amd.gpu_block_attention_backward(dout, q, k, v, ids, 64, out, lse, scale=scale)

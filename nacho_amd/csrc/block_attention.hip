@@ -13,8 +13,8 @@
 // O^T = V^T P^T (dense_tiles.hpp).  An operand of a product has to have the rows' type.  Where a
 // sequence has few rows, bound by their keys' bytes, 16-bit types take a probability in two parts,
 // so that out is what rounding it once makes it: 0.0017 of its norm off with bfloat16, 0.0002 with
-// float16.  Where it has many, bound by products, one rounded part is taken: out is 0.0021 and
-// 0.00026 off for two thirds of the time (kPartsRows).  The sum l is of the unrounded ones in
+// float16.  Where it has many, bound by products, one rounded part is taken: out is 0.0022 and
+// 0.00026 off for three quarters of the time (kPartsRows).  The sum l is of the unrounded ones in
 // float32 either way.
 //
 // Backward, with delta = dout . out and p from the stored lse: ds = p (dout . v - delta),
@@ -761,7 +761,8 @@ __global__ __launch_bounds__(kStartBlock) void start_kernel(int64_t rows, int pe
 // float16 has less range than gradients take that it can hold the sums of: the scores' gradients
 // of a small step fall below 2^-24, those of a scaled loss rise above 65504.  So a column of them
 // is multiplied by a power of two that keeps the largest so far below 2^15, and was at least 2^12
-// when it was chosen; when it has to change, the column's sums follow.
+// when it was chosen; when it has to change, the column's sums follow.  Training steps of 2 x 4096
+// queries of 16 heads of 128 take 566 us instead of 527 for it, of heads of 64 304 instead of 282.
 template <typename T>
 struct Range {
     static constexpr bool kNeeded = __is_same(T, _Float16);
@@ -834,9 +835,9 @@ __device__ __forceinline__ void score_gradient(f32x4 (&s)[N], f32x4 (&dp)[N], fl
 // ds is in two parts of the operands' type for its product (16-bit types): dq then is 0.0019 of its
 // norm off with bfloat16 instead of 0.0026, where its own rounding makes 0.0017 and delta, which is
 // of the rounded out, 0.0006.
-// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 199 us (172 without the second product), 68
-// GFLOP that are asked for and 1.6 times that with the union's.  Matrix products 38%, vector unit
-// 41% of a CU's time.
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 200 us (172 without the second product), 68
+// GFLOP that are asked for and 1.6 times that with the union's.  Matrix products 36%, vector unit
+// 37% of a CU's time.
 template <typename T, int DP, int BN, int COLS>
 __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *__restrict__ delta,
                                                          int64_t rows_of_blocks,
@@ -960,12 +961,13 @@ struct Items {
 // with float16 (0.0024 and 0.0003 with one rounded part); training steps of 2 x 4096 queries of 16
 // heads of 128 take 541 us instead of 504 for it.
 //
-// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 203 us for 90 GFLOP (rows that did not
-// select the block take no part); with one workgroup per block instead of items 1146 us.  LDS is
-// the bound, 45% of a CU's time and waits for it: a wavefront's 16 keys use each fragment once.
-// Two column tiles use it twice: for heads of 64 training steps are 32 us of 330 shorter with them;
-// for 128 they leave one wavefront to a SIMD, and the kernel takes 276 us.  32 keys to a workgroup
-// instead of 64: training steps 531 us instead of 507, heads of 64 317 instead of 298.
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 237 us for 90 GFLOP (rows that did not
+// select the block take no part; with one rounded part 203, and 1146 with one workgroup per block
+// instead of items).  LDS is the bound, 40% of a CU's time and waits for it, before matrix products
+// with 34%: a wavefront's 16 keys use each fragment once.  Two column tiles use it twice: for heads
+// of 64 training steps are 35 us of 330 shorter with them; for 128 they do not fit the registers,
+// and a step takes 920 us instead of 544.  32 keys to a workgroup instead of 64: training steps 562
+// us instead of 544, heads of 64 306 instead of 295.
 template <typename T, int DP, int COLS, int LANES>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
     Backward<T> a, const float *__restrict__ delta, Items items, unsigned group_inverse) {
@@ -1311,9 +1313,9 @@ constexpr int kFullGrid = 256;  // workgroups that occupy the device: one per CU
 // Two column tiles per wavefront share what each reads of LDS, but are half as many workgroups
 // with twice the work.  us with two and with one, by tiles of 128 rows; attention of heads of 128:
 // 192: 114 72, 320: 112 112, 512: 116 123 and 107 103, 768: 171 163, 1024: 183 202, 2048: 308 361
-// and 276 320; its training steps: 512: 265 249, 896: 450 450, 1024: 508 516, 2048: 1113 1161; of
-// heads of 96: 512: 200 184, 1024: 359 359.  Heads of 64, whose registers leave room for more
-// wavefronts with one: 512: 81 57, 1024: 127 97, 2048: 158 145; training 1024: 331 288.
+// and 276 320; its training steps: 512: 284 264, 896: 480 472, 1024: 543 540, 2048: 1031 1075; of
+// heads of 96: 512: 242 231, 1024: 473 477.  Heads of 64, whose registers leave room for more
+// wavefronts with one: 512: 81 57, 1024: 127 97, 2048: 158 145; training 1024: 344 295.
 constexpr int64_t kTwoColumns = 4 * kFullGrid;
 template <typename T, int DP>
 constexpr bool kMayShare = sizeof(T) == 2 && DP > 64;
@@ -1330,8 +1332,8 @@ constexpr int64_t kFewTiles = (sizeof(T) == 2 ? 2 : 3) * kFullGrid;
 // A sequence's rows up to which a probability reaches its product in two parts of the operands'
 // type: one tile then has all of a key head's rows, and its keys' bytes take longer than their
 // products.
-// 64 single tokens of 32 heads of 128: 51.1 us either way; 8192 queries: 307 us with one part, 416
-// with two.
+// 64 single tokens of 32 heads of 128: 51.1 us either way, 256 of them 198 and 197 (with two column
+// tiles); 8192 queries: 307 us with one part, 416 with two.
 constexpr int64_t kPartsRows = 64;
 
 // Calls f with the keys of a step, 64, or 32 where the block or float32's tiles (twice as large)
@@ -1364,8 +1366,8 @@ int with_tiles(const Shape &s, bool one_column, F f) {
 }
 
 // Training steps of 16 heads of 128, 4 key heads, in us by the target (384, 512, 768, 1024, 1536):
-// 2 x 4096 queries 570 550 507 520 518; 2 x 2048 (512, 768, 1024) 265 249 239; by the least (128,
-// 192, 256, 384): 2 x 1024 134 121 130 136, 1 x 1024 of half the heads 107 107 115 131.
+// 2 x 4096 queries 610 571 544 558 551; 2 x 2048 (512, 768, 1024) 278 264 253; by the least (128,
+// 192, 256, 384): 2 x 1024 141 128 139 144, 1 x 1024 of half the heads 103 111 120 138.
 constexpr int64_t kItemTarget = 768;
 constexpr int64_t kItemLeast = 192;  // tokens
 

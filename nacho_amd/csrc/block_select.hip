@@ -10,7 +10,9 @@
 // block of keys), so it runs on the float32 matrix instruction. A workgroup sums 16 queries'
 // heads into LDS and goes over the blocks 64 at a time, 16 to a wavefront. 8192 queries of 32
 // heads of 128 against 128 blocks: 30 us, where reading q and writing the scores would take 18.
-// 48 sequences' tokens against 512 blocks each (101 MB of means): 16 us, a copy's rate; 32 or
+// 48 sequences' tokens against the 320 of 512 blocks that they have on average (63 MB of means): 15
+// to 16 us, 4 TB/s, where a copy's rate would take 11.3: a workgroup's first means are on their way
+// only when q's heads are summed, and each step's only when the step before is multiplied.  32 or
 // 64 queries to a workgroup are no faster for many queries and 1.3 us slower there.
 //
 // select: a wavefront per query and key head. Scores become unsigned numbers of the same order,

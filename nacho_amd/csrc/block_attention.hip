@@ -430,7 +430,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
                     for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
                 }
             }
-            column_products<Lds, T, DP, COLS, BN / 16, PARTS>(s_v, p, g, c, o);
+            column_products<Lds, T, DP, COLS, BN / 16, PARTS ? kTwo : kOne>(s_v, p, g, c, o);
         });
         float wrong = 0.0f;
 #pragma unroll
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
             }
-            column_products<typename Stage::Lds, T, DP, 1, 2, true>(s_v, p, g, c, o);
+            column_products<typename Stage::Lds, T, DP, 1, 2, kTwo>(s_v, p, g, c, o);
         }
     };
     for (;; ++pass) {  // uniform
@@ -911,7 +911,7 @@ __global__ __launch_bounds__(kThreads, 2) void dq_kernel(Backward<T> a, float *_
                 Lds::make_finite(s_k, threadIdx.x, pass == kMarks);
                 __syncthreads();
             }
-            column_products<Lds, T, DP, COLS, BN / 16, true>(s_k, dp, g, c, o);
+            column_products<Lds, T, DP, COLS, BN / 16, kTwo>(s_k, dp, g, c, o);
         });
         float wrong = 0.0f;
 #pragma unroll
@@ -1127,8 +1127,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void dkv_kernel(
         }
 #pragma unroll
         for (int x = 0; x < COLS; ++x) range[x].bring(dp[x], dk[x]);
-        column_products<Lds, T, DP, COLS, kN, true>(my_do, p, g, c, dv);
-        column_products<Lds, T, DP, COLS, kN, true>(my_q, dp, g, c, dk);
+        column_products<Lds, T, DP, COLS, kN, kTwo>(my_do, p, g, c, dv);
+        column_products<Lds, T, DP, COLS, kN, kTwoOrInfinite>(my_q, dp, g, c, dk);
     };
     if (rows > 0) {  // uniform
         if (informs) {

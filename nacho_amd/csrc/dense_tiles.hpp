@@ -80,13 +80,16 @@ __device__ __forceinline__ Frag<T> result_frag(f32x4 lo, f32x4 hi) {
     return f;
 }
 
+// How the results of a product become the next one's operand: one part of its type, or two; with
+// kTwoOrInfinite infinities among them are that in the sums too (their rests are no numbers).
+enum Parts { kOne, kTwo, kTwoOrInfinite };
+
 // Two results of a product as an operand in two parts of T, a 16-bit type, that together hold what
 // one would round away: `head` is x cut off toward 0, `rest` what is left of (1 + 2^-12) x.  The
 // part of 2^-12, which kPartsScale undoes in the sums, gives the rest x's sign and keeps it from
 // being 0 where x is not, so that the products of both with an infinity are the same infinity.
-// (float16: for an x of 2^-12 or more; below, the rest may be 0.  The rest of an infinity is no
-// number.)
-template <typename T>
+// (float16: for an x of 2^-12 or more; below, the rest may be 0.)
+template <typename T, Parts PARTS>
 __device__ __forceinline__ void parts_frag(f32x4 lo, f32x4 hi, Frag<T> &head, Frag<T> &rest) {
     typedef T t2 __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -104,7 +107,11 @@ __device__ __forceinline__ void parts_frag(f32x4 lo, f32x4 hi, Frag<T> &head, Fr
             cut = f2{static_cast<float>(h[0]), static_cast<float>(h[1])};
         }
         constexpr float kMore = 1.0f + 0x1p-12f;
-        const float u = __builtin_fmaf(x, kMore, -cut[0]), v = __builtin_fmaf(y, kMore, -cut[1]);
+        float u = __builtin_fmaf(x, kMore, -cut[0]), v = __builtin_fmaf(y, kMore, -cut[1]);
+        if constexpr (PARTS == kTwoOrInfinite) {  // (no number to any finite one)
+            u = fmaxf(u, -0x1p100f);
+            v = fmaxf(v, -0x1p100f);
+        }
         if constexpr (__is_same(T, __bf16)) {
             r = t2{static_cast<T>(u), static_cast<T>(v)};
         } else {
@@ -341,19 +348,19 @@ __device__ __forceinline__ void row_products(const T *tile, const Frag<T> (&oper
 }
 
 // sums[x] += the tile's columns times p[x], the products' rows, which 16-bit types take rounded, or
-// with PARTS in two parts: a second product with the same columns, and a sum that is 1 /
-// kPartsScale times as large.
-template <typename Lds, typename T, int DP, int COLS, int N, bool PARTS>
+// in two parts: a second product with the same columns, and a sum that is 1 / kPartsScale times as
+// large.
+template <typename Lds, typename T, int DP, int COLS, int N, Parts PARTS>
 __device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[COLS][N], int g,
                                                 int c, f32x4 (&sums)[COLS][DP / 16]) {
-    constexpr bool kTwo = PARTS && sizeof(T) == 2;
+    constexpr bool kSplit = PARTS != kOne && sizeof(T) == 2;
 #pragma unroll
     for (int u = 0; u < N / 2; ++u) {
         Frag<T> f[COLS], rest[COLS];
 #pragma unroll
         for (int x = 0; x < COLS; ++x) {
-            if constexpr (kTwo) {
-                parts_frag<T>(p[x][2 * u], p[x][2 * u + 1], f[x], rest[x]);
+            if constexpr (kSplit) {
+                parts_frag<T, PARTS>(p[x][2 * u], p[x][2 * u + 1], f[x], rest[x]);
             } else {
                 f[x] = result_frag<T>(p[x][2 * u], p[x][2 * u + 1]);
             }
@@ -364,7 +371,7 @@ __device__ __forceinline__ void column_products(const T *tile, const f32x4 (&p)[
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
                 sums[x][i] = mma(v, f[x], sums[x][i]);
-                if constexpr (kTwo) sums[x][i] = mma(v, rest[x], sums[x][i]);
+                if constexpr (kSplit) sums[x][i] = mma(v, rest[x], sums[x][i]);
             }
         }
     }

@@ -102,3 +102,20 @@ def test_scales_past_the_range_are_named(gpu, scale):
         f(q.clone().requires_grad_(), k, v, ids, 64, scale=scale)
     with pytest.raises(ValueError, match="scale must be"):
         nacho_amd.gpu_block_attention_backward(dout, q, k, v, ids, 64, out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim,block", [(64, 64), (128, 64), (96, 32)])
+def test_infinite_score_gradients(gpu, dim, block, dtype):
+    """A query that sees an infinite value takes its infinity from the other keys' score gradients:
+    their dk is that infinity with the query's signs."""
+    q, k, v, _, dout = _operands(55, dtype, 1, 1, 40, 1, 1, dim, block, 1)
+    ids = torch.arange((40 + block - 1) // block, dtype=torch.int32).view(1, 1, 1, -1)
+    dout[..., 0], v[:, 7, :, 0] = 1.0, math.inf
+    q = torch.where(q.abs() < 0.25, 0.25, q)
+    dev = [x.to(gpu).requires_grad_() for x in (q, k, v)]
+    out = nacho_amd.gpu_block_attention(*dev, ids.to(gpu), block)
+    dq, dk, dv = (x.cpu() for x in torch.autograd.grad(out, dev, dout.to(gpu)))
+    assert torch.isnan(dq).all() and torch.isnan(dk[:, 7]).all() and torch.isfinite(dv).all()
+    others = torch.arange(40) != 7
+    assert torch.equal(dk[:, others].float(), (-math.inf * q.sign().float()).expand(1, 39, 1, dim))

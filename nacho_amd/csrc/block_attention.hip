@@ -276,19 +276,24 @@ __device__ __forceinline__ float base2_scale(float scale) {
     return fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f);
 }
 
-constexpr float kSlack = 8.0f;  // the running maximum follows a row's when it is 2^8 behind
+// The running maximum follows a row's when it is 2^kSlack behind.  float16's probabilities in two
+// parts are 2^kUp times as large, so that neither part of one of more than 2^-25 is 0.
+template <typename T, bool PARTS>
+constexpr int kUp = __is_same(T, _Float16) && PARTS ? 13 : 0;
+template <int UP>
+constexpr float kSlack = UP ? 15 - UP : 8;
 
 // One online-softmax step for a row (a lane's column) over 16 N keys: s are the products, the
 // first `limit` keys from the step's first (this lane's 4 g included) are seen.  s become the
 // probabilities against the running maximum m, which may stay up to kSlack below the row's own
-// (they are at most 2^kSlack then): sums are brought to a new one only when some row of the
+// (they are at most 2^(UP + kSlack) then): sums are brought to a new one only when some row of the
 // wavefront needs it.  Returns whether they were, by `factor`.
 //
 // Most steps are seen whole or not at all: a row that sees nothing of a step takes a maximum of
 // infinity there, and only steps that some row sees in part, or every one after kPlain's pass, are
 // masked key by key.  With kMarks the scores are 0, so that each key that a row sees counts, the
 // ones of the least probabilities too.
-template <int N>
+template <int UP, int N>
 __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int limit, int pass,
                                              float &m, float &l, float &factor) {
     const bool none = limit <= 0;
@@ -309,7 +314,7 @@ __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int li
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
     }
     top = column_max(none ? kNegInf : top) * scale2;
-    const bool moved = __any(top > m + kSlack);
+    const bool moved = __any(top > m + kSlack<UP>);
     factor = 1.0f;
     if (moved) {
         const float now = fmaxf(m, top);
@@ -317,7 +322,7 @@ __device__ __forceinline__ bool softmax_step(f32x4 (&s)[N], float scale2, int li
         m = now;
         l *= factor;
     }
-    const float base = none ? -kNegInf : m == kNegInf ? 0.0f : m;
+    const float base = none ? -kNegInf : m == kNegInf ? 0.0f : m - UP;
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < N; ++t) {
@@ -340,6 +345,12 @@ __device__ __forceinline__ int step_limit(bool selected, int last_key, int first
 template <typename T, bool PARTS>
 __device__ __forceinline__ float row_factor(float sum) {
     return sum > 0.0f ? (PARTS ? kPartsScale<T> : 1.0f) / sum : sum == 0.0f ? 0.0f : sum;
+}
+
+// The log of a row's sum of exponentials, from its maximum and sum of base 2.
+template <typename T, bool PARTS>
+__device__ __forceinline__ float row_lse(float m, float sum) {
+    return sum == 0.0f ? kNegInf : (m - kUp<T, PARTS> + log2_fast(sum)) * kLn2;
 }
 
 // A lane's rows of a tile: COLS of them, 16 apart.
@@ -425,7 +436,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
 #pragma unroll
             for (int x = 0; x < COLS; ++x) {
                 float factor;
-                if (softmax_step<BN / 16>(p[x], scale2, limit[x], pass, m[x], l[x], factor)) {
+                if (softmax_step<kUp<T, PARTS>>(p[x], scale2, limit[x], pass, m[x], l[x], factor)) {
 #pragma unroll
                     for (int i = 0; i < DP / 16; ++i) o[x][i] *= factor;
                 }
@@ -454,7 +465,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(Forward<T> a) {
             }
             if (a.lse && g == 0) {
                 a.lse[(static_cast<int64_t>(tile.b) * s.queries + t) * s.q_heads + head] =
-                    sum == 0.0f ? kNegInf : (m[x] + log2_fast(sum)) * kLn2;
+                    row_lse<T, PARTS>(m[x], sum);
             }
         }
         if (pass == kPlain && !__syncthreads_or(wrong != wrong)) break;
@@ -558,7 +569,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
             if (step + stride < steps) load(step + stride);
             if (!__any(limit > 0)) continue;
             float factor;
-            if (softmax_step<2>(p[0], scale2, limit, pass, m, l, factor)) {
+            if (softmax_step<kUp<T, true>>(p[0], scale2, limit, pass, m, l, factor)) {
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) o[0][i] *= factor;
             }
@@ -648,7 +659,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2) void split_kernel
             if (col < s.dim && pass != kPlain) store_again(out, v * inverse, pass);
             if (col == 0 && a.lse) {
                 a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + t) * s.q_heads + hd] =
-                    sum == 0.0f ? kNegInf : (top + log2_fast(sum)) * kLn2;
+                    row_lse<T, true>(top, sum);
             }
         }
         if (ONE || pass == kFinite) break;
@@ -682,7 +693,7 @@ __global__ __launch_bounds__(DP) void join_kernel(Forward<T> a, int splits, Part
     if (col < s.dim) a.out.row(tile.b, tile.t0 + t, hd)[col] = static_cast<T>(v * inverse);
     if (col == 0 && a.lse) {
         a.lse[(static_cast<int64_t>(tile.b) * s.queries + tile.t0 + t) * s.q_heads + hd] =
-            sum == 0.0f ? kNegInf : (top + log2_fast(sum)) * kLn2;
+            row_lse<T, true>(top, sum);
     }
 }
 

@@ -119,3 +119,25 @@ def test_infinite_score_gradients(gpu, dim, block, dtype):
     assert torch.isnan(dq).all() and torch.isnan(dk[:, 7]).all() and torch.isfinite(dv).all()
     others = torch.arange(40) != 7
     assert torch.equal(dk[:, others].float(), (-math.inf * q.sign().float()).expand(1, 39, 1, dim))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [(2, 1, 200, 4, 2, 72, 64, 4), (1, 3, 200, 4, 2, 128, 32, 7),
+                                   (64, 1, 200, 32, 8, 64, 64, 4)], ids=str)
+@pytest.mark.parametrize("behind", (8.0, 10.0, 12.0, 14.0, 16.0))
+def test_infinite_values_of_small_probabilities(gpu, sizes, behind, dtype):
+    """A value that is infinite makes the result that infinity, whatever share its key has, down to
+    the least probability that the type holds (2^-24 of the largest in float16)."""
+    batch, queries, keys, heads, kv_heads, dim, block, count = sizes
+    g = torch.Generator().manual_seed(56)
+    q = torch.zeros(batch, queries, heads, dim, dtype=dtype)
+    k = torch.zeros(batch, keys, kv_heads, dim, dtype=dtype)
+    v = torch.randn(batch, keys, kv_heads, dim, generator=g).to(dtype)
+    q[..., 0] = 1.0
+    k[:, 3, :, 0], k[:, 70, :, 0] = -behind, -behind - 0.375
+    v[:, 3, :, 1], v[:, 70, :, 2] = math.inf, -math.inf
+    ids = torch.arange(count, dtype=torch.int32).expand(batch, queries, kv_heads, count)
+    got = nacho_amd.gpu_block_attention(*(x.to(gpu) for x in (q, k, v, ids.contiguous())), block,
+                                        scale=1.0).cpu()
+    assert (got[..., 1] == math.inf).all() and (got[..., 2] == -math.inf).all()
+    assert torch.isfinite(got[..., 3:]).all()

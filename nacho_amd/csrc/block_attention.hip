@@ -972,7 +972,7 @@ struct Items {
 // with float16 (0.0024 and 0.0003 with one rounded part); training steps of 2 x 4096 queries of 16
 // heads of 128 take 541 us instead of 504 for it.
 //
-// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 237 us for 90 GFLOP (rows that did not
+// 2 x 4096 queries of 16 heads of 128, 12 of 64 blocks: 240 us for 90 GFLOP (rows that did not
 // select the block take no part; with one rounded part 203, and 1146 with one workgroup per block
 // instead of items).  LDS is the bound, 40% of a CU's time and waits for it, before matrix products
 // with 34%: a wavefront's 16 keys use each fragment once.  Two column tiles use it twice: for heads

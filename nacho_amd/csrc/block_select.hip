@@ -11,7 +11,7 @@
 // heads into LDS and goes over the blocks 64 at a time, 16 to a wavefront. 8192 queries of 32
 // heads of 128 against 128 blocks: 30 us, where reading q and writing the scores would take 18.
 // 48 sequences' tokens against the 320 of 512 blocks that they have on average (63 MB of means): 15
-// to 16 us, 4 TB/s, where a copy's rate would take 11.3: a workgroup's first means are on their way
+// to 17 us, 4 TB/s, where a copy's rate would take 11.3: a workgroup's first means are on their way
 // only when q's heads are summed, and each step's only when the step before is multiplied.  32 or
 // 64 queries to a workgroup are no faster for many queries and 1.3 us slower there.
 //

@@ -462,6 +462,79 @@ int nacho_combine_backward(int32_t dtype, int64_t tokens, int32_t per_token, int
                            const void *dout, int64_t dout_stride, void *drows, float *dweights,
                            void *stream);
 
+/* ---- the ends of a training step --------------------------------------------------------
+ * Words to rows, rows to a loss over the words, and what becomes of the gradients before they are
+ * used.  The contract is that of the entry points above: operands of one type, float32 sums in a
+ * fixed order, results in the caller's buffers, asynchronous on `stream`, nothing read back. */
+
+/* At most so many words, and so many tokens of a loss. */
+#define NACHO_MAX_WORDS ((int64_t)1 << 30)
+
+/* rows[tokens][width] = scale * table[ids[token]]: a row of zeros for an id (of `id_bytes` = 4 or 8
+ * bytes) outside [0, words).  stride: elements between the table's rows; rows are contiguous. */
+int nacho_embedding(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float scale,
+                    const void *ids, int32_t id_bytes, const void *table, int64_t stride,
+                    void *rows, void *stream);
+
+/* The gradient of nacho_embedding: dtable[words][width] = scale * the sum of dout[token] over the
+ * tokens with the word's id, in their order; 0 for a word without.  stride: elements between
+ * dout's rows; dtable is contiguous. */
+int nacho_embedding_backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width,
+                             float scale, const void *ids, int32_t id_bytes, const void *dout,
+                             int64_t stride, void *dtable, void *stream,
+                             const nacho_allocator *alloc);
+
+/* What becomes of the tokens' losses: they are the result, or their mean or sum. */
+#define NACHO_LOSS_NONE 0
+#define NACHO_LOSS_MEAN 1
+#define NACHO_LOSS_SUM 2
+/* Elements of a row of a loss, at most. */
+#define NACHO_MAX_LOSS_WIDTH ((int64_t)1 << 20)
+
+/* Cross entropy of z = scale * x[tokens][width] . table[words][width] against targets[tokens] (ids
+ * of `id_bytes` = 4 or 8 bytes): log(sum over words of exp(z)) - z[target] for each token, and 0,
+ * not counted in a mean, for a token whose target is outside [0, words).  loss: [tokens] or [1]; the
+ * mean of no tokens is 0.  stats (NULL: not wanted), for the backward pass: [2][tokens], the
+ * greatest z and the sum of exp(z - greatest); 0 and 1 for a token without a target.  The logits are
+ * never in memory.  Strides in elements, rows contiguous. */
+int nacho_linear_cross_entropy(int32_t dtype, int64_t tokens, int64_t words, int64_t width,
+                               float scale, int32_t reduction, const void *x, int64_t x_stride,
+                               const void *table, int64_t table_stride, const void *targets,
+                               int32_t id_bytes, float *loss, float *stats, void *stream,
+                               const nacho_allocator *alloc);
+
+/* The gradients of nacho_linear_cross_entropy, contiguous, from that of its result (dloss: [tokens]
+ * or [1]) and its stats: dx[tokens][width], 0 for a token without a target, and
+ * dtable[words][width].  Either may be NULL. */
+int nacho_linear_cross_entropy_backward(int32_t dtype, int64_t tokens, int64_t words,
+                                        int64_t width, float scale, int32_t reduction,
+                                        const void *x, int64_t x_stride, const void *table,
+                                        int64_t table_stride, const void *targets,
+                                        int32_t id_bytes, const float *stats, const float *dloss,
+                                        void *dx, void *dtable, void *stream,
+                                        const nacho_allocator *alloc);
+
+/* A tensor of `size` elements one after another, in `data`; `out` (nacho_clip_grad_norm only) takes
+ * its scaled elements and may be `data`.  Types: NACHO_F32 ... */
+typedef struct nacho_gradient {
+    const void *data;
+    void *out;
+    int64_t size;
+    int32_t dtype, out_dtype;
+} nacho_gradient;
+
+/* norm[1] = the root of the sum of the squares of all elements of the `count` tensors, which is
+ * summed in float64. */
+int nacho_grad_norm(const nacho_gradient *tensors, int64_t count, float *norm, void *stream,
+                    const nacho_allocator *alloc);
+
+/* The same, and every tensor's elements times min(1, max_norm / (norm + 1e-6)), that factor rounded
+ * to float32, into its `out` in `out_dtype`, the tensor's own or NACHO_F32.  A norm that is no
+ * number makes all of them that.  max_norm: 0 or more; infinity copies.  No `out` may overlap
+ * another tensor's data or `out`, nor its own data but for being it. */
+int nacho_clip_grad_norm(const nacho_gradient *tensors, int64_t count, float max_norm,
+                         float *norm, void *stream, const nacho_allocator *alloc);
+
 /* ---- input validation ------------------------------------------------------------
  * The entry points trust operand contents, as the reference's generated code does.  This
  * checks a CSR operand against the input contract on the device: pos[0] == 0, pos

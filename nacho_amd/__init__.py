@@ -7,7 +7,9 @@ libnacho_hip.so through its C ABI (include/nacho_hip.h); nothing here computes o
 except the file readers (host C++ in the same library).
 
 Beside the reference's surface: products of dense rows with structure that scores decide at run
-time, attention over selected blocks of keys (blocks.py) and tokens sorted by expert (routing.py).
+time, attention over selected blocks of keys (blocks.py) and tokens sorted by expert (routing.py);
+and the ends of a training step, words to rows and rows to a loss over the words (vocabulary.py),
+the gradients' norm and clipping (gradients.py).
 """
 
 from .blocks import (  # noqa: F401
@@ -18,6 +20,7 @@ from .blocks import (  # noqa: F401
     gpu_block_select,
 )
 from .convert import to_coo, to_coo3, to_csf3, to_csr, to_dcsr  # noqa: F401
+from .gradients import gpu_clip_grad_norm, gpu_grad_norm  # noqa: F401
 from .ops import (  # noqa: F401
     cached_bytes,
     gpu_coo3d_add_f32,
@@ -48,5 +51,11 @@ from .io import COO2D, COO3D_parsed, parse2D, parse3D_i32_f32  # noqa: F401
 from .routing import Route, gpu_combine, gpu_dispatch, gpu_route  # noqa: F401
 from .tensors import (  # noqa: F401
     COO3_gpu, COO_gpu, CSF3_gpu, CSR64_gpu, CSR_gpu, DCSR_gpu, Scalar_gpu)
+from .vocabulary import (  # noqa: F401
+    gpu_embedding,
+    gpu_embedding_backward,
+    gpu_linear_cross_entropy,
+    gpu_linear_cross_entropy_backward,
+)
 
 __version__ = "0.1.0"

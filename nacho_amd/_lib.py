@@ -161,6 +161,16 @@ class BlockAttentionArgs(ctypes.Structure):
     ]
 
 
+class Gradient(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("size", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+    ]
+
+
 class Allocator(ctypes.Structure):
     _fields_ = [
         ("ctx", ctypes.c_void_p),
@@ -206,8 +216,9 @@ ENTRY_POINTS_NOALLOC = {
 
 _I32, _I64, _PTR = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 _HEADS, _ALLOC = ctypes.POINTER(Heads), ctypes.POINTER(Allocator)
+_LOSS = (_I32, _I64, _I64, _I64, ctypes.c_float, _I32, _PTR, _I64, _PTR, _I64, _PTR, _I32)
 
-# dense rows through computed structure: name -> arguments
+# operators on dense rows: name -> arguments
 ENTRY_POINTS_DENSE = {
     "nacho_block_attention": (ctypes.POINTER(BlockAttentionArgs), _PTR, _ALLOC),
     "nacho_block_attention_backward": (ctypes.POINTER(BlockAttentionArgs), _PTR, _ALLOC),
@@ -219,6 +230,13 @@ ENTRY_POINTS_DENSE = {
     "nacho_combine": (_I32, _I64, _I32, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR),
     "nacho_combine_backward": (_I32, _I64, _I32, _I32, _I64, _PTR, _I64, _PTR, _PTR, _PTR, _PTR,
                                _I64, _PTR, _PTR, _PTR),
+    "nacho_embedding": (_I32, _I64, _I64, _I64, ctypes.c_float, _PTR, _I32, _PTR, _I64, _PTR, _PTR),
+    "nacho_embedding_backward": (_I32, _I64, _I64, _I64, ctypes.c_float, _PTR, _I32, _PTR, _I64,
+                                 _PTR, _PTR, _ALLOC),
+    "nacho_linear_cross_entropy": (*_LOSS, _PTR, _PTR, _PTR, _ALLOC),
+    "nacho_linear_cross_entropy_backward": (*_LOSS, _PTR, _PTR, _PTR, _PTR, _PTR, _ALLOC),
+    "nacho_grad_norm": (ctypes.POINTER(Gradient), _I64, _PTR, _PTR, _ALLOC),
+    "nacho_clip_grad_norm": (ctypes.POINTER(Gradient), _I64, ctypes.c_float, _PTR, _PTR, _ALLOC),
 }
 
 _lib = None

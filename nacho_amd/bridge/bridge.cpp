@@ -17,6 +17,7 @@
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <exception>
 #include <initializer_list>
@@ -703,6 +704,286 @@ PyObject *combine_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// ---- the ends of a training step ----------------------------------------------------------
+
+// Ids of any shape, contiguous, and their bytes.
+at::Tensor ids_of(PyObject *o, int device, int32_t *bytes) {
+    need(THPVariable_Check(o));
+    const at::Tensor &t = THPVariable_Unpack(o);
+    need(t.is_cuda() && t.get_device() == device && t.layout() == at::kStrided);
+    need(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt);
+    *bytes = static_cast<int32_t>(t.element_size());
+    return t.contiguous();
+}
+
+// A tensor [..., width] as rows, and the elements between them.
+at::Tensor flat_rows(PyObject *o, int device, int64_t *stride) {
+    need(THPVariable_Check(o));
+    at::Tensor t = THPVariable_Unpack(o);
+    need(t.is_cuda() && t.get_device() == device && t.dim() >= 1 && t.layout() == at::kStrided);
+    type_code(t.scalar_type());
+    const int64_t width = t.size(-1);
+    if (t.dim() != 2) t = t.reshape({width > 0 ? t.numel() / width : t.numel(), width});
+    if (t.size(1) > 1 && t.stride(1) != 1) t = t.contiguous();
+    *stride = t.size(0) > 1 ? t.stride(0) : t.size(1);
+    return t;
+}
+
+// A table's rows: no row in another.
+at::Tensor table_of(PyObject *o, int device, int64_t *stride) {
+    at::Tensor t = rows_of(o, device, stride);
+    type_code(t.scalar_type());
+    if (*stride < t.size(1)) {
+        t = t.contiguous();
+        *stride = t.size(1);
+    }
+    return t;
+}
+
+void *ids_data(const at::Tensor &t) { return t.numel() > 0 ? t.data_ptr() : nullptr; }
+
+std::vector<int64_t> with_width(at::IntArrayRef shape, int64_t width) {
+    std::vector<int64_t> out(shape.begin(), shape.end());
+    out.push_back(width);
+    return out;
+}
+
+// embedding(entry, stream, device, ids, table, scale) -> rows
+PyObject *embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 6)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        int32_t bytes = 0;
+        int64_t stride = 0;
+        const at::Tensor ids = ids_of(args[3], w.device, &bytes);
+        const at::Tensor table = table_of(args[4], w.device, &stride);
+        const float scale = float_of(args[5]);
+        at::Tensor out = at::empty(with_width(ids.sizes(), table.size(1)), table.options());
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_embedding)>(w.entry)(
+                type_code(table.scalar_type()), ids.numel(), table.size(0), table.size(1), scale,
+                ids_data(ids), bytes, rows_data(table), stride, rows_data(out), w.stream);
+        });
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// embedding_backward(entry, stream, device, dout, ids, words, scale) -> dtable
+PyObject *embedding_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 7)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        int32_t bytes = 0;
+        int64_t stride = 0;
+        const at::Tensor dout = flat_rows(args[3], w.device, &stride);
+        const at::Tensor ids = ids_of(args[4], w.device, &bytes);
+        const int64_t words = int_of(args[5]);
+        const float scale = float_of(args[6]);
+        const at::Tensor &given = THPVariable_Unpack(args[3]);
+        need(words >= 0 && given.sizes().slice(0, given.dim() - 1) == ids.sizes());
+        at::Tensor dtable = at::empty({words, dout.size(1)}, dout.options());
+        Scratch scratch(w.device);
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_embedding_backward)>(w.entry)(
+                type_code(dout.scalar_type()), ids.numel(), words, dout.size(1), scale,
+                ids_data(ids), bytes, rows_data(dout), stride, rows_data(dtable), w.stream,
+                &scratch.allocator);
+        });
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(dtable);
+    });
+}
+
+// x, table and targets of a loss.
+struct Loss {
+    at::Tensor x, table, targets;
+    int64_t x_stride = 0, table_stride = 0;
+    int32_t type = 0, id_bytes = 0;
+
+    Loss(PyObject *const *args, int device) {
+        x = flat_rows(args[0], device, &x_stride);
+        table = table_of(args[1], device, &table_stride);
+        targets = ids_of(args[2], device, &id_bytes);
+        type = type_code(x.scalar_type());
+        const at::Tensor &given = THPVariable_Unpack(args[0]);
+        need(table.scalar_type() == x.scalar_type() && table.size(1) == x.size(1) &&
+             table.size(0) > 0 && table.size(1) > 0 &&
+             given.sizes().slice(0, given.dim() - 1) == targets.sizes());
+    }
+};
+
+// linear_cross_entropy(entry, stream, device, x, table, targets, scale, reduction, want_stats)
+//     -> (loss, stats) or (loss,)
+PyObject *linear_cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 9)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        const Loss t(args + 3, w.device);
+        const float scale = float_of(args[6]);
+        const int32_t reduction = int_of(args[7]);
+        const auto options = t.x.options().dtype(at::kFloat);
+        const int64_t tokens = t.targets.numel();
+        at::Tensor loss = reduction == NACHO_LOSS_NONE ? at::empty(t.targets.sizes(), options)
+                                                       : at::empty({}, options);
+        at::Tensor stats;
+        if (args[8] == Py_True) stats = at::empty({2, tokens}, options);
+        Scratch scratch(w.device);
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_linear_cross_entropy)>(w.entry)(
+                t.type, tokens, t.table.size(0), t.table.size(1), scale, reduction,
+                rows_data(t.x), t.x_stride, rows_data(t.table), t.table_stride,
+                ids_data(t.targets), t.id_bytes, data_or_null<float>(loss),
+                stats.defined() ? data_or_null<float>(stats) : nullptr, w.stream,
+                &scratch.allocator);
+        });
+        if (rc != 0) return PyLong_FromLong(rc);
+        return stats.defined() ? tuple_of({loss, stats}) : tuple_of({loss});
+    });
+}
+
+// linear_cross_entropy_backward(entry, stream, device, x, table, targets, stats, dloss, scale,
+//                               reduction, want_dx, want_dtable) -> (dx or None, dtable or None)
+PyObject *linear_cross_entropy_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 12)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        const Loss t(args + 3, w.device);
+        const int64_t tokens = t.targets.numel();
+        const at::Tensor stats = tensor(args[6], w.device, 2, at::kFloat).contiguous();
+        const float scale = float_of(args[8]);
+        const int32_t reduction = int_of(args[9]);
+        const bool each = reduction == NACHO_LOSS_NONE;
+        const at::Tensor dloss =
+            tensor(args[7], w.device, each ? t.targets.dim() : 0, at::kFloat).contiguous();
+        need(stats.size(0) == 2 && stats.size(1) == tokens &&
+             (!each || dloss.sizes() == t.targets.sizes()));
+        at::Tensor dx, dtable;
+        if (args[10] == Py_True) {
+            dx = at::empty(THPVariable_Unpack(args[3]).sizes(), t.x.options());
+        }
+        if (args[11] == Py_True) dtable = at::empty(t.table.sizes(), t.table.options());
+        Scratch scratch(w.device);
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_linear_cross_entropy_backward)>(w.entry)(
+                t.type, tokens, t.table.size(0), t.table.size(1), scale, reduction,
+                rows_data(t.x), t.x_stride, rows_data(t.table), t.table_stride,
+                ids_data(t.targets), t.id_bytes, data_or_null<float>(stats),
+                data_or_null<float>(dloss), dx.defined() ? rows_data(dx) : nullptr,
+                dtable.defined() ? rows_data(dtable) : nullptr, w.stream, &scratch.allocator);
+        });
+        if (rc != 0) return PyLong_FromLong(rc);
+        return tuple_of({dx, dtable});  // (an undefined tensor is None)
+    });
+}
+
+// A tuple's tensors, strided, of the types that rows have.
+std::vector<at::Tensor> tensors_of(PyObject *o, int device) {
+    need(PyTuple_CheckExact(o));
+    std::vector<at::Tensor> out;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) {
+        PyObject *x = PyTuple_GET_ITEM(o, i);
+        need(THPVariable_Check(x));
+        const at::Tensor &t = THPVariable_Unpack(x);
+        need(t.is_cuda() && t.get_device() == device && t.layout() == at::kStrided);
+        type_code(t.scalar_type());
+        out.push_back(t);
+    }
+    return out;
+}
+
+nacho_gradient described(const at::Tensor &t) {
+    const int32_t type = type_code(t.scalar_type());
+    return {rows_data(t), nullptr, t.numel(), type, type};
+}
+
+// grad_norm(entry, stream, device, tensors) -> norm
+PyObject *grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 4)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        std::vector<at::Tensor> tensors = tensors_of(args[3], w.device);
+        need(!tensors.empty());
+        std::vector<nacho_gradient> list;
+        for (at::Tensor &t : tensors) {
+            if (!t.is_non_overlapping_and_dense()) t = t.clone(at::MemoryFormat::Contiguous);
+            list.push_back(described(t));
+        }
+        at::Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
+        Scratch scratch(w.device);
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_grad_norm)>(w.entry)(
+                list.data(), static_cast<int64_t>(list.size()), norm.data_ptr<float>(), w.stream,
+                &scratch.allocator);
+        });
+        return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(norm);
+    });
+}
+
+// Whether some memory that is written is another tensor's too (or its own data, moved).
+bool writes_overlap(const std::vector<nacho_gradient> &list) {
+    struct Span {
+        uintptr_t begin, end;
+        bool written;
+    };
+    std::vector<Span> spans;
+    for (const nacho_gradient &t : list) {
+        if (t.size == 0) continue;
+        auto span = [&](const void *p, int32_t type, bool written) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            spans.push_back({at, at + static_cast<uintptr_t>(t.size) * (type == NACHO_F32 ? 4 : 2),
+                             written});
+        };
+        span(t.out, t.out_dtype, true);
+        if (t.data != t.out || t.dtype != t.out_dtype) span(t.data, t.dtype, false);
+    }
+    std::sort(spans.begin(), spans.end(),
+              [](const Span &a, const Span &b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;  // the ends so far
+    for (const Span &x : spans) {
+        if (x.begin < (x.written ? any : written)) return true;
+        any = std::max(any, x.end);
+        if (x.written) written = std::max(written, x.end);
+    }
+    return false;
+}
+
+// clip_grad_norm(entry, stream, device, tensors, outs, max_norm) -> norm
+PyObject *clip_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (!arguments(n, 6)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const Where w = where(args);
+        std::vector<at::Tensor> tensors = tensors_of(args[3], w.device);
+        const std::vector<at::Tensor> outs = tensors_of(args[4], w.device);
+        const float max_norm = float_of(args[5]);
+        need(!tensors.empty() && outs.size() == tensors.size());
+        std::vector<nacho_gradient> list;
+        for (size_t i = 0; i < outs.size(); ++i) {
+            at::Tensor &t = tensors[i];
+            const at::Tensor &out = outs[i];
+            need(out.is_non_overlapping_and_dense() && out.sizes() == t.sizes() &&
+                 (out.scalar_type() == t.scalar_type() || out.scalar_type() == at::kFloat));
+            if (t.strides() != out.strides()) {  // elements in out's order
+                t = at::empty_strided(out.sizes(), out.strides(), t.options()).copy_(t);
+            }
+            list.push_back(described(t));
+            list.back().out = rows_data(out);
+            list.back().out_dtype = type_code(out.scalar_type());
+        }
+        need(!writes_overlap(list));
+        at::Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
+        Scratch scratch(w.device);
+        const int rc = unlocked([&] {
+            return reinterpret_cast<decltype(&nacho_clip_grad_norm)>(w.entry)(
+                list.data(), static_cast<int64_t>(list.size()), max_norm, norm.data_ptr<float>(),
+                w.stream, &scratch.allocator);
+        });
+        if (rc != 0) return PyLong_FromLong(rc);
+        for (const at::Tensor &out : outs) {  // (so that autograd notices the write)
+            if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+        }
+        return THPVariable_Wrap(norm);
+    });
+}
+
 // set_free(address of nacho_free)
 PyObject *set_free(PyObject *, PyObject *arg) {
     void *p = PyLong_AsVoidPtr(arg);
@@ -728,6 +1009,14 @@ PyMethodDef g_methods[] = {
     {"dispatch", fast(dispatch), METH_FASTCALL, "nacho_dispatch."},
     {"combine", fast(combine), METH_FASTCALL, "nacho_combine."},
     {"combine_backward", fast(combine_backward), METH_FASTCALL, "nacho_combine_backward."},
+    {"embedding", fast(embedding), METH_FASTCALL, "nacho_embedding."},
+    {"embedding_backward", fast(embedding_backward), METH_FASTCALL, "nacho_embedding_backward."},
+    {"linear_cross_entropy", fast(linear_cross_entropy), METH_FASTCALL,
+     "nacho_linear_cross_entropy."},
+    {"linear_cross_entropy_backward", fast(linear_cross_entropy_backward), METH_FASTCALL,
+     "nacho_linear_cross_entropy_backward."},
+    {"grad_norm", fast(grad_norm), METH_FASTCALL, "nacho_grad_norm."},
+    {"clip_grad_norm", fast(clip_grad_norm), METH_FASTCALL, "nacho_clip_grad_norm."},
     {"set_free", set_free, METH_O, "Address of nacho_free."},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -1,0 +1,830 @@
+// The loss of rows over a vocabulary, and its gradients, without the logits in memory.
+//
+// With z = scale x w^T (tokens x words), a token's loss is log s + (m - z[target]) where m is its
+// greatest logit and s the sum of exp(z - m); dz = (exp(z - m) / s - [word is target]) c with the
+// gradient c of the token's loss; dx = scale dz w, dw = scale dz^T x.
+//
+// Tokens without a target are left out before anything else: the others' rows are gathered, and
+// all products have as many rows as there are targets (a number that only the device knows; tiles
+// past it end at once).  What the rows left out hold never counts.
+//
+// forward: one product, whose tiles of logits are reduced to m and s where they stand in
+// registers, words in the result's rows: a lane has one token's logits, and only two exchanges and
+// one pass through LDS join them.  Tiles' parts are joined by a second kernel, token by token.
+// backward: the words are taken in pieces.  A piece's logits are worked out again and become dz in
+// the rows' type, in scratch; two more products take it from there.  dx is summed in float32 over
+// the pieces.
+//
+// Rounding: sums, m, s and losses are float32 (the sum of the losses float64).  dz reaches the
+// gradients' products in the rows' type, without c's size: mean and sum have the factor c in
+// common, which the results are multiplied by in float32, and else the largest |c| is taken out.
+// float16 takes 2^14 dz: probabilities down to 2^-28 keep their bits, and below 2^-38 add nothing.
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+#include <new>
+#include <type_traits>
+
+#include "dense_product.hpp"
+#include "dense_rows.hpp"
+#include "runtime.hpp"
+
+namespace nacho {
+namespace cross_entropy {
+
+using dense::Across;
+using dense::Along;
+using dense::element_aligned;
+using dense::f32x4;
+using dense::item_of;
+using dense::kLog2e;
+using dense::kNegInf;
+using dense::Matrix;
+using dense::Product;
+using dense::Shape;
+
+constexpr int kThreads = 256;
+
+// ---- the tokens that have a target ------------------------------------------------------
+
+struct Targets {
+    const void *ids;
+    int bytes;  // 4 or 8
+    int64_t words;
+
+    // Word of a token, -1 for one without.
+    __device__ __forceinline__ int operator()(int64_t t) const {
+        const int64_t id = bytes == 8 ? static_cast<const int64_t *>(ids)[t]
+                                      : static_cast<const int32_t *>(ids)[t];
+        return id >= 0 && id < words ? static_cast<int>(id) : -1;
+    }
+};
+
+// What the kernels know of the tokens: `held` of them have a target.
+struct Held {
+    int *count;     // [1]
+    int *slot;      // [tokens]: place among them, -1 for one without a target
+    int *token;     // [held]
+    int *target;    // [held]
+    float *factor;  // [held]: gradient of the token's loss over `common` (the backward pass)
+    float *common;  // [1]
+};
+
+enum Reduction { kNone = NACHO_LOSS_NONE, kMean = NACHO_LOSS_MEAN, kSum = NACHO_LOSS_SUM };
+
+constexpr int kListThreads = 1024;
+constexpr int kListPer = 8;  // tokens of a thread and step
+
+// One workgroup: places in order of the tokens and, with dloss, the gradients' factors.
+__global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int tokens,
+                                                            int reduction,
+                                                            const float *__restrict__ dloss,
+                                                            Held held) {
+    __shared__ int s_sums[kListThreads / dev::kWave];
+    __shared__ float s_max[kListThreads / dev::kWave];
+    int carry = 0;
+    float most = 0.0f;
+    for (int64_t t0 = 0; t0 < tokens; t0 += kListThreads * kListPer) {
+        const int64_t first = t0 + static_cast<int>(threadIdx.x) * kListPer;
+        int id[kListPer];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < kListPer; ++i) {
+            id[i] = first + i < tokens ? targets(first + i) : -1;
+            mine += id[i] >= 0 ? 1 : 0;
+        }
+        int total = 0;
+        int at = carry + dev::block_exclusive_sum<kListThreads>(mine, s_sums, total);
+        carry += total;
+#pragma unroll
+        for (int i = 0; i < kListPer; ++i) {
+            const int64_t t = first + i;
+            if (t < tokens) held.slot[t] = id[i] >= 0 ? at : -1;
+            if (id[i] >= 0) {
+                held.token[at] = static_cast<int>(t);
+                held.target[at] = id[i];
+                if (dloss && reduction == kNone) {
+                    const float c = fabsf(dloss[t]);
+                    most = most < c || c != c ? c : most;  // (no number stays)
+                }
+                ++at;
+            }
+        }
+    }
+    if (threadIdx.x == 0) *held.count = carry;
+    if (!dloss) return;
+    float common = 0.0f;
+    if (reduction == kNone) {
+#pragma unroll
+        for (int off = dev::kWave / 2; off > 0; off >>= 1) {
+            const float other = __shfl_xor(most, off, dev::kWave);
+            most = most < other || other != other ? other : most;
+        }
+        if (dev::lane() == 0) s_max[threadIdx.x / dev::kWave] = most;
+        __syncthreads();
+        for (int w = 0; w < kListThreads / dev::kWave; ++w) {
+            const float other = s_max[w];
+            common = common < other || other != other ? other : common;
+        }
+    } else {
+        common = reduction == kMean ? dloss[0] / static_cast<float>(max(carry, 1)) : dloss[0];
+    }
+    if (reduction == kNone && !(common < dense::kInf)) common = 1.0f;
+    if (threadIdx.x == 0) *held.common = common;
+    if (reduction != kNone) return;
+    for (int64_t t = threadIdx.x; t < tokens; t += kListThreads) {
+        const int id = targets(t);
+        if (id >= 0) held.factor[held.slot[t]] = common == 0.0f ? 0.0f : dloss[t] / common;
+    }
+}
+
+// Rows of `width` elements, one after another `padded` elements apart and zeros behind the width:
+// those of the listed tokens (token), or the first `rows` (null).
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict__ count,
+                                                          const int *__restrict__ token,
+                                                          int64_t rows, int64_t width,
+                                                          int64_t padded,
+                                                          const T *__restrict__ from,
+                                                          int64_t stride, T *__restrict__ to) {
+    const int64_t there = count ? *count : rows;
+    const int64_t per = padded / N;
+    const int64_t all = there * per;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all;
+         i += gridDim.x * static_cast<int64_t>(kThreads)) {
+        const int64_t row = i / per, col = i % per * N;
+        const int64_t source = token ? token[row] : row;
+        dense::Piece<T, N> piece;
+        if (col < width) {
+            piece = *reinterpret_cast<const dense::Piece<T, N> *>(from + source * stride + col);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) piece.v[j] = static_cast<T>(0.0f);
+        }
+        *reinterpret_cast<dense::Piece<T, N> *>(to + row * padded + col) = piece;
+    }
+}
+
+// ---- logits -----------------------------------------------------------------------------
+
+struct Logits {
+    const int *held;
+    int64_t width;         // of the gathered rows, and of the table's
+    const void *rows;      // [held][width]
+    const void *table;
+    int64_t table_stride;
+    int words;             // of this piece
+    int first;             // its first word
+    unsigned m_tiles, n_tiles;
+    const int *target;
+    float scale;
+    // the forward pass
+    float2 *parts;         // [held][m_tiles]: m and s of a tile's words
+    float *mine;           // [held]: the target's logit
+    // the backward pass
+    const float *most;     // m by token of the whole batch
+    const float *total;    // s
+    const int *token;
+    const float *factor;   // null: 1
+    void *dz;              // [held][dz_stride]
+    int64_t dz_stride;     // a multiple of the rows of a tile: words past the piece's get zeros
+};
+
+template <typename T>
+constexpr float kDzScale = __is_same(T, _Float16) ? 0x1p14f : 1.0f;
+
+// The tile's product of table and rows.
+template <typename T, typename S>
+__device__ __forceinline__ void logits_of(const Logits &a, int64_t v0, int64_t n0, int held,
+                                          T *lds, f32x4 (&z)[S::MT][S::NT]) {
+    const Matrix<T> table{static_cast<const T *>(a.table) + (a.first + v0) * a.table_stride,
+                          a.table_stride};
+    const Matrix<T> rows{static_cast<const T *>(a.rows) + n0 * a.width, a.width};
+    Product<T, S, Along, Along>::run(
+        table, static_cast<int>(min(a.words - v0, static_cast<int64_t>(S::BM))), rows,
+        static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))), a.width, lds, z);
+}
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void parts_kernel(Logits a) {
+    __shared__ __attribute__((aligned(16))) T lds[Product<T, S, Along, Along>::kLdsElements];
+    unsigned mt, nt;
+    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
+    const int held = *a.held;
+    const int64_t v0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
+    if (n0 >= held) return;
+    f32x4 z[S::MT][S::NT];
+    logits_of<T, S>(a, v0, n0, held, lds, z);
+    const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+    float2(*s_part)[S::BN] = reinterpret_cast<float2(*)[S::BN]>(lds);
+    __syncthreads();  // (the tiles have been read)
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int col = (wn * S::NT + t) * 16 + c;
+        const int64_t n = n0 + col;
+        // the target's place among this lane's words, if it is one of them
+        const int64_t target = n < held ? a.target[n] - v0 : -1;
+        float most = kNegInf;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int v = (wm * S::MT + i) * 16 + 4 * g + j;
+                float x = z[i][t][j] * a.scale;
+                if (v == target) a.mine[n] = x;
+                if (v0 + v >= a.words) x = kNegInf;
+                z[i][t][j] = x;
+                most = fmaxf(most, x);
+            }
+        }
+        most = dense::column_max(most);
+        // (with no finite logit: exp(-inf) of each)
+        const float base = most == kNegInf ? 0.0f : most;
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) total += dense::exp2_fast((z[i][t][j] - base) * kLog2e);
+        }
+        total = dense::column_sum(total);
+        if (g == 0) s_part[wm][col] = float2{most, total};
+    }
+    __syncthreads();
+    for (int col = threadIdx.x; col < S::BN; col += S::kThreads) {
+        if (n0 + col >= held) break;
+        float most = kNegInf, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < S::WM; ++w) most = fmaxf(most, s_part[w][col].x);
+        const float base = most == kNegInf ? 0.0f : most;
+#pragma unroll
+        for (int w = 0; w < S::WM; ++w) {
+            const float2 p = s_part[w][col];
+            total += p.y * dense::exp2_fast((p.x - base) * kLog2e);
+        }
+        a.parts[(n0 + col) * a.m_tiles + mt] = float2{most, total};
+    }
+}
+
+// A wavefront per token: its tiles' parts to m, s and the loss.
+__global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ slot,
+                                                        int tokens, unsigned tiles,
+                                                        const float2 *__restrict__ parts,
+                                                        const float *__restrict__ mine,
+                                                        float *__restrict__ most_of,
+                                                        float *__restrict__ total_of,
+                                                        float *__restrict__ loss) {
+    const int64_t t = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / dev::kWave;
+    if (t >= tokens) return;
+    const int at = slot[t];
+    if (at < 0) {
+        if (dev::lane() == 0) {
+            most_of[t] = 0.0f;
+            total_of[t] = 1.0f;
+            loss[t] = 0.0f;
+        }
+        return;
+    }
+    const float2 *from = parts + static_cast<int64_t>(at) * tiles;
+    float most = kNegInf, total = 0.0f;
+    for (unsigned i = dev::lane(); i < tiles; i += dev::kWave) {
+        const float2 p = from[i];
+        const float higher = fmaxf(most, p.x);
+        const float base = higher == kNegInf ? 0.0f : higher;
+        total = total * dense::exp2_fast((most - base) * kLog2e) +
+                p.y * dense::exp2_fast((p.x - base) * kLog2e);
+        most = higher;
+    }
+#pragma unroll
+    for (int off = dev::kWave / 2; off > 0; off >>= 1) {
+        const float other = __shfl_xor(most, off, dev::kWave);
+        const float other_total = __shfl_xor(total, off, dev::kWave);
+        const float higher = fmaxf(most, other);
+        const float base = higher == kNegInf ? 0.0f : higher;
+        total = total * dense::exp2_fast((most - base) * kLog2e) +
+                other_total * dense::exp2_fast((other - base) * kLog2e);
+        most = higher;
+    }
+    if (dev::lane() == 0) {
+        most_of[t] = most;
+        total_of[t] = total;
+        loss[t] = logf(total) + (most - mine[at]);
+    }
+}
+
+// The sum of the losses, or their mean over the tokens that have a target.
+__global__ __launch_bounds__(1024) void sum_kernel(const int *__restrict__ count, int64_t tokens,
+                                                   const float *__restrict__ each, int mean,
+                                                   float *__restrict__ loss) {
+    __shared__ double s_sum[1024 / dev::kWave];
+    double sum = 0.0;
+    for (int64_t t = threadIdx.x; t < tokens; t += 1024) sum += static_cast<double>(each[t]);
+    sum = dev::wave_sum(sum);
+    if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = sum;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    sum = 0.0;
+    for (int w = 0; w < 1024 / dev::kWave; ++w) sum += s_sum[w];
+    *loss = static_cast<float>(mean ? sum / max(*count, 1) : sum);
+}
+
+// dz of a piece.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dz_kernel(Logits a) {
+    __shared__ __attribute__((aligned(16))) T lds[Product<T, S, Along, Along>::kLdsElements];
+    unsigned mt, nt;
+    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
+    const int held = *a.held;
+    const int64_t v0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
+    if (n0 >= held) return;
+    f32x4 z[S::MT][S::NT];
+    logits_of<T, S>(a, v0, n0, held, lds, z);
+    const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
+        if (n >= held) continue;
+        const int64_t target = a.target[n] - static_cast<int64_t>(a.first) - v0;
+        const int token = a.token[n];
+        const float most = a.most[token], part = 1.0f / a.total[token];
+        const float factor = kDzScale<T> * (a.factor ? a.factor[n] : 1.0f);
+        T *to = static_cast<T *>(a.dz) + n * a.dz_stride + v0;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+            const int v = (wm * S::MT + i) * 16 + 4 * g;
+            f32x4 d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = z[i][t][j] * a.scale;
+                float p = dense::exp2_fast((x - most) * kLog2e) * part;
+                if (v + j == target) p -= 1.0f;
+                d[j] = v0 + v + j < a.words ? p * factor : 0.0f;
+            }
+            dense::store4<T>(to + v, d);
+        }
+    }
+}
+
+// ---- the gradients' products ------------------------------------------------------------
+
+struct Gradients {
+    const int *held;
+    const void *dz;
+    int64_t dz_stride;
+    const void *rows;     // gathered
+    const void *table;    // of the piece
+    int64_t table_stride;
+    int64_t words, width; // of the piece; of the results
+    int64_t padded;       // columns that the operands' rows have
+    unsigned m_tiles, n_tiles;
+    int64_t split;        // words of a split of dx's sums
+    int64_t tokens;       // rows of a split's sums
+    float *sums;          // [split][tokens][sums_stride]
+    int64_t sums_stride;
+    int first;            // whether the piece is the first
+    const float *common;
+    float scale;
+    void *dtable;         // of the piece, [words][width]
+};
+
+// dx: the columns of the table's rows by the tokens, over the words of a split.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dx_kernel(Gradients a) {
+    using P = Product<T, S, Across, Along>;
+    __shared__ __attribute__((aligned(16))) T lds[P::kLdsElements];
+    unsigned mt, nt;
+    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
+    const int held = *a.held;
+    const int64_t d0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
+    if (n0 >= held) return;
+    const int64_t v0 = blockIdx.y * a.split;
+    const Matrix<T> table{static_cast<const T *>(a.table) + v0 * a.table_stride + d0,
+                          a.table_stride};
+    const Matrix<T> dz{static_cast<const T *>(a.dz) + n0 * a.dz_stride + v0, a.dz_stride};
+    f32x4 sums[S::MT][S::NT];
+    P::run(table, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
+           static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))),
+           min(a.split, a.words - v0), lds, sums);
+    const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
+        if (n >= held) continue;
+        float *to = a.sums + (blockIdx.y * a.tokens + n) * a.sums_stride;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+            const int64_t d = d0 + (wm * S::MT + i) * 16 + 4 * g;
+            if (d < a.sums_stride) {
+                f32x4 *p = reinterpret_cast<f32x4 *>(to + d);
+                *p = a.first ? sums[i][t] : *p + sums[i][t];
+            }
+        }
+    }
+}
+
+// dx of every token: the splits' sums in their order, and 0 for a token without a target.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dx_join_kernel(const int *__restrict__ slot,
+                                                           int64_t tokens, int64_t width,
+                                                           const float *__restrict__ sums,
+                                                           int64_t stride, int splits,
+                                                           const float *__restrict__ common,
+                                                           float scale, T *__restrict__ dx) {
+    const float factor = *common * scale * (1.0f / kDzScale<T>);
+    const int64_t per = (width + 3) / 4;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < tokens * per;
+         i += gridDim.x * static_cast<int64_t>(kThreads)) {
+        const int64_t t = i / per, d = i % per * 4;
+        const int at = slot[t];
+        f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0) {
+            for (int s = 0; s < splits; ++s) {
+                sum += *reinterpret_cast<const f32x4 *>(sums + (s * tokens + at) * stride + d);
+            }
+            sum *= factor;
+        }
+        T *to = dx + t * width + d;
+        if (width % 4 == 0) {
+            dense::store4<T>(to, sum);
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                if (d + j < width) to[j] = static_cast<T>(sum[j]);
+            }
+        }
+    }
+}
+
+// dw of a piece: the columns of the gathered rows by the words, over the tokens.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dtable_kernel(Gradients a) {
+    using P = Product<T, S, Across, Across>;
+    __shared__ __attribute__((aligned(16))) T lds[P::kLdsElements];
+    unsigned mt, nt;
+    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
+    const int64_t d0 = static_cast<int64_t>(mt) * S::BM, v0 = static_cast<int64_t>(nt) * S::BN;
+    const Matrix<T> rows{static_cast<const T *>(a.rows) + d0, a.padded};
+    const Matrix<T> dz{static_cast<const T *>(a.dz) + v0, a.dz_stride};
+    f32x4 sums[S::MT][S::NT];
+    P::run(rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
+           static_cast<int>(min(a.dz_stride - v0, static_cast<int64_t>(S::BN))), *a.held, lds,
+           sums);
+    const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
+    const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
+    const int wm = wave / S::WN, wn = wave % S::WN;
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int64_t v = v0 + (wn * S::NT + t) * 16 + c;
+        if (v >= a.words) continue;
+        T *to = static_cast<T *>(a.dtable) + v * a.width;
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+            const int64_t d = d0 + (wm * S::MT + i) * 16 + 4 * g;
+            const f32x4 x = sums[i][t] * factor;
+            if (a.width % 4 == 0) {
+                if (d < a.width) dense::store4<T>(to + d, x);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (d + j < a.width) to[d + j] = static_cast<T>(x[j]);
+                }
+            }
+        }
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+struct Args {
+    int32_t dtype;
+    int64_t tokens, words, width;
+    float scale;
+    int32_t reduction;
+    const void *x;
+    int64_t x_stride;
+    const void *table;
+    int64_t table_stride;
+    const void *targets;
+    int32_t id_bytes;
+};
+
+int check(const Args &a) {
+    if (a.dtype < NACHO_F32 || a.dtype > NACHO_BF16 || a.tokens < 0 || a.words < 1 ||
+        a.width < 1 || !(a.scale - a.scale == 0.0f) || a.reduction < NACHO_LOSS_NONE ||
+        a.reduction > NACHO_LOSS_SUM || (a.id_bytes != 4 && a.id_bytes != 8)) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if (a.words > NACHO_MAX_WORDS || a.tokens > NACHO_MAX_WORDS || a.width > NACHO_MAX_LOSS_WIDTH) {
+        return NACHO_ERR_INDEX_OVERFLOW;
+    }
+    const int item = item_of(a.dtype);
+    if (!a.table || !element_aligned(a.table, item) || a.table_stride < a.width) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if (a.tokens > 0 && (!a.x || !a.targets || !element_aligned(a.x, item) ||
+                         !element_aligned(a.targets, a.id_bytes))) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    return NACHO_OK;
+}
+
+// The operands as the kernels take them: rows gathered and, where a table's rows are not whole
+// aligned pieces, a copy of it whose are.
+template <typename T>
+struct Operands {
+    Held held{};
+    T *rows = nullptr;
+    const T *table = nullptr;
+    int64_t width = 0;  // of rows, a multiple of a piece
+    int64_t table_stride = 0;
+
+    int start(Call &call, const Args &a, const float *dloss) {
+        constexpr int64_t kPer = 16 / sizeof(T);
+        const hipStream_t s = call.stream();
+        const size_t n = static_cast<size_t>(a.tokens);
+        int *ints = nullptr;
+        float *floats = nullptr;
+        NACHO_TRY(call.scratch_n(3 * n + 1, &ints));
+        held.count = ints;
+        held.slot = ints + 1;
+        held.token = held.slot + n;
+        held.target = held.token + n;
+        if (dloss) {
+            const size_t factors = a.reduction == NACHO_LOSS_NONE ? n : 0;
+            NACHO_TRY(call.scratch_n(1 + factors, &floats));
+            held.common = floats;
+            held.factor = factors ? floats + 1 : nullptr;
+        }
+        list_kernel<<<1, kListThreads, 0, s>>>(Targets{a.targets, a.id_bytes, a.words},
+                                               static_cast<int>(a.tokens), a.reduction, dloss,
+                                               held);
+        NACHO_TRY_HIP(hipGetLastError());
+        width = up(a.width, kPer);
+        NACHO_TRY(call.scratch_n(n * static_cast<size_t>(width), &rows));
+        NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, a.x, a.x_stride, rows));
+        table = static_cast<const T *>(a.table);
+        table_stride = a.table_stride;
+        if (!dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
+            table_stride * static_cast<int64_t>(sizeof(T)) > kMostStride) {
+            T *copy = nullptr;
+            NACHO_TRY(call.scratch_n(static_cast<size_t>(a.words * width), &copy));
+            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, a.table, a.table_stride, copy));
+            table = copy;
+            table_stride = width;
+        }
+        return NACHO_OK;
+    }
+
+    // (256 rows of a tile within the loads' 2 GB)
+    static constexpr int64_t kMostStride = int64_t{1} << 22;
+
+    int gather(hipStream_t s, const int *count, const int *token, int64_t n, int64_t columns,
+               const void *from, int64_t stride, T *to) const {
+        constexpr int kPer = 16 / sizeof(T);
+        const bool whole = dense::pieces(from, stride, columns, sizeof(T));
+        const int64_t threads = n * (width / (whole ? kPer : 1));
+        const int64_t groups = (threads + kThreads - 1) / kThreads;
+        const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
+        if (whole) {
+            gather_kernel<T, kPer><<<grid, kThreads, 0, s>>>(
+                count, token, n, columns, width, static_cast<const T *>(from), stride, to);
+        } else {
+            gather_kernel<T, 1><<<grid, kThreads, 0, s>>>(
+                count, token, n, columns, width, static_cast<const T *>(from), stride, to);
+        }
+        NACHO_TRY_HIP(hipGetLastError());
+        return NACHO_OK;
+    }
+};
+
+// Tiles by the number of tokens: a tile's products of a few tokens would be of nothing.
+template <typename T, typename F>
+int with_shape(int64_t tokens, F f) {
+    if constexpr (sizeof(T) == 4) {
+        if (tokens <= 16) return f(Shape<128, 16, 4, 1>{});
+        return f(Shape<128, 128, 2, 2>{});
+    } else {
+        if (tokens <= 16) return f(Shape<256, 16, 4, 1>{});
+        if (tokens <= 128) return f(Shape<256, 64, 4, 1>{});
+        return f(Shape<256, 256, 2, 4>{});
+    }
+}
+
+template <typename F>
+int with_type(int32_t dtype, F f) {
+    if (dtype == NACHO_F32) return f(float{});
+    if (dtype == NACHO_F16) return f(_Float16{});
+    return f(__bf16{});
+}
+
+// Tiles of a launch; 0 for more than a launch has.
+template <typename S>
+int64_t tiles_of(int64_t m, int64_t n, unsigned *m_tiles, unsigned *n_tiles) {
+    const int64_t a = up(m, S::BM) / S::BM, b = up(n, S::BN) / S::BN;
+    *m_tiles = static_cast<unsigned>(a);
+    *n_tiles = static_cast<unsigned>(b);
+    return a * b < (int64_t{1} << 32) / S::kThreads ? a * b : 0;
+}
+
+int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_allocator *alloc) {
+    NACHO_TRY(check(a));
+    if (!loss && (a.tokens > 0 || a.reduction != NACHO_LOSS_NONE)) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if (a.tokens == 0 && a.reduction == NACHO_LOSS_NONE) return NACHO_OK;
+    Call call(stream, alloc);
+    const hipStream_t s = call.stream();
+    return with_type(a.dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        return with_shape<T>(a.tokens, [&](auto shape) -> int {
+            using S = decltype(shape);
+            unsigned m_tiles = 0, n_tiles = 0;
+            const int64_t tiles = tiles_of<S>(a.words, a.tokens, &m_tiles, &n_tiles);
+            if (a.tokens > 0 && tiles == 0) return NACHO_ERR_INDEX_OVERFLOW;
+            Operands<T> ops;
+            const size_t n = static_cast<size_t>(a.tokens);
+            float *each = loss;
+            if (a.tokens > 0) {
+                NACHO_TRY(ops.start(call, a, nullptr));
+                float2 *parts = nullptr;
+                float *floats = nullptr;
+                const bool keep = stats != nullptr, sums = a.reduction != NACHO_LOSS_NONE;
+                NACHO_TRY(call.scratch_n(n * m_tiles, &parts));
+                NACHO_TRY(call.scratch_n(n * (1 + (keep ? 0 : 2) + (sums ? 1 : 0)), &floats));
+                float *most = keep ? stats : floats + n;
+                if (sums) each = floats + n * (keep ? 1 : 3);
+                Logits l{};
+                l.held = ops.held.count;
+                l.width = ops.width;
+                l.rows = ops.rows;
+                l.table = ops.table;
+                l.table_stride = ops.table_stride;
+                l.words = static_cast<int>(a.words);
+                l.m_tiles = m_tiles;
+                l.n_tiles = n_tiles;
+                l.target = ops.held.target;
+                l.scale = a.scale;
+                l.parts = parts;
+                l.mine = floats;
+                parts_kernel<T, S><<<static_cast<unsigned>(tiles), S::kThreads, 0, s>>>(l);
+                NACHO_TRY_HIP(hipGetLastError());
+                join_kernel<<<ceil_div(n, kThreads / dev::kWave), kThreads, 0, s>>>(
+                    ops.held.slot, static_cast<int>(a.tokens), m_tiles, parts, floats, most,
+                    most + n, each);
+                NACHO_TRY_HIP(hipGetLastError());
+            }
+            if (a.reduction != NACHO_LOSS_NONE) {
+                sum_kernel<<<1, 1024, 0, s>>>(ops.held.count, a.tokens, each,
+                                              a.tokens > 0 && a.reduction == NACHO_LOSS_MEAN,
+                                              loss);
+                NACHO_TRY_HIP(hipGetLastError());
+            }
+            return NACHO_OK;
+        });
+    });
+}
+
+// Bytes of a piece's dz, about, and its least words.
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+constexpr int64_t kPieceWords = 2048;
+// Workgroups that dx's products are split into, about, where there are few tiles, and a split's
+// least words.
+constexpr int64_t kSplitGroups = 512, kSplitWords = 512;
+
+int backward(const Args &a, const float *stats, const float *dloss, void *dx, void *dtable,
+             void *stream, const nacho_allocator *alloc) {
+    NACHO_TRY(check(a));
+    const int item = item_of(a.dtype);
+    if (!element_aligned(dx, item) || !element_aligned(dtable, item) ||
+        (a.tokens > 0 && (!stats || !dloss))) {
+        return NACHO_ERR_INVALID_ARGUMENT;
+    }
+    if ((!dx || a.tokens == 0) && !dtable) return NACHO_OK;
+    Call call(stream, alloc);
+    const hipStream_t s = call.stream();
+    return with_type(a.dtype, [&](auto type) -> int {
+        using T = decltype(type);
+        using Wide = std::conditional_t<sizeof(T) == 4, Shape<128, 128, 2, 2>,
+                                        Shape<256, 256, 2, 4>>;
+        if (a.tokens == 0) {
+            return dense::clear(s, static_cast<T *>(dtable), a.words * a.width);
+        }
+        return with_shape<T>(a.tokens, [&](auto shape) -> int {
+            using S = decltype(shape);
+            const size_t n = static_cast<size_t>(a.tokens);
+            int64_t piece = up(kPieceBytes / (a.tokens * item), 256);
+            if (piece < kPieceWords) piece = kPieceWords;
+            if (piece > up(a.words, 256)) piece = up(a.words, 256);
+            Logits l{};
+            Gradients d{};
+            unsigned dx_m = 0, dx_n = 0, dw_m = 0, dw_n = 0;
+            const int64_t dx_tiles = tiles_of<S>(a.width, a.tokens, &dx_m, &dx_n);
+            if (!dx_tiles || !tiles_of<S>(piece, a.tokens, &l.m_tiles, &l.n_tiles) ||
+                !tiles_of<Wide>(a.width, piece, &dw_m, &dw_n)) {
+                return NACHO_ERR_INDEX_OVERFLOW;
+            }
+            Operands<T> ops;
+            NACHO_TRY(ops.start(call, a, dloss));
+            T *dz = nullptr;
+            NACHO_TRY(call.scratch_n(n * static_cast<size_t>(piece), &dz));
+            int64_t splits = kSplitGroups / dx_tiles;
+            if (splits > piece / kSplitWords) splits = piece / kSplitWords;
+            if (splits < 1) splits = 1;
+            d.split = up((piece + splits - 1) / splits, 64);
+            splits = (piece + d.split - 1) / d.split;
+            d.sums_stride = up(a.width, 4);
+            if (dx) {
+                NACHO_TRY(call.scratch_n(static_cast<size_t>(splits) * n *
+                                             static_cast<size_t>(d.sums_stride), &d.sums));
+            }
+            l.held = d.held = ops.held.count;
+            l.width = d.padded = ops.width;
+            l.rows = d.rows = ops.rows;
+            l.table_stride = d.table_stride = ops.table_stride;
+            l.target = ops.held.target;
+            l.scale = d.scale = a.scale;
+            l.most = stats;
+            l.total = stats + n;
+            l.token = ops.held.token;
+            l.factor = ops.held.factor;
+            l.dz = dz;
+            d.dz = dz;
+            l.dz_stride = d.dz_stride = piece;
+            l.table = ops.table;
+            d.width = a.width;
+            d.tokens = a.tokens;
+            d.common = ops.held.common;
+            for (int64_t v = 0; v < a.words; v += piece) {
+                const int64_t words = a.words - v < piece ? a.words - v : piece;
+                l.first = static_cast<int>(v);
+                l.words = static_cast<int>(words);
+                const int64_t tiles = tiles_of<S>(words, a.tokens, &l.m_tiles, &l.n_tiles);
+                dz_kernel<T, S><<<static_cast<unsigned>(tiles), S::kThreads, 0, s>>>(l);
+                NACHO_TRY_HIP(hipGetLastError());
+                d.words = words;
+                d.table = ops.table + v * ops.table_stride;
+                d.first = v == 0;
+                if (dx) {
+                    d.m_tiles = dx_m, d.n_tiles = dx_n;
+                    dx_kernel<T, S><<<dim3(static_cast<unsigned>(dx_tiles),
+                                           static_cast<unsigned>(splits)), S::kThreads, 0, s>>>(d);
+                    NACHO_TRY_HIP(hipGetLastError());
+                }
+                if (dtable) {
+                    const int64_t dw_tiles =
+                        tiles_of<Wide>(a.width, words, &d.m_tiles, &d.n_tiles);
+                    d.dtable = static_cast<T *>(dtable) + v * a.width;
+                    dtable_kernel<T, Wide><<<static_cast<unsigned>(dw_tiles), Wide::kThreads, 0,
+                                             s>>>(d);
+                    NACHO_TRY_HIP(hipGetLastError());
+                }
+            }
+            if (dx) {
+                const int64_t groups =
+                    (a.tokens * ((a.width + 3) / 4) + kThreads - 1) / kThreads;
+                const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
+                dx_join_kernel<T><<<grid, kThreads, 0, s>>>(
+                    ops.held.slot, a.tokens, a.width, d.sums, d.sums_stride,
+                    static_cast<int>(splits), ops.held.common, a.scale, static_cast<T *>(dx));
+                NACHO_TRY_HIP(hipGetLastError());
+            }
+            return NACHO_OK;
+        });
+    });
+}
+
+}  // namespace cross_entropy
+}  // namespace nacho
+
+extern "C" int nacho_linear_cross_entropy(int32_t dtype, int64_t tokens, int64_t words,
+                                          int64_t width, float scale, int32_t reduction,
+                                          const void *x, int64_t x_stride, const void *table,
+                                          int64_t table_stride, const void *targets,
+                                          int32_t id_bytes, float *loss, float *stats,
+                                          void *stream, const nacho_allocator *alloc) {
+    try {
+        return nacho::cross_entropy::forward({dtype, tokens, words, width, scale, reduction, x,
+                                              x_stride, table, table_stride, targets, id_bytes},
+                                             loss, stats, stream, alloc);
+    } catch (const std::bad_alloc &) {
+        return NACHO_ERR_OUT_OF_MEMORY;
+    }
+}
+
+extern "C" int nacho_linear_cross_entropy_backward(
+    int32_t dtype, int64_t tokens, int64_t words, int64_t width, float scale, int32_t reduction,
+    const void *x, int64_t x_stride, const void *table, int64_t table_stride, const void *targets,
+    int32_t id_bytes, const float *stats, const float *dloss, void *dx, void *dtable,
+    void *stream, const nacho_allocator *alloc) {
+    try {
+        return nacho::cross_entropy::backward({dtype, tokens, words, width, scale, reduction, x,
+                                               x_stride, table, table_stride, targets, id_bytes},
+                                              stats, dloss, dx, dtable, stream, alloc);
+    } catch (const std::bad_alloc &) {
+        return NACHO_ERR_OUT_OF_MEMORY;
+    }
+}

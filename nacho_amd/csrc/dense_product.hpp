@@ -1,0 +1,261 @@
+// Matrix products of dense operands in memory: tiles of C = A B on the matrix cores, A's rows (m)
+// against B's columns (n), sums in float32.
+//
+// An operand lies in memory either with its k next to each other ("along": rows of k, one for each
+// m or n) or with its m or n next to each other ("across": a row for each k).  A workgroup takes a
+// tile of BM x BN and goes over k in steps of 128 bytes of k (64 16-bit elements, 32 float32).  The
+// next step's tiles are on their way from memory to LDS, without registers, while the wavefronts
+// multiply this one's: two buffers, one barrier a step.  Products take eight consecutive k per
+// lane (lane = 16 g + c: row or column c, k = 8 g + j); operands that lie across are read with the
+// transposing LDS read.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "dense_tiles.hpp"
+#include "device_utils.hpp"
+
+namespace nacho {
+namespace dense {
+
+// Elements of k in a step.
+template <typename T>
+constexpr int kStepK = 128 / static_cast<int>(sizeof(T));
+
+// Offsets past any buffer's end, where a load gives zeros.  Buffers are described as kBufferEnd
+// bytes long whatever they are: what lies in them is decided by the loads' offsets alone.
+constexpr unsigned kBufferEnd = 0x80000000u, kNowhere = 0xffffff00u;
+
+template <typename T>
+__device__ __forceinline__ void load_pieces(const T *base, T *lds, unsigned offset) {
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass does not know buffer descriptors)
+    using Shared = __attribute__((address_space(3))) void *;
+    const auto buffer =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, kBufferEnd, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (Shared)lds, 16, static_cast<int>(offset), 0,
+                                             0, 0);
+#endif
+}
+
+// ROWS rows of a step's k.  In LDS a row is 128 bytes, eight pieces of 16, piece p of row r at
+// place p ^ swizzle(r): the 16 rows that a fragment reads lie in different banks.
+template <typename T, int ROWS, int THREADS>
+struct Along {
+    static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+    static constexpr int kPieces = 8;
+    static constexpr int kElements = ROWS * kStepK<T>;
+    static constexpr int kAll = ROWS * kPieces;
+    static constexpr int kLoads = (kAll + THREADS - 1) / THREADS;
+    static_assert(kAll % dev::kWave == 0 && THREADS % 128 == 0, "whole wavefronts");
+
+    unsigned offset[kLoads];
+    unsigned piece;  // of every load of this thread: swizzle repeats after 16 rows
+
+    __device__ __forceinline__ static int swizzle(int row) {
+        return (row & 6) | ((row >> 3) & 1);
+    }
+
+    // Rows from `there` on are zeros.  stride: elements from row to row.
+    __device__ __forceinline__ void start(int thread, int64_t stride, int there) {
+        piece = static_cast<unsigned>(thread % kPieces ^ swizzle(thread / kPieces));
+        const unsigned bytes = static_cast<unsigned>(stride * static_cast<int>(sizeof(T)));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = thread / kPieces + i * (THREADS / kPieces);
+            offset[i] = r < there ? static_cast<unsigned>(r) * bytes + 16u * piece : kNowhere;
+        }
+    }
+    __device__ __forceinline__ static int64_t advance(int64_t) { return kStepK<T>; }
+
+    // k from `left` on are zeros (left: a multiple of a piece's elements).
+    __device__ __forceinline__ void load(int thread, const T *base, int64_t left, T *tile) const {
+        const int wave_first = __builtin_amdgcn_readfirstlane(thread & ~(dev::kWave - 1));
+        const bool cut = left < kStepK<T> && static_cast<int>(piece) * kPer >= left;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            if (kAll % THREADS != 0 && wave_first + i * THREADS >= kAll) break;
+            load_pieces(base, tile + (i * THREADS + wave_first) * kPer,
+                        cut ? kNowhere : offset[i]);
+        }
+    }
+
+    // k 32 kk + 8 g .. + 8 of row 16 t + c.
+    __device__ __forceinline__ static Frag<T> frag(const T *tile, int t, int kk, int g, int c) {
+        const T *p = tile + (16 * t + c) * kStepK<T>;
+        const int x = swizzle(c);
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(p + ((2 * g) ^ x) * kPer);
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(p + ((2 * g + 1) ^ x) * kPer);
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const Frag<T> *>(p + ((4 * kk + g) ^ x) * kPer);
+        }
+    }
+};
+
+// A step's k, COLS elements of each.
+template <typename T, int COLS, int THREADS>
+struct Across {
+    static constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+    static constexpr int kPieces = COLS / kPer;
+    static constexpr int kElements = COLS * kStepK<T>;
+    static constexpr int kLoads = kStepK<T> * kPieces / THREADS;
+    static_assert(kStepK<T> * kPieces % THREADS == 0 && kPieces >= 16, "whole pieces per thread");
+
+    unsigned offset[kLoads];
+
+    // What a fragment reads at a time lies in different banks: two neighbouring pieces of eight
+    // rows (16-bit types), four of four rows.
+    __device__ __forceinline__ static int swizzle(int row) {
+        if constexpr (sizeof(T) == 4) {
+            return (row >> 3 & 3) << 2;
+        } else {
+            return ((row & 3) | (row >> 3 & 1) << 2) << 1;
+        }
+    }
+
+    // Columns from `there` on, which is a multiple of a piece's elements, are zeros.
+    __device__ __forceinline__ void start(int thread, int64_t stride, int there) {
+        const unsigned bytes = static_cast<unsigned>(stride * static_cast<int>(sizeof(T)));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = thread + i * THREADS;
+            const int r = at / kPieces, piece = (at % kPieces) ^ swizzle(r);
+            offset[i] = piece * kPer < there
+                            ? static_cast<unsigned>(r) * bytes + 16u * static_cast<unsigned>(piece)
+                            : kNowhere;
+        }
+    }
+    __device__ __forceinline__ static int64_t advance(int64_t stride) {
+        return stride * kStepK<T>;
+    }
+
+    __device__ __forceinline__ void load(int thread, const T *base, int64_t left, T *tile) const {
+        const int wave_first = __builtin_amdgcn_readfirstlane(thread & ~(dev::kWave - 1));
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (thread + i * THREADS) / kPieces;
+            load_pieces(base, tile + (i * THREADS + wave_first) * kPer,
+                        r < left ? offset[i] : kNowhere);
+        }
+    }
+
+    // k 32 kk + 8 g .. + 8 of column 16 t + c.  16-bit types: the 16 lanes of a group name four
+    // rows of 16 elements, four lanes a row, and lane c receives column c of the four rows.
+    __device__ __forceinline__ static Frag<T> frag(const T *tile, int t, int kk, int g, int c) {
+        if constexpr (sizeof(T) == 4) {
+            Frag<T> f;
+            const int piece = (4 * t + (c >> 2)) ^ swizzle(8 * g);
+            const T *p = tile + 8 * g * COLS + piece * kPer + (c & 3);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = p[j * COLS];
+            return f;
+        } else {
+            using Shared = __attribute__((address_space(3))) s16x4 *;
+            const int r = 32 * kk + 8 * g + (c >> 2);
+            const int at = r * COLS + ((2 * t + ((c >> 1) & 1)) ^ swizzle(r)) * kPer + 4 * (c & 1);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + at)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + at + 4 * COLS)));
+            const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(Frag<T>, both);
+        }
+    }
+};
+
+// A tile's shape: BM x BN by WM x WN wavefronts.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+    static constexpr int kThreads = WM * WN * dev::kWave;
+    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // 16 x 16 tiles of a wavefront
+};
+
+// An operand of a tile: its first element (m or n, and k, of the tile) and the elements from a row
+// to the next.
+template <typename T>
+struct Matrix {
+    const T *data;
+    int64_t stride;
+};
+
+template <typename T, typename S, template <typename, int, int> class OfA,
+          template <typename, int, int> class OfB>
+struct Product {
+    using A = OfA<T, S::BM, S::kThreads>;
+    using B = OfB<T, S::BN, S::kThreads>;
+    static constexpr int kLdsElements = 2 * (A::kElements + B::kElements);
+    static constexpr size_t kLdsBytes = kLdsElements * sizeof(T);
+
+    // sums[i][t]: rows 16 (wm MT + i) + 4 g .. + 4 of column 16 (wn NT + t) + c, over k < `depth`.
+    // Every thread of the workgroup calls this; m and n: rows and columns that there are.
+    __device__ __forceinline__ static void run(Matrix<T> a, int m, Matrix<T> b, int n,
+                                               int64_t depth, T *lds, f32x4 (&sums)[S::MT][S::NT]) {
+        const int thread = static_cast<int>(threadIdx.x);
+        const int wave = __builtin_amdgcn_readfirstlane(thread / dev::kWave);
+        const int wm = wave / S::WN, wn = wave % S::WN;
+        const int lane = dev::lane(), g = lane >> 4, c = lane & 15;
+        A from_a;
+        B from_b;
+        from_a.start(thread, a.stride, m);
+        from_b.start(thread, b.stride, n);
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+            for (int t = 0; t < S::NT; ++t) sums[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int64_t step_a = A::advance(a.stride), step_b = B::advance(b.stride);
+        T *tile_a = lds, *tile_b = lds + A::kElements;
+        T *next_a = lds + A::kElements + B::kElements, *next_b = next_a + A::kElements;
+        if (depth > 0) {
+            from_a.load(thread, a.data, depth, tile_a);
+            from_b.load(thread, b.data, depth, tile_b);
+        }
+        for (int64_t left = depth; left > 0; left -= kStepK<T>) {
+            rows_arrived();
+            a.data += step_a;
+            b.data += step_b;
+            if (left > kStepK<T>) {
+                from_a.load(thread, a.data, left - kStepK<T>, next_a);
+                from_b.load(thread, b.data, left - kStepK<T>, next_b);
+            }
+#pragma unroll
+            for (int kk = 0; kk < kStepK<T> / 32; ++kk) {
+                Frag<T> fb[S::NT];
+#pragma unroll
+                for (int t = 0; t < S::NT; ++t) fb[t] = B::frag(tile_b, wn * S::NT + t, kk, g, c);
+#pragma unroll
+                for (int i = 0; i < S::MT; ++i) {
+                    const Frag<T> fa = A::frag(tile_a, wm * S::MT + i, kk, g, c);
+#pragma unroll
+                    for (int t = 0; t < S::NT; ++t) sums[i][t] = mma(fa, fb[t], sums[i][t]);
+                }
+            }
+            T *const swap_a = tile_a, *const swap_b = tile_b;
+            tile_a = next_a, tile_b = next_b;
+            next_a = swap_a, next_b = swap_b;
+        }
+    }
+};
+
+// Tile `at` of m_tiles x n_tiles.  Workgroups go to the eight dies in turn, each with a cache of
+// its own: a die gets tiles next to each other, in groups of kGroup along n, so that it reads few
+// different rows at a time.
+__device__ __forceinline__ void tile_of(unsigned at, unsigned m_tiles, unsigned n_tiles,
+                                        unsigned &m, unsigned &n) {
+    constexpr unsigned kDies = 8, kGroup = 8;
+    const unsigned all = m_tiles * n_tiles;
+    const unsigned die = at % kDies, per = all / kDies, more = all % kDies;
+    unsigned i = die * per + min(die, more) + at / kDies;
+    const unsigned group = i / (kGroup * m_tiles);
+    const unsigned first = group * kGroup, wide = min(kGroup, n_tiles - first);
+    i -= first * m_tiles;
+    n = first + i % wide;
+    m = i / wide;
+}
+
+}  // namespace dense
+}  // namespace nacho

@@ -434,7 +434,8 @@ __device__ __forceinline__ float not_finite(const f32x4 (&v)[N]) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNegInf = -__builtin_inff();
+constexpr float kInf = __builtin_inff();
+constexpr float kNegInf = -kInf;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }

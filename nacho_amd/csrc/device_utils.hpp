@@ -81,6 +81,18 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// Lanes of the wavefront with the same number (of `bits` bits).
+__device__ __forceinline__ unsigned long long peers_of(int x, int bits) {
+    unsigned long long same = ~0ull;
+    for (int i = 0; i < bits; ++i) {
+        const unsigned long long set = __ballot(x >> i & 1);
+        same &= (x >> i & 1) ? set : ~set;
+    }
+    return same;
+}
+
+__device__ __forceinline__ int bits_for(int n) { return n > 0 ? 32 - __clz(n) : 0; }
+
 // Sum over the 64 lanes, result in every lane.
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {

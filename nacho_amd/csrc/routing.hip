@@ -21,11 +21,21 @@
 #include <new>
 #include <type_traits>
 
+#include "dense_rows.hpp"
 #include "dense_tiles.hpp"
 #include "runtime.hpp"
 
 namespace nacho {
 namespace routing {
+
+using dense::element_aligned;
+using dense::item_of;
+using dense::load_piece;
+using dense::Piece;
+using dense::pieces;
+using dense::store_piece;
+using dev::bits_for;
+using dev::peers_of;
 
 constexpr int kThreads = 256;
 constexpr int kRun = 256;  // entries that one wavefront ranks
@@ -46,18 +56,6 @@ __device__ __forceinline__ int expert_of(const RouteArgs &a, int e) {
                                          : static_cast<const int *>(a.experts)[e];
     return id >= 0 && id < a.n_experts ? static_cast<int>(id) : a.n_experts;
 }
-
-// Lanes of the wavefront with the same number (of `bits` bits).
-__device__ __forceinline__ unsigned long long peers_of(int x, int bits) {
-    unsigned long long same = ~0ull;
-    for (int i = 0; i < bits; ++i) {
-        const unsigned long long set = __ballot(x >> i & 1);
-        same &= (x >> i & 1) ? set : ~set;
-    }
-    return same;
-}
-
-__device__ __forceinline__ int bits_for(int n) { return n > 0 ? 32 - __clz(n) : 0; }
 
 // A run's entries, counted into the wavefront's own counters in LDS.
 __device__ void count_run(const RouteArgs &a, int first, int bits, int *counters) {
@@ -209,33 +207,6 @@ __global__ __launch_bounds__(kThreads) void place_kernel(RouteArgs a, int runs,
 }
 
 // ---- rows -----------------------------------------------------------------------------
-
-// N elements that are read or written together: 16 bytes where rows allow it, one element where
-// a row starts between (odd widths and strides).
-template <typename T, int N>
-struct alignas(N * sizeof(T)) Piece {
-    T v[N];
-};
-
-// Rows are too many to be read again from a cache by what comes next: they go past it.
-template <typename T, int N>
-__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
-    if constexpr (N * sizeof(T) == 16) {
-        return __builtin_bit_cast(Piece<T, N>, __builtin_nontemporal_load(
-                                                   reinterpret_cast<const dense::u32x4 *>(p)));
-    } else {
-        return *reinterpret_cast<const Piece<T, N> *>(p);
-    }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
-    if constexpr (N * sizeof(T) == 16) {
-        __builtin_nontemporal_store(__builtin_bit_cast(dense::u32x4, v),
-                                    reinterpret_cast<dense::u32x4 *>(p));
-    } else {
-        *reinterpret_cast<Piece<T, N> *>(p) = v;
-    }
-}
 
 struct Rows {
     int64_t tokens, width;
@@ -427,18 +398,6 @@ int check_rows(int32_t dtype, int64_t tokens, int32_t per_token, int64_t width) 
     }
     if (tokens > kMostEntries / per_token) return NACHO_ERR_INDEX_OVERFLOW;
     return NACHO_OK;
-}
-
-int item_of(int32_t dtype) { return dtype == NACHO_F32 ? 4 : 2; }
-
-// Whether rows of `width` elements at `p`, `stride` apart, are whole aligned 16-byte pieces.
-bool pieces(const void *p, int64_t stride, int64_t width, int item) {
-    const int64_t per = 16 / item;
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % per == 0 && width % per == 0;
-}
-
-bool element_aligned(const void *p, int item) {
-    return reinterpret_cast<uintptr_t>(p) % static_cast<unsigned>(item) == 0;
 }
 
 // Calls f with the element type, the elements of a piece and the threads per token: a wavefront

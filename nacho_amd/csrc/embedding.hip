@@ -23,12 +23,44 @@ namespace embedding {
 
 using dense::element_aligned;
 using dense::item_of;
-using dense::load_piece;
-using dense::Piece;
-using dense::pieces;
-using dense::store_piece;
 
 constexpr int kThreads = 256;
+
+// N elements that are read or written together, wherever they start: 16 bytes, or one element where
+// a row is shorter.  (Rows of odd widths start between 16-byte pieces; loads and stores of 16 bytes
+// take any address.)
+template <typename T, int N>
+struct alignas(sizeof(T)) Piece {
+    T v[N];
+};
+typedef dense::u32x4 u32x4_any __attribute__((aligned(2)));
+
+// Rows are too many to be read again from a cache by what comes next: they go past it.
+template <typename T, int N>
+__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
+    if constexpr (N * sizeof(T) == 16) {
+        return __builtin_bit_cast(
+            Piece<T, N>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p)));
+    } else {
+        return *reinterpret_cast<const Piece<T, N> *>(p);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
+    if constexpr (N * sizeof(T) == 16) {
+        __builtin_nontemporal_store(__builtin_bit_cast(dense::u32x4, v),
+                                    reinterpret_cast<u32x4_any *>(p));
+    } else {
+        *reinterpret_cast<Piece<T, N> *>(p) = v;
+    }
+}
+
+// Where the piece that starts at col < width lies: a row's last piece ends with the row, over
+// elements that the one before has too (and both give them the same value).
+template <int N>
+__device__ __forceinline__ int64_t within(int64_t col, int64_t width) {
+    return min(col, width - N);
+}
 
 struct Ids {
     const void *ids;
@@ -64,7 +96,8 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, int64_t token
                 const int64_t col = col0 + s * LANES * N;
                 if (col < width) {
                     if (id >= 0) {
-                        piece[s] = *reinterpret_cast<const Piece<T, N> *>(from + col);
+                        piece[s] = *reinterpret_cast<const Piece<T, N> *>(
+                            from + within<N>(col, width));
                     } else {
                         for (int j = 0; j < N; ++j) piece[s].v[j] = static_cast<T>(0.0f);
                     }
@@ -81,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, int64_t token
                                 static_cast<T>(scale * static_cast<float>(piece[s].v[j]));
                         }
                     }
-                    store_piece<T, N>(to + col, piece[s]);
+                    store_piece<T, N>(to + within<N>(col, width), piece[s]);
                 }
             }
         }
@@ -91,104 +124,175 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, int64_t token
 // ---- tokens in order of (word, token) ---------------------------------------------------
 //
 // keys[place] and order[place]: the word and the token at a place; tokens without a word are behind
-// with the key `words`.
+// with the key `words`.  Sorting keeps a few workgroups busy with waits for memory; the others of
+// its launches clear the table's gradient meanwhile, each launch a share of it.
+
+struct Clear {
+    dense::u32x4 *pieces;
+    int64_t from, to;      // of 16 bytes, in this launch
+    unsigned first;        // the first workgroup that clears
+
+    // Whether the workgroup is one of those, and has done its part.
+    __device__ __forceinline__ bool done() const {
+        if (blockIdx.x < first) return false;
+        const dense::u32x4 zero{0u, 0u, 0u, 0u};
+        const int64_t all = (gridDim.x - first) * static_cast<int64_t>(blockDim.x);
+        for (int64_t i = from + (blockIdx.x - first) * static_cast<int64_t>(blockDim.x) +
+                         threadIdx.x; i < to; i += all) {
+            __builtin_nontemporal_store(zero, pieces + i);
+        }
+        return true;
+    }
+};
 
 // Up to kRankMost tokens: a token's place is the number of tokens before it, counted.  A workgroup
 // has 64 tokens, one a lane, and its wavefronts share the tokens to count.
-constexpr int kRankMost = 8192;
+constexpr int kRankMost = 16384;
 constexpr int kRankThreads = 1024;
 constexpr int kRankWaves = kRankThreads / dev::kWave;
 
 __global__ __launch_bounds__(kRankThreads) void rank_kernel(Ids ids, int tokens,
                                                             int *__restrict__ keys,
-                                                            int *__restrict__ order) {
+                                                            int *__restrict__ order,
+                                                            Clear clear) {
     __shared__ __attribute__((aligned(16))) int s_key[kRankMost];
     __shared__ int s_before[kRankWaves][dev::kWave];
-    const int lane = dev::lane(), wave = static_cast<int>(threadIdx.x) / dev::kWave;
+    if (clear.done()) return;
+    const int lane = dev::lane();
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / dev::kWave);
     const int none = static_cast<int>(ids.words);
     // (past the tokens: a key that is before no other)
-    const int filled = (tokens + 4 * kRankWaves - 1) / (4 * kRankWaves) * (4 * kRankWaves);
-    for (int t = threadIdx.x; t < filled; t += kRankThreads) {
-        const int64_t id = t < tokens ? ids(t) : -1;
-        s_key[t] = t >= tokens ? INT_MAX : id < 0 ? none : static_cast<int>(id);
-    }
-    __syncthreads();
-    const int mine = static_cast<int>(blockIdx.x) * dev::kWave + lane;
-    const int key = mine < tokens ? s_key[mine] : none;
-    const int per = filled / kRankWaves;
-    int before = 0;
-    for (int t = wave * per; t < wave * per + per; t += 4) {
+    constexpr int kStep = 8;
+    const int filled = (tokens + kStep * kRankWaves - 1) / (kStep * kRankWaves) *
+                       (kStep * kRankWaves);
+    for (int t0 = threadIdx.x; t0 < filled; t0 += kRankThreads * kStep) {
+        int64_t id[kStep];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int other = s_key[t + j];
-            before += other < key || (other == key && t + j < mine) ? 1 : 0;
+        for (int s = 0; s < kStep; ++s) {
+            const int t = t0 + s * kRankThreads;
+            id[s] = t < tokens ? ids(t) : -1;
+        }
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) {
+            const int t = t0 + s * kRankThreads;
+            if (t < filled) {
+                s_key[t] = t >= tokens ? INT_MAX : id[s] < 0 ? none : static_cast<int>(id[s]);
+            }
         }
     }
-    s_before[wave][lane] = before;
+    __syncthreads();
+    const int group = static_cast<int>(blockIdx.x) * dev::kWave;
+    const int mine = group + lane;
+    const int key = mine < tokens ? s_key[mine] : none;
+    const int per = filled / kRankWaves;
+    const int from = wave * per, to = from + per;
+    // Tokens before this group's count with an equal key too, those behind without; among its own
+    // 64 the lane decides.
+    auto count = [&](int a, int b, auto before) {
+        int n = 0;
+        for (int t = a; t < b; t += kStep) {
+            int other[kStep];
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) other[j] = s_key[t + j];
+#pragma unroll
+            for (int j = 0; j < kStep; ++j) n += before(other[j], t + j) ? 1 : 0;
+        }
+        return n;
+    };
+    const int a = min(max(group, from), to), b = min(max(group + dev::kWave, from), to);
+    int n = count(from, a, [&](int other, int) { return other <= key; });
+    n += count(a, b, [&](int other, int t) { return other < key || (other == key && t < mine); });
+    n += count(b, to, [&](int other, int) { return other < key; });
+    s_before[wave][lane] = n;
     __syncthreads();
     if (wave == 0 && mine < tokens) {
         int at = 0;
+#pragma unroll
         for (int w = 0; w < kRankWaves; ++w) at += s_before[w][lane];
         keys[at] = key;
         order[at] = mine;
     }
 }
 
-// More tokens: a stable counting sort by kDigitBits bits at a time, lowest first.  Tokens are cut
-// into runs of kRun, one wavefront each: counts per (digit, run), their exclusive scan, and each
-// token's place from its run's offset and the equal digits before it in the run.
+// More tokens: a stable counting sort by kDigitBits bits at a time, lowest first.  A workgroup has
+// a block of kBlock tokens, its wavefronts runs of kRun of them.  A token's place is its digit's
+// first, and the equal digits of the blocks before, of the block's runs before, and before it in
+// its run.
 constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kRun = 512;
-constexpr int kRunSteps = kRun / dev::kWave;
-constexpr int kRunWaves = kThreads / dev::kWave;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / dev::kWave;
+constexpr int kRunSteps = 2;
+constexpr int kRun = kRunSteps * dev::kWave;
+constexpr int kBlock = kRun * kSortWaves;
+// Up to so many blocks, the workgroups that place tokens add up the blocks' counts themselves.
+constexpr int kFewBlocks = 256;
 
 struct Pass {
     Ids ids;             // the first pass: tokens in their own order
     const int *keys_in;  // else the last one's
     const int *order_in;
-    int tokens, runs, shift;
+    int tokens, blocks, shift;
     int *keys, *order;
 };
 
-__device__ __forceinline__ int pass_key(const Pass &p, int i) {
-    if (p.keys_in) return p.keys_in[i];
-    const int64_t id = p.ids(i);
-    return id < 0 ? static_cast<int>(p.ids.words) : static_cast<int>(id);
+// Keys of a wavefront's run; -1 past the tokens.
+__device__ __forceinline__ void run_keys(const Pass &p, int first, int (&keys)[kRunSteps]) {
+#pragma unroll
+    for (int step = 0; step < kRunSteps; ++step) {
+        const int i = first + step * dev::kWave + dev::lane();
+        keys[step] = -1;
+        if (i < p.tokens) {
+            if (p.keys_in) {
+                keys[step] = p.keys_in[i];
+            } else {
+                const int64_t id = p.ids(i);
+                keys[step] = static_cast<int>(id < 0 ? p.ids.words : id);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ int run_first() {
+    return static_cast<int>(blockIdx.x) * kBlock +
+           static_cast<int>(threadIdx.x) / dev::kWave * kRun;
 }
 
 __device__ __forceinline__ int digit_of(int key, int shift) {
     return key >> shift & (kDigits - 1);
 }
 
-__global__ __launch_bounds__(kThreads) void count_kernel(Pass p, int *__restrict__ counts) {
-    __shared__ int s_count[kRunWaves][kDigits];
-    const int wave = static_cast<int>(threadIdx.x) / dev::kWave, lane = dev::lane();
-    const int run = static_cast<int>(blockIdx.x) * kRunWaves + wave;
-    for (int i = lane; i < kDigits; i += dev::kWave) s_count[wave][i] = 0;
-    dev::wave_sync();
-    if (run >= p.runs) return;
+// counts[block][digit]
+__global__ __launch_bounds__(kSortThreads) void count_kernel(Pass p, int *__restrict__ counts,
+                                                             Clear clear) {
+    __shared__ int s_count[kDigits];
+    if (clear.done()) return;
+    int keys[kRunSteps];
+    run_keys(p, run_first(), keys);
+    if (threadIdx.x < kDigits) s_count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
     for (int step = 0; step < kRunSteps; ++step) {
-        const int i = run * kRun + step * dev::kWave + lane;
         // (only the count matters here: the order of these additions decides nothing)
-        if (i < p.tokens) atomicAdd(&s_count[wave][digit_of(pass_key(p, i), p.shift)], 1);
+        if (keys[step] >= 0) atomicAdd(&s_count[digit_of(keys[step], p.shift)], 1);
     }
-    dev::wave_sync();
-    for (int i = lane; i < kDigits; i += dev::kWave) {
-        counts[static_cast<int64_t>(run) * kDigits + i] = s_count[wave][i];
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+        counts[static_cast<int64_t>(blockIdx.x) * kDigits + threadIdx.x] = s_count[threadIdx.x];
     }
 }
 
-// counts[run][digit] become the offsets of each run's tokens within their digit, and totals[digit]
-// the digit's tokens: a workgroup per 64 digits, its wavefronts over the runs.
-__global__ __launch_bounds__(1024) void scan_kernel(int runs, int *__restrict__ counts,
-                                                    int *__restrict__ totals) {
+// counts[block][digit] become the tokens of the digit in the blocks before, and totals[digit] the
+// digit's tokens: a workgroup per 64 digits, its wavefronts over the blocks.
+__global__ __launch_bounds__(1024) void scan_kernel(int blocks, int *__restrict__ counts,
+                                                    int *__restrict__ totals, Clear clear) {
     constexpr int kParts = 1024 / dev::kWave;
     __shared__ int s_part[kParts][dev::kWave];
+    if (clear.done()) return;
     const int lane = dev::lane(), part = static_cast<int>(threadIdx.x) / dev::kWave;
     int *mine = counts + blockIdx.x * dev::kWave + lane;
-    const int per = (runs + kParts - 1) / kParts;
-    const int from = min(runs, part * per), to = min(runs, from + per);
+    const int per = (blocks + kParts - 1) / kParts;
+    const int from = min(blocks, part * per), to = min(blocks, from + per);
     int sum = 0;
 #pragma unroll 8
     for (int r = from; r < to; ++r) sum += mine[static_cast<int64_t>(r) * kDigits];
@@ -208,42 +312,77 @@ __global__ __launch_bounds__(1024) void scan_kernel(int runs, int *__restrict__ 
     if (part == 0) totals[blockIdx.x * dev::kWave + lane] = all;
 }
 
-__global__ __launch_bounds__(kThreads) void place_kernel(Pass p, const int *__restrict__ counts,
-                                                         const int *__restrict__ totals) {
-    __shared__ int s_next[kRunWaves][kDigits];
-    __shared__ int s_first[kDigits];
-    __shared__ int s_sums[kRunWaves];
-    int carry = 0;
-    for (int x0 = 0; x0 < kDigits; x0 += kThreads) {
-        const int x = x0 + static_cast<int>(threadIdx.x);
-        int total = 0;
-        s_first[x] = carry + dev::block_exclusive_sum<kThreads>(totals[x], s_sums, total);
-        carry += total;
+// totals: null for few blocks, whose counts are as counted.
+__global__ __launch_bounds__(kSortThreads) void place_kernel(Pass p,
+                                                             const int *__restrict__ counts,
+                                                             const int *__restrict__ totals,
+                                                             Clear clear) {
+    __shared__ int s_next[kSortWaves][kDigits];
+    __shared__ int s_half[2][2][kDigits];
+    __shared__ int s_sums[kSortWaves];
+    if (clear.done()) return;
+    const int wave = static_cast<int>(threadIdx.x) / dev::kWave, lane = dev::lane();
+    const int block = static_cast<int>(blockIdx.x);
+    int keys[kRunSteps];
+    run_keys(p, run_first(), keys);
+    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) {
+        (&s_next[0][0])[i] = 0;
+    }
+    // The digits' sizes, and their tokens in the blocks before: every digit has two threads, which
+    // take the blocks in turn.
+    static_assert(kSortThreads == 2 * kDigits, "two threads a digit");
+    const int digit = static_cast<int>(threadIdx.x) % kDigits;
+    const int half = static_cast<int>(threadIdx.x) / kDigits;
+    int before = 0, size = 0;
+    if (totals) {
+        if (half == 0) {
+            before = counts[static_cast<int64_t>(block) * kDigits + digit];
+            size = totals[digit];
+        }
+    } else {
+#pragma unroll 8
+        for (int b = half; b < p.blocks; b += 2) {
+            const int n = counts[static_cast<int64_t>(b) * kDigits + digit];
+            before += b < block ? n : 0;
+            size += n;
+        }
+    }
+    s_half[half][0][digit] = before;
+    s_half[half][1][digit] = size;
+    __syncthreads();
+    int *mine = s_next[wave];
+#pragma unroll
+    for (int step = 0; step < kRunSteps; ++step) {
+        if (keys[step] >= 0) atomicAdd(&mine[digit_of(keys[step], p.shift)], 1);
+    }
+    size = half == 0 ? s_half[0][1][digit] + s_half[1][1][digit] : 0;
+    int all = 0;
+    int at = dev::block_exclusive_sum<kSortThreads>(size, s_sums, all);
+    if (half == 0) {
+        at += s_half[0][0][digit] + s_half[1][0][digit];
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = s_next[w][digit];
+            s_next[w][digit] = at;
+            at += n;
+        }
     }
     __syncthreads();
-    const int wave = static_cast<int>(threadIdx.x) / dev::kWave, lane = dev::lane();
-    const int run = static_cast<int>(blockIdx.x) * kRunWaves + wave;
-    if (run >= p.runs) return;
-    int *next = s_next[wave];
-    for (int i = lane; i < kDigits; i += dev::kWave) {
-        next[i] = s_first[i] + counts[static_cast<int64_t>(run) * kDigits + i];
-    }
-    dev::wave_sync();
+#pragma unroll
     for (int step = 0; step < kRunSteps; ++step) {
-        const int i = run * kRun + step * dev::kWave + lane;
-        const bool there = i < p.tokens;
-        const int key = there ? pass_key(p, i) : 0;
-        // (a lane past the tokens is no one's peer: digits have kDigitBits bits)
-        const int digit = there ? digit_of(key, p.shift) : kDigits;
-        const unsigned long long peers = dev::peers_of(digit, kDigitBits + 1);
+        const int i = run_first() + step * dev::kWave + lane;
+        const bool there = keys[step] >= 0;
+        const int x = digit_of(keys[step], p.shift);
+        // (a lane past the tokens is no one's peer)
+        const unsigned long long peers = dev::peers_of(x, kDigitBits) & __ballot(there);
         const int rank = __popcll(peers & ((1ull << lane) - 1ull));
-        const int at = there ? next[digit] + rank : 0;
+        const int place = mine[x] + rank;
         dev::wave_sync();
-        if (there && rank == 0) next[digit] += __popcll(peers);
+        if (there && rank == 0) mine[x] += __popcll(peers);
         dev::wave_sync();
         if (there) {
-            p.keys[at] = key;
-            p.order[at] = p.order_in ? p.order_in[i] : i;
+            p.keys[place] = keys[step];
+            p.order[place] = p.order_in ? p.order_in[i] : i;
         }
     }
 }
@@ -254,7 +393,7 @@ constexpr int kChunk = 32;  // sorted tokens of a run
 
 struct Sums {
     const int *keys, *order;
-    int tokens, words;
+    int tokens, words, chunks;
     int64_t width;
     float scale;
     float *parts;  // [run][2][width]: sums of the run's first and last word, where these have
@@ -275,15 +414,31 @@ __device__ __forceinline__ void store_part(float *to, const float (&sum)[N]) {
     for (int j = 0; j < N; ++j) to[j] = sum[j];
 }
 
-template <typename T, int N>
+// The run of this thread, of which LANES threads have a slice of the columns each, and the thread's
+// first column.
+template <int N, int LANES>
+struct Part {
+    int run;
+    int64_t col;
+    bool there;
+
+    __device__ __forceinline__ explicit Part(const Sums &a)
+        : run(static_cast<int>(blockIdx.x) * (kThreads / LANES) +
+              __builtin_amdgcn_readfirstlane(threadIdx.x / LANES)),
+          col((blockIdx.y * static_cast<int64_t>(LANES) + threadIdx.x % LANES) * N),
+          there(run < a.chunks && col < a.width) {
+        col = within<N>(col, a.width);
+    }
+};
+
+template <typename T, int N, int LANES>
 __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restrict__ dout,
                                                        int64_t stride, T *__restrict__ dtable) {
     constexpr int kStep = 8;
-    const int first = static_cast<int>(blockIdx.x) * kChunk;
-    const int end = min(first + kChunk, a.tokens);
-    const int64_t col =
-        (blockIdx.y * static_cast<int64_t>(kThreads) + threadIdx.x) * N;
-    if (col >= a.width) return;
+    const Part<N, LANES> part(a);
+    if (!part.there) return;
+    const int first = part.run * kChunk, end = min(first + kChunk, a.tokens);
+    const int64_t col = part.col;
     const int before = first > 0 ? a.keys[first - 1] : -1;
     const int behind = end < a.tokens ? a.keys[end] : -1;
     float sum[N] = {};
@@ -307,9 +462,9 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restri
             if (next == key[s] && e + 1 < end) continue;
             // the word's last token in this run
             if (key[s] == before) {
-                store_part<N>(a.parts + (blockIdx.x * 2ll) * a.width + col, sum);
+                store_part<N>(a.parts + (part.run * 2ll) * a.width + col, sum);
             } else if (next == key[s]) {
-                store_part<N>(a.parts + (blockIdx.x * 2ll + 1) * a.width + col, sum);
+                store_part<N>(a.parts + (part.run * 2ll + 1) * a.width + col, sum);
             } else {
                 store_sum<T, N>(dtable + static_cast<int64_t>(key[s]) * a.width + col, sum,
                                 a.scale);
@@ -321,36 +476,36 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restri
 }
 
 // Words that begin in a run and go on behind it: their parts in the order of the runs.
-template <typename T, int N>
+template <typename T, int N, int LANES>
 __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, T *__restrict__ dtable) {
     constexpr int kStep = 8;
-    const int first = static_cast<int>(blockIdx.x) * kChunk, end = first + kChunk;
-    if (end >= a.tokens) return;
+    const Part<N, LANES> own(a);
+    if (own.run + 1 >= a.chunks) return;
+    const int first = own.run * kChunk, end = first + kChunk;
     const int key = a.keys[end - 1];
     if (key >= a.words || a.keys[end] != key || (first > 0 && a.keys[first - 1] == key)) return;
-    const int64_t col =
-        (blockIdx.y * static_cast<int64_t>(kThreads) + threadIdx.x) * N;
-    if (col >= a.width) return;
-    // the word's last token: keys are sorted
-    int lo = end, hi = a.tokens - 1;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (a.keys[mid] == key) {
-            lo = mid;
-        } else {
-            hi = mid - 1;
-        }
+    // The last run that begins with the word: keys are sorted, and the lanes look at 64 runs at a
+    // time, the same number apart.
+    int last = own.run + 1, most = a.chunks - 1;
+    while (last < most) {
+        const int step = (most - last) / dev::kWave + 1;
+        const int64_t run = last + static_cast<int64_t>(dev::lane()) * step;
+        const bool with = run <= most && a.keys[run * kChunk] == key;
+        const int n = __popcll(__ballot(with));  // (1 or more: `last` begins with the word)
+        last += (n - 1) * step;
+        most = min(most, last + step - 1);
     }
-    const int64_t last = lo / kChunk;
+    if (!own.there) return;
+    const int64_t col = own.col;
     float sum[N];
-    const float *mine = a.parts + (blockIdx.x * 2ll + 1) * a.width + col;
+    const float *mine = a.parts + (own.run * 2ll + 1) * a.width + col;
 #pragma unroll
     for (int j = 0; j < N; ++j) sum[j] = mine[j];
-    for (int64_t run = blockIdx.x + 1ll; run <= last; run += kStep) {
+    for (int run = own.run + 1; run <= last; run += kStep) {
         float part[kStep][N];
 #pragma unroll
         for (int s = 0; s < kStep; ++s) {
-            const float *from = a.parts + min(run + s, last) * 2 * a.width + col;
+            const float *from = a.parts + min(run + s, last) * 2ll * a.width + col;
 #pragma unroll
             for (int j = 0; j < N; ++j) part[s][j] = from[j];
         }
@@ -371,7 +526,7 @@ int check(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sca
         !(scale - scale == 0.0f) || (id_bytes != 4 && id_bytes != 8)) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
-    if (words > NACHO_MAX_WORDS || tokens > INT32_MAX - kRun * kRunWaves) {
+    if (words > NACHO_MAX_WORDS || tokens > INT32_MAX - kBlock) {
         return NACHO_ERR_INDEX_OVERFLOW;
     }
     if (tokens > 0 && (!ids || !element_aligned(ids, id_bytes))) {
@@ -380,12 +535,13 @@ int check(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sca
     return NACHO_OK;
 }
 
-// Calls f with the element type and the elements of a piece.
+// Calls f with the element type and the elements of a piece.  (In us with pieces of 16 bytes and of
+// one element: 30001 rows of 333 float32, lookup 8 and 12, sums 12 and 20.)
 template <typename F>
-int with_type(int32_t dtype, bool whole, F f) {
+int with_type(int32_t dtype, int64_t width, F f) {
     auto typed = [&](auto type) {
         using T = decltype(type);
-        if (whole) return f(type, std::integral_constant<int, 16 / sizeof(T)>{});
+        if (width * static_cast<int64_t>(sizeof(T)) >= 16) return f(type, std::integral_constant<int, 16 / sizeof(T)>{});
         return f(type, std::integral_constant<int, 1>{});
     };
     if (dtype == NACHO_F32) return typed(float{});
@@ -404,8 +560,7 @@ int lookup(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sc
         return NACHO_ERR_INVALID_ARGUMENT;
     }
     const Ids of{ids, id_bytes, words};
-    const bool whole = pieces(table, stride, width, item) && pieces(rows, width, width, item);
-    return with_type(dtype, whole, [&](auto type, auto n) -> int {
+    return with_type(dtype, width, [&](auto type, auto n) -> int {
         using T = decltype(type);
         auto launch = [&](auto lanes) -> int {
             const int64_t groups = (tokens * lanes() + kThreads - 1) / kThreads;
@@ -422,38 +577,56 @@ int lookup(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sc
     });
 }
 
-// The tokens sorted by word into keys and order.
-int sort_tokens(Call &call, const Ids &ids, int tokens, int *keys, int *order) {
+// The tokens sorted by word into keys and order, and `pieces` of 16 bytes cleared.
+int sort_tokens(Call &call, const Ids &ids, int tokens, int *keys, int *order,
+                dense::u32x4 *pieces, int64_t n_pieces) {
     const hipStream_t s = call.stream();
+    // Launch i of n: its share of the pieces, and a grid with workgroups for them.
+    auto share = [&](unsigned groups, int threads, int i, int n, unsigned *grid) {
+        const Clear c{pieces, n_pieces * i / n, n_pieces * (i + 1) / n, groups};
+        const int64_t want = (c.to - c.from + threads * 4 - 1) / (threads * 4);
+        const int64_t most = 2048 * 256 / threads;
+        *grid = groups + static_cast<unsigned>(want < most ? want : most);
+        return c;
+    };
+    unsigned grid = 0;
     if (tokens <= kRankMost) {
-        rank_kernel<<<ceil_div(static_cast<size_t>(tokens), dev::kWave), kRankThreads, 0, s>>>(
-            ids, tokens, keys, order);
+        const Clear clear = share(ceil_div(static_cast<size_t>(tokens), dev::kWave), kRankThreads,
+                                  0, 1, &grid);
+        rank_kernel<<<grid, kRankThreads, 0, s>>>(ids, tokens, keys, order, clear);
         NACHO_TRY_HIP(hipGetLastError());
         return NACHO_OK;
     }
-    const int runs = (tokens + kRun - 1) / kRun;
+    const int blocks = (tokens + kBlock - 1) / kBlock;
     int bits = 1;
     while (ids.words >> bits) ++bits;  // of the key `words`
     const int passes = (bits + kDigitBits - 1) / kDigitBits;
+    const bool few = blocks <= kFewBlocks;
+    const int launches = passes * (few ? 2 : 3);
     int *counts = nullptr, *totals = nullptr, *other_keys = nullptr, *other_order = nullptr;
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(runs) * kDigits, &counts));
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(kDigits), &totals));
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(blocks) * kDigits, &counts));
+    if (!few) NACHO_TRY(call.scratch_n(static_cast<size_t>(kDigits), &totals));
     if (passes > 1) {
         NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &other_keys));
         NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &other_order));
     }
-    const unsigned groups = ceil_div(static_cast<size_t>(runs), kRunWaves);
-    Pass p{ids, nullptr, nullptr, tokens, runs, 0, nullptr, nullptr};
-    for (int i = 0; i < passes; ++i) {
+    const unsigned groups = static_cast<unsigned>(blocks);
+    Pass p{ids, nullptr, nullptr, tokens, blocks, 0, nullptr, nullptr};
+    for (int i = 0, launch = 0; i < passes; ++i) {
         const bool to_result = (passes - i) % 2 == 1;
         p.keys = to_result ? keys : other_keys;
         p.order = to_result ? order : other_order;
         p.shift = i * kDigitBits;
-        count_kernel<<<groups, kThreads, 0, s>>>(p, counts);
+        Clear clear = share(groups, kSortThreads, launch++, launches, &grid);
+        count_kernel<<<grid, kSortThreads, 0, s>>>(p, counts, clear);
         NACHO_TRY_HIP(hipGetLastError());
-        scan_kernel<<<kDigits / dev::kWave, 1024, 0, s>>>(runs, counts, totals);
-        NACHO_TRY_HIP(hipGetLastError());
-        place_kernel<<<groups, kThreads, 0, s>>>(p, counts, totals);
+        if (!few) {
+            clear = share(kDigits / dev::kWave, 1024, launch++, launches, &grid);
+            scan_kernel<<<grid, 1024, 0, s>>>(blocks, counts, totals, clear);
+            NACHO_TRY_HIP(hipGetLastError());
+        }
+        clear = share(groups, kSortThreads, launch++, launches, &grid);
+        place_kernel<<<grid, kSortThreads, 0, s>>>(p, counts, totals, clear);
         NACHO_TRY_HIP(hipGetLastError());
         p.keys_in = p.keys;
         p.order_in = p.order;
@@ -471,35 +644,50 @@ int backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float 
         !element_aligned(dtable, item)) {
         return NACHO_ERR_INVALID_ARGUMENT;
     }
-    const bool whole = pieces(dout, stride, width, item) && pieces(dtable, width, width, item);
     const int64_t chunks = (tokens + kChunk - 1) / kChunk;
-    const int64_t per = whole ? kThreads * (16 / item) : kThreads;
-    const int64_t slices = (width + per - 1) / per;
-    if (slices > 65535 || chunks * slices > dense::kMostGroups) return NACHO_ERR_INDEX_OVERFLOW;
+    // Threads of a run: a row's pieces, if they are few.
+    const int64_t row = width * item >= 16 ? (width * item + 15) / 16 : width;
+    const int lanes = row <= 64 ? 64 : row <= 128 ? 128 : kThreads;
+    const int64_t slices = (row + lanes - 1) / lanes;
+    const int64_t groups_x = (chunks * lanes + kThreads - 1) / kThreads;
+    if (slices > 65535 || groups_x * slices > dense::kMostGroups) return NACHO_ERR_INDEX_OVERFLOW;
     Call call(stream, alloc);
     const hipStream_t s = call.stream();
-    return with_type(dtype, whole, [&](auto type, auto n) -> int {
+    return with_type(dtype, width, [&](auto type, auto n) -> int {
         using T = decltype(type);
-        NACHO_TRY(dense::clear(s, static_cast<T *>(dtable), words * width));
-        if (tokens == 0) return NACHO_OK;
+        if (tokens == 0) return dense::clear(s, static_cast<T *>(dtable), words * width);
         int *keys = nullptr, *order = nullptr;
         float *parts = nullptr;
         NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &keys));
         NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &order));
         if (chunks > 1) NACHO_TRY(call.scratch_n(static_cast<size_t>(chunks * 2 * width), &parts));
+        // The gradient's whole 16-byte pieces are cleared with the sort, the few elements before
+        // and behind them by themselves, where there are any.
+        T *const table = static_cast<T *>(dtable);
+        const int64_t all = words * width, per = 16 / item;
+        int64_t head = static_cast<int64_t>((-reinterpret_cast<uintptr_t>(table) & 15) / item);
+        if (head > all) head = all;
+        const int64_t n_pieces = (all - head) / per, tail = all - head - n_pieces * per;
+        if (head > 0) NACHO_TRY(dense::clear(s, table, head));
+        if (tail > 0) NACHO_TRY(dense::clear(s, table + all - tail, tail));
         NACHO_TRY(sort_tokens(call, Ids{ids, id_bytes, words}, static_cast<int>(tokens), keys,
-                              order));
+                              order, reinterpret_cast<dense::u32x4 *>(table + head), n_pieces));
         const Sums a{keys, order, static_cast<int>(tokens), static_cast<int>(words),
-                     width, scale, parts};
-        const dim3 all(static_cast<unsigned>(chunks), static_cast<unsigned>(slices));
-        sum_kernel<T, n()><<<all, kThreads, 0, s>>>(a, static_cast<const T *>(dout), stride,
-                                                    static_cast<T *>(dtable));
-        NACHO_TRY_HIP(hipGetLastError());
-        if (chunks > 1) {
-            join_kernel<T, n()><<<all, kThreads, 0, s>>>(a, static_cast<T *>(dtable));
+                     static_cast<int>(chunks), width, scale, parts};
+        const dim3 groups(static_cast<unsigned>(groups_x), static_cast<unsigned>(slices));
+        auto sums = [&](auto of) -> int {
+            sum_kernel<T, n(), of()><<<groups, kThreads, 0, s>>>(a, static_cast<const T *>(dout),
+                                                                 stride, table);
             NACHO_TRY_HIP(hipGetLastError());
-        }
-        return NACHO_OK;
+            if (chunks > 1) {
+                join_kernel<T, n(), of()><<<groups, kThreads, 0, s>>>(a, table);
+                NACHO_TRY_HIP(hipGetLastError());
+            }
+            return NACHO_OK;
+        };
+        if (lanes == 64) return sums(std::integral_constant<int, 64>{});
+        if (lanes == 128) return sums(std::integral_constant<int, 128>{});
+        return sums(std::integral_constant<int, kThreads>{});
     });
 }
 

@@ -4,13 +4,16 @@
 // tensors are read for the norm, then read again and written.  Squares are summed in float64, which
 // costs nothing beside the bytes and neither overflows nor loses small tensors next to large ones.
 //
-// The tensors' addresses travel in the kernels' arguments, kTensors a launch, cut into chunks of
-// kChunk elements: a workgroup finds the tensor of its chunk by a search of their first chunks.
+// The tensors are cut into chunks of kChunk elements, one a workgroup, which finds the tensor of its
+// chunk by a search of their first chunks.  The tensors' addresses travel in the kernels'
+// arguments; those of more than kTensors are first written into memory by small launches (with
+// passes of kTensors at a time instead, 611 tensors of 120 M elements took 204 us a call).
 #include <hip/hip_runtime.h>
 
 #include <climits>
 #include <cstdint>
 #include <new>
+#include <type_traits>
 
 #include "dense_rows.hpp"
 #include "runtime.hpp"
@@ -24,31 +27,63 @@ using dense::Piece;
 
 constexpr int kThreads = 256;
 constexpr int64_t kChunk = 32768;
-constexpr int kTensors = 96;
+constexpr int kTensors = 96;  // (of a launch's arguments)
+// Up to so many chunks, every workgroup that scales adds up the chunks' sums itself (8 KB from a
+// cache), instead of a launch between: 14 small tensors 12 us a call instead of 16.
+constexpr int64_t kFewChunks = 1024;
+
+struct Tensor {
+    const void *data;
+    void *out;
+    int64_t size;
+    unsigned first;  // chunk
+    unsigned char dtype, out_dtype;
+};
 
 // (arguments of a launch: less than 4 KB)
 struct Table {
-    const void *data[kTensors];
-    void *out[kTensors];
-    int64_t size[kTensors];
-    unsigned first[kTensors + 1];  // chunk
-    unsigned char dtype[kTensors], out_dtype[kTensors];
+    Tensor tensors[kTensors];
     int count;
 };
 static_assert(sizeof(Table) <= 3584, "a launch's arguments");
 
-// The tensor of a chunk: the last whose first chunk is not after it.
-__device__ __forceinline__ int tensor_of(const Table &t, unsigned chunk) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (t.first[mid] <= chunk) {
-            lo = mid;
-        } else {
-            hi = mid - 1;
+// Where a kernel finds the tensors: in its arguments, or in memory.
+struct InArguments {
+    Table table;
+
+    // The tensor of a chunk, the last whose first chunk is not after it, and that chunk's place.
+    __device__ __forceinline__ const Tensor &of(unsigned chunk) const {
+        int lo = 0, hi = table.count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (table.tensors[mid].first <= chunk) {
+                lo = mid;
+            } else {
+                hi = mid - 1;
+            }
         }
+        return table.tensors[lo];
     }
-    return lo;
+};
+struct InMemory {
+    const Tensor *tensors;
+    int64_t count;
+
+    // (the lanes look at 64 tensors at a time, the same number apart)
+    __device__ __forceinline__ const Tensor &of(unsigned chunk) const {
+        int64_t lo = 0, hi = count - 1;
+        while (lo < hi) {
+            const int64_t step = (hi - lo) / dev::kWave + 1, i = lo + dev::lane() * step;
+            const bool there = i <= hi && tensors[i].first <= chunk;
+            lo += (__popcll(__ballot(there)) - 1) * step;
+            hi = min(hi, lo + step - 1);
+        }
+        return tensors[lo];
+    }
+};
+
+__global__ __launch_bounds__(dev::kWave) void table_kernel(Table t, Tensor *__restrict__ tensors) {
+    for (int i = threadIdx.x; i < t.count; i += dev::kWave) tensors[i] = t.tensors[i];
 }
 
 // Calls f with the element type of a code.
@@ -96,62 +131,86 @@ __device__ __forceinline__ double squares_of(const T *p, int64_t n) {
     return sum;
 }
 
-__device__ __forceinline__ double group_sum(double sum, double *s_sum, int waves) {
+// The sum of the threads' values, for all of them.
+__device__ __forceinline__ double group_sum(double sum) {
+    __shared__ double s_sum[kThreads / dev::kWave];
     sum = dev::wave_sum(sum);
     if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = sum;
     __syncthreads();
     sum = 0.0;
-    for (int w = 0; w < waves; ++w) sum += s_sum[w];
+#pragma unroll
+    for (int w = 0; w < kThreads / dev::kWave; ++w) sum += s_sum[w];
     return sum;
 }
 
-__global__ __launch_bounds__(kThreads) void square_kernel(Table t, double *__restrict__ sums) {
-    __shared__ double s_sum[kThreads / dev::kWave];
-    const int i = tensor_of(t, blockIdx.x);
-    const int64_t at = (blockIdx.x - t.first[i]) * kChunk;
-    const int64_t n = min(kChunk, t.size[i] - at);
+template <typename Tensors>
+__global__ __launch_bounds__(kThreads) void square_kernel(Tensors tensors,
+                                                          double *__restrict__ sums) {
+    const Tensor t = tensors.of(blockIdx.x);
+    const int64_t at = (blockIdx.x - t.first) * kChunk;
+    const int64_t n = min(kChunk, t.size - at);
     double sum = 0.0;
-    typed(t.dtype[i], [&](auto type) {
-        sum = squares_of(static_cast<const decltype(type) *>(t.data[i]) + at, n);
+    typed(t.dtype, [&](auto type) {
+        sum = squares_of(static_cast<const decltype(type) *>(t.data) + at, n);
     });
-    sum = group_sum(sum, s_sum, kThreads / dev::kWave);
+    sum = group_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(1024) void norm_kernel(const double *__restrict__ sums, int64_t n,
-                                                    float max_norm, float *__restrict__ norm,
-                                                    float *__restrict__ factor) {
-    __shared__ double s_sum[1024 / dev::kWave];
+// The norm from the chunks' sums, whose order is that of a workgroup's threads wherever this runs.
+__device__ __forceinline__ double norm_of(const double *__restrict__ sums, int64_t n) {
+    constexpr int kStep = 16;
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) sum += sums[i];
-    sum = group_sum(sum, s_sum, 1024 / dev::kWave);
-    if (threadIdx.x != 0) return;
-    const double root = sqrt(sum);
-    *norm = static_cast<float>(root);
-    const double f = static_cast<double>(max_norm) / (root + 1e-6);
+    for (int64_t i0 = threadIdx.x; i0 < n; i0 += kThreads * kStep) {
+        double x[kStep];
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) {
+            const int64_t i = i0 + s * kThreads;
+            x[s] = i < n ? sums[i] : 0.0;
+        }
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) sum += x[s];
+    }
+    return sqrt(group_sum(sum));
+}
+
+__device__ __forceinline__ float factor_of(double norm, float max_norm) {
+    const double f = static_cast<double>(max_norm) / (norm + 1e-6);
     // (no number stays; a limit of infinity is none)
-    *factor = max_norm == dense::kInf && root == root ? 1.0f
-              : f >= 1.0                              ? 1.0f
-                                                      : static_cast<float>(f);
+    return max_norm == dense::kInf && norm == norm ? 1.0f
+           : f >= 1.0                              ? 1.0f
+                                                   : static_cast<float>(f);
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double *__restrict__ sums, int64_t n,
+                                                        float max_norm, float *__restrict__ norm,
+                                                        float *__restrict__ factor) {
+    const double x = norm_of(sums, n);
+    if (threadIdx.x != 0) return;
+    *norm = static_cast<float>(x);
+    *factor = factor_of(x, max_norm);
 }
 
 template <typename T, typename O>
 __device__ __forceinline__ void scale_of(const T *p, O *out, int64_t n, float factor) {
-    constexpr int kN = 16 / sizeof(T), kStep = 4;
+    // (16 bytes of the wider of the two: a wavefront's stores lie next to each other)
+    constexpr int kN = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
+    constexpr int kStep = sizeof(T) == sizeof(O) ? 4 : 8;
+    constexpr uintptr_t kAlign = kN * sizeof(T) - 1;
     auto scaled = [&](T v) { return static_cast<O>(factor * static_cast<float>(v)); };
-    int64_t head =
-        min(n, static_cast<int64_t>((-reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T)));
+    const int64_t head =
+        min(n, static_cast<int64_t>((-reinterpret_cast<uintptr_t>(p) & kAlign) / sizeof(T)));
     // (both sides in whole pieces, or element by element)
-    const bool both = (reinterpret_cast<uintptr_t>(out + head) & 15) == 0;
+    const bool both = (reinterpret_cast<uintptr_t>(out + head) & (kN * sizeof(O) - 1)) == 0;
     if (!both) {
-        for (int64_t i0 = threadIdx.x; i0 < n; i0 += kThreads * 2 * kStep) {
-            T v[2 * kStep];
+        for (int64_t i0 = threadIdx.x; i0 < n; i0 += kThreads * kStep) {
+            T v[kStep];
 #pragma unroll
-            for (int s = 0; s < 2 * kStep; ++s) {
+            for (int s = 0; s < kStep; ++s) {
                 if (i0 + s * kThreads < n) v[s] = p[i0 + s * kThreads];
             }
 #pragma unroll
-            for (int s = 0; s < 2 * kStep; ++s) {
+            for (int s = 0; s < kStep; ++s) {
                 if (i0 + s * kThreads < n) out[i0 + s * kThreads] = scaled(v[s]);
             }
         }
@@ -170,16 +229,10 @@ __device__ __forceinline__ void scale_of(const T *p, O *out, int64_t n, float fa
         for (int s = 0; s < kStep; ++s) {
             const int64_t i = i0 + s * kThreads;
             if (i < whole) {
-                // (16 or 32 bytes)
-                constexpr int kM = 16 / sizeof(O);
-                Piece<O, kM> *to = reinterpret_cast<Piece<O, kM> *>(out + head + i * kN);
+                Piece<O, kN> o;
 #pragma unroll
-                for (int h = 0; h < kN / kM; ++h) {
-                    Piece<O, kM> o;
-#pragma unroll
-                    for (int j = 0; j < kM; ++j) o.v[j] = scaled(piece[s].v[h * kM + j]);
-                    dense::store_piece<O, kM>(reinterpret_cast<O *>(to + h), o);
-                }
+                for (int j = 0; j < kN; ++j) o.v[j] = scaled(piece[s].v[j]);
+                dense::store_piece<O, kN>(out + head + i * kN, o);
             }
         }
     }
@@ -190,20 +243,38 @@ __device__ __forceinline__ void scale_of(const T *p, O *out, int64_t n, float fa
     }
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(Table t,
-                                                         const float *__restrict__ factor) {
-    const int i = tensor_of(t, blockIdx.x);
-    const int64_t at = (blockIdx.x - t.first[i]) * kChunk;
-    const int64_t n = min(kChunk, t.size[i] - at);
-    const float f = *factor;
-    if (f == 1.0f && t.data[i] == t.out[i]) return;  // (as they are)
-    typed(t.dtype[i], [&](auto type) {
+// What the chunks are scaled by: `factor`, or where that is null, what the chunks' sums give.
+struct Limit {
+    const float *factor;
+    const double *sums;
+    int64_t chunks;
+    float max_norm;
+    float *norm;
+};
+
+// Chunks go from the last to the first: those that the norm has read last are still in a cache.
+template <typename Tensors>
+__global__ __launch_bounds__(kThreads) void scale_kernel(Tensors tensors, Limit limit) {
+    float f;
+    if (limit.factor) {
+        f = *limit.factor;
+    } else {
+        const double norm = norm_of(limit.sums, limit.chunks);
+        f = factor_of(norm, limit.max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *limit.norm = static_cast<float>(norm);
+    }
+    const unsigned chunk = gridDim.x - 1 - blockIdx.x;
+    const Tensor t = tensors.of(chunk);
+    const int64_t at = (chunk - t.first) * kChunk;
+    const int64_t n = min(kChunk, t.size - at);
+    if (f == 1.0f && t.data == t.out) return;  // (as they are)
+    typed(t.dtype, [&](auto type) {
         using T = decltype(type);
-        const T *from = static_cast<const T *>(t.data[i]) + at;
-        if (t.out_dtype[i] == t.dtype[i]) {
-            scale_of(from, static_cast<T *>(t.out[i]) + at, n, f);
+        const T *from = static_cast<const T *>(t.data) + at;
+        if (t.out_dtype == t.dtype) {
+            scale_of(from, static_cast<T *>(t.out) + at, n, f);
         } else {
-            scale_of(from, static_cast<float *>(t.out[i]) + at, n, f);
+            scale_of(from, static_cast<float *>(t.out) + at, n, f);
         }
     });
 }
@@ -211,8 +282,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t,
 // ---- host -----------------------------------------------------------------------------
 
 int check(const nacho_gradient *tensors, int64_t count, bool clip, const float *norm,
-          int64_t *chunks) {
-    *chunks = 0;
+          int64_t *held, int64_t *chunks) {
+    *held = *chunks = 0;
     if (count < 0 || (count > 0 && !tensors) || !norm) return NACHO_ERR_INVALID_ARGUMENT;
     for (int64_t i = 0; i < count; ++i) {
         const nacho_gradient &t = tensors[i];
@@ -226,34 +297,31 @@ int check(const nacho_gradient *tensors, int64_t count, bool clip, const float *
                      (t.size > 0 && (!t.out || !element_aligned(t.out, item_of(t.out_dtype)))))) {
             return NACHO_ERR_INVALID_ARGUMENT;
         }
-        if (t.size > int64_t{1} << 46) return NACHO_ERR_INDEX_OVERFLOW;
-        *chunks += (t.size + kChunk - 1) / kChunk;
+        *held += t.size > 0;
+        *chunks += t.size / kChunk + (t.size % kChunk > 0);
+        if (*chunks > dense::kMostGroups) return NACHO_ERR_INDEX_OVERFLOW;
     }
-    // (also the chunks of each launch)
-    return *chunks > dense::kMostGroups ? NACHO_ERR_INDEX_OVERFLOW : NACHO_OK;
+    return NACHO_OK;
 }
 
-// Calls f(table, chunks, chunks before) for each launch's tensors.
+// Calls f(table, tensors before) with the tensors that have elements, kTensors at a time.
 template <typename F>
 int each_table(const nacho_gradient *tensors, int64_t count, F f) {
     Table t;
     t.count = 0;
-    t.first[0] = 0;
     int64_t before = 0;
+    unsigned chunk = 0;
     for (int64_t i = 0; i < count; ++i) {
         const nacho_gradient &x = tensors[i];
         if (x.size > 0) {
-            const int n = t.count++;
-            t.data[n] = x.data;
-            t.out[n] = x.out;
-            t.size[n] = x.size;
-            t.dtype[n] = static_cast<unsigned char>(x.dtype);
-            t.out_dtype[n] = static_cast<unsigned char>(x.out_dtype);
-            t.first[n + 1] = t.first[n] + static_cast<unsigned>((x.size + kChunk - 1) / kChunk);
+            t.tensors[t.count++] = {x.data, x.out, x.size, chunk,
+                                    static_cast<unsigned char>(x.dtype),
+                                    static_cast<unsigned char>(x.out_dtype)};
+            chunk += static_cast<unsigned>((x.size + kChunk - 1) / kChunk);
         }
-        if (t.count > 0 && (t.count == kTensors || i + 1 == count)) {
-            NACHO_TRY(f(t, t.first[t.count], before));
-            before += t.first[t.count];
+        if (t.count == kTensors || (i + 1 == count && t.count > 0)) {
+            NACHO_TRY(f(t, before));
+            before += t.count;
             t.count = 0;
         }
     }
@@ -262,27 +330,50 @@ int each_table(const nacho_gradient *tensors, int64_t count, F f) {
 
 int run(const nacho_gradient *tensors, int64_t count, bool clip, float max_norm, float *norm,
         void *stream, const nacho_allocator *alloc) {
-    int64_t chunks = 0;
+    int64_t held = 0, chunks = 0;
     if (clip && !(max_norm >= 0.0f)) return NACHO_ERR_INVALID_ARGUMENT;
-    NACHO_TRY(check(tensors, count, clip, norm, &chunks));
+    NACHO_TRY(check(tensors, count, clip, norm, &held, &chunks));
     Call call(stream, alloc);
     const hipStream_t s = call.stream();
     double *sums = nullptr;  // and the factor
     NACHO_TRY(call.scratch_n(static_cast<size_t>(chunks) + 1, &sums));
     float *factor = reinterpret_cast<float *>(sums + chunks);
-    NACHO_TRY(each_table(tensors, count, [&](const Table &t, unsigned n, int64_t before) -> int {
-        square_kernel<<<n, kThreads, 0, s>>>(t, sums + before);
+    const unsigned grid = static_cast<unsigned>(chunks);
+    auto with = [&](const auto &from) -> int {
+        using Tensors = std::decay_t<decltype(from)>;
+        if (grid > 0) {
+            square_kernel<Tensors><<<grid, kThreads, 0, s>>>(from, sums);
+            NACHO_TRY_HIP(hipGetLastError());
+        }
+        const bool few = clip && grid > 0 && chunks <= kFewChunks;
+        if (!few) {
+            norm_kernel<<<1, kThreads, 0, s>>>(sums, chunks, max_norm, norm, factor);
+            NACHO_TRY_HIP(hipGetLastError());
+        }
+        if (clip && grid > 0) {
+            const Limit limit{few ? nullptr : factor, sums, chunks, max_norm, norm};
+            scale_kernel<Tensors><<<grid, kThreads, 0, s>>>(from, limit);
+            NACHO_TRY_HIP(hipGetLastError());
+        }
+        return NACHO_OK;
+    };
+    if (held <= kTensors) {
+        InArguments from;
+        from.table.count = 0;
+        NACHO_TRY(each_table(tensors, count, [&](const Table &t, int64_t) -> int {
+            from.table = t;
+            return NACHO_OK;
+        }));
+        return with(from);
+    }
+    Tensor *list = nullptr;
+    NACHO_TRY(call.scratch_n(static_cast<size_t>(held), &list));
+    NACHO_TRY(each_table(tensors, count, [&](const Table &t, int64_t before) -> int {
+        table_kernel<<<1, dev::kWave, 0, s>>>(t, list + before);
         NACHO_TRY_HIP(hipGetLastError());
         return NACHO_OK;
     }));
-    norm_kernel<<<1, 1024, 0, s>>>(sums, chunks, max_norm, norm, factor);
-    NACHO_TRY_HIP(hipGetLastError());
-    if (!clip) return NACHO_OK;
-    return each_table(tensors, count, [&](const Table &t, unsigned n, int64_t) -> int {
-        scale_kernel<<<n, kThreads, 0, s>>>(t, factor);
-        NACHO_TRY_HIP(hipGetLastError());
-        return NACHO_OK;
-    });
+    return with(InMemory{list, held});
 }
 
 }  // namespace grad_norm

@@ -166,6 +166,25 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict_
     }
 }
 
+// ---- tiles ------------------------------------------------------------------------------
+
+// Workgroups that run at a time, one a compute unit.
+constexpr unsigned kUnits = 256;
+
+// All tiles are of 512 threads.  Wide ones are those of calls with many tokens, whose products bound
+// them; a tile at the end of the tokens, the words or the columns takes as little of each as it
+// needs.
+constexpr int kTileThreads = 512;
+template <int BM, int BN>
+using Tile = std::conditional_t<
+    BM == 256, std::conditional_t<BN == 256, Shape<256, 256, 2, 4>,
+                                  std::conditional_t<BN == 16, Shape<256, 16, 8, 1>,
+                                                     Shape<256, BN, 4, 2>>>,
+    std::conditional_t<BN == 256, Shape<64, 256, 1, 8>,
+                       std::conditional_t<BN == 16, Shape<64, 16, 4, 1>, Shape<64, 64, 2, 4>>>>;
+template <int N>
+using Number = std::integral_constant<int, N>;
+
 // ---- logits -----------------------------------------------------------------------------
 
 struct Logits {
@@ -176,11 +195,11 @@ struct Logits {
     int64_t table_stride;
     int words;             // of this piece
     int first;             // its first word
-    unsigned m_tiles, n_tiles;
     const int *target;
     float scale;
     // the forward pass
     float2 *parts;         // [held][m_tiles]: m and s of a tile's words
+    unsigned m_tiles;
     float *mine;           // [held]: the target's logit
     // the backward pass
     const float *most;     // m by token of the whole batch
@@ -188,11 +207,52 @@ struct Logits {
     const int *token;
     const float *factor;   // null: 1
     void *dz;              // [held][dz_stride]
-    int64_t dz_stride;     // a multiple of the rows of a tile: words past the piece's get zeros
+    int64_t dz_stride;     // a multiple of 256: words past the piece's get zeros
 };
 
 template <typename T>
 constexpr float kDzScale = __is_same(T, _Float16) ? 0x1p14f : 1.0f;
+
+// Calls f(shape, first word, its tile, first token) for this workgroup's tile of BM x BN.
+//
+// Where BN is 256 the tiles of the last round, if they are few, are cut along the tokens so that
+// more compute units have one: 1000 tokens of 50001 words are 784 tiles, three rounds and 16 tiles.
+template <int BM, int BN, typename F>
+__device__ __forceinline__ void with_tile(int words, int held, F f) {
+    const unsigned m_tiles = (words + BM - 1) / BM, n_tiles = (held + BN - 1) / BN;
+    const unsigned all = m_tiles * n_tiles;
+    unsigned mt = 0, nt = 0;
+    if constexpr (BN == 256) {
+        const unsigned rest = all % kUnits;
+        const unsigned cut = rest == 0 ? 1 : rest <= kUnits / 4 ? 4 : rest <= kUnits / 2 ? 2 : 1;
+        const unsigned whole = cut == 1 ? all : all - rest;
+        const unsigned late = blockIdx.x - whole;
+        int wide = 256, n0 = 0;
+        if (blockIdx.x < whole) {
+            dense::tile_of(dense::order_of(blockIdx.x, whole), m_tiles, n_tiles, mt, nt);
+        } else {
+            if (cut == 1 || late >= rest * cut) return;
+            dense::tile_of(whole + late / cut, m_tiles, n_tiles, mt, nt);
+            wide = 256 / static_cast<int>(cut);
+            n0 = static_cast<int>(late % cut) * wide;
+        }
+        n0 += static_cast<int>(nt) * 256;
+        const int left = held - n0;
+        if (left <= 0) return;
+        const int64_t v0 = static_cast<int64_t>(mt) * BM;
+        if (wide <= 64 || left <= 64) {
+            f(Tile<BM, 64>{}, v0, mt, n0);
+        } else if (wide <= 128 || left <= 128) {
+            f(Tile<BM, 128>{}, v0, mt, n0);
+        } else {
+            f(Tile<BM, 256>{}, v0, mt, n0);
+        }
+    } else {
+        if (blockIdx.x >= all) return;
+        dense::tile_of(dense::order_of(blockIdx.x, all), m_tiles, n_tiles, mt, nt);
+        f(Tile<BM, BN>{}, static_cast<int64_t>(mt) * BM, mt, static_cast<int>(nt) * BN);
+    }
+}
 
 // The tile's product of table and rows.
 template <typename T, typename S>
@@ -206,26 +266,25 @@ __device__ __forceinline__ void logits_of(const Logits &a, int64_t v0, int64_t n
         static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))), a.width, lds, z);
 }
 
+// m and s of a tile's words for each of its tokens, and the logits of targets among them.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void parts_kernel(Logits a) {
-    __shared__ __attribute__((aligned(16))) T lds[Product<T, S, Along, Along>::kLdsElements];
-    unsigned mt, nt;
-    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
-    const int held = *a.held;
-    const int64_t v0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
-    if (n0 >= held) return;
-    f32x4 z[S::MT][S::NT];
-    logits_of<T, S>(a, v0, n0, held, lds, z);
+__device__ __forceinline__ void tile_parts(const Logits &a, int64_t v0, unsigned mt, int64_t n0,
+                                           int held, T *lds) {
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
+    int64_t target[S::NT];  // among the tile's words
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
+        target[t] = n < held ? a.target[n] - v0 : -1;
+    }
+    f32x4 z[S::MT][S::NT];
+    logits_of<T, S>(a, v0, n0, held, lds, z);
     float2(*s_part)[S::BN] = reinterpret_cast<float2(*)[S::BN]>(lds);
     __syncthreads();  // (the tiles have been read)
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int col = (wn * S::NT + t) * 16 + c;
-        const int64_t n = n0 + col;
-        // the target's place among this lane's words, if it is one of them
-        const int64_t target = n < held ? a.target[n] - v0 : -1;
         float most = kNegInf;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
@@ -233,7 +292,7 @@ __global__ __launch_bounds__(S::kThreads) void parts_kernel(Logits a) {
             for (int j = 0; j < 4; ++j) {
                 const int v = (wm * S::MT + i) * 16 + 4 * g + j;
                 float x = z[i][t][j] * a.scale;
-                if (v == target) a.mine[n] = x;
+                if (v == target[t]) a.mine[n0 + col] = x;
                 if (v0 + v >= a.words) x = kNegInf;
                 z[i][t][j] = x;
                 most = fmaxf(most, x);
@@ -265,6 +324,20 @@ __global__ __launch_bounds__(S::kThreads) void parts_kernel(Logits a) {
         }
         a.parts[(n0 + col) * a.m_tiles + mt] = float2{most, total};
     }
+}
+
+// LDS of the largest tile that a kernel of BM x BN tiles has.
+template <typename T, int BM, int BN, template <typename, int, int> class A,
+          template <typename, int, int> class B>
+constexpr int kLds = Product<T, Tile<BM, BN>, A, B>::kLdsElements;
+
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__((Tile<BM, BN>::kThreads)) void parts_kernel(Logits a) {
+    __shared__ __attribute__((aligned(16))) T lds[kLds<T, BM, BN, Along, Along>];
+    const int held = *a.held;
+    with_tile<BM, BN>(a.words, held, [&](auto shape, int64_t v0, unsigned mt, int n0) {
+        tile_parts<T, decltype(shape)>(a, v0, mt, n0, held, lds);
+    });
 }
 
 // A wavefront per token: its tiles' parts to m, s and the loss.
@@ -329,27 +402,30 @@ __global__ __launch_bounds__(1024) void sum_kernel(const int *__restrict__ count
     *loss = static_cast<float>(mean ? sum / max(*count, 1) : sum);
 }
 
-// dz of a piece.
+// dz of a tile's words and tokens.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void dz_kernel(Logits a) {
-    __shared__ __attribute__((aligned(16))) T lds[Product<T, S, Along, Along>::kLdsElements];
-    unsigned mt, nt;
-    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
-    const int held = *a.held;
-    const int64_t v0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
-    if (n0 >= held) return;
-    f32x4 z[S::MT][S::NT];
-    logits_of<T, S>(a, v0, n0, held, lds, z);
+__device__ __forceinline__ void tile_dz(const Logits &a, int64_t v0, int64_t n0, int held,
+                                        T *lds) {
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
+    // (on their way before the product: nothing is left to wait for behind it)
+    int target[S::NT];
+    float most[S::NT], part[S::NT], factor[S::NT];
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t) {
+        const int64_t n = min(n0 + (wn * S::NT + t) * 16 + c, static_cast<int64_t>(held - 1));
+        const int token = a.token[n];
+        target[t] = static_cast<int>(a.target[n] - a.first - v0);
+        most[t] = a.most[token];
+        part[t] = 1.0f / a.total[token];
+        factor[t] = kDzScale<T> * (a.factor ? a.factor[n] : 1.0f);
+    }
+    f32x4 z[S::MT][S::NT];
+    logits_of<T, S>(a, v0, n0, held, lds, z);
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
         if (n >= held) continue;
-        const int64_t target = a.target[n] - static_cast<int64_t>(a.first) - v0;
-        const int token = a.token[n];
-        const float most = a.most[token], part = 1.0f / a.total[token];
-        const float factor = kDzScale<T> * (a.factor ? a.factor[n] : 1.0f);
         T *to = static_cast<T *>(a.dz) + n * a.dz_stride + v0;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
@@ -358,13 +434,22 @@ __global__ __launch_bounds__(S::kThreads) void dz_kernel(Logits a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float x = z[i][t][j] * a.scale;
-                float p = dense::exp2_fast((x - most) * kLog2e) * part;
-                if (v + j == target) p -= 1.0f;
-                d[j] = v0 + v + j < a.words ? p * factor : 0.0f;
+                float p = dense::exp2_fast((x - most[t]) * kLog2e) * part[t];
+                if (v + j == target[t]) p -= 1.0f;
+                d[j] = v0 + v + j < a.words ? p * factor[t] : 0.0f;
             }
             dense::store4<T>(to + v, d);
         }
     }
+}
+
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__((Tile<BM, BN>::kThreads)) void dz_kernel(Logits a) {
+    __shared__ __attribute__((aligned(16))) T lds[kLds<T, BM, BN, Along, Along>];
+    const int held = *a.held;
+    with_tile<BM, BN>(a.words, held, [&](auto shape, int64_t v0, unsigned, int n0) {
+        tile_dz<T, decltype(shape)>(a, v0, n0, held, lds);
+    });
 }
 
 // ---- the gradients' products ------------------------------------------------------------
@@ -378,42 +463,70 @@ struct Gradients {
     int64_t table_stride;
     int64_t words, width; // of the piece; of the results
     int64_t padded;       // columns that the operands' rows have
-    unsigned m_tiles, n_tiles;
-    int64_t split;        // words of a split of dx's sums
-    int64_t tokens;       // rows of a split's sums
-    float *sums;          // [split][tokens][sums_stride]
+    int64_t piece;        // words of a whole piece
+    int64_t most_rows;    // that the sums have room for, at least all tokens
+    float *sums;          // [split][held][sums_stride]; null: no dx
     int64_t sums_stride;
     int first;            // whether the piece is the first
     const float *common;
     float scale;
-    void *dtable;         // of the piece, [words][width]
+    void *dtable;         // of the piece, [words][width]; null: none
 };
 
-// dx: the columns of the table's rows by the tokens, over the words of a split.
+// How dx's products, tiles of its columns by the tokens, are split over the words: into items of
+// about half of a compute unit's work, that of dtable included where one launch has both, so that
+// the units' work is even.  The same for every piece, and known to the device alone.
+struct Splits {
+    unsigned m_tiles, n_tiles, count;
+    int64_t words;  // of a split
+
+    __device__ __forceinline__ unsigned items() const { return m_tiles * n_tiles * count; }
+};
+
+constexpr unsigned kMostItems = 512, kMostSplits = 64;
+
+template <typename T, int BN>
+__device__ __forceinline__ Splits splits_of(int64_t piece, int64_t width, int64_t most_rows,
+                                            int held, bool both) {
+    constexpr int kStep = dense::kStepK<T>;
+    Splits s;
+    s.m_tiles = static_cast<unsigned>((width + 255) / 256);
+    s.n_tiles = static_cast<unsigned>((held + BN - 1) / BN);
+    const int64_t steps = (piece + kStep - 1) / kStep;
+    const int64_t tiles = static_cast<int64_t>(s.m_tiles) * s.n_tiles;
+    int64_t load = tiles * steps;
+    if (both) load += (piece + 255) / 256 * s.m_tiles * ((held + kStep - 1) / kStep);
+    // (0.55 of it: two and a bit to a unit are one each and no third)
+    const int64_t wanted = load * 11 / (20 * static_cast<int64_t>(kUnits));
+    const int64_t per = wanted < 8 ? 8 : wanted;
+    int64_t n = (steps + per - 1) / per;
+    n = min(n, static_cast<int64_t>(kMostItems) / max(tiles, int64_t{1}));
+    n = min(n, static_cast<int64_t>(kMostSplits));
+    n = min(n, most_rows / max(held, 1));
+    n = max(n, int64_t{1});
+    s.words = (steps + n - 1) / n * kStep;
+    s.count = static_cast<unsigned>((piece + s.words - 1) / s.words);
+    return s;
+}
+
+// A tile of dx's sums: columns of the table's rows by the tokens, over the words of a split.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void dx_kernel(Gradients a) {
-    using P = Product<T, S, Across, Along>;
-    __shared__ __attribute__((aligned(16))) T lds[P::kLdsElements];
-    unsigned mt, nt;
-    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
-    const int held = *a.held;
-    const int64_t d0 = static_cast<int64_t>(mt) * S::BM, n0 = static_cast<int64_t>(nt) * S::BN;
-    if (n0 >= held) return;
-    const int64_t v0 = blockIdx.y * a.split;
+__device__ __forceinline__ void tile_dx(const Gradients &a, int64_t d0, int64_t n0, unsigned split,
+                                        int64_t v0, int64_t words, int held, T *lds) {
     const Matrix<T> table{static_cast<const T *>(a.table) + v0 * a.table_stride + d0,
                           a.table_stride};
     const Matrix<T> dz{static_cast<const T *>(a.dz) + n0 * a.dz_stride + v0, a.dz_stride};
     f32x4 sums[S::MT][S::NT];
-    P::run(table, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
-           static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))),
-           min(a.split, a.words - v0), lds, sums);
+    Product<T, S, Across, Along>::run(
+        table, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
+        static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))), words, lds, sums);
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
         if (n >= held) continue;
-        float *to = a.sums + (blockIdx.y * a.tokens + n) * a.sums_stride;
+        float *to = a.sums + (static_cast<int64_t>(split) * held + n) * a.sums_stride;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
             const int64_t d = d0 + (wm * S::MT + i) * 16 + 4 * g;
@@ -425,52 +538,16 @@ __global__ __launch_bounds__(S::kThreads) void dx_kernel(Gradients a) {
     }
 }
 
-// dx of every token: the splits' sums in their order, and 0 for a token without a target.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void dx_join_kernel(const int *__restrict__ slot,
-                                                           int64_t tokens, int64_t width,
-                                                           const float *__restrict__ sums,
-                                                           int64_t stride, int splits,
-                                                           const float *__restrict__ common,
-                                                           float scale, T *__restrict__ dx) {
-    const float factor = *common * scale * (1.0f / kDzScale<T>);
-    const int64_t per = (width + 3) / 4;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < tokens * per;
-         i += gridDim.x * static_cast<int64_t>(kThreads)) {
-        const int64_t t = i / per, d = i % per * 4;
-        const int at = slot[t];
-        f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-        if (at >= 0) {
-            for (int s = 0; s < splits; ++s) {
-                sum += *reinterpret_cast<const f32x4 *>(sums + (s * tokens + at) * stride + d);
-            }
-            sum *= factor;
-        }
-        T *to = dx + t * width + d;
-        if (width % 4 == 0) {
-            dense::store4<T>(to, sum);
-        } else {
-            for (int j = 0; j < 4; ++j) {
-                if (d + j < width) to[j] = static_cast<T>(sum[j]);
-            }
-        }
-    }
-}
-
-// dw of a piece: the columns of the gathered rows by the words, over the tokens.
+// A tile of dtable: columns of the gathered rows by the words, over the tokens.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void dtable_kernel(Gradients a) {
-    using P = Product<T, S, Across, Across>;
-    __shared__ __attribute__((aligned(16))) T lds[P::kLdsElements];
-    unsigned mt, nt;
-    dense::tile_of(blockIdx.x, a.m_tiles, a.n_tiles, mt, nt);
-    const int64_t d0 = static_cast<int64_t>(mt) * S::BM, v0 = static_cast<int64_t>(nt) * S::BN;
+__device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int64_t v0, int held,
+                                            T *lds) {
     const Matrix<T> rows{static_cast<const T *>(a.rows) + d0, a.padded};
     const Matrix<T> dz{static_cast<const T *>(a.dz) + v0, a.dz_stride};
     f32x4 sums[S::MT][S::NT];
-    P::run(rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
-           static_cast<int>(min(a.dz_stride - v0, static_cast<int64_t>(S::BN))), *a.held, lds,
-           sums);
+    Product<T, S, Across, Across>::run(
+        rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
+        static_cast<int>(min(a.dz_stride - v0, static_cast<int64_t>(S::BN))), held, lds, sums);
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
@@ -490,6 +567,95 @@ __global__ __launch_bounds__(S::kThreads) void dtable_kernel(Gradients a) {
                 for (int j = 0; j < 4; ++j) {
                     if (d + j < a.width) to[d + j] = static_cast<T>(x[j]);
                 }
+            }
+        }
+    }
+}
+
+// Calls f with the tile of at most BM x BN that `m` by `n` need.
+template <int BN, typename F>
+__device__ __forceinline__ void with_ends(int64_t m, int64_t n, F f) {
+    if (BN <= 64 || n <= 64) {
+        constexpr int kBN = BN <= 64 ? BN : 64;
+        f(Tile<256, kBN>{});
+    } else if (m <= 64) {
+        f(Tile<64, BN>{});
+    } else {
+        f(Tile<256, BN>{});
+    }
+}
+
+// dx's items, then dtable's tiles: one launch for calls of many tokens (BN 256), else one for each.
+template <typename T, int BN, bool DX, bool DTABLE>
+__global__ __launch_bounds__(kTileThreads) void gradients_kernel(Gradients a) {
+    constexpr int kLdsX = DX ? kLds<T, 256, BN, Across, Along> : 0;
+    constexpr int kLdsT = DTABLE ? kLds<T, 256, (BN <= 64 ? 64 : BN), Across, Across> : 0;
+    __shared__ __attribute__((aligned(16))) T lds[kLdsX > kLdsT ? kLdsX : kLdsT];
+    const int held = *a.held;
+    unsigned at = blockIdx.x, mt = 0, nt = 0;
+    if constexpr (DX) {
+        const Splits s = splits_of<T, BN>(a.piece, a.width, a.most_rows, held, DTABLE);
+        const unsigned items = s.items();
+        if (at < items) {
+            at = dense::order_of(at, items);
+            const unsigned tiles = s.m_tiles * s.n_tiles, split = at / tiles;
+            dense::tile_of(at % tiles, s.m_tiles, s.n_tiles, mt, nt);
+            const int64_t d0 = mt * int64_t{256}, n0 = nt * static_cast<int64_t>(BN);
+            const int64_t v0 = split * s.words;
+            // (a short last piece has fewer splits; a first one's sums are all written)
+            if (v0 >= a.words && !a.first) return;
+            with_ends<BN>(a.padded - d0, held - n0, [&](auto shape) {
+                tile_dx<T, decltype(shape)>(a, d0, n0, split, v0, min(s.words, a.words - v0),
+                                            held, lds);
+            });
+            return;
+        }
+        at -= items;
+    }
+    if constexpr (DTABLE) {
+        constexpr int kBN = BN <= 64 ? 64 : BN;
+        const unsigned m_tiles = static_cast<unsigned>((a.width + 255) / 256);
+        const unsigned n_tiles = static_cast<unsigned>((a.words + kBN - 1) / kBN);
+        const unsigned tiles = m_tiles * n_tiles;
+        if (at >= tiles) return;
+        dense::tile_of(dense::order_of(at, tiles), m_tiles, n_tiles, mt, nt);
+        const int64_t d0 = mt * int64_t{256}, v0 = nt * static_cast<int64_t>(kBN);
+        with_ends<kBN>(a.padded - d0, a.words - v0, [&](auto shape) {
+            tile_dtable<T, decltype(shape)>(a, d0, v0, held, lds);
+        });
+    }
+}
+
+// dx of every token: the splits' sums in their order, and 0 for a token without a target.
+template <typename T, int BN>
+__global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
+                                                           const int *__restrict__ slot,
+                                                           int64_t tokens, bool both,
+                                                           T *__restrict__ dx) {
+    const int held = *a.held;
+    const unsigned splits =
+        splits_of<T, BN>(a.piece, a.width, a.most_rows, held, both).count;
+    const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
+    const int64_t per = (a.width + 3) / 4;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < tokens * per;
+         i += gridDim.x * static_cast<int64_t>(kThreads)) {
+        const int64_t t = i / per, d = i % per * 4;
+        const int at = slot[t];
+        f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0) {
+            const float *from = a.sums + at * a.sums_stride + d;
+#pragma unroll 4
+            for (unsigned s = 0; s < splits; ++s) {
+                sum += *reinterpret_cast<const f32x4 *>(from + s * (held * a.sums_stride));
+            }
+            sum *= factor;
+        }
+        T *to = dx + t * a.width + d;
+        if (a.width % 4 == 0) {
+            dense::store4<T>(to, sum);
+        } else {
+            for (int j = 0; j < 4; ++j) {
+                if (d + j < a.width) to[j] = static_cast<T>(sum[j]);
             }
         }
     }
@@ -601,17 +767,15 @@ struct Operands {
     }
 };
 
-// Tiles by the number of tokens: a tile's products of a few tokens would be of nothing.
-template <typename T, typename F>
-int with_shape(int64_t tokens, F f) {
-    if constexpr (sizeof(T) == 4) {
-        if (tokens <= 16) return f(Shape<128, 16, 4, 1>{});
-        return f(Shape<128, 128, 2, 2>{});
-    } else {
-        if (tokens <= 16) return f(Shape<256, 16, 4, 1>{});
-        if (tokens <= 128) return f(Shape<256, 64, 4, 1>{});
-        return f(Shape<256, 256, 2, 4>{});
-    }
+// Calls f with the words and the tokens of a tile of logits, by the number of tokens: a tile's
+// products of a few tokens would be of nothing.  Few tokens are bound by the table's bytes, of which
+// small tiles of a small vocabulary have more on their way.
+template <typename F>
+int with_shape(int64_t tokens, int64_t words, F f) {
+    if (tokens <= 16 && words < 65536) return f(Number<64>{}, Number<16>{});
+    if (tokens <= 16) return f(Number<256>{}, Number<16>{});
+    if (tokens <= 128) return f(Number<256>{}, Number<64>{});
+    return f(Number<256>{}, Number<256>{});
 }
 
 template <typename F>
@@ -621,13 +785,10 @@ int with_type(int32_t dtype, F f) {
     return f(__bf16{});
 }
 
-// Tiles of a launch; 0 for more than a launch has.
-template <typename S>
-int64_t tiles_of(int64_t m, int64_t n, unsigned *m_tiles, unsigned *n_tiles) {
-    const int64_t a = up(m, S::BM) / S::BM, b = up(n, S::BN) / S::BN;
-    *m_tiles = static_cast<unsigned>(a);
-    *n_tiles = static_cast<unsigned>(b);
-    return a * b < (int64_t{1} << 32) / S::kThreads ? a * b : 0;
+// Workgroups of a launch, and of those at the end that cut tiles make; 0 for more than a launch has.
+unsigned groups_of(int64_t m, int64_t bm, int64_t n, int64_t bn, int64_t more) {
+    const int64_t all = up(m, bm) / bm * (up(n, bn) / bn) + more;
+    return all < (int64_t{1} << 32) / kTileThreads ? static_cast<unsigned>(all) : 0u;
 }
 
 int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_allocator *alloc) {
@@ -640,11 +801,11 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
     const hipStream_t s = call.stream();
     return with_type(a.dtype, [&](auto type) -> int {
         using T = decltype(type);
-        return with_shape<T>(a.tokens, [&](auto shape) -> int {
-            using S = decltype(shape);
-            unsigned m_tiles = 0, n_tiles = 0;
-            const int64_t tiles = tiles_of<S>(a.words, a.tokens, &m_tiles, &n_tiles);
-            if (a.tokens > 0 && tiles == 0) return NACHO_ERR_INDEX_OVERFLOW;
+        return with_shape(a.tokens, a.words, [&](auto bm, auto bn) -> int {
+            const unsigned m_tiles = static_cast<unsigned>(up(a.words, bm()) / bm());
+            const unsigned groups =
+                groups_of(a.words, bm(), a.tokens, bn(), bn() == 256 ? kUnits : 0);
+            if (a.tokens > 0 && groups == 0) return NACHO_ERR_INDEX_OVERFLOW;
             Operands<T> ops;
             const size_t n = static_cast<size_t>(a.tokens);
             float *each = loss;
@@ -665,12 +826,12 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
                 l.table_stride = ops.table_stride;
                 l.words = static_cast<int>(a.words);
                 l.m_tiles = m_tiles;
-                l.n_tiles = n_tiles;
                 l.target = ops.held.target;
                 l.scale = a.scale;
                 l.parts = parts;
                 l.mine = floats;
-                parts_kernel<T, S><<<static_cast<unsigned>(tiles), S::kThreads, 0, s>>>(l);
+                constexpr int kShapeThreads = Tile<bm(), bn()>::kThreads;
+                parts_kernel<T, bm(), bn()><<<groups, kShapeThreads, 0, s>>>(l);
                 NACHO_TRY_HIP(hipGetLastError());
                 join_kernel<<<ceil_div(n, kThreads / dev::kWave), kThreads, 0, s>>>(
                     ops.held.slot, static_cast<int>(a.tokens), m_tiles, parts, floats, most,
@@ -691,10 +852,6 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
 // Bytes of a piece's dz, about, and its least words.
 constexpr int64_t kPieceBytes = int64_t{256} << 20;
 constexpr int64_t kPieceWords = 2048;
-// Workgroups that dx's products are split into, about, where there are few tiles, and a split's
-// least words.
-constexpr int64_t kSplitGroups = 512, kSplitWords = 512;
-
 int backward(const Args &a, const float *stats, const float *dloss, void *dx, void *dtable,
              void *stream, const nacho_allocator *alloc) {
     NACHO_TRY(check(a));
@@ -708,38 +865,36 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
     const hipStream_t s = call.stream();
     return with_type(a.dtype, [&](auto type) -> int {
         using T = decltype(type);
-        using Wide = std::conditional_t<sizeof(T) == 4, Shape<128, 128, 2, 2>,
-                                        Shape<256, 256, 2, 4>>;
         if (a.tokens == 0) {
             return dense::clear(s, static_cast<T *>(dtable), a.words * a.width);
         }
-        return with_shape<T>(a.tokens, [&](auto shape) -> int {
-            using S = decltype(shape);
+        return with_shape(a.tokens, a.words, [&](auto bm, auto bn) -> int {
+            constexpr int kBM = bm(), kBN = bn();
             const size_t n = static_cast<size_t>(a.tokens);
             int64_t piece = up(kPieceBytes / (a.tokens * item), 256);
             if (piece < kPieceWords) piece = kPieceWords;
             if (piece > up(a.words, 256)) piece = up(a.words, 256);
-            Logits l{};
-            Gradients d{};
-            unsigned dx_m = 0, dx_n = 0, dw_m = 0, dw_n = 0;
-            const int64_t dx_tiles = tiles_of<S>(a.width, a.tokens, &dx_m, &dx_n);
-            if (!dx_tiles || !tiles_of<S>(piece, a.tokens, &l.m_tiles, &l.n_tiles) ||
-                !tiles_of<Wide>(a.width, piece, &dw_m, &dw_n)) {
+            const int64_t cut = kBN == 256 ? kUnits : 0;
+            const unsigned dx_groups = groups_of(a.width, 256, a.tokens, kBN, kMostItems);
+            if (!groups_of(piece, kBM, a.tokens, kBN, cut) || !dx_groups ||
+                !groups_of(a.width, 256, piece, 64, dx_groups)) {
                 return NACHO_ERR_INDEX_OVERFLOW;
             }
             Operands<T> ops;
             NACHO_TRY(ops.start(call, a, dloss));
             T *dz = nullptr;
             NACHO_TRY(call.scratch_n(n * static_cast<size_t>(piece), &dz));
-            int64_t splits = kSplitGroups / dx_tiles;
-            if (splits > piece / kSplitWords) splits = piece / kSplitWords;
-            if (splits < 1) splits = 1;
-            d.split = up((piece + splits - 1) / splits, 64);
-            splits = (piece + d.split - 1) / d.split;
+            Logits l{};
+            Gradients d{};
             d.sums_stride = up(a.width, 4);
+            // Room for the sums of as many splits as are made: tiles of 256 columns by kBN tokens,
+            // at most kMostItems of them where they are split.
+            const int64_t most = kMostItems / (up(a.width, 256) / 256) * kBN;
+            d.most_rows = a.tokens * kMostSplits < most ? a.tokens * kMostSplits : most;
+            if (d.most_rows < a.tokens) d.most_rows = a.tokens;
             if (dx) {
-                NACHO_TRY(call.scratch_n(static_cast<size_t>(splits) * n *
-                                             static_cast<size_t>(d.sums_stride), &d.sums));
+                NACHO_TRY(call.scratch_n(static_cast<size_t>(d.most_rows * d.sums_stride),
+                                         &d.sums));
             }
             l.held = d.held = ops.held.count;
             l.width = d.padded = ops.width;
@@ -756,30 +911,35 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             l.dz_stride = d.dz_stride = piece;
             l.table = ops.table;
             d.width = a.width;
-            d.tokens = a.tokens;
+            d.piece = piece;
             d.common = ops.held.common;
+            const bool both = kBN == 256 && dx && dtable;
             for (int64_t v = 0; v < a.words; v += piece) {
                 const int64_t words = a.words - v < piece ? a.words - v : piece;
                 l.first = static_cast<int>(v);
                 l.words = static_cast<int>(words);
-                const int64_t tiles = tiles_of<S>(words, a.tokens, &l.m_tiles, &l.n_tiles);
-                dz_kernel<T, S><<<static_cast<unsigned>(tiles), S::kThreads, 0, s>>>(l);
+                dz_kernel<T, kBM, kBN><<<groups_of(words, kBM, a.tokens, kBN, cut),
+                                         Tile<kBM, kBN>::kThreads, 0, s>>>(l);
                 NACHO_TRY_HIP(hipGetLastError());
                 d.words = words;
                 d.table = ops.table + v * ops.table_stride;
                 d.first = v == 0;
+                if (dtable) d.dtable = static_cast<T *>(dtable) + v * a.width;
+                const unsigned dtable_groups =
+                    groups_of(a.width, 256, words, kBN <= 64 ? 64 : kBN, 0);
+                if (both) {
+                    gradients_kernel<T, 256, true, true>
+                        <<<dx_groups + dtable_groups, kTileThreads, 0, s>>>(d);
+                    NACHO_TRY_HIP(hipGetLastError());
+                    continue;
+                }
                 if (dx) {
-                    d.m_tiles = dx_m, d.n_tiles = dx_n;
-                    dx_kernel<T, S><<<dim3(static_cast<unsigned>(dx_tiles),
-                                           static_cast<unsigned>(splits)), S::kThreads, 0, s>>>(d);
+                    gradients_kernel<T, kBN, true, false><<<dx_groups, kTileThreads, 0, s>>>(d);
                     NACHO_TRY_HIP(hipGetLastError());
                 }
                 if (dtable) {
-                    const int64_t dw_tiles =
-                        tiles_of<Wide>(a.width, words, &d.m_tiles, &d.n_tiles);
-                    d.dtable = static_cast<T *>(dtable) + v * a.width;
-                    dtable_kernel<T, Wide><<<static_cast<unsigned>(dw_tiles), Wide::kThreads, 0,
-                                             s>>>(d);
+                    gradients_kernel<T, kBN, false, true>
+                        <<<dtable_groups, kTileThreads, 0, s>>>(d);
                     NACHO_TRY_HIP(hipGetLastError());
                 }
             }
@@ -787,9 +947,8 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
                 const int64_t groups =
                     (a.tokens * ((a.width + 3) / 4) + kThreads - 1) / kThreads;
                 const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
-                dx_join_kernel<T><<<grid, kThreads, 0, s>>>(
-                    ops.held.slot, a.tokens, a.width, d.sums, d.sums_stride,
-                    static_cast<int>(splits), ops.held.common, a.scale, static_cast<T *>(dx));
+                dx_join_kernel<T, kBN><<<grid, kThreads, 0, s>>>(d, ops.held.slot, a.tokens, both,
+                                                                 static_cast<T *>(dx));
                 NACHO_TRY_HIP(hipGetLastError());
             }
             return NACHO_OK;

@@ -102,7 +102,8 @@ struct Across {
     static constexpr int kPieces = COLS / kPer;
     static constexpr int kElements = COLS * kStepK<T>;
     static constexpr int kLoads = kStepK<T> * kPieces / THREADS;
-    static_assert(kStepK<T> * kPieces % THREADS == 0 && kPieces >= 16, "whole pieces per thread");
+    static_assert(kStepK<T> * kPieces % THREADS == 0 && kPieces * 128 / kStepK<T> >= 16,
+                  "whole pieces per thread, and banks for what is read at a time");
 
     unsigned offset[kLoads];
 
@@ -111,6 +112,8 @@ struct Across {
     __device__ __forceinline__ static int swizzle(int row) {
         if constexpr (sizeof(T) == 4) {
             return (row >> 3 & 3) << 2;
+        } else if constexpr (kPieces == 8) {  // (two rows in all banks)
+            return ((row >> 1 & 1) | (row >> 3 & 1) << 1) << 1;
         } else {
             return ((row & 3) | (row >> 3 & 1) << 2) << 1;
         }
@@ -241,17 +244,20 @@ struct Product {
     }
 };
 
-// Tile `at` of m_tiles x n_tiles.  Workgroups go to the eight dies in turn, each with a cache of
-// its own: a die gets tiles next to each other, in groups of kGroup along n, so that it reads few
-// different rows at a time.
-__device__ __forceinline__ void tile_of(unsigned at, unsigned m_tiles, unsigned n_tiles,
-                                        unsigned &m, unsigned &n) {
-    constexpr unsigned kDies = 8, kGroup = 8;
-    const unsigned all = m_tiles * n_tiles;
+// The order of workgroup `at` of `all`.  Workgroups go to the eight dies in turn, each with a cache
+// of its own: a die gets neighbours.
+__device__ __forceinline__ unsigned order_of(unsigned at, unsigned all) {
+    constexpr unsigned kDies = 8;
     const unsigned die = at % kDies, per = all / kDies, more = all % kDies;
-    unsigned i = die * per + min(die, more) + at / kDies;
-    const unsigned group = i / (kGroup * m_tiles);
-    const unsigned first = group * kGroup, wide = min(kGroup, n_tiles - first);
+    return die * per + min(die, more) + at / kDies;
+}
+
+// Tile i of m_tiles x n_tiles, in groups of kGroup along n, so that neighbours read few different
+// rows.
+__device__ __forceinline__ void tile_of(unsigned i, unsigned m_tiles, unsigned n_tiles,
+                                        unsigned &m, unsigned &n) {
+    constexpr unsigned kGroup = 8;
+    const unsigned first = i / (kGroup * m_tiles) * kGroup, wide = min(kGroup, n_tiles - first);
     i -= first * m_tiles;
     n = first + i % wide;
     m = i / wide;

@@ -131,6 +131,8 @@ struct Clear {
     dense::u32x4 *pieces;
     int64_t from, to;      // of 16 bytes, in this launch
     unsigned first;        // the first workgroup that clears
+    uint16_t *ends[2];     // before and behind all pieces, in the launch that clears the first
+    int in_ends[2];
 
     // Whether the workgroup is one of those, and has done its part.
     __device__ __forceinline__ bool done() const {
@@ -140,6 +142,12 @@ struct Clear {
         for (int64_t i = from + (blockIdx.x - first) * static_cast<int64_t>(blockDim.x) +
                          threadIdx.x; i < to; i += all) {
             __builtin_nontemporal_store(zero, pieces + i);
+        }
+        if (from == 0 && blockIdx.x == first) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (static_cast<int>(threadIdx.x) < in_ends[e]) ends[e][threadIdx.x] = 0;
+            }
         }
         return true;
     }
@@ -434,7 +442,7 @@ struct Part {
 template <typename T, int N, int LANES>
 __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restrict__ dout,
                                                        int64_t stride, T *__restrict__ dtable) {
-    constexpr int kStep = 8;
+    constexpr int kStep = 16;
     const Part<N, LANES> part(a);
     if (!part.there) return;
     const int first = part.run * kChunk, end = min(first + kChunk, a.tokens);
@@ -577,23 +585,44 @@ int lookup(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sc
     });
 }
 
-// The tokens sorted by word into keys and order, and `pieces` of 16 bytes cleared.
-int sort_tokens(Call &call, const Ids &ids, int tokens, int *keys, int *order,
-                dense::u32x4 *pieces, int64_t n_pieces) {
+// Memory that is cleared: 16-byte pieces, and what is before and behind them in units of 2 bytes.
+struct Cleared {
+    dense::u32x4 *pieces;
+    int64_t n;
+    uint16_t *ends[2];
+    int in_ends[2];
+
+    Cleared(void *p, int64_t bytes) {
+        char *const at = static_cast<char *>(p);
+        int64_t head = static_cast<int64_t>(-reinterpret_cast<uintptr_t>(p) & 15);
+        if (head > bytes) head = bytes;
+        n = (bytes - head) / 16;
+        pieces = reinterpret_cast<dense::u32x4 *>(at + head);
+        ends[0] = reinterpret_cast<uint16_t *>(at);
+        ends[1] = reinterpret_cast<uint16_t *>(at + head + 16 * n);
+        in_ends[0] = static_cast<int>(head / 2);
+        in_ends[1] = static_cast<int>((bytes - head - 16 * n) / 2);
+    }
+};
+
+// The tokens sorted by word: keys of all places, then their tokens.  Clears `all` meanwhile.
+int sort_tokens(Call &call, const Ids &ids, int tokens, const Cleared &all, int **sorted) {
     const hipStream_t s = call.stream();
     // Launch i of n: its share of the pieces, and a grid with workgroups for them.
     auto share = [&](unsigned groups, int threads, int i, int n, unsigned *grid) {
-        const Clear c{pieces, n_pieces * i / n, n_pieces * (i + 1) / n, groups};
+        const Clear c{all.pieces, all.n * i / n, all.n * (i + 1) / n, groups,
+                      {all.ends[0], all.ends[1]}, {all.in_ends[0], all.in_ends[1]}};
         const int64_t want = (c.to - c.from + threads * 4 - 1) / (threads * 4);
         const int64_t most = 2048 * 256 / threads;
-        *grid = groups + static_cast<unsigned>(want < most ? want : most);
+        *grid = groups + static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
         return c;
     };
     unsigned grid = 0;
+    const size_t n = static_cast<size_t>(tokens);
     if (tokens <= kRankMost) {
-        const Clear clear = share(ceil_div(static_cast<size_t>(tokens), dev::kWave), kRankThreads,
-                                  0, 1, &grid);
-        rank_kernel<<<grid, kRankThreads, 0, s>>>(ids, tokens, keys, order, clear);
+        NACHO_TRY(call.scratch_n(2 * n, sorted));
+        const Clear clear = share(ceil_div(n, dev::kWave), kRankThreads, 0, 1, &grid);
+        rank_kernel<<<grid, kRankThreads, 0, s>>>(ids, tokens, *sorted, *sorted + n, clear);
         NACHO_TRY_HIP(hipGetLastError());
         return NACHO_OK;
     }
@@ -603,19 +632,16 @@ int sort_tokens(Call &call, const Ids &ids, int tokens, int *keys, int *order,
     const int passes = (bits + kDigitBits - 1) / kDigitBits;
     const bool few = blocks <= kFewBlocks;
     const int launches = passes * (few ? 2 : 3);
-    int *counts = nullptr, *totals = nullptr, *other_keys = nullptr, *other_order = nullptr;
-    NACHO_TRY(call.scratch_n(static_cast<size_t>(blocks) * kDigits, &counts));
-    if (!few) NACHO_TRY(call.scratch_n(static_cast<size_t>(kDigits), &totals));
-    if (passes > 1) {
-        NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &other_keys));
-        NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &other_order));
-    }
+    const size_t n_counts = static_cast<size_t>(blocks) * kDigits;
+    NACHO_TRY(call.scratch_n(4 * n + n_counts + kDigits, sorted));
+    int *const other = *sorted + 2 * n;
+    int *const counts = other + 2 * n, *const totals = few ? nullptr : counts + n_counts;
     const unsigned groups = static_cast<unsigned>(blocks);
     Pass p{ids, nullptr, nullptr, tokens, blocks, 0, nullptr, nullptr};
     for (int i = 0, launch = 0; i < passes; ++i) {
         const bool to_result = (passes - i) % 2 == 1;
-        p.keys = to_result ? keys : other_keys;
-        p.order = to_result ? order : other_order;
+        p.keys = to_result ? *sorted : other;
+        p.order = p.keys + n;
         p.shift = i * kDigitBits;
         Clear clear = share(groups, kSortThreads, launch++, launches, &grid);
         count_kernel<<<grid, kSortThreads, 0, s>>>(p, counts, clear);
@@ -656,23 +682,13 @@ int backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float 
     return with_type(dtype, width, [&](auto type, auto n) -> int {
         using T = decltype(type);
         if (tokens == 0) return dense::clear(s, static_cast<T *>(dtable), words * width);
-        int *keys = nullptr, *order = nullptr;
+        int *sorted = nullptr;
         float *parts = nullptr;
-        NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &keys));
-        NACHO_TRY(call.scratch_n(static_cast<size_t>(tokens), &order));
         if (chunks > 1) NACHO_TRY(call.scratch_n(static_cast<size_t>(chunks * 2 * width), &parts));
-        // The gradient's whole 16-byte pieces are cleared with the sort, the few elements before
-        // and behind them by themselves, where there are any.
         T *const table = static_cast<T *>(dtable);
-        const int64_t all = words * width, per = 16 / item;
-        int64_t head = static_cast<int64_t>((-reinterpret_cast<uintptr_t>(table) & 15) / item);
-        if (head > all) head = all;
-        const int64_t n_pieces = (all - head) / per, tail = all - head - n_pieces * per;
-        if (head > 0) NACHO_TRY(dense::clear(s, table, head));
-        if (tail > 0) NACHO_TRY(dense::clear(s, table + all - tail, tail));
-        NACHO_TRY(sort_tokens(call, Ids{ids, id_bytes, words}, static_cast<int>(tokens), keys,
-                              order, reinterpret_cast<dense::u32x4 *>(table + head), n_pieces));
-        const Sums a{keys, order, static_cast<int>(tokens), static_cast<int>(words),
+        NACHO_TRY(sort_tokens(call, Ids{ids, id_bytes, words}, static_cast<int>(tokens),
+                              Cleared(table, words * width * item), &sorted));
+        const Sums a{sorted, sorted + tokens, static_cast<int>(tokens), static_cast<int>(words),
                      static_cast<int>(chunks), width, scale, parts};
         const dim3 groups(static_cast<unsigned>(groups_x), static_cast<unsigned>(slices));
         auto sums = [&](auto of) -> int {

@@ -139,15 +139,16 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
     }
 }
 
-// Rows of `width` elements, one after another `padded` elements apart and zeros behind the width:
-// those of the listed tokens (token), or the first `rows` (null).
+// Rows of `width` elements with zeros behind them up to `padded`: those of the listed tokens (token),
+// or the first `rows` (null).
 template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict__ count,
                                                           const int *__restrict__ token,
                                                           int64_t rows, int64_t width,
                                                           int64_t padded,
                                                           const T *__restrict__ from,
-                                                          int64_t stride, T *__restrict__ to) {
+                                                          int64_t stride, T *__restrict__ to,
+                                                          int64_t to_stride) {
     const int64_t there = count ? *count : rows;
     const int64_t per = padded / N;
     const int64_t all = there * per;
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict_
 #pragma unroll
             for (int j = 0; j < N; ++j) piece.v[j] = static_cast<T>(0.0f);
         }
-        *reinterpret_cast<dense::Piece<T, N> *>(to + row * padded + col) = piece;
+        *reinterpret_cast<dense::Piece<T, N> *>(to + row * to_stride + col) = piece;
     }
 }
 
@@ -190,7 +191,8 @@ using Number = std::integral_constant<int, N>;
 struct Logits {
     const int *held;
     int64_t width;         // of the gathered rows, and of the table's
-    const void *rows;      // [held][width]
+    const void *rows;      // [held][rows_stride]
+    int64_t rows_stride;
     const void *table;
     int64_t table_stride;
     int words;             // of this piece
@@ -207,7 +209,7 @@ struct Logits {
     const int *token;
     const float *factor;   // null: 1
     void *dz;              // [held][dz_stride]
-    int64_t dz_stride;     // a multiple of 256: words past the piece's get zeros
+    int64_t dz_stride;     // at least the piece's tiles: words past the piece's get zeros
 };
 
 template <typename T>
@@ -260,7 +262,7 @@ __device__ __forceinline__ void logits_of(const Logits &a, int64_t v0, int64_t n
                                           T *lds, f32x4 (&z)[S::MT][S::NT]) {
     const Matrix<T> table{static_cast<const T *>(a.table) + (a.first + v0) * a.table_stride,
                           a.table_stride};
-    const Matrix<T> rows{static_cast<const T *>(a.rows) + n0 * a.width, a.width};
+    const Matrix<T> rows{static_cast<const T *>(a.rows) + n0 * a.rows_stride, a.rows_stride};
     Product<T, S, Along, Along>::run(
         table, static_cast<int>(min(a.words - v0, static_cast<int64_t>(S::BM))), rows,
         static_cast<int>(min(held - n0, static_cast<int64_t>(S::BN))), a.width, lds, z);
@@ -285,18 +287,33 @@ __device__ __forceinline__ void tile_parts(const Logits &a, int64_t v0, unsigned
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int col = (wn * S::NT + t) * 16 + c;
+        // (a wavefront seldom has a token's target: it looks for one only then)
+        const int64_t there = target[t] - wm * S::MT * 16 - 4 * g;
+        if (__ballot(there >= 0 && there < S::MT * 16 && (there & 15) < 4)) {
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (16 * i + j == there) a.mine[n0 + col] = z[i][t][j] * a.scale;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) z[i][t] *= a.scale;
+        if (v0 + S::BM > a.words) {  // words that there are not
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (v0 + (wm * S::MT + i) * 16 + 4 * g + j >= a.words) z[i][t][j] = kNegInf;
+                }
+            }
+        }
         float most = kNegInf;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = (wm * S::MT + i) * 16 + 4 * g + j;
-                float x = z[i][t][j] * a.scale;
-                if (v == target[t]) a.mine[n0 + col] = x;
-                if (v0 + v >= a.words) x = kNegInf;
-                z[i][t][j] = x;
-                most = fmaxf(most, x);
-            }
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, z[i][t][j]);
         }
         most = dense::column_max(most);
         // (with no finite logit: exp(-inf) of each)
@@ -417,15 +434,17 @@ __device__ __forceinline__ void tile_dz(const Logits &a, int64_t v0, int64_t n0,
         const int token = a.token[n];
         target[t] = static_cast<int>(a.target[n] - a.first - v0);
         most[t] = a.most[token];
-        part[t] = 1.0f / a.total[token];
         factor[t] = kDzScale<T> * (a.factor ? a.factor[n] : 1.0f);
+        part[t] = factor[t] / a.total[token];
     }
     f32x4 z[S::MT][S::NT];
     logits_of<T, S>(a, v0, n0, held, lds, z);
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
-        if (n >= held) continue;
+        // the target's probability less 1, where the wavefront has a target
+        const int there = target[t] - wm * S::MT * 16 - 4 * g;
+        const bool some = __ballot(there >= 0 && there < S::MT * 16 && (there & 15) < 4) != 0;
         T *to = static_cast<T *>(a.dz) + n * a.dz_stride + v0;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
@@ -434,11 +453,17 @@ __device__ __forceinline__ void tile_dz(const Logits &a, int64_t v0, int64_t n0,
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float x = z[i][t][j] * a.scale;
-                float p = dense::exp2_fast((x - most[t]) * kLog2e) * part[t];
-                if (v + j == target[t]) p -= 1.0f;
-                d[j] = v0 + v + j < a.words ? p * factor[t] : 0.0f;
+                d[j] = dense::exp2_fast((x - most[t]) * kLog2e) * part[t];
             }
-            dense::store4<T>(to + v, d);
+            if (some) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] -= 16 * i + j == there ? factor[t] : 0.0f;
+            }
+            if (v0 + S::BM > a.words) {  // words that there are not
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = v0 + v + j < a.words ? d[j] : 0.0f;
+            }
+            if (n < held) dense::store4<T>(to + v, d);
         }
     }
 }
@@ -463,6 +488,7 @@ struct Gradients {
     int64_t table_stride;
     int64_t words, width; // of the piece; of the results
     int64_t padded;       // columns that the operands' rows have
+    int64_t rows_stride;
     int64_t piece;        // words of a whole piece
     int64_t most_rows;    // that the sums have room for, at least all tokens
     float *sums;          // [split][held][sums_stride]; null: no dx
@@ -542,12 +568,12 @@ __device__ __forceinline__ void tile_dx(const Gradients &a, int64_t d0, int64_t 
 template <typename T, typename S>
 __device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int64_t v0, int held,
                                             T *lds) {
-    const Matrix<T> rows{static_cast<const T *>(a.rows) + d0, a.padded};
+    const Matrix<T> rows{static_cast<const T *>(a.rows) + d0, a.rows_stride};
     const Matrix<T> dz{static_cast<const T *>(a.dz) + v0, a.dz_stride};
     f32x4 sums[S::MT][S::NT];
     Product<T, S, Across, Across>::run(
         rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
-        static_cast<int>(min(a.dz_stride - v0, static_cast<int64_t>(S::BN))), held, lds, sums);
+        static_cast<int>(min(a.piece - v0, static_cast<int64_t>(S::BN))), held, lds, sums);
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
@@ -665,6 +691,14 @@ __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// Elements from row to row of a matrix in scratch: an odd number of 128-byte lines.  (Rows a power of
+// two apart share few of the memory's channels, and a tile reads 256 rows at the same column.)
+template <typename T>
+int64_t scratch_stride(int64_t width) {
+    const int64_t line = 128 / static_cast<int64_t>(sizeof(T));
+    return up(width, line) / line % 2 ? up(width, line) : up(width, line) + line;
+}
+
 struct Args {
     int32_t dtype;
     int64_t tokens, words, width;
@@ -706,6 +740,7 @@ struct Operands {
     T *rows = nullptr;
     const T *table = nullptr;
     int64_t width = 0;  // of rows, a multiple of a piece
+    int64_t rows_stride = 0;
     int64_t table_stride = 0;
 
     int start(Call &call, const Args &a, const float *dloss) {
@@ -730,17 +765,20 @@ struct Operands {
                                                held);
         NACHO_TRY_HIP(hipGetLastError());
         width = up(a.width, kPer);
-        NACHO_TRY(call.scratch_n(n * static_cast<size_t>(width), &rows));
-        NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, a.x, a.x_stride, rows));
+        rows_stride = scratch_stride<T>(width);
+        NACHO_TRY(call.scratch_n(n * static_cast<size_t>(rows_stride), &rows));
+        NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, a.x, a.x_stride, rows,
+                         rows_stride));
         table = static_cast<const T *>(a.table);
         table_stride = a.table_stride;
         if (!dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
             table_stride * static_cast<int64_t>(sizeof(T)) > kMostStride) {
             T *copy = nullptr;
-            NACHO_TRY(call.scratch_n(static_cast<size_t>(a.words * width), &copy));
-            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, a.table, a.table_stride, copy));
+            table_stride = scratch_stride<T>(width);
+            NACHO_TRY(call.scratch_n(static_cast<size_t>(a.words * table_stride), &copy));
+            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, a.table, a.table_stride, copy,
+                             table_stride));
             table = copy;
-            table_stride = width;
         }
         return NACHO_OK;
     }
@@ -749,7 +787,7 @@ struct Operands {
     static constexpr int64_t kMostStride = int64_t{1} << 22;
 
     int gather(hipStream_t s, const int *count, const int *token, int64_t n, int64_t columns,
-               const void *from, int64_t stride, T *to) const {
+               const void *from, int64_t stride, T *to, int64_t to_stride) const {
         constexpr int kPer = 16 / sizeof(T);
         const bool whole = dense::pieces(from, stride, columns, sizeof(T));
         const int64_t threads = n * (width / (whole ? kPer : 1));
@@ -757,10 +795,12 @@ struct Operands {
         const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
         if (whole) {
             gather_kernel<T, kPer><<<grid, kThreads, 0, s>>>(
-                count, token, n, columns, width, static_cast<const T *>(from), stride, to);
+                count, token, n, columns, width, static_cast<const T *>(from), stride, to,
+                to_stride);
         } else {
             gather_kernel<T, 1><<<grid, kThreads, 0, s>>>(
-                count, token, n, columns, width, static_cast<const T *>(from), stride, to);
+                count, token, n, columns, width, static_cast<const T *>(from), stride, to,
+                to_stride);
         }
         NACHO_TRY_HIP(hipGetLastError());
         return NACHO_OK;
@@ -822,6 +862,7 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
                 l.held = ops.held.count;
                 l.width = ops.width;
                 l.rows = ops.rows;
+                l.rows_stride = ops.rows_stride;
                 l.table = ops.table;
                 l.table_stride = ops.table_stride;
                 l.words = static_cast<int>(a.words);
@@ -882,10 +923,11 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             }
             Operands<T> ops;
             NACHO_TRY(ops.start(call, a, dloss));
-            T *dz = nullptr;
-            NACHO_TRY(call.scratch_n(n * static_cast<size_t>(piece), &dz));
             Logits l{};
             Gradients d{};
+            T *dz = nullptr;
+            l.dz_stride = d.dz_stride = scratch_stride<T>(piece);
+            NACHO_TRY(call.scratch_n(n * static_cast<size_t>(l.dz_stride), &dz));
             d.sums_stride = up(a.width, 4);
             // Room for the sums of as many splits as are made: tiles of 256 columns by kBN tokens,
             // at most kMostItems of them where they are split.
@@ -899,6 +941,7 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             l.held = d.held = ops.held.count;
             l.width = d.padded = ops.width;
             l.rows = d.rows = ops.rows;
+            l.rows_stride = d.rows_stride = ops.rows_stride;
             l.table_stride = d.table_stride = ops.table_stride;
             l.target = ops.held.target;
             l.scale = d.scale = a.scale;
@@ -908,7 +951,6 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             l.factor = ops.held.factor;
             l.dz = dz;
             d.dz = dz;
-            l.dz_stride = d.dz_stride = piece;
             l.table = ops.table;
             d.width = a.width;
             d.piece = piece;

@@ -53,8 +53,14 @@ struct Along {
     unsigned offset[kLoads];
     unsigned piece;  // of every load of this thread: swizzle repeats after 16 rows
 
+    // A 16-byte read takes 16 lanes at a time: rows 0-3 and 12-15 of one g and 4-11 of the next, and
+    // the other way round.  Of the eight rows in each half of the banks those two groups have
+    // numbers whose second and third bits differ, so that what g adds to a piece, its last bits,
+    // keeps them apart.  (With any numbers that differ between all rows half of the LDS's cycles
+    // were conflicts.)
     __device__ __forceinline__ static int swizzle(int row) {
-        return (row & 6) | ((row >> 3) & 1);
+        const int k = row >> 1;
+        return ((k >> 1 ^ k >> 2) & 1) << 2 | (k >> 2 & 1) << 1 | (k & 1);
     }
 
     // Rows from `there` on are zeros.  stride: elements from row to row.
@@ -191,7 +197,12 @@ struct Product {
     using A = OfA<T, S::BM, S::kThreads>;
     using B = OfB<T, S::BN, S::kThreads>;
     static constexpr int kLdsElements = 2 * (A::kElements + B::kElements);
-    static constexpr size_t kLdsBytes = kLdsElements * sizeof(T);
+    // 16-bit operands that both lie along k.  (Across, a fragment is two reads and a half of a step
+    // 24, more than a wavefront can have on its way: 2163 us instead of 1111 for the gradients of a
+    // piece of 16384 words.)
+    static constexpr bool kHalves =
+        sizeof(T) == 2 && __is_same(A, Along<T, S::BM, S::kThreads>) &&
+        __is_same(B, Along<T, S::BN, S::kThreads>);
 
     // sums[i][t]: rows 16 (wm MT + i) + 4 g .. + 4 of column 16 (wn NT + t) + c, over k < `depth`.
     // Every thread of the workgroup calls this; m and n: rows and columns that there are.
@@ -210,36 +221,73 @@ struct Product {
 #pragma unroll
             for (int t = 0; t < S::NT; ++t) sums[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        if (depth <= 0) return;
         const int64_t step_a = A::advance(a.stride), step_b = B::advance(b.stride);
         T *tile_a = lds, *tile_b = lds + A::kElements;
         T *next_a = lds + A::kElements + B::kElements, *next_b = next_a + A::kElements;
-        if (depth > 0) {
-            from_a.load(thread, a.data, depth, tile_a);
-            from_b.load(thread, b.data, depth, tile_b);
-        }
-        for (int64_t left = depth; left > 0; left -= kStepK<T>) {
-            rows_arrived();
+        int64_t left = depth;  // of the step that is loaded next
+        auto load = [&](T *to_a, T *to_b) {
+            from_a.load(thread, a.data, left, to_a);
+            from_b.load(thread, b.data, left, to_b);
             a.data += step_a;
             b.data += step_b;
-            if (left > kStepK<T>) {
-                from_a.load(thread, a.data, left - kStepK<T>, next_a);
-                from_b.load(thread, b.data, left - kStepK<T>, next_b);
-            }
-#pragma unroll
-            for (int kk = 0; kk < kStepK<T> / 32; ++kk) {
-                Frag<T> fb[S::NT];
-#pragma unroll
-                for (int t = 0; t < S::NT; ++t) fb[t] = B::frag(tile_b, wn * S::NT + t, kk, g, c);
-#pragma unroll
-                for (int i = 0; i < S::MT; ++i) {
-                    const Frag<T> fa = A::frag(tile_a, wm * S::MT + i, kk, g, c);
-#pragma unroll
-                    for (int t = 0; t < S::NT; ++t) sums[i][t] = mma(fa, fb[t], sums[i][t]);
-                }
-            }
-            T *const swap_a = tile_a, *const swap_b = tile_b;
+            left -= kStepK<T>;
+        };
+        auto swap = [&] {
+            T *const was_a = tile_a, *const was_b = tile_b;
             tile_a = next_a, tile_b = next_b;
-            next_a = swap_a, next_b = swap_b;
+            next_a = was_a, next_b = was_b;
+        };
+        auto read = [&](int kk, Frag<T> (&fa)[S::MT], Frag<T> (&fb)[S::NT]) {
+#pragma unroll
+            for (int t = 0; t < S::NT; ++t) fb[t] = B::frag(tile_b, wn * S::NT + t, kk, g, c);
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) fa[i] = A::frag(tile_a, wm * S::MT + i, kk, g, c);
+        };
+        auto multiply = [&](const Frag<T> (&fa)[S::MT], const Frag<T> (&fb)[S::NT]) {
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+                for (int t = 0; t < S::NT; ++t) sums[i][t] = mma(fa[i], fb[t], sums[i][t]);
+            }
+        };
+        load(tile_a, tile_b);
+        if constexpr (!kHalves) {
+            for (int64_t steps = (depth + kStepK<T> - 1) / kStepK<T>; steps > 0; --steps) {
+                rows_arrived();
+                if (left > 0) load(next_a, next_b);
+#pragma unroll
+                for (int kk = 0; kk < kStepK<T> / 32; ++kk) {
+                    Frag<T> fa[S::MT], fb[S::NT];
+                    read(kk, fa, fb);
+                    multiply(fa, fb);
+                }
+                swap();
+            }
+        } else {
+            // A step's products are two halves of 32 k.  The barrier that ends a step for its
+            // buffer stands between them: by then a wavefront has read the second half's fragments
+            // into registers, so that its matrix instructions go on behind it, while the next
+            // step's first half is read and the step after that is loaded.
+            Frag<T> fa0[S::MT], fb0[S::NT], fa1[S::MT], fb1[S::NT];
+            rows_arrived();
+            if (left > 0) load(next_a, next_b);
+            read(0, fa0, fb0);
+            for (int64_t steps = (depth + kStepK<T> - 1) / kStepK<T>; steps > 0; --steps) {
+                read(1, fa1, fb1);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(fa0, fb0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (steps > 1) {
+                    rows_arrived();
+                    if (left > 0) load(tile_a, tile_b);
+                    swap();
+                    read(0, fa0, fb0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(fa1, fb1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 };

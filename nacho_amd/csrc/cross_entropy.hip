@@ -200,8 +200,8 @@ struct Logits {
     const int *target;
     float scale;
     // the forward pass
-    float2 *parts;         // [held][m_tiles]: m and s of a tile's words
     unsigned m_tiles;
+    float2 *parts;         // [held][m_tiles]: m and s of a tile's words
     float *mine;           // [held]: the target's logit
     // the backward pass
     const float *most;     // m by token of the whole batch
@@ -274,32 +274,38 @@ __device__ __forceinline__ void tile_parts(const Logits &a, int64_t v0, unsigned
                                            int held, T *lds) {
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
-    int64_t target[S::NT];  // among the tile's words
+    const float scale = a.scale;
+    int target[S::NT];  // among the tile's words
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int64_t n = n0 + (wn * S::NT + t) * 16 + c;
-        target[t] = n < held ? a.target[n] - v0 : -1;
+        target[t] = n < held ? static_cast<int>(a.target[n] - v0) : -1;
     }
     f32x4 z[S::MT][S::NT];
     logits_of<T, S>(a, v0, n0, held, lds, z);
-    float2(*s_part)[S::BN] = reinterpret_cast<float2(*)[S::BN]>(lds);
+    float(*s_most)[S::BN] = reinterpret_cast<float(*)[S::BN]>(lds);
+    float(*s_total)[S::BN] = s_most + S::WM;
     __syncthreads();  // (the tiles have been read)
 #pragma unroll
     for (int t = 0; t < S::NT; ++t) {
         const int col = (wn * S::NT + t) * 16 + c;
         // (a wavefront seldom has a token's target: it looks for one only then)
-        const int64_t there = target[t] - wm * S::MT * 16 - 4 * g;
-        if (__ballot(there >= 0 && there < S::MT * 16 && (there & 15) < 4)) {
+        const int there = target[t] - wm * S::MT * 16 - 4 * g;
+        const bool mine = there >= 0 && there < S::MT * 16 && (there & 15) < 4;
+        if (__ballot(mine)) {
+            float x = 0.0f;
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (16 * i + j == there) a.mine[n0 + col] = z[i][t][j] * a.scale;
-                }
+                for (int j = 0; j < 4; ++j) x = 16 * i + j == there ? z[i][t][j] : x;
             }
+            if (mine) a.mine[n0 + col] = x * scale;
         }
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i) z[i][t] *= a.scale;
+        for (int i = 0; i < S::MT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[i][t][j] *= scale;
+        }
         if (v0 + S::BM > a.words) {  // words that there are not
 #pragma unroll
             for (int i = 0; i < S::MT; ++i) {
@@ -325,19 +331,21 @@ __device__ __forceinline__ void tile_parts(const Logits &a, int64_t v0, unsigned
             for (int j = 0; j < 4; ++j) total += dense::exp2_fast((z[i][t][j] - base) * kLog2e);
         }
         total = dense::column_sum(total);
-        if (g == 0) s_part[wm][col] = float2{most, total};
+        if (g == 0) {
+            s_most[wm][col] = most;
+            s_total[wm][col] = total;
+        }
     }
     __syncthreads();
     for (int col = threadIdx.x; col < S::BN; col += S::kThreads) {
         if (n0 + col >= held) break;
         float most = kNegInf, total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < S::WM; ++w) most = fmaxf(most, s_part[w][col].x);
+        for (int w = 0; w < S::WM; ++w) most = fmaxf(most, s_most[w][col]);
         const float base = most == kNegInf ? 0.0f : most;
 #pragma unroll
         for (int w = 0; w < S::WM; ++w) {
-            const float2 p = s_part[w][col];
-            total += p.y * dense::exp2_fast((p.x - base) * kLog2e);
+            total += s_total[w][col] * dense::exp2_fast((s_most[w][col] - base) * kLog2e);
         }
         a.parts[(n0 + col) * a.m_tiles + mt] = float2{most, total};
     }

@@ -13,12 +13,24 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 #include "dense_tiles.hpp"
 #include "device_utils.hpp"
 
 namespace nacho {
 namespace dense {
+
+// f(0), f(1) .. f(N - 1), each number a type: arrays that f indexes by it stay in registers.
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+    each_of(std::make_integer_sequence<int, N>{}, f);
+}
 
 // Elements of k in a step.
 template <typename T>
@@ -197,13 +209,6 @@ struct Product {
     using A = OfA<T, S::BM, S::kThreads>;
     using B = OfB<T, S::BN, S::kThreads>;
     static constexpr int kLdsElements = 2 * (A::kElements + B::kElements);
-    // 16-bit operands that both lie along k.  (Across, a fragment is two reads and a half of a step
-    // 24, more than a wavefront can have on its way: 2163 us instead of 1111 for the gradients of a
-    // piece of 16384 words.)
-    static constexpr bool kHalves =
-        sizeof(T) == 2 && __is_same(A, Along<T, S::BM, S::kThreads>) &&
-        __is_same(B, Along<T, S::BN, S::kThreads>);
-
     // sums[i][t]: rows 16 (wm MT + i) + 4 g .. + 4 of column 16 (wn NT + t) + c, over k < `depth`.
     // Every thread of the workgroup calls this; m and n: rows and columns that there are.
     __device__ __forceinline__ static void run(Matrix<T> a, int m, Matrix<T> b, int n,
@@ -238,56 +243,64 @@ struct Product {
             tile_a = next_a, tile_b = next_b;
             next_a = was_a, next_b = was_b;
         };
-        auto read = [&](int kk, Frag<T> (&fa)[S::MT], Frag<T> (&fb)[S::NT]) {
-#pragma unroll
-            for (int t = 0; t < S::NT; ++t) fb[t] = B::frag(tile_b, wn * S::NT + t, kk, g, c);
-#pragma unroll
-            for (int i = 0; i < S::MT; ++i) fa[i] = A::frag(tile_a, wm * S::MT + i, kk, g, c);
-        };
-        auto multiply = [&](const Frag<T> (&fa)[S::MT], const Frag<T> (&fb)[S::NT]) {
-#pragma unroll
-            for (int i = 0; i < S::MT; ++i) {
-#pragma unroll
-                for (int t = 0; t < S::NT; ++t) sums[i][t] = mma(fa[i], fb[t], sums[i][t]);
+        // Fragment f of a half of the step's k: B's, then A's.
+        auto read = [&](auto f, int kk, Frag<T> (&fa)[S::MT], Frag<T> (&fb)[S::NT]) {
+            if constexpr (f() < S::NT) {
+                fb[f()] = B::frag(tile_b, wn * S::NT + f(), kk, g, c);
+            } else {
+                fa[f() - S::NT] = A::frag(tile_a, wm * S::MT + f() - S::NT, kk, g, c);
             }
         };
+        constexpr int kFrags = S::MT + S::NT;
+        auto multiply = [&](auto i, const Frag<T> (&fa)[S::MT], const Frag<T> (&fb)[S::NT]) {
+            each<S::NT>([&](auto t) { sums[i()][t()] = mma(fa[i()], fb[t()], sums[i()][t()]); });
+        };
         load(tile_a, tile_b);
-        if constexpr (!kHalves) {
-            for (int64_t steps = (depth + kStepK<T> - 1) / kStepK<T>; steps > 0; --steps) {
+        int64_t steps = (depth + kStepK<T> - 1) / kStepK<T>;
+        if constexpr (sizeof(T) == 4) {
+            for (; steps > 0; --steps) {
                 rows_arrived();
                 if (left > 0) load(next_a, next_b);
-#pragma unroll
-                for (int kk = 0; kk < kStepK<T> / 32; ++kk) {
-                    Frag<T> fa[S::MT], fb[S::NT];
-                    read(kk, fa, fb);
-                    multiply(fa, fb);
-                }
+                Frag<T> fa[S::MT], fb[S::NT];
+                each<kFrags>([&](auto f) { read(f, 0, fa, fb); });
+                each<S::MT>([&](auto i) { multiply(i, fa, fb); });
                 swap();
             }
         } else {
-            // A step's products are two halves of 32 k.  The barrier that ends a step for its
-            // buffer stands between them: by then a wavefront has read the second half's fragments
-            // into registers, so that its matrix instructions go on behind it, while the next
-            // step's first half is read and the step after that is loaded.
+            // A step's products are two halves of 32 k, and while one half is multiplied the next
+            // one's fragments are read, a few between the matrix instructions of each row.  The
+            // barrier that ends a step for its buffer stands between its halves: by then a
+            // wavefront has the second half's fragments in registers, so that its matrix
+            // instructions go on behind it, while the next step's first half is read and the step
+            // after that is loaded.
             Frag<T> fa0[S::MT], fb0[S::NT], fa1[S::MT], fb1[S::NT];
+            auto half = [&](const Frag<T> (&fa)[S::MT], const Frag<T> (&fb)[S::NT], auto reads,
+                            int kk, Frag<T> (&next_fa)[S::MT], Frag<T> (&next_fb)[S::NT]) {
+                each<S::MT>([&](auto i) {
+                    if constexpr (reads()) {
+                        constexpr int kFrom = i() * kFrags / S::MT;
+                        each<(i() + 1) * kFrags / S::MT - kFrom>([&](auto f) {
+                            read(std::integral_constant<int, kFrom + f()>{}, kk, next_fa, next_fb);
+                        });
+                    }
+                    multiply(i, fa, fb);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            };
+            constexpr std::true_type kReads{};
+            constexpr std::false_type kLast{};
             rows_arrived();
             if (left > 0) load(next_a, next_b);
-            read(0, fa0, fb0);
-            for (int64_t steps = (depth + kStepK<T> - 1) / kStepK<T>; steps > 0; --steps) {
-                read(1, fa1, fb1);
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(fa0, fb0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (steps > 1) {
-                    rows_arrived();
-                    if (left > 0) load(tile_a, tile_b);
-                    swap();
-                    read(0, fa0, fb0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                multiply(fa1, fb1);
-                __builtin_amdgcn_sched_barrier(0);
+            each<kFrags>([&](auto f) { read(f, 0, fa0, fb0); });
+            for (; steps > 1; --steps) {
+                half(fa0, fb0, kReads, 1, fa1, fb1);
+                rows_arrived();
+                if (left > 0) load(tile_a, tile_b);
+                swap();
+                half(fa1, fb1, kReads, 0, fa0, fb0);
             }
+            half(fa0, fb0, kReads, 1, fa1, fb1);
+            half(fa1, fb1, kLast, 0, fa0, fb0);
         }
     }
 };

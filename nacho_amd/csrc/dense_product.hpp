@@ -203,15 +203,78 @@ struct Matrix {
     int64_t stride;
 };
 
+// Eight float32 in three parts of bfloat16, each what the one before leaves, rounded: together they
+// are the number (8 + 8 + 8 bits).
+struct Split {
+    bf16x8 part[3];
+};
+__device__ __forceinline__ Split split(f32x8 x) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    Split s;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        float u = x[j], v = x[j + 1];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const b2 h{static_cast<__bf16>(u), static_cast<__bf16>(v)};
+            s.part[p][j] = h[0], s.part[p][j + 1] = h[1];
+            if (p < 2) {
+                const unsigned bits = __builtin_bit_cast(unsigned, h);
+                u -= __uint_as_float(bits << 16);
+                v -= __uint_as_float(bits & 0xffff0000u);
+            }
+        }
+    }
+    return s;
+}
+// c += a * b over 32 k, from the smallest parts to the largest.  Left out are the products of a
+// second and a third part and of two third ones, together at most 2^-24 of |a| |b|.
+__device__ __forceinline__ f32x4 mma(const Split &a, const Split &b, f32x4 c) {
+    c = mma(a.part[1], b.part[1], c);
+    c = mma(a.part[0], b.part[2], c);
+    c = mma(a.part[2], b.part[0], c);
+    c = mma(a.part[0], b.part[1], c);
+    c = mma(a.part[1], b.part[0], c);
+    return mma(a.part[0], b.part[0], c);
+}
+
 template <typename T, typename S, template <typename, int, int> class OfA,
           template <typename, int, int> class OfB>
 struct Product {
     using A = OfA<T, S::BM, S::kThreads>;
     using B = OfB<T, S::BN, S::kThreads>;
     static constexpr int kLdsElements = 2 * (A::kElements + B::kElements);
+    // float32: six products of bfloat16 parts take 96 cycles of the matrix cores where eight steps
+    // of the float32 instruction take 256, and splitting the operands, which the rows of a fragment
+    // share, runs beside them (1024 x 16384 by 2048, us: 300 instead of 500).  Narrow tiles are
+    // bound by memory.
+    static constexpr bool kSplit = sizeof(T) == 4 && S::BN > 16;
+
     // sums[i][t]: rows 16 (wm MT + i) + 4 g .. + 4 of column 16 (wn NT + t) + c, over k < `depth`.
     // Every thread of the workgroup calls this; m and n: rows and columns that there are.
     __device__ __forceinline__ static void run(Matrix<T> a, int m, Matrix<T> b, int n,
+                                               int64_t depth, T *lds, f32x4 (&sums)[S::MT][S::NT]) {
+        run_as<kSplit>(a, m, b, n, depth, lds, sums);
+        if constexpr (kSplit) {
+            // The parts of an infinity are one and numbers that are none.  A tile with a sum that
+            // is not finite is worked out again without parts.
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i) x += not_finite(sums[i]);
+            volatile int *again = reinterpret_cast<volatile int *>(lds);
+            __syncthreads();
+            if (threadIdx.x == 0) *again = 0;
+            __syncthreads();
+            if (x != x) *again = 1;
+            __syncthreads();
+            const bool redo = *again != 0;
+            __syncthreads();
+            if (redo) run_as<false>(a, m, b, n, depth, lds, sums);
+        }
+    }
+
+    template <bool SPLIT>
+    __device__ __forceinline__ static void run_as(Matrix<T> a, int m, Matrix<T> b, int n,
                                                int64_t depth, T *lds, f32x4 (&sums)[S::MT][S::NT]) {
         const int thread = static_cast<int>(threadIdx.x);
         const int wave = __builtin_amdgcn_readfirstlane(thread / dev::kWave);
@@ -263,7 +326,18 @@ struct Product {
                 if (left > 0) load(next_a, next_b);
                 Frag<T> fa[S::MT], fb[S::NT];
                 each<kFrags>([&](auto f) { read(f, 0, fa, fb); });
-                each<S::MT>([&](auto i) { multiply(i, fa, fb); });
+                if constexpr (SPLIT) {
+                    Split pb[S::NT];
+                    each<S::NT>([&](auto t) { pb[t()] = split(fb[t()]); });
+                    each<S::MT>([&](auto i) {
+                        const Split pa = split(fa[i()]);
+                        each<S::NT>([&](auto t) {
+                            sums[i()][t()] = mma(pa, pb[t()], sums[i()][t()]);
+                        });
+                    });
+                } else {
+                    each<S::MT>([&](auto i) { multiply(i, fa, fb); });
+                }
                 swap();
             }
         } else {

@@ -195,6 +195,35 @@ def test_values_that_are_not_finite(gpu):
     assert torch.equal(loss[keep], want[keep]) and torch.equal(got[0][keep], dx[keep])
 
 
+@pytest.mark.parametrize("value", (float("nan"), float("inf"), 3.4e38))
+@pytest.mark.parametrize("tokens", (20, 300))
+def test_float32_next_to_values_that_are_not_finite(gpu, tokens, value):
+    """Products in parts are none where an operand is not finite: those of the others stay right."""
+    x, table, targets = _operands(gpu, 27, tokens, 600, 72, torch.float32, left=0.0)
+    want = Loss(x, table, targets, reduction="none", dloss=torch.ones(tokens, device=gpu))
+    x[7, 5] = value
+    xd = x.requires_grad_()
+    loss = nacho_amd.gpu_linear_cross_entropy(xd, table, targets, reduction="none")
+    dx, = torch.autograd.grad(loss, xd, torch.ones(tokens, device=gpu))
+    keep = torch.arange(tokens, device=gpu) != 7
+    near(loss[keep], want.loss[keep], want.loss_off[keep], "loss")
+    near(dx[keep], want.dx[keep], want.dx_off[keep], "dx")
+    assert not torch.isfinite(loss[7]) or abs(value) < float("inf")
+
+
+@pytest.mark.parametrize("size", (2.0 ** -60, 2.0 ** 60, 2.0 ** 100))
+def test_float32_of_all_sizes(gpu, size):
+    x, table, targets = _operands(gpu, 28, 40, 300, 64, torch.float32, left=0.0)
+    dloss = _dloss(gpu, "mean", targets.shape)
+    want = Loss(x, table, targets, dloss=dloss)
+    xd, td = (x * size).requires_grad_(), (table / size).requires_grad_()
+    loss = nacho_amd.gpu_linear_cross_entropy(xd, td, targets)
+    dx, dtable = torch.autograd.grad(loss, (xd, td), dloss)
+    near(loss, want.loss, want.loss_off, "loss")
+    near(dx * size, want.dx, want.dx_off, "dx")
+    near(dtable / size, want.dtable, want.dtable_off, "dtable")
+
+
 def test_words_of_minus_infinity(gpu):
     """A word whose logits are all minus infinity has probability 0."""
     x = torch.ones(20, 32, device=gpu)

@@ -227,16 +227,10 @@ __device__ __forceinline__ Split split(f32x8 x) {
     }
     return s;
 }
-// c += a * b over 32 k, from the smallest parts to the largest.  Left out are the products of a
-// second and a third part and of two third ones, together at most 2^-24 of |a| |b|.
-__device__ __forceinline__ f32x4 mma(const Split &a, const Split &b, f32x4 c) {
-    c = mma(a.part[1], b.part[1], c);
-    c = mma(a.part[0], b.part[2], c);
-    c = mma(a.part[2], b.part[0], c);
-    c = mma(a.part[0], b.part[1], c);
-    c = mma(a.part[1], b.part[0], c);
-    return mma(a.part[0], b.part[0], c);
-}
+// The products of parts that make a product, from the smallest to the largest: a's part and b's.
+// Left out are those of a second and a third part and of two third ones, together at most 2^-24 of
+// |a| |b|.
+constexpr int kSplitProducts[6][2] = {{1, 1}, {0, 2}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
 
 template <typename T, typename S, template <typename, int, int> class OfA,
           template <typename, int, int> class OfB>
@@ -325,16 +319,33 @@ struct Product {
                 rows_arrived();
                 if (left > 0) load(next_a, next_b);
                 Frag<T> fa[S::MT], fb[S::NT];
-                each<kFrags>([&](auto f) { read(f, 0, fa, fb); });
+                constexpr int kFirst = SPLIT ? S::NT + 2 : kFrags;
+                each<(kFirst < kFrags ? kFirst : kFrags)>([&](auto f) { read(f, 0, fa, fb); });
                 if constexpr (SPLIT) {
-                    Split pb[S::NT];
+                    // (a row's operand is split between the matrix instructions of the row before,
+                    // and read between those of the one before that)
+                    Split pb[S::NT], pa[2];
                     each<S::NT>([&](auto t) { pb[t()] = split(fb[t()]); });
+                    pa[0] = split(fa[0]);
                     each<S::MT>([&](auto i) {
-                        const Split pa = split(fa[i()]);
-                        each<S::NT>([&](auto t) {
-                            sums[i()][t()] = mma(pa, pb[t()], sums[i()][t()]);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (i() + 2 < S::MT) {
+                            read(std::integral_constant<int, S::NT + i() + 2>{}, 0, fa, fb);
+                        }
+                        if constexpr (i() + 1 < S::MT) pa[(i() + 1) % 2] = split(fa[i() + 1]);
+                        each<6>([&](auto p) {
+                            each<S::NT>([&](auto t) {
+                                sums[i()][t()] = mma(pa[i() % 2].part[kSplitProducts[p()][0]],
+                                                     pb[t()].part[kSplitProducts[p()][1]],
+                                                     sums[i()][t()]);
+                            });
+                        });
+                        each<6 * S::NT>([&](auto) {
+                            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // matrix
+                            __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);  // vector
                         });
                     });
+                    __builtin_amdgcn_sched_barrier(0);
                 } else {
                     each<S::MT>([&](auto i) { multiply(i, fa, fb); });
                 }

@@ -34,6 +34,7 @@ namespace nacho {
 namespace cross_entropy {
 
 using dense::Across;
+using dense::AcrossPairs;
 using dense::Along;
 using dense::element_aligned;
 using dense::f32x4;
@@ -63,7 +64,7 @@ struct Targets {
 
 // What the kernels know of the tokens: `held` of them have a target.
 struct Held {
-    int *count;     // [1]
+    int *count;     // [2]: and a counter that starts at 0
     int *slot;      // [tokens]: place among them, -1 for one without a target
     int *token;     // [held]
     int *target;    // [held]
@@ -112,7 +113,10 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
             }
         }
     }
-    if (threadIdx.x == 0) *held.count = carry;
+    if (threadIdx.x == 0) {
+        held.count[0] = carry;
+        held.count[1] = 0;
+    }
     if (!dloss) return;
     float common = 0.0f;
     if (reduction == kNone) {
@@ -139,9 +143,30 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
     }
 }
 
-// Rows of `width` elements with zeros behind them up to `padded`: those of the listed tokens (token),
-// or the first `rows` (null).
-template <typename T, int N>
+// A row of `width` elements, with zeros behind them up to `padded`, by LANES threads.
+template <typename T, int LANES>
+__device__ __forceinline__ void copy_row(const T *__restrict__ from, int64_t width,
+                                         T *__restrict__ to, int64_t padded, int lane) {
+    constexpr int kN = 16 / sizeof(T);
+    typedef T piece_t __attribute__((ext_vector_type(kN)));
+    // (a row starts anywhere: loads of 16 bytes take any address)
+    typedef piece_t any_t __attribute__((aligned(sizeof(T))));
+    for (int64_t col = static_cast<int64_t>(lane) * kN; col < padded; col += LANES * kN) {
+        piece_t v;
+        if (col + kN <= width) {
+            v = *reinterpret_cast<const any_t *>(from + col);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                v[j] = col + j < width ? from[col + j] : static_cast<T>(0.0f);
+            }
+        }
+        *reinterpret_cast<piece_t *>(to + col) = v;
+    }
+}
+
+// Those of the listed tokens (token), or the first `rows` (null).
+template <typename T, int LANES>
 __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict__ count,
                                                           const int *__restrict__ token,
                                                           int64_t rows, int64_t width,
@@ -149,21 +174,109 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict_
                                                           const T *__restrict__ from,
                                                           int64_t stride, T *__restrict__ to,
                                                           int64_t to_stride) {
+    constexpr int kPer = kThreads / LANES;
     const int64_t there = count ? *count : rows;
-    const int64_t per = padded / N;
-    const int64_t all = there * per;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < all;
-         i += gridDim.x * static_cast<int64_t>(kThreads)) {
-        const int64_t row = i / per, col = i % per * N;
-        const int64_t source = token ? token[row] : row;
-        dense::Piece<T, N> piece;
-        if (col < width) {
-            piece = *reinterpret_cast<const dense::Piece<T, N> *>(from + source * stride + col);
-        } else {
+    int64_t row = blockIdx.x * static_cast<int64_t>(kPer) +
+                  __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    for (; row < there; row += gridDim.x * static_cast<int64_t>(kPer)) {
+        copy_row<T, LANES>(from + (token ? token[row] : row) * stride, width, to + row * to_stride,
+                           padded, threadIdx.x % LANES);
+    }
+}
+
+// Both of the above for up to kListMost tokens: every workgroup counts the targets before its own
+// kListRows tokens.  (8192 tokens of 2048 bfloat16: 29 us, and 27 for the two; 3000 of 776: 9 and 9;
+// few: a launch less, 5 us.)
+constexpr int kListMost = 2048;
+constexpr int kListRows = 8;
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, int tokens,
+                                                             int reduction,
+                                                             const float *__restrict__ dloss,
+                                                             Held held, int64_t width,
+                                                             int64_t padded,
+                                                             const T *__restrict__ from,
+                                                             int64_t stride, T *__restrict__ to,
+                                                             int64_t to_stride) {
+    constexpr int kWaves = kThreads / dev::kWave, kStep = 8;
+    __shared__ int s_before[kWaves], s_all[kWaves], s_token[kListRows];
+    __shared__ float s_most[kWaves];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / dev::kWave), lane = dev::lane();
+    const int first = static_cast<int>(blockIdx.x) * kListRows;
+    const bool each = dloss && reduction == kNone;
+    int before = 0, all = 0;
+    float most = 0.0f;
+    for (int t0 = threadIdx.x; t0 < tokens; t0 += kThreads * kStep) {
+        int id[kStep];
+        float c[kStep];
 #pragma unroll
-            for (int j = 0; j < N; ++j) piece.v[j] = static_cast<T>(0.0f);
+        for (int s = 0; s < kStep; ++s) {
+            const int t = t0 + s * kThreads;
+            id[s] = t < tokens ? targets(t) : -1;
+            c[s] = each && t < tokens ? fabsf(dloss[t]) : 0.0f;
         }
-        *reinterpret_cast<dense::Piece<T, N> *>(to + row * to_stride + col) = piece;
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) {
+            const int t = t0 + s * kThreads;
+            if (id[s] >= 0) {
+                ++all;
+                before += t < first ? 1 : 0;
+                most = most < c[s] || c[s] != c[s] ? c[s] : most;  // (no number stays)
+            }
+        }
+    }
+    before = dev::wave_sum(before);
+    all = dev::wave_sum(all);
+#pragma unroll
+    for (int off = dev::kWave / 2; off > 0; off >>= 1) {
+        const float other = __shfl_xor(most, off, dev::kWave);
+        most = most < other || other != other ? other : most;
+    }
+    if (lane == 0) {
+        s_before[wave] = before;
+        s_all[wave] = all;
+        s_most[wave] = most;
+    }
+    __syncthreads();
+    before = all = 0;
+    float common = 0.0f;
+    for (int w = 0; w < kWaves; ++w) {
+        before += s_before[w];
+        all += s_all[w];
+        common = common < s_most[w] || s_most[w] != s_most[w] ? s_most[w] : common;
+    }
+    if (each) {
+        if (!(common < dense::kInf)) common = 1.0f;
+    } else if (dloss) {
+        common = reduction == kMean ? dloss[0] / static_cast<float>(max(all, 1)) : dloss[0];
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        held.count[0] = all;
+        held.count[1] = 0;
+        if (dloss) *held.common = common;
+    }
+    // the workgroup's own tokens, a lane each
+    if (wave == 0) {
+        const int t = first + lane;
+        const int id = lane < kListRows && t < tokens ? targets(t) : -1;
+        const unsigned long long there = __ballot(id >= 0);
+        const int at = before + __popcll(there & ((1ull << lane) - 1ull));
+        if (lane < kListRows && t < tokens) held.slot[t] = id >= 0 ? at : -1;
+        if (id >= 0) {
+            held.token[at] = t;
+            held.target[at] = id;
+            if (each) held.factor[at] = common == 0.0f ? 0.0f : dloss[t] / common;
+        }
+        if (lane < kListRows) s_token[lane] = id >= 0 ? at : -1;
+    }
+    __syncthreads();
+    for (int i = wave; i < kListRows; i += kWaves) {
+        const int at = s_token[i];
+        if (at >= 0) {
+            copy_row<T, dev::kWave>(from + (first + i) * stride, width, to + at * to_stride, padded,
+                                    lane);
+        }
     }
 }
 
@@ -177,12 +290,20 @@ constexpr unsigned kUnits = 256;
 // needs.
 constexpr int kTileThreads = 512;
 template <int BM, int BN>
-using Tile = std::conditional_t<
-    BM == 256, std::conditional_t<BN == 256, Shape<256, 256, 2, 4>,
-                                  std::conditional_t<BN == 16, Shape<256, 16, 8, 1>,
-                                                     Shape<256, BN, 4, 2>>>,
-    std::conditional_t<BN == 256, Shape<64, 256, 1, 8>,
-                       std::conditional_t<BN == 16, Shape<64, 16, 4, 1>, Shape<64, 64, 2, 4>>>>;
+struct TileOf;
+template <> struct TileOf<256, 256> { using type = Shape<256, 256, 2, 4>; };
+template <> struct TileOf<256, 192> { using type = Shape<256, 192, 2, 4>; };
+template <> struct TileOf<256, 128> { using type = Shape<256, 128, 4, 2>; };
+template <> struct TileOf<256, 64> { using type = Shape<256, 64, 4, 2>; };
+template <> struct TileOf<256, 16> { using type = Shape<256, 16, 8, 1>; };
+template <> struct TileOf<128, 256> { using type = Shape<128, 256, 2, 4>; };
+template <> struct TileOf<128, 192> { using type = Shape<128, 192, 2, 4>; };
+template <> struct TileOf<128, 128> { using type = Shape<128, 128, 2, 4>; };
+template <> struct TileOf<128, 64> { using type = Shape<128, 64, 4, 2>; };
+template <> struct TileOf<64, 256> { using type = Shape<64, 256, 1, 8>; };
+template <> struct TileOf<64, 16> { using type = Shape<64, 16, 4, 1>; };
+template <int BM, int BN>
+using Tile = typename TileOf<BM, BN>::type;
 template <int N>
 using Number = std::integral_constant<int, N>;
 
@@ -246,6 +367,8 @@ __device__ __forceinline__ void with_tile(int words, int held, F f) {
             f(Tile<BM, 64>{}, v0, mt, n0);
         } else if (wide <= 128 || left <= 128) {
             f(Tile<BM, 128>{}, v0, mt, n0);
+        } else if (left <= 192) {
+            f(Tile<BM, 192>{}, v0, mt, n0);
         } else {
             f(Tile<BM, 256>{}, v0, mt, n0);
         }
@@ -365,27 +488,25 @@ __global__ __launch_bounds__((Tile<BM, BN>::kThreads)) void parts_kernel(Logits 
     });
 }
 
-// A wavefront per token: its tiles' parts to m, s and the loss.
-__global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ slot,
-                                                        int tokens, unsigned tiles,
-                                                        const float2 *__restrict__ parts,
-                                                        const float *__restrict__ mine,
-                                                        float *__restrict__ most_of,
-                                                        float *__restrict__ total_of,
-                                                        float *__restrict__ loss) {
-    const int64_t t = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / dev::kWave;
-    if (t >= tokens) return;
-    const int at = slot[t];
-    if (at < 0) {
-        if (dev::lane() == 0) {
-            most_of[t] = 0.0f;
-            total_of[t] = 1.0f;
-            loss[t] = 0.0f;
-        }
-        return;
-    }
-    const float2 *from = parts + static_cast<int64_t>(at) * tiles;
+// The sum of the threads' values, over a number if there is one, as a float.
+template <int THREADS>
+__device__ __forceinline__ void store_sum(double all, const int *count, float *to) {
+    __shared__ double s_sum[THREADS / dev::kWave];
+    all = dev::wave_sum(all);
+    if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = all;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    all = 0.0;
+    for (int w = 0; w < THREADS / dev::kWave; ++w) all += s_sum[w];
+    *to = static_cast<float>(count ? all / max(*count, 1) : all);
+}
+
+// A token's tiles' parts to m, s and the loss, by a wavefront.
+__device__ __forceinline__ void join_token(const float2 *__restrict__ from, unsigned tiles,
+                                           const float *__restrict__ mine, float *most_of,
+                                           float *total_of, float *loss) {
     float most = kNegInf, total = 0.0f;
+#pragma unroll 4
     for (unsigned i = dev::lane(); i < tiles; i += dev::kWave) {
         const float2 p = from[i];
         const float higher = fmaxf(most, p.x);
@@ -405,26 +526,99 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ 
         most = higher;
     }
     if (dev::lane() == 0) {
-        most_of[t] = most;
-        total_of[t] = total;
-        loss[t] = logf(total) + (most - mine[at]);
+        *most_of = most;
+        *total_of = total;
+        *loss = logf(total) + (most - *mine);
     }
+}
+
+// A wavefront per token; with `sum`, for up to kJoinMost tokens, also the sum of the losses or (mean)
+// their mean.  (What makes the losses of all workgroups visible to the last costs each of them:
+// 5 us less than two launches for 64 tokens, 60 us more for 3000.)
+constexpr int64_t kJoinMost = 64;
+
+__global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ slot,
+                                                        int tokens, unsigned tiles,
+                                                        const float2 *__restrict__ parts,
+                                                        const float *__restrict__ mine,
+                                                        float *__restrict__ most_of,
+                                                        float *__restrict__ total_of, float *each,
+                                                        int *count, int mean, float *sum) {
+    const int64_t t = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / dev::kWave;
+    const int at = t < tokens ? slot[t] : -1;
+    if (t < tokens && at < 0 && dev::lane() == 0) {
+        most_of[t] = 0.0f;
+        total_of[t] = 1.0f;
+        each[t] = 0.0f;
+    }
+    if (at >= 0) join_token(parts + static_cast<int64_t>(at) * tiles, tiles, mine + at,
+                            most_of + t, total_of + t, each + t);
+    if (!sum) return;
+    // The workgroup that finds all others done adds the losses up, in their order.
+    __shared__ int s_last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s_last = atomicAdd(count + 1, 1) == static_cast<int>(gridDim.x) - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!s_last) return;
+    double all = 0.0;
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < tokens; i += kThreads) {
+        all += static_cast<double>(
+            __hip_atomic_load(each + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    }
+    store_sum<kThreads>(all, mean ? count : nullptr, sum);
 }
 
 // The sum of the losses, or their mean over the tokens that have a target.
 __global__ __launch_bounds__(1024) void sum_kernel(const int *__restrict__ count, int64_t tokens,
                                                    const float *__restrict__ each, int mean,
                                                    float *__restrict__ loss) {
-    __shared__ double s_sum[1024 / dev::kWave];
-    double sum = 0.0;
-    for (int64_t t = threadIdx.x; t < tokens; t += 1024) sum += static_cast<double>(each[t]);
-    sum = dev::wave_sum(sum);
-    if (dev::lane() == 0) s_sum[threadIdx.x / dev::kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    sum = 0.0;
-    for (int w = 0; w < 1024 / dev::kWave; ++w) sum += s_sum[w];
-    *loss = static_cast<float>(mean ? sum / max(*count, 1) : sum);
+    double all = 0.0;
+#pragma unroll 8
+    for (int64_t t = threadIdx.x; t < tokens; t += 1024) all += static_cast<double>(each[t]);
+    store_sum<1024>(all, mean ? count : nullptr, loss);
+}
+
+// Four results of a row, or those of them that are within its width.
+template <typename T>
+__device__ __forceinline__ void store_row4(T *row, int64_t d, int64_t width, f32x4 v) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    typedef t4 any_t __attribute__((aligned(sizeof(T))));
+    if (d + 4 <= width) {
+        t4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = static_cast<T>(v[j]);
+        *reinterpret_cast<any_t *>(row + d) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (d + j < width) row[d + j] = static_cast<T>(v[j]);
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row8(T *row, int64_t d, int64_t width, f32x4 lo, f32x4 hi) {
+    if constexpr (sizeof(T) == 2) {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        typedef t8 any_t __attribute__((aligned(sizeof(T))));
+        if (d + 8 <= width) {
+            t8 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = static_cast<T>(lo[j]);
+                o[4 + j] = static_cast<T>(hi[j]);
+            }
+            *reinterpret_cast<any_t *>(row + d) = o;
+            return;
+        }
+    }
+    store_row4<T>(row, d, width, lo);
+    store_row4<T>(row, d + 4, width, hi);
 }
 
 // dz of a tile's words and tokens.
@@ -502,45 +696,66 @@ struct Gradients {
     float *sums;          // [split][held][sums_stride]; null: no dx
     int64_t sums_stride;
     int first;            // whether the piece is the first
+    int64_t most_parts;   // splits that `parts` has room for; 1 without it
+    float *parts;         // [split][piece][sums_stride]: dtable's
     const float *common;
     float scale;
     void *dtable;         // of the piece, [words][width]; null: none
 };
 
-// How dx's products, tiles of its columns by the tokens, are split over the words: into items of
-// about half of a compute unit's work, that of dtable included where one launch has both, so that
-// the units' work is even.  The same for every piece, and known to the device alone.
+// How the gradients' products are split: dx's tiles, of its columns by the tokens, over the words,
+// and dtable's, of its columns by the words, over the tokens.  An item is at most about three
+// quarters of a compute unit's work, that of both where one launch has both, so that the units' work
+// is even.
+// The same for every piece, and known to the device alone.
 struct Splits {
     unsigned m_tiles, n_tiles, count;
-    int64_t words;  // of a split
+    int64_t depth;  // words, or tokens, of a split
 
-    __device__ __forceinline__ unsigned items() const { return m_tiles * n_tiles * count; }
+    __device__ __forceinline__ unsigned tiles() const { return m_tiles * n_tiles; }
+    __device__ __forceinline__ unsigned items() const { return tiles() * count; }
 };
 
 constexpr unsigned kMostItems = 512, kMostSplits = 64;
 
-template <typename T, int BN>
-__device__ __forceinline__ Splits splits_of(int64_t piece, int64_t width, int64_t most_rows,
-                                            int held, bool both) {
-    constexpr int kStep = dense::kStepK<T>;
+// n rows by the width, over `depth`, in whole steps, of a load of `load` steps; most: splits that
+// the sums have room for.
+__device__ __forceinline__ Splits split_up(int64_t n, int bn, int64_t width, int64_t depth,
+                                           int step, int64_t load, int64_t most) {
     Splits s;
     s.m_tiles = static_cast<unsigned>((width + 255) / 256);
-    s.n_tiles = static_cast<unsigned>((held + BN - 1) / BN);
-    const int64_t steps = (piece + kStep - 1) / kStep;
-    const int64_t tiles = static_cast<int64_t>(s.m_tiles) * s.n_tiles;
-    int64_t load = tiles * steps;
-    if (both) load += (piece + 255) / 256 * s.m_tiles * ((held + kStep - 1) / kStep);
-    // (0.55 of it: two and a bit to a unit are one each and no third)
-    const int64_t wanted = load * 11 / (20 * static_cast<int64_t>(kUnits));
+    s.n_tiles = static_cast<unsigned>((n + bn - 1) / bn);
+    const int64_t steps = (depth + step - 1) / step;
+    const int64_t wanted = load * 3 / (4 * static_cast<int64_t>(kUnits));
     const int64_t per = wanted < 8 ? 8 : wanted;
-    int64_t n = (steps + per - 1) / per;
-    n = min(n, static_cast<int64_t>(kMostItems) / max(tiles, int64_t{1}));
-    n = min(n, static_cast<int64_t>(kMostSplits));
-    n = min(n, most_rows / max(held, 1));
-    n = max(n, int64_t{1});
-    s.words = (steps + n - 1) / n * kStep;
-    s.count = static_cast<unsigned>((piece + s.words - 1) / s.words);
+    int64_t k = (steps + per - 1) / per;
+    k = min(k, static_cast<int64_t>(kMostItems) / max(static_cast<int64_t>(s.tiles()), int64_t{1}));
+    k = max(min(min(k, static_cast<int64_t>(kMostSplits)), most), int64_t{1});
+    s.depth = max((steps + k - 1) / k, int64_t{1}) * step;
+    s.count = static_cast<unsigned>(max((depth + s.depth - 1) / s.depth, int64_t{1}));
     return s;
+}
+
+// The steps of dx's and of dtable's products.
+template <typename T, int BN>
+__device__ __forceinline__ int64_t load_of(const Gradients &a, int held, bool dx, bool dtable) {
+    constexpr int kStep = dense::kStepK<T>, kBN = BN <= 64 ? 64 : BN;
+    const int64_t m_tiles = (a.width + 255) / 256;
+    const int64_t x = (held + BN - 1) / BN * ((a.piece + kStep - 1) / kStep);
+    const int64_t t = (a.piece + kBN - 1) / kBN * ((held + kStep - 1) / kStep);
+    return m_tiles * ((dx ? x : 0) + (dtable ? t : 0));
+}
+
+template <typename T, int BN>
+__device__ __forceinline__ Splits dx_splits(const Gradients &a, int held, int64_t load) {
+    return split_up(held, BN, a.width, a.piece, dense::kStepK<T>, load,
+                    a.most_rows / max(held, 1));
+}
+
+template <typename T, int BN>
+__device__ __forceinline__ Splits dtable_splits(const Gradients &a, int held, int64_t load) {
+    return split_up(a.piece, BN <= 64 ? 64 : BN, a.width, held, dense::kStepK<T>, load,
+                    a.most_parts);
 }
 
 // A tile of dx's sums: columns of the table's rows by the tokens, over the words of a split.
@@ -572,16 +787,21 @@ __device__ __forceinline__ void tile_dx(const Gradients &a, int64_t d0, int64_t 
     }
 }
 
-// A tile of dtable: columns of the gathered rows by the words, over the tokens.
-template <typename T, typename S>
-__device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int64_t v0, int held,
-                                            T *lds) {
-    const Matrix<T> rows{static_cast<const T *>(a.rows) + d0, a.rows_stride};
-    const Matrix<T> dz{static_cast<const T *>(a.dz) + v0, a.dz_stride};
+// A tile of dtable: columns of the gathered rows by the words, over the tokens or (not whole) those
+// of a split.
+template <typename T, typename S, bool PAIRS>
+__device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int64_t v0,
+                                            unsigned split, int64_t t0, int64_t tokens,
+                                            bool whole, T *lds) {
+    const Matrix<T> rows{static_cast<const T *>(a.rows) + t0 * a.rows_stride + d0, a.rows_stride};
+    const Matrix<T> dz{static_cast<const T *>(a.dz) + t0 * a.dz_stride + v0, a.dz_stride};
     f32x4 sums[S::MT][S::NT];
-    Product<T, S, Across, Across>::run(
+    // (few tokens are bound by the stores of the results: 8 elements together)
+    using P = std::conditional_t<PAIRS, Product<T, S, AcrossPairs, Across>,
+                                 Product<T, S, Across, Across>>;
+    P::run(
         rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
-        static_cast<int>(min(a.piece - v0, static_cast<int64_t>(S::BN))), held, lds, sums);
+        static_cast<int>(min(a.piece - v0, static_cast<int64_t>(S::BN))), tokens, lds, sums);
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;
@@ -590,107 +810,148 @@ __device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int6
         const int64_t v = v0 + (wn * S::NT + t) * 16 + c;
         if (v >= a.words) continue;
         T *to = static_cast<T *>(a.dtable) + v * a.width;
+        float *part = a.parts + (split * a.piece + v) * a.sums_stride;
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int i = 0; i < S::MT; i += 2) {
+                const int64_t d = d0 + (wm * S::MT + i) * 16 + 8 * g;
+                store_row8<T>(to, d, a.width, sums[i][t] * factor, sums[i + 1][t] * factor);
+            }
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < S::MT; ++i) {
             const int64_t d = d0 + (wm * S::MT + i) * 16 + 4 * g;
-            const f32x4 x = sums[i][t] * factor;
-            if (a.width % 4 == 0) {
-                if (d < a.width) dense::store4<T>(to + d, x);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (d + j < a.width) to[d + j] = static_cast<T>(x[j]);
-                }
+            if (whole) {
+                store_row4<T>(to, d, a.width, sums[i][t] * factor);
+            } else if (d < a.sums_stride) {
+                *reinterpret_cast<f32x4 *>(part + d) = sums[i][t];
             }
         }
     }
 }
 
-// Calls f with the tile of at most BM x BN that `m` by `n` need.
-template <int BN, typename F>
+// Calls f with the tile of at most 256 x BN that `m` by `n` need.
+template <int BN, bool ALONG, typename F>
 __device__ __forceinline__ void with_ends(int64_t m, int64_t n, F f) {
-    if (BN <= 64 || n <= 64) {
-        constexpr int kBN = BN <= 64 ? BN : 64;
-        f(Tile<256, kBN>{});
-    } else if (m <= 64) {
-        f(Tile<64, BN>{});
-    } else {
+    if constexpr (BN <= 64) {
         f(Tile<256, BN>{});
+    } else {
+        if (n <= 64) return f(Tile<256, 64>{});
+        if (m <= 64) return f(Tile<64, 256>{});
+        if (m <= 128) return f(Tile<128, 256>{});
+        if (n <= 128) return f(Tile<256, 128>{});
+        if constexpr (ALONG) {
+            if (n <= 192) return f(Tile<256, 192>{});
+        }
+        f(Tile<256, 256>{});
     }
 }
 
-// dx's items, then dtable's tiles: one launch for calls of many tokens (BN 256), else one for each.
+// dx's items, then dtable's: one launch for calls of many tokens (BN 256), else one for each.
 template <typename T, int BN, bool DX, bool DTABLE>
 __global__ __launch_bounds__(kTileThreads) void gradients_kernel(Gradients a) {
     constexpr int kLdsX = DX ? kLds<T, 256, BN, Across, Along> : 0;
     constexpr int kLdsT = DTABLE ? kLds<T, 256, (BN <= 64 ? 64 : BN), Across, Across> : 0;
     __shared__ __attribute__((aligned(16))) T lds[kLdsX > kLdsT ? kLdsX : kLdsT];
     const int held = *a.held;
+    const int64_t load = load_of<T, BN>(a, held, DX, DTABLE);
     unsigned at = blockIdx.x, mt = 0, nt = 0;
     if constexpr (DX) {
-        const Splits s = splits_of<T, BN>(a.piece, a.width, a.most_rows, held, DTABLE);
-        const unsigned items = s.items();
-        if (at < items) {
-            at = dense::order_of(at, items);
-            const unsigned tiles = s.m_tiles * s.n_tiles, split = at / tiles;
-            dense::tile_of(at % tiles, s.m_tiles, s.n_tiles, mt, nt);
+        const Splits s = dx_splits<T, BN>(a, held, load);
+        if (at < s.items()) {
+            at = dense::order_of(at, s.items());
+            const unsigned split = at / s.tiles();
+            dense::tile_of(at % s.tiles(), s.m_tiles, s.n_tiles, mt, nt);
             const int64_t d0 = mt * int64_t{256}, n0 = nt * static_cast<int64_t>(BN);
-            const int64_t v0 = split * s.words;
+            const int64_t v0 = split * s.depth;
             // (a short last piece has fewer splits; a first one's sums are all written)
             if (v0 >= a.words && !a.first) return;
-            with_ends<BN>(a.padded - d0, held - n0, [&](auto shape) {
-                tile_dx<T, decltype(shape)>(a, d0, n0, split, v0, min(s.words, a.words - v0),
-                                            held, lds);
+            with_ends<BN, true>(a.padded - d0, held - n0, [&](auto shape) {
+                tile_dx<T, decltype(shape)>(a, d0, n0, split, v0, min(s.depth, a.words - v0), held,
+                                            lds);
             });
             return;
         }
-        at -= items;
+        at -= s.items();
     }
     if constexpr (DTABLE) {
+        const Splits s = dtable_splits<T, BN>(a, held, load);
+        if (at >= s.items()) return;
+        at = dense::order_of(at, s.items());
+        const unsigned split = at / s.tiles();
+        dense::tile_of(at % s.tiles(), s.m_tiles, s.n_tiles, mt, nt);
         constexpr int kBN = BN <= 64 ? 64 : BN;
-        const unsigned m_tiles = static_cast<unsigned>((a.width + 255) / 256);
-        const unsigned n_tiles = static_cast<unsigned>((a.words + kBN - 1) / kBN);
-        const unsigned tiles = m_tiles * n_tiles;
-        if (at >= tiles) return;
-        dense::tile_of(dense::order_of(at, tiles), m_tiles, n_tiles, mt, nt);
         const int64_t d0 = mt * int64_t{256}, v0 = nt * static_cast<int64_t>(kBN);
-        with_ends<kBN>(a.padded - d0, a.words - v0, [&](auto shape) {
-            tile_dtable<T, decltype(shape)>(a, d0, v0, held, lds);
+        const int64_t t0 = split * s.depth;
+        if (v0 >= a.words) return;
+        with_ends<kBN, false>(a.padded - d0, a.words - v0, [&](auto shape) {
+            // (with few tokens never split)
+            tile_dtable<T, decltype(shape), BN <= 64>(a, d0, v0, split, t0,
+                                                      min(s.depth, held - t0), s.count == 1, lds);
         });
     }
 }
 
-// dx of every token: the splits' sums in their order, and 0 for a token without a target.
+// Four sums of the splits, `stride` apart, in their order; kStep of them on their way at a time.
+__device__ __forceinline__ f32x4 splits_sum(const float *from, int64_t stride, unsigned splits) {
+    constexpr unsigned kStep = 8;
+    f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned s0 = 0; s0 < splits; s0 += kStep) {
+        f32x4 x[kStep];
+#pragma unroll
+        for (unsigned s = 0; s < kStep; ++s) {
+            x[s] = *reinterpret_cast<const f32x4 *>(from + min(s0 + s, splits - 1) * stride);
+        }
+#pragma unroll
+        for (unsigned s = 0; s < kStep; ++s) {
+            if (s0 + s < splits) sum += x[s];
+        }
+    }
+    return sum;
+}
+
+// dtable of a piece whose products were split: the splits' sums in their order.
 template <typename T, int BN>
+__global__ __launch_bounds__(kThreads) void dtable_join_kernel(Gradients a, bool both) {
+    const int held = *a.held;
+    const unsigned splits =
+        dtable_splits<T, BN>(a, held, load_of<T, BN>(a, held, both, true)).count;
+    if (splits == 1) return;
+    const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
+    constexpr int kPer = kThreads / dev::kWave;
+    int64_t v = blockIdx.x * static_cast<int64_t>(kPer) +
+                __builtin_amdgcn_readfirstlane(threadIdx.x / dev::kWave);
+    for (; v < a.words; v += gridDim.x * static_cast<int64_t>(kPer)) {
+        const float *from = a.parts + v * a.sums_stride;
+        for (int64_t d = 4ll * dev::lane(); d < a.width; d += 4 * dev::kWave) {
+            const f32x4 sum = splits_sum(from + d, a.piece * a.sums_stride, splits);
+            store_row4<T>(static_cast<T *>(a.dtable) + v * a.width, d, a.width, sum * factor);
+        }
+    }
+}
+
+// dx of every token: the splits' sums in their order, and 0 for a token without a target.
+template <typename T, int BN, int LANES>
 __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
                                                            const int *__restrict__ slot,
                                                            int64_t tokens, bool both,
                                                            T *__restrict__ dx) {
     const int held = *a.held;
-    const unsigned splits =
-        splits_of<T, BN>(a.piece, a.width, a.most_rows, held, both).count;
+    const unsigned splits = dx_splits<T, BN>(a, held, load_of<T, BN>(a, held, true, both)).count;
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
-    const int64_t per = (a.width + 3) / 4;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < tokens * per;
-         i += gridDim.x * static_cast<int64_t>(kThreads)) {
-        const int64_t t = i / per, d = i % per * 4;
+    constexpr int kPer = kThreads / LANES;
+    int64_t t = blockIdx.x * static_cast<int64_t>(kPer) +
+                __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    for (; t < tokens; t += gridDim.x * static_cast<int64_t>(kPer)) {
         const int at = slot[t];
-        f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-        if (at >= 0) {
-            const float *from = a.sums + at * a.sums_stride + d;
-#pragma unroll 4
-            for (unsigned s = 0; s < splits; ++s) {
-                sum += *reinterpret_cast<const f32x4 *>(from + s * (held * a.sums_stride));
+        for (int64_t d = 4ll * (threadIdx.x % LANES); d < a.width; d += 4 * LANES) {
+            f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+            if (at >= 0) {
+                sum = splits_sum(a.sums + at * a.sums_stride + d, held * a.sums_stride, splits);
+                sum *= factor;
             }
-            sum *= factor;
-        }
-        T *to = dx + t * a.width + d;
-        if (a.width % 4 == 0) {
-            dense::store4<T>(to, sum);
-        } else {
-            for (int j = 0; j < 4; ++j) {
-                if (d + j < a.width) to[j] = static_cast<T>(sum[j]);
-            }
+            store_row4<T>(dx + t * a.width, d, a.width, sum);
         }
     }
 }
@@ -740,6 +1001,31 @@ int check(const Args &a) {
     return NACHO_OK;
 }
 
+// A call's scratch: one allocation for all that it asks for.
+struct Wanted {
+    struct Piece {
+        void **to;
+        size_t bytes;
+    } pieces[12];
+    int n = 0;
+
+    template <typename T>
+    void add(T **to, int64_t count) {
+        pieces[n++] = {reinterpret_cast<void **>(to), static_cast<size_t>(count) * sizeof(T)};
+    }
+    int get(Call &call) {
+        size_t all = 0;
+        for (int i = 0; i < n; ++i) all += (pieces[i].bytes + 255) / 256 * 256;
+        char *p = nullptr;
+        NACHO_TRY(call.scratch(all, reinterpret_cast<void **>(&p)));
+        for (int i = 0; i < n; ++i) {
+            *pieces[i].to = p;
+            p += (pieces[i].bytes + 255) / 256 * 256;
+        }
+        return NACHO_OK;
+    }
+};
+
 // The operands as the kernels take them: rows gathered and, where a table's rows are not whole
 // aligned pieces, a copy of it whose are.
 template <typename T>
@@ -747,82 +1033,89 @@ struct Operands {
     Held held{};
     T *rows = nullptr;
     const T *table = nullptr;
+    T *copy = nullptr;
     int64_t width = 0;  // of rows, a multiple of a piece
     int64_t rows_stride = 0;
     int64_t table_stride = 0;
+    bool copied = false;
 
-    int start(Call &call, const Args &a, const float *dloss) {
-        constexpr int64_t kPer = 16 / sizeof(T);
-        const hipStream_t s = call.stream();
-        const size_t n = static_cast<size_t>(a.tokens);
-        int *ints = nullptr;
-        float *floats = nullptr;
-        NACHO_TRY(call.scratch_n(3 * n + 1, &ints));
-        held.count = ints;
-        held.slot = ints + 1;
-        held.token = held.slot + n;
-        held.target = held.token + n;
-        if (dloss) {
-            const size_t factors = a.reduction == NACHO_LOSS_NONE ? n : 0;
-            NACHO_TRY(call.scratch_n(1 + factors, &floats));
-            held.common = floats;
-            held.factor = factors ? floats + 1 : nullptr;
-        }
-        list_kernel<<<1, kListThreads, 0, s>>>(Targets{a.targets, a.id_bytes, a.words},
-                                               static_cast<int>(a.tokens), a.reduction, dloss,
-                                               held);
-        NACHO_TRY_HIP(hipGetLastError());
-        width = up(a.width, kPer);
+    // (256 rows of a tile within the loads' 2 GB)
+    static constexpr int64_t kMostStride = int64_t{1} << 22;
+
+    void want(Wanted &wanted, const Args &a, const float *dloss) {
+        width = up(a.width, 16 / sizeof(T));
         rows_stride = scratch_stride<T>(width);
-        NACHO_TRY(call.scratch_n(n * static_cast<size_t>(rows_stride), &rows));
-        NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, a.x, a.x_stride, rows,
-                         rows_stride));
+        wanted.add(&held.count, 2);
+        wanted.add(&held.slot, a.tokens);
+        wanted.add(&held.token, a.tokens);
+        wanted.add(&held.target, a.tokens);
+        if (dloss) wanted.add(&held.common, 1);
+        if (dloss && a.reduction == NACHO_LOSS_NONE) wanted.add(&held.factor, a.tokens);
+        wanted.add(&rows, a.tokens * rows_stride);
         table = static_cast<const T *>(a.table);
         table_stride = a.table_stride;
-        if (!dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
-            table_stride * static_cast<int64_t>(sizeof(T)) > kMostStride) {
-            T *copy = nullptr;
+        copied = !dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
+                 table_stride * static_cast<int64_t>(sizeof(T)) > kMostStride;
+        if (copied) {
             table_stride = scratch_stride<T>(width);
-            NACHO_TRY(call.scratch_n(static_cast<size_t>(a.words * table_stride), &copy));
-            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, a.table, a.table_stride, copy,
+            wanted.add(&copy, a.words * table_stride);
+        }
+    }
+
+    int start(hipStream_t s, const Args &a, const float *dloss) {
+        const Targets targets{a.targets, a.id_bytes, a.words};
+        const int tokens = static_cast<int>(a.tokens);
+        const T *x = static_cast<const T *>(a.x);
+        if (tokens <= kListMost) {
+            list_rows_kernel<T><<<ceil_div(static_cast<size_t>(tokens), kListRows), kThreads, 0,
+                                  s>>>(targets, tokens, a.reduction, dloss, held, a.width, width,
+                                       x, a.x_stride, rows, rows_stride);
+            NACHO_TRY_HIP(hipGetLastError());
+        } else {
+            list_kernel<<<1, kListThreads, 0, s>>>(targets, tokens, a.reduction, dloss, held);
+            NACHO_TRY_HIP(hipGetLastError());
+            NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, x, a.x_stride, rows,
+                             rows_stride));
+        }
+        if (copied) {
+            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, table, a.table_stride, copy,
                              table_stride));
             table = copy;
         }
         return NACHO_OK;
     }
 
-    // (256 rows of a tile within the loads' 2 GB)
-    static constexpr int64_t kMostStride = int64_t{1} << 22;
-
     int gather(hipStream_t s, const int *count, const int *token, int64_t n, int64_t columns,
-               const void *from, int64_t stride, T *to, int64_t to_stride) const {
-        constexpr int kPer = 16 / sizeof(T);
-        const bool whole = dense::pieces(from, stride, columns, sizeof(T));
-        const int64_t threads = n * (width / (whole ? kPer : 1));
-        const int64_t groups = (threads + kThreads - 1) / kThreads;
-        const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
-        if (whole) {
-            gather_kernel<T, kPer><<<grid, kThreads, 0, s>>>(
-                count, token, n, columns, width, static_cast<const T *>(from), stride, to,
-                to_stride);
-        } else {
-            gather_kernel<T, 1><<<grid, kThreads, 0, s>>>(
-                count, token, n, columns, width, static_cast<const T *>(from), stride, to,
-                to_stride);
-        }
-        NACHO_TRY_HIP(hipGetLastError());
-        return NACHO_OK;
+               const T *from, int64_t stride, T *to, int64_t to_stride) const {
+        auto launch = [&](auto lanes) -> int {
+            const int64_t groups = (n * lanes() + kThreads - 1) / kThreads;
+            const unsigned grid = static_cast<unsigned>(groups < (1 << 20) ? groups : 1 << 20);
+            gather_kernel<T, lanes()><<<grid, kThreads, 0, s>>>(
+                count, token, n, columns, width, from, stride, to, to_stride);
+            NACHO_TRY_HIP(hipGetLastError());
+            return NACHO_OK;
+        };
+        if (width * static_cast<int64_t>(sizeof(T)) <= 4096) return launch(Number<dev::kWave>{});
+        return launch(Number<kThreads>{});
     }
 };
 
 // Calls f with the words and the tokens of a tile of logits, by the number of tokens: a tile's
 // products of a few tokens would be of nothing.  Few tokens are bound by the table's bytes, of which
-// small tiles of a small vocabulary have more on their way.
+// small tiles of a small vocabulary have more on their way; and tiles are smaller where there are
+// fewer than compute units.
 template <typename F>
 int with_shape(int64_t tokens, int64_t words, F f) {
-    if (tokens <= 16 && words < 65536) return f(Number<64>{}, Number<16>{});
-    if (tokens <= 16) return f(Number<256>{}, Number<16>{});
-    if (tokens <= 128) return f(Number<256>{}, Number<64>{});
+    auto tiles = [&](int64_t bn) { return up(words, 256) / 256 * (up(tokens, bn) / bn); };
+    if (tokens <= 16) {
+        if (words < 65536) return f(Number<64>{}, Number<16>{});
+        return f(Number<256>{}, Number<16>{});
+    }
+    if (tokens <= 128) {
+        if (tiles(64) < 2 * kUnits) return f(Number<128>{}, Number<64>{});
+        return f(Number<256>{}, Number<64>{});
+    }
+    if (tiles(256) < kUnits) return f(Number<128>{}, Number<256>{});
     return f(Number<256>{}, Number<256>{});
 }
 
@@ -854,43 +1147,48 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
             const unsigned groups =
                 groups_of(a.words, bm(), a.tokens, bn(), bn() == 256 ? kUnits : 0);
             if (a.tokens > 0 && groups == 0) return NACHO_ERR_INDEX_OVERFLOW;
-            Operands<T> ops;
-            const size_t n = static_cast<size_t>(a.tokens);
-            float *each = loss;
-            if (a.tokens > 0) {
-                NACHO_TRY(ops.start(call, a, nullptr));
-                float2 *parts = nullptr;
-                float *floats = nullptr;
-                const bool keep = stats != nullptr, sums = a.reduction != NACHO_LOSS_NONE;
-                NACHO_TRY(call.scratch_n(n * m_tiles, &parts));
-                NACHO_TRY(call.scratch_n(n * (1 + (keep ? 0 : 2) + (sums ? 1 : 0)), &floats));
-                float *most = keep ? stats : floats + n;
-                if (sums) each = floats + n * (keep ? 1 : 3);
-                Logits l{};
-                l.held = ops.held.count;
-                l.width = ops.width;
-                l.rows = ops.rows;
-                l.rows_stride = ops.rows_stride;
-                l.table = ops.table;
-                l.table_stride = ops.table_stride;
-                l.words = static_cast<int>(a.words);
-                l.m_tiles = m_tiles;
-                l.target = ops.held.target;
-                l.scale = a.scale;
-                l.parts = parts;
-                l.mine = floats;
-                constexpr int kShapeThreads = Tile<bm(), bn()>::kThreads;
-                parts_kernel<T, bm(), bn()><<<groups, kShapeThreads, 0, s>>>(l);
+            if (a.tokens == 0) {  // (a reduction of none)
+                sum_kernel<<<1, 1024, 0, s>>>(nullptr, 0, nullptr, 0, loss);
                 NACHO_TRY_HIP(hipGetLastError());
-                join_kernel<<<ceil_div(n, kThreads / dev::kWave), kThreads, 0, s>>>(
-                    ops.held.slot, static_cast<int>(a.tokens), m_tiles, parts, floats, most,
-                    most + n, each);
-                NACHO_TRY_HIP(hipGetLastError());
+                return NACHO_OK;
             }
-            if (a.reduction != NACHO_LOSS_NONE) {
-                sum_kernel<<<1, 1024, 0, s>>>(ops.held.count, a.tokens, each,
-                                              a.tokens > 0 && a.reduction == NACHO_LOSS_MEAN,
-                                              loss);
+            const int64_t n = a.tokens;
+            const bool sums = a.reduction != NACHO_LOSS_NONE;
+            Operands<T> ops;
+            Wanted wanted;
+            float2 *parts = nullptr;
+            float *mine = nullptr, *most = stats, *each = loss;
+            ops.want(wanted, a, nullptr);
+            wanted.add(&parts, n * m_tiles);
+            wanted.add(&mine, n);
+            if (!stats) wanted.add(&most, 2 * n);
+            if (sums) wanted.add(&each, n);
+            NACHO_TRY(wanted.get(call));
+            NACHO_TRY(ops.start(s, a, nullptr));
+            Logits l{};
+            l.held = ops.held.count;
+            l.width = ops.width;
+            l.rows = ops.rows;
+            l.rows_stride = ops.rows_stride;
+            l.table = ops.table;
+            l.table_stride = ops.table_stride;
+            l.words = static_cast<int>(a.words);
+            l.m_tiles = m_tiles;
+            l.target = ops.held.target;
+            l.scale = a.scale;
+            l.parts = parts;
+            l.mine = mine;
+            constexpr int kShapeThreads = Tile<bm(), bn()>::kThreads;
+            parts_kernel<T, bm(), bn()><<<groups, kShapeThreads, 0, s>>>(l);
+            NACHO_TRY_HIP(hipGetLastError());
+            const int mean = a.reduction == NACHO_LOSS_MEAN;
+            join_kernel<<<ceil_div(static_cast<size_t>(n), kThreads / dev::kWave), kThreads, 0,
+                          s>>>(ops.held.slot, static_cast<int>(n), m_tiles, parts, mine, most,
+                               most + n, each, ops.held.count, mean,
+                               sums && n <= kJoinMost ? loss : nullptr);
+            NACHO_TRY_HIP(hipGetLastError());
+            if (sums && n > kJoinMost) {
+                sum_kernel<<<1, 1024, 0, s>>>(ops.held.count, n, each, mean, loss);
                 NACHO_TRY_HIP(hipGetLastError());
             }
             return NACHO_OK;
@@ -919,33 +1217,41 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
         }
         return with_shape(a.tokens, a.words, [&](auto bm, auto bn) -> int {
             constexpr int kBM = bm(), kBN = bn();
-            const size_t n = static_cast<size_t>(a.tokens);
             int64_t piece = up(kPieceBytes / (a.tokens * item), 256);
             if (piece < kPieceWords) piece = kPieceWords;
             if (piece > up(a.words, 256)) piece = up(a.words, 256);
             const int64_t cut = kBN == 256 ? kUnits : 0;
             const unsigned dx_groups = groups_of(a.width, 256, a.tokens, kBN, kMostItems);
             if (!groups_of(piece, kBM, a.tokens, kBN, cut) || !dx_groups ||
-                !groups_of(a.width, 256, piece, 64, dx_groups)) {
+                !groups_of(a.width, 256, piece, 64, dx_groups + kMostItems)) {
                 return NACHO_ERR_INDEX_OVERFLOW;
             }
             Operands<T> ops;
-            NACHO_TRY(ops.start(call, a, dloss));
+            Wanted wanted;
             Logits l{};
             Gradients d{};
             T *dz = nullptr;
+            ops.want(wanted, a, dloss);
             l.dz_stride = d.dz_stride = scratch_stride<T>(piece);
-            NACHO_TRY(call.scratch_n(n * static_cast<size_t>(l.dz_stride), &dz));
+            wanted.add(&dz, a.tokens * l.dz_stride);
             d.sums_stride = up(a.width, 4);
             // Room for the sums of as many splits as are made: tiles of 256 columns by kBN tokens,
-            // at most kMostItems of them where they are split.
-            const int64_t most = kMostItems / (up(a.width, 256) / 256) * kBN;
+            // at most kMostItems of them where they are split; the same for dtable.
+            const int64_t m_tiles = up(a.width, 256) / 256;
+            const int64_t most = kMostItems / m_tiles * kBN;
             d.most_rows = a.tokens * kMostSplits < most ? a.tokens * kMostSplits : most;
             if (d.most_rows < a.tokens) d.most_rows = a.tokens;
-            if (dx) {
-                NACHO_TRY(call.scratch_n(static_cast<size_t>(d.most_rows * d.sums_stride),
-                                         &d.sums));
+            if (dx) wanted.add(&d.sums, d.most_rows * d.sums_stride);
+            const int64_t tiles = m_tiles * (up(piece, 256) / 256);
+            const int64_t deep = up(a.tokens, 512) / 512;  // (splits are 8 steps or more)
+            d.most_parts = kMostItems / tiles < deep ? kMostItems / tiles : deep;
+            if (d.most_parts > kMostSplits) d.most_parts = kMostSplits;
+            if (kBN < 256 || d.most_parts < 2) d.most_parts = 1;
+            if (dtable && d.most_parts > 1) {
+                wanted.add(&d.parts, d.most_parts * piece * d.sums_stride);
             }
+            NACHO_TRY(wanted.get(call));
+            NACHO_TRY(ops.start(s, a, dloss));
             l.held = d.held = ops.held.count;
             l.width = d.padded = ops.width;
             l.rows = d.rows = ops.rows;
@@ -954,7 +1260,7 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             l.target = ops.held.target;
             l.scale = d.scale = a.scale;
             l.most = stats;
-            l.total = stats + n;
+            l.total = stats + a.tokens;
             l.token = ops.held.token;
             l.factor = ops.held.factor;
             l.dz = dz;
@@ -975,31 +1281,40 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
                 d.table = ops.table + v * ops.table_stride;
                 d.first = v == 0;
                 if (dtable) d.dtable = static_cast<T *>(dtable) + v * a.width;
-                const unsigned dtable_groups =
-                    groups_of(a.width, 256, words, kBN <= 64 ? 64 : kBN, 0);
+                const unsigned dtable_groups = groups_of(
+                    a.width, 256, piece, kBN <= 64 ? 64 : kBN, d.most_parts > 1 ? kMostItems : 0);
                 if (both) {
                     gradients_kernel<T, 256, true, true>
                         <<<dx_groups + dtable_groups, kTileThreads, 0, s>>>(d);
                     NACHO_TRY_HIP(hipGetLastError());
-                    continue;
                 }
-                if (dx) {
+                if (dx && !both) {
                     gradients_kernel<T, kBN, true, false><<<dx_groups, kTileThreads, 0, s>>>(d);
                     NACHO_TRY_HIP(hipGetLastError());
                 }
-                if (dtable) {
+                if (dtable && !both) {
                     gradients_kernel<T, kBN, false, true>
                         <<<dtable_groups, kTileThreads, 0, s>>>(d);
                     NACHO_TRY_HIP(hipGetLastError());
                 }
+                if (dtable && d.most_parts > 1) {
+                    const int64_t rows = (words + 3) / 4;
+                    dtable_join_kernel<T, kBN>
+                        <<<static_cast<unsigned>(rows < (1 << 20) ? rows : 1 << 20), kThreads, 0,
+                           s>>>(d, both);
+                    NACHO_TRY_HIP(hipGetLastError());
+                }
             }
             if (dx) {
-                const int64_t groups =
-                    (a.tokens * ((a.width + 3) / 4) + kThreads - 1) / kThreads;
-                const unsigned grid = static_cast<unsigned>(groups < (1 << 16) ? groups : 1 << 16);
-                dx_join_kernel<T, kBN><<<grid, kThreads, 0, s>>>(d, ops.held.slot, a.tokens, both,
-                                                                 static_cast<T *>(dx));
-                NACHO_TRY_HIP(hipGetLastError());
+                auto join = [&](auto lanes) -> int {
+                    const int64_t groups = (a.tokens * lanes() + kThreads - 1) / kThreads;
+                    dx_join_kernel<T, kBN, lanes()>
+                        <<<static_cast<unsigned>(groups < (1 << 20) ? groups : 1 << 20), kThreads,
+                           0, s>>>(d, ops.held.slot, a.tokens, both, static_cast<T *>(dx));
+                    NACHO_TRY_HIP(hipGetLastError());
+                    return NACHO_OK;
+                };
+                NACHO_TRY(a.width <= 1024 ? join(Number<dev::kWave>{}) : join(Number<kThreads>{}));
             }
             return NACHO_OK;
         });

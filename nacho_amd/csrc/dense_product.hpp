@@ -187,6 +187,35 @@ struct Across {
     }
 };
 
+// The same with a product's rows in another order: the results of tiles 2 p and 2 p + 1 in a lane are
+// eight consecutive rows, 32 p + 8 g .. + 8, for wider stores.  Reads take the LDS twice as long.
+template <typename T, int COLS, int THREADS>
+struct AcrossPairs : Across<T, COLS, THREADS> {
+    using Base = Across<T, COLS, THREADS>;
+
+    __device__ __forceinline__ static Frag<T> frag(const T *tile, int t, int kk, int g, int c) {
+        if constexpr (sizeof(T) == 4) {
+            Frag<T> f;
+            const int piece = (8 * (t >> 1) + 2 * (c >> 2) + (t & 1)) ^ Base::swizzle(8 * g);
+            const T *p = tile + 8 * g * COLS + piece * Base::kPer + (c & 3);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = p[j * COLS];
+            return f;
+        } else {
+            using Shared = __attribute__((address_space(3))) s16x4 *;
+            const int r = 32 * kk + 8 * g + (c >> 2);
+            const int at = r * COLS + ((4 * (t >> 1) + (c & 3)) ^ Base::swizzle(r)) * Base::kPer +
+                           4 * (t & 1);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + at)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (Shared)(reinterpret_cast<const s16x4 *>(tile + at + 4 * COLS)));
+            const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(Frag<T>, both);
+        }
+    }
+};
+
 // A tile's shape: BM x BN by WM x WN wavefronts.
 template <int BM_, int BN_, int WM_, int WN_>
 struct Shape {

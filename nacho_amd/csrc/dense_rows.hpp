@@ -39,7 +39,7 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
     }
 }
 
-// Elements to zero, 16 bytes a thread and step; `head` of them before the first aligned ones.
+// Elements to zero, 16 bytes a thread; `head` of them before the first aligned ones.
 constexpr int kClearThreads = 256;
 
 template <typename T>
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kClearThreads) void clear_kernel(T *__restrict__ p,
     const int64_t all = gridDim.x * static_cast<int64_t>(kClearThreads);
     const u32x4 zero{0u, 0u, 0u, 0u};
     for (int64_t i = at; i < whole; i += all) {
-        __builtin_nontemporal_store(zero, reinterpret_cast<u32x4 *>(p + head) + i);
+        reinterpret_cast<u32x4 *>(p + head)[i] = zero;
     }
     if (at < head) p[at] = static_cast<T>(0.0f);
     if (at < n - head - whole * kN) p[head + whole * kN + at] = static_cast<T>(0.0f);
@@ -76,7 +76,8 @@ template <typename T>
 int clear(hipStream_t stream, T *p, int64_t n) {
     const int64_t bytes = n * static_cast<int64_t>(sizeof(T)), per = 16 * kClearThreads;
     const int64_t groups = (bytes + per - 1) / per;
-    const unsigned grid = static_cast<unsigned>(groups < 1 ? 1 : groups < 8192 ? groups : 8192);
+    const unsigned grid =
+        static_cast<unsigned>(groups < 1 ? 1 : groups < kMostGroups ? groups : kMostGroups);
     clear_kernel<T><<<grid, kClearThreads, 0, stream>>>(p, n);
     NACHO_TRY_HIP(hipGetLastError());
     return NACHO_OK;

@@ -141,7 +141,7 @@ struct Clear {
         const int64_t all = (gridDim.x - first) * static_cast<int64_t>(blockDim.x);
         for (int64_t i = from + (blockIdx.x - first) * static_cast<int64_t>(blockDim.x) +
                          threadIdx.x; i < to; i += all) {
-            __builtin_nontemporal_store(zero, pieces + i);
+            pieces[i] = zero;
         }
         if (from == 0 && blockIdx.x == first) {
 #pragma unroll
@@ -612,8 +612,10 @@ int sort_tokens(Call &call, const Ids &ids, int tokens, const Cleared &all, int 
     auto share = [&](unsigned groups, int threads, int i, int n, unsigned *grid) {
         const Clear c{all.pieces, all.n * i / n, all.n * (i + 1) / n, groups,
                       {all.ends[0], all.ends[1]}, {all.in_ends[0], all.in_ends[1]}};
-        const int64_t want = (c.to - c.from + threads * 4 - 1) / (threads * 4);
-        const int64_t most = 2048 * 256 / threads;
+        // (16 bytes a thread: 1.5 GB of zeros take 216 us so, and 290 us with as many workgroups as
+        // run at a time)
+        const int64_t want = (c.to - c.from + threads - 1) / threads;
+        const int64_t most = dense::kMostGroups * 256 / threads - groups;
         *grid = groups + static_cast<unsigned>(want < 1 ? 1 : want < most ? want : most);
         return c;
     };

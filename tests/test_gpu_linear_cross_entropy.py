@@ -12,7 +12,8 @@ TYPES = (torch.float32, torch.float16, torch.bfloat16)
 # tokens, words, width
 SIZES = [(1, 1, 1), (1, 5, 8), (2, 1, 64), (3, 100, 64), (16, 257, 72), (17, 300, 40),
          (65, 513, 136), (128, 256, 64), (129, 700, 264), (300, 1000, 104), (700, 2300, 520),
-         (450, 300, 776), (321, 66000, 24), (1100, 1025, 328), (260, 20, 1032)]
+         (450, 300, 776), (321, 66000, 24), (1100, 1025, 328), (260, 20, 1032), (180, 600, 192),
+         (3000, 300, 72), (9000, 1000, 40), (20000, 50, 16), (600, 700, 333)]
 
 
 def _operands(gpu, seed, tokens, words, width, dtype, left=0.2, ids=torch.int64, lean=4.0):

@@ -1199,8 +1199,10 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
     });
 }
 
-// Bytes of a piece's dz, about, and its least words.
-constexpr int64_t kPieceBytes = int64_t{256} << 20;
+// Bytes of a piece's dz, about, and its least words.  (8192 tokens of 131072 words of 2048, us a step:
+// 128 MB 15,407, 256 MB 15,642, which no longer stays in the cache that the dies share; 64 MB has too
+// few tiles a launch.)
+constexpr int64_t kPieceBytes = int64_t{128} << 20;
 constexpr int64_t kPieceWords = 2048;
 int backward(const Args &a, const float *stats, const float *dloss, void *dx, void *dtable,
              void *stream, const nacho_allocator *alloc) {
@@ -1249,6 +1251,10 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             const int64_t deep = up(a.tokens, 512) / 512;  // (splits are 8 steps or more)
             d.most_parts = kMostItems / tiles < deep ? kMostItems / tiles : deep;
             if (d.most_parts > kMostSplits) d.most_parts = kMostSplits;
+            // (dx's products are as many: with both, or enough of one, no split is worth its while)
+            const int64_t full = up(piece, 256) / 256 * (a.width > 64 ? a.width : 64) / 256;
+            const bool both = kBN == 256 && dx && dtable;
+            if (full * (both ? 2 : 1) * 3 >= 4 * kUnits) d.most_parts = 1;
             if (kBN < 256 || d.most_parts < 2) d.most_parts = 1;
             if (dtable && d.most_parts > 1) {
                 wanted.add(&d.parts, d.most_parts * piece * d.sums_stride);
@@ -1272,7 +1278,6 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             d.width = a.width;
             d.piece = piece;
             d.common = ops.held.common;
-            const bool both = kBN == 256 && dx && dtable;
             for (int64_t v = 0; v < a.words; v += piece) {
                 const int64_t words = a.words - v < piece ? a.words - v : piece;
                 l.first = static_cast<int>(v);

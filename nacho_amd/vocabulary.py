@@ -73,7 +73,7 @@ class _Embedding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
-        return gpu_embedding_backward(dout, ids, *ctx.how), None, None
+        return _call("embedding_backward", dout.device, dout, ids, *ctx.how), None, None
 
 
 def gpu_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:

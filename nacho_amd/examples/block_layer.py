@@ -1,5 +1,6 @@
 """One layer of a language model on computed sparsity: attention over selected blocks of keys, and
-experts that tokens are routed to.  Trains on a synthetic task, then decodes with a cache.
+experts that tokens are routed to, between an embedding and a loss over the vocabulary.  Trains on a
+synthetic task, its gradients clipped, then decodes with a cache.
 
     python -m nacho_amd.examples.block_layer [--steps 160]
 
@@ -77,14 +78,25 @@ class Layer(nn.Module):
         self.norms = nn.ModuleList(nn.LayerNorm(dim) for _ in range(3))
         self.head = nn.Linear(dim, words, bias=False)
 
+    def rows(self, tokens, places):
+        return nacho_amd.gpu_embedding(tokens, self.words.weight) + places
+
     def rest(self, x, attended):
         x = x + attended
         x = x + self.experts(self.norms[1](x))
-        return self.head(self.norms[2](x))
+        return self.norms[2](x)
+
+    def hidden(self, tokens, places):
+        x = self.rows(tokens, places[:tokens.shape[1]])
+        return self.rest(x, self.attention(self.norms[0](x)))
 
     def forward(self, tokens, places):
-        x = self.words(tokens) + places[:tokens.shape[1]]
-        return self.rest(x, self.attention(self.norms[0](x)))
+        return self.head(self.hidden(tokens, places))
+
+    def loss(self, tokens, places, wanted):
+        """The mean loss of the tokens whose wanted word is one; the logits are never in memory."""
+        return nacho_amd.gpu_linear_cross_entropy(self.hidden(tokens, places), self.head.weight,
+                                                  wanted)
 
 
 class Cache:
@@ -101,7 +113,7 @@ class Cache:
 def decode(layer, cache, token, place):
     """Logits of one more token of each sequence, [batch, 1, words]."""
     attention = layer.attention
-    x = layer.words(token) + place
+    x = layer.rows(token, place)
     q, k, v = attention.project(layer.norms[0](x))
     at = int(cache.lengths[0])
     cache.k[:, at], cache.v[:, at] = k[:, 0], v[:, 0]
@@ -111,7 +123,8 @@ def decode(layer, cache, token, place):
     mine = cache.k[:, first:first + attention.block]
     cache.means[:, at // attention.block] = nacho_amd.gpu_block_means(
         mine, attention.block, cache.lengths - first)[:, 0]
-    return layer.rest(x, attention.attend(q, cache.k, cache.v, cache.means, cache.lengths))
+    return layer.head(layer.rest(x, attention.attend(q, cache.k, cache.v, cache.means,
+                                                     cache.lengths)))
 
 
 def main(argv=None):
@@ -130,15 +143,17 @@ def main(argv=None):
     def sequences():
         said = torch.randint(1, words, (batch, phrase), device=device)
         blanks = torch.zeros(batch, length - phrase, dtype=torch.long, device=device)
-        return torch.cat((said, blanks), 1), said.repeat(1, length // phrase)
+        wanted = said.repeat(1, length // phrase)
+        wanted[:, :phrase] = -1  # what is said first has no target
+        return torch.cat((said, blanks), 1), wanted
 
     losses = []
     for step in range(args.steps):
         tokens, wanted = sequences()
-        logits = layer(tokens, places)
-        loss = F.cross_entropy(logits[:, phrase:].flatten(0, 1), wanted[:, phrase:].flatten())
+        loss = layer.loss(tokens, places, wanted)
         optimiser.zero_grad()
         loss.backward()
+        nacho_amd.gpu_clip_grad_norm([p.grad for p in layer.parameters()], 1.0)
         optimiser.step()
         losses.append(float(loss.detach()))
         if step % 20 == 0 or step + 1 == args.steps:

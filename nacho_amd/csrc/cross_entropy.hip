@@ -19,6 +19,10 @@
 // gradients' products in the rows' type, without c's size: mean and sum have the factor c in
 // common, which the results are multiplied by in float32, and else the largest |c| is taken out.
 // float16 takes 2^14 dz: probabilities down to 2^-28 keep their bits, and below 2^-38 add nothing.
+// Up to kPartsMost tokens of 16 bits have dz in two parts, a row for what the first has rounded away
+// behind all first ones and the gathered rows a second time with it: with few tokens the results
+// have little else to average a rounding of dz with (a single token's gradient of its target's row
+// was up to 0.004 of it off in bfloat16, of which its own rounding is 0.0017).
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -107,7 +111,7 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
                 held.target[at] = id[i];
                 if (dloss && reduction == kNone) {
                     const float c = fabsf(dloss[t]);
-                    most = most < c || c != c ? c : most;  // (no number stays)
+                    most = c < dense::kInf ? fmaxf(most, c) : most;
                 }
                 ++at;
             }
@@ -122,24 +126,20 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
     if (reduction == kNone) {
 #pragma unroll
         for (int off = dev::kWave / 2; off > 0; off >>= 1) {
-            const float other = __shfl_xor(most, off, dev::kWave);
-            most = most < other || other != other ? other : most;
+            most = fmaxf(most, __shfl_xor(most, off, dev::kWave));
         }
         if (dev::lane() == 0) s_max[threadIdx.x / dev::kWave] = most;
         __syncthreads();
-        for (int w = 0; w < kListThreads / dev::kWave; ++w) {
-            const float other = s_max[w];
-            common = common < other || other != other ? other : common;
-        }
+        for (int w = 0; w < kListThreads / dev::kWave; ++w) common = fmaxf(common, s_max[w]);
+        if (common == 0.0f) common = 1.0f;
     } else {
         common = reduction == kMean ? dloss[0] / static_cast<float>(max(carry, 1)) : dloss[0];
     }
-    if (reduction == kNone && !(common < dense::kInf)) common = 1.0f;
     if (threadIdx.x == 0) *held.common = common;
     if (reduction != kNone) return;
     for (int64_t t = threadIdx.x; t < tokens; t += kListThreads) {
         const int id = targets(t);
-        if (id >= 0) held.factor[held.slot[t]] = common == 0.0f ? 0.0f : dloss[t] / common;
+        if (id >= 0) held.factor[held.slot[t]] = dloss[t] / common;
     }
 }
 
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
                                                              int64_t padded,
                                                              const T *__restrict__ from,
                                                              int64_t stride, T *__restrict__ to,
-                                                             int64_t to_stride) {
+                                                             int64_t to_stride, int copies) {
     constexpr int kWaves = kThreads / dev::kWave, kStep = 8;
     __shared__ int s_before[kWaves], s_all[kWaves], s_token[kListRows];
     __shared__ float s_most[kWaves];
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
             if (id[s] >= 0) {
                 ++all;
                 before += t < first ? 1 : 0;
-                most = most < c[s] || c[s] != c[s] ? c[s] : most;  // (no number stays)
+                most = c[s] < dense::kInf ? fmaxf(most, c[s]) : most;
             }
         }
     }
@@ -230,8 +230,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
     all = dev::wave_sum(all);
 #pragma unroll
     for (int off = dev::kWave / 2; off > 0; off >>= 1) {
-        const float other = __shfl_xor(most, off, dev::kWave);
-        most = most < other || other != other ? other : most;
+        most = fmaxf(most, __shfl_xor(most, off, dev::kWave));
     }
     if (lane == 0) {
         s_before[wave] = before;
@@ -244,10 +243,10 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
     for (int w = 0; w < kWaves; ++w) {
         before += s_before[w];
         all += s_all[w];
-        common = common < s_most[w] || s_most[w] != s_most[w] ? s_most[w] : common;
+        common = fmaxf(common, s_most[w]);
     }
     if (each) {
-        if (!(common < dense::kInf)) common = 1.0f;
+        if (common == 0.0f) common = 1.0f;
     } else if (dloss) {
         common = reduction == kMean ? dloss[0] / static_cast<float>(max(all, 1)) : dloss[0];
     }
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
         if (id >= 0) {
             held.token[at] = t;
             held.target[at] = id;
-            if (each) held.factor[at] = common == 0.0f ? 0.0f : dloss[t] / common;
+            if (each) held.factor[at] = dloss[t] / common;
         }
         if (lane < kListRows) s_token[lane] = id >= 0 ? at : -1;
     }
@@ -274,8 +273,10 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
     for (int i = wave; i < kListRows; i += kWaves) {
         const int at = s_token[i];
         if (at >= 0) {
-            copy_row<T, dev::kWave>(from + (first + i) * stride, width, to + at * to_stride, padded,
-                                    lane);
+            for (int c = 0; c < copies; ++c) {
+                copy_row<T, dev::kWave>(from + (first + i) * stride, width,
+                                        to + (c * all + at) * to_stride, padded, lane);
+            }
         }
     }
 }
@@ -329,7 +330,8 @@ struct Logits {
     const float *total;    // s
     const int *token;
     const float *factor;   // null: 1
-    void *dz;              // [held][dz_stride]
+    int copies;            // parts of dz, 1 or 2
+    void *dz;              // [copies][held][dz_stride]
     int64_t dz_stride;     // at least the piece's tiles: words past the piece's get zeros
 };
 
@@ -665,7 +667,20 @@ __device__ __forceinline__ void tile_dz(const Logits &a, int64_t v0, int64_t n0,
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[j] = v0 + v + j < a.words ? d[j] : 0.0f;
             }
-            if (n < held) dense::store4<T>(to + v, d);
+            if (n >= held) continue;
+            dense::store4<T>(to + v, d);
+            if constexpr (sizeof(T) == 2) {
+                if (a.copies == 2) {
+                    f32x4 rest;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        rest[j] = d[j] - static_cast<float>(static_cast<T>(d[j]));
+                        // (of an infinity or what is no number: nothing)
+                        if (rest[j] != rest[j]) rest[j] = 0.0f;
+                    }
+                    dense::store4<T>(to + held * a.dz_stride + v, rest);
+                }
+            }
         }
     }
 }
@@ -683,6 +698,7 @@ __global__ __launch_bounds__((Tile<BM, BN>::kThreads)) void dz_kernel(Logits a) 
 
 struct Gradients {
     const int *held;
+    int copies;           // of dz and the rows: as many tokens as held times copies
     const void *dz;
     int64_t dz_stride;
     const void *rows;     // gathered
@@ -693,7 +709,7 @@ struct Gradients {
     int64_t rows_stride;
     int64_t piece;        // words of a whole piece
     int64_t most_rows;    // that the sums have room for, at least all tokens
-    float *sums;          // [split][held][sums_stride]; null: no dx
+    float *sums;          // [split][copies][held][sums_stride]; null: no dx
     int64_t sums_stride;
     int first;            // whether the piece is the first
     int64_t most_parts;   // splits that `parts` has room for; 1 without it
@@ -718,6 +734,13 @@ struct Splits {
 
 constexpr unsigned kMostItems = 512, kMostSplits = 64;
 
+// Tenths of a tile of 256 columns that the width takes: one at the end, of 64 or of 128 columns, takes
+// 0.4 or 0.6 as long as a whole one.
+__device__ __host__ __forceinline__ int64_t tenths_of(int64_t width) {
+    const int64_t rest = width % 256;
+    return width / 256 * 10 + (rest == 0 ? 0 : rest <= 64 ? 4 : rest <= 128 ? 6 : 10);
+}
+
 // n rows by the width, over `depth`, in whole steps, of a load of `load` steps; most: splits that
 // the sums have room for.
 __device__ __forceinline__ Splits split_up(int64_t n, int bn, int64_t width, int64_t depth,
@@ -730,8 +753,8 @@ __device__ __forceinline__ Splits split_up(int64_t n, int bn, int64_t width, int
     const int64_t per = wanted < 8 ? 8 : wanted;
     int64_t k = (steps + per - 1) / per;
     // (a few more make a round of all units: 2048 tokens of 16384 words 1290 us instead of 1380)
-    const int64_t round = 256 * static_cast<int64_t>(kUnits) /
-                          max(s.n_tiles * max(width, int64_t{64}), int64_t{1});
+    const int64_t round = 10 * static_cast<int64_t>(kUnits) /
+                          max(s.n_tiles * tenths_of(width), int64_t{1});
     if (k > 1 && k < round && 2 * round <= 3 * k) k = round;
     k = min(k, static_cast<int64_t>(kMostItems) / max(static_cast<int64_t>(s.tiles()), int64_t{1}));
     k = max(min(min(k, static_cast<int64_t>(kMostSplits)), most), int64_t{1});
@@ -740,13 +763,13 @@ __device__ __forceinline__ Splits split_up(int64_t n, int bn, int64_t width, int
     return s;
 }
 
-// The steps of dx's and of dtable's products, those of tiles of fewer columns in proportion.
+// The steps of dx's and of dtable's products, in those of whole tiles.
 template <typename T, int BN>
 __device__ __forceinline__ int64_t load_of(const Gradients &a, int held, bool dx, bool dtable) {
     constexpr int kStep = dense::kStepK<T>, kBN = BN <= 64 ? 64 : BN;
     const int64_t x = (held + BN - 1) / BN * ((a.piece + kStep - 1) / kStep);
     const int64_t t = (a.piece + kBN - 1) / kBN * ((held + kStep - 1) / kStep);
-    return ((dx ? x : 0) + (dtable ? t : 0)) * max(a.width, int64_t{64}) / 256;
+    return ((dx ? x : 0) + (dtable ? t : 0)) * tenths_of(a.width) / 10;
 }
 
 template <typename T, int BN>
@@ -857,7 +880,7 @@ __global__ __launch_bounds__(kTileThreads) void gradients_kernel(Gradients a) {
     constexpr int kLdsX = DX ? kLds<T, 256, BN, Across, Along> : 0;
     constexpr int kLdsT = DTABLE ? kLds<T, 256, (BN <= 64 ? 64 : BN), Across, Across> : 0;
     __shared__ __attribute__((aligned(16))) T lds[kLdsX > kLdsT ? kLdsX : kLdsT];
-    const int held = *a.held;
+    const int held = *a.held * a.copies;
     const int64_t load = load_of<T, BN>(a, held, DX, DTABLE);
     unsigned at = blockIdx.x, mt = 0, nt = 0;
     if constexpr (DX) {
@@ -917,7 +940,7 @@ __device__ __forceinline__ f32x4 splits_sum(const float *from, int64_t stride, u
 // dtable of a piece whose products were split: the splits' sums in their order.
 template <typename T, int BN>
 __global__ __launch_bounds__(kThreads) void dtable_join_kernel(Gradients a, bool both) {
-    const int held = *a.held;
+    const int held = *a.held * a.copies;
     const unsigned splits =
         dtable_splits<T, BN>(a, held, load_of<T, BN>(a, held, both, true)).count;
     if (splits == 1) return;
@@ -940,7 +963,7 @@ __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
                                                            const int *__restrict__ slot,
                                                            int64_t tokens, bool both,
                                                            T *__restrict__ dx) {
-    const int held = *a.held;
+    const int held = *a.held * a.copies;
     const unsigned splits = dx_splits<T, BN>(a, held, load_of<T, BN>(a, held, true, both)).count;
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
     constexpr int kPer = kThreads / LANES;
@@ -951,7 +974,11 @@ __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
         for (int64_t d = 4ll * (threadIdx.x % LANES); d < a.width; d += 4 * LANES) {
             f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
             if (at >= 0) {
-                sum = splits_sum(a.sums + at * a.sums_stride + d, held * a.sums_stride, splits);
+                const float *from = a.sums + at * a.sums_stride + d;
+                sum = splits_sum(from, held * a.sums_stride, splits);
+                if (a.copies == 2) {
+                    sum += splits_sum(from + held / 2 * a.sums_stride, held * a.sums_stride, splits);
+                }
                 sum *= factor;
             }
             store_row4<T>(dx + t * a.width, d, a.width, sum);
@@ -1029,6 +1056,9 @@ struct Wanted {
     }
 };
 
+// (within kListMost)
+constexpr int64_t kPartsMost = 128;
+
 // The operands as the kernels take them: rows gathered and, where a table's rows are not whole
 // aligned pieces, a copy of it whose are.
 template <typename T>
@@ -1041,6 +1071,7 @@ struct Operands {
     int64_t rows_stride = 0;
     int64_t table_stride = 0;
     bool copied = false;
+    int copies = 1;  // of the rows
 
     // (256 rows of a tile within the loads' 2 GB)
     static constexpr int64_t kMostStride = int64_t{1} << 22;
@@ -1054,7 +1085,8 @@ struct Operands {
         wanted.add(&held.target, a.tokens);
         if (dloss) wanted.add(&held.common, 1);
         if (dloss && a.reduction == NACHO_LOSS_NONE) wanted.add(&held.factor, a.tokens);
-        wanted.add(&rows, a.tokens * rows_stride);
+        if (dloss && sizeof(T) == 2 && a.tokens <= kPartsMost) copies = 2;
+        wanted.add(&rows, copies * a.tokens * rows_stride);
         table = static_cast<const T *>(a.table);
         table_stride = a.table_stride;
         copied = !dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
@@ -1072,7 +1104,7 @@ struct Operands {
         if (tokens <= kListMost) {
             list_rows_kernel<T><<<ceil_div(static_cast<size_t>(tokens), kListRows), kThreads, 0,
                                   s>>>(targets, tokens, a.reduction, dloss, held, a.width, width,
-                                       x, a.x_stride, rows, rows_stride);
+                                       x, a.x_stride, rows, rows_stride, copies);
             NACHO_TRY_HIP(hipGetLastError());
         } else {
             list_kernel<<<1, kListThreads, 0, s>>>(targets, tokens, a.reduction, dloss, held);
@@ -1120,6 +1152,19 @@ int with_shape(int64_t tokens, int64_t words, F f) {
     }
     if (tiles(256) < kUnits) return f(Number<128>{}, Number<256>{});
     return f(Number<256>{}, Number<256>{});
+}
+
+// The same, and the columns of the gradients' tiles.
+template <typename F>
+int with_shapes(int64_t tokens, int copies, int64_t words, F f) {
+    return with_shape(tokens, words, [&](auto bm, auto bn) -> int {
+        if constexpr (bn() == 16) {
+            if (tokens * copies <= 16) return f(bm, bn, Number<16>{});
+            return f(bm, bn, Number<64>{});
+        } else {
+            return f(bm, bn, bn);
+        }
+    });
 }
 
 template <typename F>
@@ -1199,11 +1244,21 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
     });
 }
 
-// Bytes of a piece's dz, about, and its least words.  (8192 tokens of 131072 words of 2048, us a step:
-// 128 MB 15,407, 256 MB 15,642, which no longer stays in the cache that the dies share; 64 MB has too
-// few tiles a launch.)
+// Words of a piece whose dz has `bytes` a word: all where that is little, or equal pieces that stay in
+// the cache that the dies share.  (8192 tokens of 131072 words of 2048, us a step with pieces of 128
+// MB 15,407, of 256 MB 15,642, of 64 MB, with too few tiles a launch, 16,900; 3001 of 32003 words of
+// 776, 192 MB, in one piece 440, in one of 128 MB and a rest 589.)
 constexpr int64_t kPieceBytes = int64_t{128} << 20;
 constexpr int64_t kPieceWords = 2048;
+
+int64_t piece_of(int64_t words, int64_t bytes) {
+    const int64_t all = up(words, 256);
+    if (all * bytes <= 2 * kPieceBytes) return all;
+    const int64_t pieces = (all * bytes + kPieceBytes - 1) / kPieceBytes;
+    const int64_t piece = up((words + pieces - 1) / pieces, 256);
+    return piece < kPieceWords ? (kPieceWords < all ? kPieceWords : all) : piece;
+}
+
 int backward(const Args &a, const float *stats, const float *dloss, void *dx, void *dtable,
              void *stream, const nacho_allocator *alloc) {
     NACHO_TRY(check(a));
@@ -1220,14 +1275,15 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
         if (a.tokens == 0) {
             return dense::clear(s, static_cast<T *>(dtable), a.words * a.width);
         }
-        return with_shape(a.tokens, a.words, [&](auto bm, auto bn) -> int {
-            constexpr int kBM = bm(), kBN = bn();
-            int64_t piece = up(kPieceBytes / (a.tokens * item), 256);
-            if (piece < kPieceWords) piece = kPieceWords;
-            if (piece > up(a.words, 256)) piece = up(a.words, 256);
-            const int64_t cut = kBN == 256 ? kUnits : 0;
-            const unsigned dx_groups = groups_of(a.width, 256, a.tokens, kBN, kMostItems);
-            if (!groups_of(piece, kBM, a.tokens, kBN, cut) || !dx_groups ||
+        const int copies = sizeof(T) == 2 && a.tokens <= kPartsMost ? 2 : 1;
+        return with_shapes(a.tokens, copies, a.words, [&](auto bm, auto tokens, auto bn) -> int {
+            // of the logits' tiles, and of the gradients'
+            constexpr int kBM = bm(), kTokens = tokens(), kBN = bn();
+            const int64_t piece = piece_of(a.words, a.tokens * copies * item);
+            const int64_t cut = kTokens == 256 ? kUnits : 0;
+            const int64_t columns = a.tokens * copies;
+            const unsigned dx_groups = groups_of(a.width, 256, columns, kBN, kMostItems);
+            if (!groups_of(piece, kBM, a.tokens, kTokens, cut) || !dx_groups ||
                 !groups_of(a.width, 256, piece, 64, dx_groups + kMostItems)) {
                 return NACHO_ERR_INDEX_OVERFLOW;
             }
@@ -1238,21 +1294,21 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             T *dz = nullptr;
             ops.want(wanted, a, dloss);
             l.dz_stride = d.dz_stride = scratch_stride<T>(piece);
-            wanted.add(&dz, a.tokens * l.dz_stride);
+            wanted.add(&dz, columns * l.dz_stride);
             d.sums_stride = up(a.width, 4);
             // Room for the sums of as many splits as are made: tiles of 256 columns by kBN tokens,
             // at most kMostItems of them where they are split; the same for dtable.
             const int64_t m_tiles = up(a.width, 256) / 256;
             const int64_t most = kMostItems / m_tiles * kBN;
-            d.most_rows = a.tokens * kMostSplits < most ? a.tokens * kMostSplits : most;
-            if (d.most_rows < a.tokens) d.most_rows = a.tokens;
+            d.most_rows = columns * kMostSplits < most ? columns * kMostSplits : most;
+            if (d.most_rows < columns) d.most_rows = columns;
             if (dx) wanted.add(&d.sums, d.most_rows * d.sums_stride);
             const int64_t tiles = m_tiles * (up(piece, 256) / 256);
             const int64_t deep = up(a.tokens, 512) / 512;  // (splits are 8 steps or more)
             d.most_parts = kMostItems / tiles < deep ? kMostItems / tiles : deep;
             if (d.most_parts > kMostSplits) d.most_parts = kMostSplits;
             // (dx's products are as many: with both, or enough of one, no split is worth its while)
-            const int64_t full = up(piece, 256) / 256 * (a.width > 64 ? a.width : 64) / 256;
+            const int64_t full = up(piece, 256) / 256 * tenths_of(a.width) / 10;
             const bool both = kBN == 256 && dx && dtable;
             if (full * (both ? 2 : 1) * 3 >= 4 * kUnits) d.most_parts = 1;
             if (kBN < 256 || d.most_parts < 2) d.most_parts = 1;
@@ -1262,6 +1318,7 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             NACHO_TRY(wanted.get(call));
             NACHO_TRY(ops.start(s, a, dloss));
             l.held = d.held = ops.held.count;
+            l.copies = d.copies = copies;
             l.width = d.padded = ops.width;
             l.rows = d.rows = ops.rows;
             l.rows_stride = d.rows_stride = ops.rows_stride;
@@ -1282,8 +1339,8 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
                 const int64_t words = a.words - v < piece ? a.words - v : piece;
                 l.first = static_cast<int>(v);
                 l.words = static_cast<int>(words);
-                dz_kernel<T, kBM, kBN><<<groups_of(words, kBM, a.tokens, kBN, cut),
-                                         Tile<kBM, kBN>::kThreads, 0, s>>>(l);
+                dz_kernel<T, kBM, kTokens><<<groups_of(words, kBM, a.tokens, kTokens, cut),
+                                             Tile<kBM, kTokens>::kThreads, 0, s>>>(l);
                 NACHO_TRY_HIP(hipGetLastError());
                 d.words = words;
                 d.table = ops.table + v * ops.table_stride;

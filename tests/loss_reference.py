@@ -3,7 +3,8 @@ float32 sums and operands of 16 bits may be off.
 
 Bounds: u is the unit roundoff of the operands' type (2^-24, 2^-11, 2^-8) and e = 2^-24.  A sum of n
 float32 products is within n e of the sum of their magnitudes whatever its order.  A gradient's
-products take dz rounded to the operands' type (u), and results are rounded once (u).
+products take dz rounded to the operands' type (u), 16-bit ones of up to 128 tokens in two parts
+(u^2), and results are rounded once (u).
 """
 
 import torch
@@ -59,12 +60,13 @@ class Loss:
         c = torch.where(held, c, 0.0)[:, None]
         one = torch.zeros_like(p).scatter_(1, at, 1.0)
         dz = (p - one) * c
+        dz_u = u * u if len(x) <= 128 and x.dtype != torch.float32 else u
         off = (p * (pe + total_e) + 2 * E * one + 4 * E * (p - one).abs() +
-               u * (p - one).abs()) * c.abs() + DZ_TINY[x.dtype] * c.abs().amax()
+               dz_u * (p - one).abs()) * c.abs() + DZ_TINY[x.dtype] * c.abs().amax()
         s = abs(f32)
         dx, dtable = dz @ w * f32, dz.T @ wide * f32
-        dx_off = s * (off @ w.abs() + (words + 4) * E * (dz.abs() @ w.abs()))
-        dtable_off = s * (off.T @ wide.abs() + (n + 4) * E * (dz.abs().T @ wide.abs()))
+        dx_off = s * (off @ w.abs() + (words + 8) * E * (dz.abs() @ w.abs()))
+        dtable_off = s * (off.T @ wide.abs() + (2 * n + 4) * E * (dz.abs().T @ wide.abs()))
         self.dx, self.dx_off = dx.view(shape), (dx_off + u * dx.abs() + tiny).view(shape)
         self.dtable, self.dtable_off = dtable, dtable_off + u * dtable.abs() + tiny
 

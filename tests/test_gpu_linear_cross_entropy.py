@@ -225,6 +225,24 @@ def test_float32_of_all_sizes(gpu, size):
     near(dtable / size, want.dtable, want.dtable_off, "dtable")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_of_losses_that_are_not_finite(gpu, dtype):
+    """They reach their own token's dx and the whole dtable, and no other token's dx."""
+    x, table, targets = _operands(gpu, 29, 50, 300, 64, dtype, left=0.0)
+    stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, reduction="none",
+                                               return_stats=True)[1]
+    dloss = 1000.0 * torch.rand(50, device=gpu) + 1.0
+    want = Loss(x, table, targets, reduction="none", dloss=dloss)
+    for value in (float("inf"), float("nan")):
+        c = dloss.clone()
+        c[9] = value
+        dx, dtable = nacho_amd.gpu_linear_cross_entropy_backward(c, x, table, targets, stats,
+                                                                 reduction="none")
+        keep = torch.arange(50, device=gpu) != 9
+        near(dx[keep], want.dx[keep], want.dx_off[keep], "dx")
+        assert not torch.isfinite(dx[9]).any() and not torch.isfinite(dtable[targets[9]]).any()
+
+
 def test_words_of_minus_infinity(gpu):
     """A word whose logits are all minus infinity has probability 0."""
     x = torch.ones(20, 32, device=gpu)

@@ -959,6 +959,8 @@ PyObject *clip_grad_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
         for (size_t i = 0; i < outs.size(); ++i) {
             at::Tensor &t = tensors[i];
             const at::Tensor &out = outs[i];
+            // (a leaf that requires a gradient is a parameter, not one's gradient)
+            need(!(out.requires_grad() && out.is_leaf()));
             need(out.is_non_overlapping_and_dense() && out.sizes() == t.sizes() &&
                  (out.scalar_type() == t.scalar_type() || out.scalar_type() == at::kFloat));
             if (t.strides() != out.strides()) {  // elements in out's order

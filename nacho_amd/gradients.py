@@ -64,8 +64,9 @@ def gpu_grad_norm(tensors) -> torch.Tensor:
 
 
 def gpu_clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
-    """Scale tensors so that their common norm is at most max_norm, and give the norm that they
-    had (float32, on the device): every element times min(1, max_norm / (norm + 1e-6)).
+    """Scale tensors (gradients, not the parameters that have them) so that their common norm is at
+    most max_norm, and give the norm that they had (float32, on the device): every element times
+    min(1, max_norm / (norm + 1e-6)).
 
     In place, or into the tensors of `out`, of the same shapes, each of its tensor's type or
     float32 (as an optimiser's own copies are).  A tensor that is written has to have its elements
@@ -92,6 +93,11 @@ def gpu_clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
 
 def _refuse_clip(tensors, outs, device, in_place):
     _check(tensors, "tensors", device)
+    name = "tensors" if in_place else "out"
+    for i, o in enumerate(outs):
+        if o is not None and o.requires_grad and o.is_leaf:
+            raise ValueError(f"{name}[{i}] is a leaf that requires a gradient: expected the "
+                             "gradients (parameter.grad), not the parameters")
     for i, (t, o) in enumerate(zip(tensors, outs)):
         if t is None or (in_place and _dense(t)):
             continue

@@ -196,6 +196,10 @@ def test_refusals(gpu):
             (lambda: f([a], -1.0), ValueError, "max_norm"),
             (lambda: f([a], math.nan), ValueError, "max_norm"),
             (lambda: f([a], 1e39), ValueError, "max_norm"),
+            (lambda: f([a, torch.ones(3, device=gpu, requires_grad=True)], 1.0), ValueError,
+             "not the parameters"),
+            (lambda: f([a], 1.0, out=[a.clone().requires_grad_()]), ValueError,
+             "not the parameters"),
             (lambda: f([a, a], 1.0), ValueError, "share memory"),
             (lambda: f([a, a[3:7]], 1.0), ValueError, "share memory"),
             (lambda: f([a[:90], b], 1.0, out=[a[10:], b]), ValueError, "share memory"),

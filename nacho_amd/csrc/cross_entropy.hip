@@ -536,7 +536,7 @@ __device__ __forceinline__ void join_token(const float2 *__restrict__ from, unsi
 
 // A wavefront per token; with `sum`, for up to kJoinMost tokens, also the sum of the losses or (mean)
 // their mean.  (What makes the losses of all workgroups visible to the last costs each of them:
-// 5 us less than two launches for 64 tokens, 60 us more for 3000.)
+// 5 us less than two launches for 64 tokens, 49 us more for 3001.)
 constexpr int64_t kJoinMost = 64;
 
 __global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ slot,
@@ -752,7 +752,7 @@ __device__ __forceinline__ Splits split_up(int64_t n, int bn, int64_t width, int
     const int64_t wanted = load * 3 / (4 * static_cast<int64_t>(kUnits));
     const int64_t per = wanted < 8 ? 8 : wanted;
     int64_t k = (steps + per - 1) / per;
-    // (a few more make a round of all units: 2048 tokens of 16384 words 1290 us instead of 1380)
+    // (a few more make a round of all units: a step of 2048 tokens of 16384 words 1287 us instead of 1350)
     const int64_t round = 10 * static_cast<int64_t>(kUnits) /
                           max(s.n_tiles * tenths_of(width), int64_t{1});
     if (k > 1 && k < round && 2 * round <= 3 * k) k = round;
@@ -1245,9 +1245,9 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
 }
 
 // Words of a piece whose dz has `bytes` a word: all where that is little, or equal pieces that stay in
-// the cache that the dies share.  (8192 tokens of 131072 words of 2048, us a step with pieces of 128
-// MB 15,407, of 256 MB 15,642, of 64 MB, with too few tiles a launch, 16,900; 3001 of 32003 words of
-// 776, 192 MB, in one piece 440, in one of 128 MB and a rest 589.)
+// the cache that the dies share.  (8192 tokens of 131072 words of 2048, us a step with pieces of 64 MB,
+// which have too few tiles a launch, 16,550, of 128 MB 15,050, of 256 MB 15,600, of 512 MB 15,720;
+// 3001 of 32003 words of 776, 192 MB, in one piece 440, in one of 128 MB and a rest 589.)
 constexpr int64_t kPieceBytes = int64_t{128} << 20;
 constexpr int64_t kPieceWords = 2048;
 

@@ -544,7 +544,7 @@ int check(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float sca
 }
 
 // Calls f with the element type and the elements of a piece.  (In us with pieces of 16 bytes and of
-// one element: 30001 rows of 333 float32, lookup 8 and 12, sums 12 and 20.)
+// one element: 30001 rows of 333 float32, lookup 11 and 12, sums 14 and 20.)
 template <typename F>
 int with_type(int32_t dtype, int64_t width, F f) {
     auto typed = [&](auto type) {

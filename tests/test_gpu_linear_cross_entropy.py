@@ -386,3 +386,23 @@ def test_refusals(gpu):
             (lambda: b(one, x, table, targets, stats, reduction="none"), ValueError, "dloss")]:
         with pytest.raises(error, match=text):
             call()
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 16])
+def test_few_float32_tokens_sum_wide_rows_in_steps(gpu, tokens):
+    """Logits of few float32 tokens are summed over 32 columns at a time, and these sums added: for
+    D columns 32 + D / 32 roundings, each at most 2^-24 of a sum of terms of one sign.
+
+    All terms are c = 1 + 0.9 2^-13.  In one sum of all the last 8192 terms each lose 0.9 2^-13, one
+    by one or four together (sums from 2^13 on are multiples of 2^-10): 0.9 of 16386, 5.5e-5, where
+    32 + 512 roundings are at most 3.3e-5."""
+    width, scale = 16384, 2.0 ** -14
+    x = torch.ones(tokens, width, device=gpu)
+    table = torch.zeros(3, width, device=gpu)
+    table[1] = 1 + 0.9 * 2.0 ** -13
+    targets = torch.ones(tokens, dtype=torch.int64, device=gpu)
+    _, stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, scale=scale,
+                                                  return_stats=True)
+    exact = table[1].double().sum().item() * scale
+    # (the multiplication by the scale is exact)
+    assert (stats[0].double() - exact).abs().max().item() <= (32 + width // 32) * 2.0 ** -24 * exact

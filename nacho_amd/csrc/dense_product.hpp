@@ -8,6 +8,9 @@
 // multiply this one's: two buffers, one barrier a step.  Products take eight consecutive k per
 // lane (lane = 16 g + c: row or column c, k = 8 g + j); operands that lie across are read with the
 // transposing LDS read.
+//
+// Measured, bfloat16, 8028 x 131072 by 2048, matrix cores' share of the time in brackets: both operands
+// along k 1.27 PFLOP/s (60%), across k 1.07 for a mix of the two (46%, 47% of it waits).
 #pragma once
 
 #include <hip/hip_runtime.h>

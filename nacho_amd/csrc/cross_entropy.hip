@@ -550,15 +550,20 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const int *__restrict__ 
                                                         float *__restrict__ most_of,
                                                         float *__restrict__ total_of, float *each,
                                                         int *count, int mean, float *sum) {
-    const int64_t t = (blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x) / dev::kWave;
-    const int at = t < tokens ? slot[t] : -1;
-    if (t < tokens && at < 0 && dev::lane() == 0) {
-        most_of[t] = 0.0f;
-        total_of[t] = 1.0f;
-        each[t] = 0.0f;
+    constexpr int kPer = kThreads / dev::kWave;
+    int64_t t = blockIdx.x * static_cast<int64_t>(kPer) +
+                __builtin_amdgcn_readfirstlane(threadIdx.x / dev::kWave);
+    for (; t < tokens; t += gridDim.x * static_cast<int64_t>(kPer)) {
+        const int at = slot[t];
+        if (at >= 0) {
+            join_token(parts + static_cast<int64_t>(at) * tiles, tiles, mine + at, most_of + t,
+                       total_of + t, each + t);
+        } else if (dev::lane() == 0) {
+            most_of[t] = 0.0f;
+            total_of[t] = 1.0f;
+            each[t] = 0.0f;
+        }
     }
-    if (at >= 0) join_token(parts + static_cast<int64_t>(at) * tiles, tiles, mine + at,
-                            most_of + t, total_of + t, each + t);
     if (!sum) return;
     // The workgroup that finds all others done adds the losses up, in their order.
     __shared__ int s_last;
@@ -1234,7 +1239,8 @@ int forward(const Args &a, float *loss, float *stats, void *stream, const nacho_
             parts_kernel<T, bm(), bn()><<<groups, kShapeThreads, 0, s>>>(l);
             NACHO_TRY_HIP(hipGetLastError());
             const int mean = a.reduction == NACHO_LOSS_MEAN;
-            join_kernel<<<ceil_div(static_cast<size_t>(n), kThreads / dev::kWave), kThreads, 0,
+            const int64_t joins = up(n, kThreads / dev::kWave) / (kThreads / dev::kWave);
+            join_kernel<<<static_cast<unsigned>(joins < (1 << 20) ? joins : 1 << 20), kThreads, 0,
                           s>>>(ops.held.slot, static_cast<int>(n), m_tiles, parts, mine, most,
                                most + n, each, ops.held.count, mean,
                                sums && n <= kJoinMost ? loss : nullptr);

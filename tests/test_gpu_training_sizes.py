@@ -81,3 +81,48 @@ def test_loss_of_a_large_table(gpu):
     w = table.detach().double()
     off = (2 * u + 1e-4) * (dz.abs() @ w.abs())
     assert ((dx.double() - dz @ w).abs() <= off + 1e-30).all()
+
+
+def test_loss_of_more_tokens_than_a_launch_has_workgroups(gpu):
+    tokens, some, words, width = (1 << 26) + 8, 300, 5, 8  # four wavefronts of a workgroup have one each
+    g = torch.Generator(device=gpu).manual_seed(3)
+    few = torch.randn(some, width, generator=g, device=gpu).bfloat16()
+    table = torch.randn(words, width, generator=g, device=gpu).bfloat16()
+    few_targets = torch.randint(-1, words, (some,), generator=g, device=gpu)
+    # (copies: torch's index of so many rows has the same fault that is looked for here)
+    x = few.repeat(tokens // some + 1, 1)[:tokens]
+    targets = few_targets.repeat(tokens // some + 1)[:tokens]
+    assert torch.equal(x[-1], few[(tokens - 1) % some])
+    want = Loss(few, table, few_targets, reduction="none", dloss=torch.ones(some, device=gpu))
+    loss, stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, reduction="none",
+                                                     return_stats=True)
+
+    def repeated(got, right, off):
+        """Rows that come again and again, in parts of which each is the same."""
+        whole = tokens // some * some
+        got = got.reshape(tokens, -1)
+        first = got[:some]
+        near(first, right.reshape(some, -1), off.reshape(some, -1))
+        assert torch.equal(got[:whole].view(-1, some, got.shape[1]),
+                           first.expand(tokens // some, -1, -1))
+        assert torch.equal(got[whole:], first[:tokens - whole])
+
+    repeated(loss, want.each, want.each_off)
+    dloss = torch.ones(tokens, device=gpu)
+    dx, dtable = nacho_amd.gpu_linear_cross_entropy_backward(dloss, x, table, targets, stats,
+                                                             reduction="none")
+    # (dz of many tokens is rounded; this many are not in two parts)
+    u = 2.0 ** -8
+    held = (few_targets >= 0)[:, None]
+    z = few.double() @ table.double().T
+    dz = torch.softmax(z, -1).scatter_add_(1, few_targets.clamp(min=0)[:, None],
+                                           torch.full((some, 1), -1.0, device=gpu).double())
+    dz = torch.where(held, dz, 0.0)
+    repeated(dx, want.dx, want.dx_off + u * (dz.abs() @ table.double().abs()).view_as(want.dx))
+    # Tokens are summed in at most 64 splits of 2^20 and a few, the splits' sums one by one: no more
+    # than 2^20 + 1000 roundings; and dz's and the result's.
+    times = (tokens // some + (torch.arange(some, device=gpu) < tokens % some)).double()[:, None]
+    right = (dz * times).T @ few.double()
+    size = (dz.abs() * times).T @ few.double().abs()
+    off = ((1 << 20) + 1000) * 2.0 ** -24 * size + u * size + u * right.abs()
+    assert ((dtable.double() - right).abs() <= off).all()

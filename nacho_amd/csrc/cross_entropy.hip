@@ -831,12 +831,16 @@ __device__ __forceinline__ void tile_dtable(const Gradients &a, int64_t d0, int6
     const Matrix<T> rows{static_cast<const T *>(a.rows) + t0 * a.rows_stride + d0, a.rows_stride};
     const Matrix<T> dz{static_cast<const T *>(a.dz) + t0 * a.dz_stride + v0, a.dz_stride};
     f32x4 sums[S::MT][S::NT];
+    // Words up to a whole 16 bytes are zeros in dz; behind them nothing has been written (or by another
+    // piece), and a product of float32 would be worked out again for what is no number there.
+    constexpr int64_t kN = 16 / sizeof(T);
+    const int64_t there = (a.words + kN - 1) / kN * kN;
     // (few tokens are bound by the stores of the results: 8 elements together)
     using P = std::conditional_t<PAIRS, Product<T, S, AcrossPairs, Across>,
                                  Product<T, S, Across, Across>>;
     P::run(
         rows, static_cast<int>(min(a.padded - d0, static_cast<int64_t>(S::BM))), dz,
-        static_cast<int>(min(a.piece - v0, static_cast<int64_t>(S::BN))), tokens, lds, sums);
+        static_cast<int>(min(there - v0, static_cast<int64_t>(S::BN))), tokens, lds, sums);
     const float factor = *a.common * a.scale * (1.0f / kDzScale<T>);
     const int wave = threadIdx.x / dev::kWave, lane = dev::lane(), g = lane >> 4, c = lane & 15;
     const int wm = wave / S::WN, wn = wave % S::WN;

@@ -1,0 +1,53 @@
+"""Gradients of the linear cross entropy where tokens count differently; and that nothing in them comes
+from scratch memory."""
+
+import pytest
+import torch
+
+import nacho_amd
+
+pytestmark = pytest.mark.gpu
+
+HALVES = (torch.float16, torch.bfloat16)
+
+
+def _operands(gpu, seed, tokens, words, width, dtype, lean=4.0):
+    """Rows that lean towards their targets."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    normal = lambda *s: torch.randn(*s, generator=g, device=gpu)  # noqa: E731
+    table = (normal(words, width) * width ** -0.5).to(dtype)
+    targets = torch.randint(0, words, (tokens,), generator=g, device=gpu)
+    x = normal(tokens, width) + lean * torch.rand(tokens, 1, generator=g, device=gpu) * \
+        table[targets].float()
+    return x.to(dtype), table, targets
+
+
+def _gradients(x, table, targets, dloss, reduction="none", scale=1.0):
+    stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, scale=scale, reduction=reduction,
+                                               return_stats=True)[1]
+    return nacho_amd.gpu_linear_cross_entropy_backward(dloss, x, table, targets, stats,
+                                                       scale=scale, reduction=reduction)
+
+
+def _after(value, gpu, call):
+    """A call whose memory held bytes of `value` before."""
+    pool = torch.cuda.MemPool()
+    with torch.cuda.use_mem_pool(pool):
+        block = torch.full((1 << 28,), value, dtype=torch.uint8, device=gpu)
+        del block
+        got = [t.cpu() for t in call()]
+    torch.cuda.synchronize()
+    return got
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, *HALVES), ids=str)
+@pytest.mark.parametrize("sizes", ((300, 1100, 64), (300, 600, 72), (200, 1100, 136), (30, 70, 64),
+                                   (9, 300, 40), (2100, 1100, 333), (3000, 22600, 72)), ids=str)
+def test_nothing_comes_from_scratch(gpu, sizes, dtype):
+    """The same bits whatever the call's memory held: zeros, or bytes that are no numbers."""
+    x, table, targets = _operands(gpu, 2, *sizes, dtype)
+    targets[::5] = -1
+    dloss = torch.rand(targets.shape, device=gpu)
+    call = lambda: _gradients(x, table, targets, dloss)  # noqa: E731
+    for a, b in zip(_after(0, gpu, call), _after(0xff, gpu, call)):
+        assert torch.equal(a, b)

@@ -1,10 +1,11 @@
-"""Gradients of the linear cross entropy where tokens count differently; and that nothing in them comes
-from scratch memory."""
+"""Gradients of the linear cross entropy where tokens count differently: weights of
+every size; and that nothing in them comes from scratch memory."""
 
 import pytest
 import torch
 
 import nacho_amd
+from tests.loss_reference import TINY, Loss, near
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +52,23 @@ def test_nothing_comes_from_scratch(gpu, sizes, dtype):
     call = lambda: _gradients(x, table, targets, dloss)  # noqa: E731
     for a, b in zip(_after(0, gpu, call), _after(0xff, gpu, call)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tokens", (40, 140, 2100))
+@pytest.mark.parametrize("dtype", (torch.float32, *HALVES), ids=str)
+def test_a_tokens_dx_is_as_exact_as_its_own_weight_allows(gpu, dtype, tokens):
+    """Weights from 2^16 down to 2^-4 in one call, and nearly even probabilities of 2^-15: what
+    another token weighs is nothing to a token's own gradient.
+
+    A token's dx and how far it may be off are those of a weight of 1, times its own, whose product
+    is rounded to the result's type."""
+    words, width = 33000, 64
+    g = torch.Generator(device=gpu).manual_seed(3)
+    table = (0.5 + 0.1 * torch.randn(words, width, generator=g, device=gpu)).to(dtype)
+    x = (0.02 * torch.randn(tokens, width, generator=g, device=gpu)).to(dtype)
+    targets = torch.randint(0, words, (tokens,), generator=g, device=gpu)
+    c = 2.0 ** torch.linspace(16, -4, tokens, device=gpu)
+    dx, _ = _gradients(x, table, targets, c)
+    one = Loss(x, table, targets, reduction="none", dloss=torch.ones(tokens, device=gpu))
+    c = c.double()[:, None]
+    near(dx, one.dx * c, one.dx_off * c + TINY[dtype], "dx")

@@ -23,9 +23,9 @@
 // their own, without these for dx, and with them, over the largest, for dtable, whose sums join the
 // tokens (both gradients of 1000 tokens of 1024 and 50,001 words take 472 us instead of 413 with one
 // dz, of 8192 of 2048 and 131,072 words 14.2 ms instead of 12.4).
-// Up to kPartsMost tokens of 16 bits have dz in two parts, a row for what the first has rounded away
-// behind all first ones and the gathered rows a second time with it: with few tokens the results
-// have little else to average a rounding of dz with (a single token's gradient of its target's row
+// Up to kPartsMost tokens with a target, of 16 bits, have dz in two parts, a row for what the first has
+// rounded away behind all first ones and the gathered rows a second time with it: with few tokens the
+// results have little else to average a rounding of dz with (a single token's gradient of its target's row
 // was up to 0.004 of it off in bfloat16, of which its own rounding is 0.0017).
 //
 // Bound by the matrix cores, and by the table's bytes for few tokens.  Measured, bfloat16: 8192 tokens
@@ -83,6 +83,19 @@ struct Held {
     float *factor;  // [held]: gradient of the token's loss over `common` (the backward pass)
     float *common;  // [1]
 };
+
+// The parts of dz, of which a token's gathered row has as many copies, by the tokens that have a target;
+// and the rows that all of them take at most.
+constexpr int kPartsMost = 128;
+template <typename T>
+__device__ __forceinline__ int copies_of(int held) {
+    return sizeof(T) == 2 && held <= kPartsMost ? 2 : 1;
+}
+template <typename T>
+int64_t most_copies(int64_t tokens) {
+    const int64_t few = tokens < kPartsMost ? tokens : kPartsMost;
+    return sizeof(T) == 2 && 2 * few > tokens ? 2 * few : tokens;
+}
 
 enum Reduction { kNone = NACHO_LOSS_NONE, kMean = NACHO_LOSS_MEAN, kSum = NACHO_LOSS_SUM };
 
@@ -173,11 +186,11 @@ __device__ __forceinline__ void copy_row(const T *__restrict__ from, int64_t wid
     }
 }
 
-// Those of the listed tokens (token), or the first `rows` (null).
+// Those of the listed tokens (token), with copies for the parts of dz, or the first `rows` (null).
 template <typename T, int LANES>
 __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict__ count,
                                                           const int *__restrict__ token,
-                                                          int64_t rows, int64_t width,
+                                                          bool parts, int64_t rows, int64_t width,
                                                           int64_t padded,
                                                           const T *__restrict__ from,
                                                           int64_t stride, T *__restrict__ to,
@@ -186,9 +199,13 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(const int *__restrict_
     const int64_t there = count ? *count : rows;
     int64_t row = blockIdx.x * static_cast<int64_t>(kPer) +
                   __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+    const int copies = parts ? copies_of<T>(static_cast<int>(there)) : 1;
     for (; row < there; row += gridDim.x * static_cast<int64_t>(kPer)) {
-        copy_row<T, LANES>(from + (token ? token[row] : row) * stride, width, to + row * to_stride,
-                           padded, threadIdx.x % LANES);
+        const T *mine = from + (token ? token[row] : row) * stride;
+        for (int c = 0; c < copies; ++c) {
+            copy_row<T, LANES>(mine, width, to + (c * there + row) * to_stride, padded,
+                               threadIdx.x % LANES);
+        }
     }
 }
 
@@ -206,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
                                                              int64_t padded,
                                                              const T *__restrict__ from,
                                                              int64_t stride, T *__restrict__ to,
-                                                             int64_t to_stride, int copies) {
+                                                             int64_t to_stride, bool parts) {
     constexpr int kWaves = kThreads / dev::kWave, kStep = 8;
     __shared__ int s_before[kWaves], s_all[kWaves], s_token[kListRows];
     __shared__ float s_most[kWaves];
@@ -278,6 +295,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
         if (lane < kListRows) s_token[lane] = id >= 0 ? at : -1;
     }
     __syncthreads();
+    const int copies = parts ? copies_of<T>(all) : 1;
     for (int i = wave; i < kListRows; i += kWaves) {
         const int at = s_token[i];
         if (at >= 0) {
@@ -338,8 +356,7 @@ struct Logits {
     const float *total;    // s
     const int *token;
     const float *factor;   // null: 1
-    int copies;            // parts of dz, 1 or 2
-    void *dz;              // [copies][held][dz_stride]; null: only the next
+    void *dz;              // [parts][held][dz_stride]; null: only the next
     void *own_dz;          // the same without the factors, for dx; null: dz serves
     int64_t dz_stride;     // at least the piece's tiles: words past the piece's get zeros
 };
@@ -642,7 +659,7 @@ template <typename T>
 __device__ __forceinline__ void store_dz(const Logits &a, T *to, int held, f32x4 d) {
     dense::store4<T>(to, d);
     if constexpr (sizeof(T) == 2) {
-        if (a.copies == 2) {
+        if (copies_of<T>(held) == 2) {
             f32x4 rest;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -727,8 +744,7 @@ __global__ __launch_bounds__((Tile<BM, BN>::kThreads)) void dz_kernel(Logits a) 
 
 struct Gradients {
     const int *held;
-    int copies;           // of dz and the rows: as many tokens as held times copies
-    const void *dz;       // for dtable
+    const void *dz;       // [parts][held][dz_stride], for dtable
     const void *dx_dz;    // for dx: the same, or (own) without the tokens' gradients
     const float *own;     // these gradients, by token; null: dx's are `common`
     int64_t dz_stride;
@@ -740,7 +756,7 @@ struct Gradients {
     int64_t rows_stride;
     int64_t piece;        // words of a whole piece
     int64_t most_rows;    // that the sums have room for, at least all tokens
-    float *sums;          // [split][copies][held][sums_stride]; null: no dx
+    float *sums;          // [split][parts][held][sums_stride]; null: no dx
     int64_t sums_stride;
     int first;            // whether the piece is the first
     int64_t most_parts;   // splits that `parts` has room for; 1 without it
@@ -915,7 +931,7 @@ __global__ __launch_bounds__(kTileThreads) void gradients_kernel(Gradients a) {
     constexpr int kLdsX = DX ? kLds<T, 256, BN, Across, Along> : 0;
     constexpr int kLdsT = DTABLE ? kLds<T, 256, (BN <= 64 ? 64 : BN), Across, Across> : 0;
     __shared__ __attribute__((aligned(16))) T lds[kLdsX > kLdsT ? kLdsX : kLdsT];
-    const int held = *a.held * a.copies;
+    const int held = *a.held * copies_of<T>(*a.held);
     const int64_t load = load_of<T, BN>(a, held, DX, DTABLE);
     unsigned at = blockIdx.x, mt = 0, nt = 0;
     if constexpr (DX) {
@@ -975,7 +991,7 @@ __device__ __forceinline__ f32x4 splits_sum(const float *from, int64_t stride, u
 // dtable of a piece whose products were split: the splits' sums in their order.
 template <typename T, int BN>
 __global__ __launch_bounds__(kThreads) void dtable_join_kernel(Gradients a, bool both) {
-    const int held = *a.held * a.copies;
+    const int held = *a.held * copies_of<T>(*a.held);
     const unsigned splits =
         dtable_splits<T, BN>(a, held, load_of<T, BN>(a, held, both, true)).count;
     if (splits == 1) return;
@@ -998,7 +1014,7 @@ __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
                                                            const int *__restrict__ slot,
                                                            int64_t tokens, bool both,
                                                            T *__restrict__ dx) {
-    const int held = *a.held * a.copies;
+    const int copies = copies_of<T>(*a.held), held = *a.held * copies;
     const unsigned splits = dx_splits<T, BN>(a, held, load_of<T, BN>(a, held, true, both)).count;
     constexpr int kPer = kThreads / LANES;
     int64_t t = blockIdx.x * static_cast<int64_t>(kPer) +
@@ -1011,7 +1027,7 @@ __global__ __launch_bounds__(kThreads) void dx_join_kernel(Gradients a,
             if (at >= 0) {
                 const float *from = a.sums + at * a.sums_stride + d;
                 sum = splits_sum(from, held * a.sums_stride, splits);
-                if (a.copies == 2) {
+                if (copies == 2) {
                     sum += splits_sum(from + held / 2 * a.sums_stride, held * a.sums_stride, splits);
                 }
                 sum *= factor;
@@ -1091,9 +1107,6 @@ struct Wanted {
     }
 };
 
-// (within kListMost)
-constexpr int64_t kPartsMost = 128;
-
 // The operands as the kernels take them: rows gathered and, where a table's rows are not whole
 // aligned pieces, a copy of it whose are.
 template <typename T>
@@ -1106,7 +1119,7 @@ struct Operands {
     int64_t rows_stride = 0;
     int64_t table_stride = 0;
     bool copied = false;
-    int copies = 1;  // of the rows
+    bool parts = false;  // whether rows may have copies
 
     // (256 rows of a tile within the loads' 2 GB)
     static constexpr int64_t kMostStride = int64_t{1} << 22;
@@ -1120,8 +1133,8 @@ struct Operands {
         wanted.add(&held.target, a.tokens);
         if (dloss) wanted.add(&held.common, 1);
         if (dloss && a.reduction == NACHO_LOSS_NONE) wanted.add(&held.factor, a.tokens);
-        if (dloss && sizeof(T) == 2 && a.tokens <= kPartsMost) copies = 2;
-        wanted.add(&rows, copies * a.tokens * rows_stride);
+        parts = dloss;
+        wanted.add(&rows, (parts ? most_copies<T>(a.tokens) : a.tokens) * rows_stride);
         table = static_cast<const T *>(a.table);
         table_stride = a.table_stride;
         copied = !dense::pieces(a.table, a.table_stride, a.width, sizeof(T)) ||
@@ -1139,29 +1152,29 @@ struct Operands {
         if (tokens <= kListMost) {
             list_rows_kernel<T><<<ceil_div(static_cast<size_t>(tokens), kListRows), kThreads, 0,
                                   s>>>(targets, tokens, a.reduction, dloss, held, a.width, width,
-                                       x, a.x_stride, rows, rows_stride, copies);
+                                       x, a.x_stride, rows, rows_stride, parts);
             NACHO_TRY_HIP(hipGetLastError());
         } else {
             list_kernel<<<1, kListThreads, 0, s>>>(targets, tokens, a.reduction, dloss, held);
             NACHO_TRY_HIP(hipGetLastError());
-            NACHO_TRY(gather(s, held.count, held.token, a.tokens, a.width, x, a.x_stride, rows,
+            NACHO_TRY(gather(s, held.count, held.token, parts, a.tokens, a.width, x, a.x_stride, rows,
                              rows_stride));
         }
         if (copied) {
-            NACHO_TRY(gather(s, nullptr, nullptr, a.words, a.width, table, a.table_stride, copy,
-                             table_stride));
+            NACHO_TRY(gather(s, nullptr, nullptr, false, a.words, a.width, table, a.table_stride,
+                             copy, table_stride));
             table = copy;
         }
         return NACHO_OK;
     }
 
-    int gather(hipStream_t s, const int *count, const int *token, int64_t n, int64_t columns,
-               const T *from, int64_t stride, T *to, int64_t to_stride) const {
+    int gather(hipStream_t s, const int *count, const int *token, bool with_parts, int64_t n,
+               int64_t columns, const T *from, int64_t stride, T *to, int64_t to_stride) const {
         auto launch = [&](auto lanes) -> int {
             const int64_t groups = (n * lanes() + kThreads - 1) / kThreads;
             const unsigned grid = static_cast<unsigned>(groups < (1 << 20) ? groups : 1 << 20);
             gather_kernel<T, lanes()><<<grid, kThreads, 0, s>>>(
-                count, token, n, columns, width, from, stride, to, to_stride);
+                count, token, with_parts, n, columns, width, from, stride, to, to_stride);
             NACHO_TRY_HIP(hipGetLastError());
             return NACHO_OK;
         };
@@ -1189,12 +1202,12 @@ int with_shape(int64_t tokens, int64_t words, F f) {
     return f(Number<256>{}, Number<256>{});
 }
 
-// The same, and the columns of the gradients' tiles.
+// The same, and the columns of the gradients' tiles, whose rows are `columns` with the parts of dz.
 template <typename F>
-int with_shapes(int64_t tokens, int copies, int64_t words, F f) {
+int with_shapes(int64_t tokens, int64_t columns, int64_t words, F f) {
     return with_shape(tokens, words, [&](auto bm, auto bn) -> int {
         if constexpr (bn() == 16) {
-            if (tokens * copies <= 16) return f(bm, bn, Number<16>{});
+            if (columns <= 16) return f(bm, bn, Number<16>{});
             return f(bm, bn, Number<64>{});
         } else {
             return f(bm, bn, bn);
@@ -1311,15 +1324,14 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
         if (a.tokens == 0) {
             return dense::clear(s, static_cast<T *>(dtable), a.words * a.width);
         }
-        const int copies = sizeof(T) == 2 && a.tokens <= kPartsMost ? 2 : 1;
-        return with_shapes(a.tokens, copies, a.words, [&](auto bm, auto tokens, auto bn) -> int {
+        const int64_t columns = most_copies<T>(a.tokens);
+        return with_shapes(a.tokens, columns, a.words, [&](auto bm, auto tokens, auto bn) -> int {
             // of the logits' tiles, and of the gradients'
             constexpr int kBM = bm(), kTokens = tokens(), kBN = bn();
             // dz by the tokens' own gradients, and without them for dx
             const bool own = __is_same(T, _Float16) && a.reduction == NACHO_LOSS_NONE && dx;
-            const int64_t piece = piece_of(a.words, a.tokens * copies * item);
+            const int64_t piece = piece_of(a.words, columns * item);
             const int64_t cut = kTokens == 256 ? kUnits : 0;
-            const int64_t columns = a.tokens * copies;
             const unsigned dx_groups = groups_of(a.width, 256, columns, kBN, kMostItems);
             if (!groups_of(piece, kBM, a.tokens, kTokens, cut) || !dx_groups ||
                 !groups_of(a.width, 256, piece, 64, dx_groups + kMostItems)) {
@@ -1343,7 +1355,7 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             if (d.most_rows < columns) d.most_rows = columns;
             if (dx) wanted.add(&d.sums, d.most_rows * d.sums_stride);
             const int64_t tiles = m_tiles * (up(piece, 256) / 256);
-            const int64_t deep = up(a.tokens, 512) / 512;  // (splits are 8 steps or more)
+            const int64_t deep = up(columns, 512) / 512;  // (splits are 8 steps or more)
             d.most_parts = kMostItems / tiles < deep ? kMostItems / tiles : deep;
             if (d.most_parts > kMostSplits) d.most_parts = kMostSplits;
             // (dx's products are as many: with both, or enough of one, no split is worth its while)
@@ -1357,7 +1369,6 @@ int backward(const Args &a, const float *stats, const float *dloss, void *dx, vo
             NACHO_TRY(wanted.get(call));
             NACHO_TRY(ops.start(s, a, dloss));
             l.held = d.held = ops.held.count;
-            l.copies = d.copies = copies;
             l.width = d.padded = ops.width;
             l.rows = d.rows = ops.rows;
             l.rows_stride = d.rows_stride = ops.rows_stride;

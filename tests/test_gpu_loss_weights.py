@@ -1,5 +1,5 @@
 """Gradients of the linear cross entropy where tokens count differently: weights of
-every size; and that nothing in them comes from scratch memory."""
+every size, few targets among many tokens; and that nothing in them comes from scratch memory."""
 
 import pytest
 import torch
@@ -72,3 +72,26 @@ def test_a_tokens_dx_is_as_exact_as_its_own_weight_allows(gpu, dtype, tokens):
     one = Loss(x, table, targets, reduction="none", dloss=torch.ones(tokens, device=gpu))
     c = c.double()[:, None]
     near(dx, one.dx * c, one.dx_off * c + TINY[dtype], "dx")
+
+
+@pytest.mark.parametrize("reduction", ("mean", "none"))
+@pytest.mark.parametrize("held", (1, 3, 128))
+@pytest.mark.parametrize("tokens", (129, 1000, 3000))
+@pytest.mark.parametrize("dtype", HALVES, ids=str)
+def test_few_targets_among_many_tokens(gpu, dtype, tokens, held, reduction):
+    """The gradients of up to 128 tokens that have a target are as exact as those of a call that has
+    these tokens alone: rounded once, for the result."""
+    x, table, targets = _operands(gpu, 4, tokens, 900, 72, dtype)
+    some = torch.randperm(tokens, generator=torch.Generator().manual_seed(5))[:held].sort()[0]
+    some = some.to(gpu)
+    left = torch.full_like(targets, -1)
+    left[some] = targets[some]
+    dloss = torch.rand(tokens, device=gpu) if reduction == "none" else torch.tensor(0.7, device=gpu)
+    own = dloss[some] if reduction == "none" else dloss
+    dx, dtable = _gradients(x, table, left, dloss, reduction)
+    want = Loss(x[some], table, targets[some], 1.0, reduction, own)
+    near(dx[some], want.dx, want.dx_off, "dx")
+    near(dtable, want.dtable, want.dtable_off, "dtable")
+    none = torch.ones(tokens, dtype=torch.bool, device=gpu)
+    none[some] = False
+    assert not dx[none].any()

@@ -99,6 +99,13 @@ int64_t most_copies(int64_t tokens) {
 
 enum Reduction { kNone = NACHO_LOSS_NONE, kMean = NACHO_LOSS_MEAN, kSum = NACHO_LOSS_SUM };
 
+// The gradient of each token's loss from that of their mean or sum.  (Of no token: 0, so that sums of
+// nothing are that whatever the gradient.)
+__device__ __forceinline__ float common_of(int held, int reduction, float dloss) {
+    if (held == 0) return 0.0f;
+    return reduction == kMean ? dloss / static_cast<float>(held) : dloss;
+}
+
 constexpr int kListThreads = 1024;
 constexpr int kListPer = 8;  // tokens of a thread and step
 
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(Targets targets, int
         for (int w = 0; w < kListThreads / dev::kWave; ++w) common = fmaxf(common, s_max[w]);
         if (common == 0.0f) common = 1.0f;
     } else {
-        common = reduction == kMean ? dloss[0] / static_cast<float>(max(carry, 1)) : dloss[0];
+        common = common_of(carry, reduction, dloss[0]);
     }
     if (threadIdx.x == 0) *held.common = common;
     if (reduction != kNone) return;
@@ -273,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void list_rows_kernel(Targets targets, in
     if (each) {
         if (common == 0.0f) common = 1.0f;
     } else if (dloss) {
-        common = reduction == kMean ? dloss[0] / static_cast<float>(max(all, 1)) : dloss[0];
+        common = common_of(all, reduction, dloss[0]);
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         held.count[0] = all;

@@ -1,5 +1,6 @@
 """Gradients of the linear cross entropy where tokens count differently: weights of
-every size, few targets among many tokens; and that nothing in them comes from scratch memory."""
+every size, few targets among many tokens, no target at all; and that nothing in them comes from
+scratch memory."""
 
 import pytest
 import torch
@@ -95,3 +96,16 @@ def test_few_targets_among_many_tokens(gpu, dtype, tokens, held, reduction):
     none = torch.ones(tokens, dtype=torch.bool, device=gpu)
     none[some] = False
     assert not dx[none].any()
+
+
+@pytest.mark.parametrize("value", (float("inf"), float("-inf"), float("nan"), 3e38))
+@pytest.mark.parametrize("dtype", (torch.float32, *HALVES), ids=str)
+def test_no_target_has_no_gradient(gpu, dtype, value):
+    """A sum over no tokens is 0, whatever the gradient of its result."""
+    for tokens in (1, 40, 200, 3000):
+        x, table, targets = _operands(gpu, 1, tokens, 300, 64, dtype)
+        for reduction in ("mean", "sum", "none"):
+            shape = targets.shape if reduction == "none" else ()
+            dx, dtable = _gradients(x, table, torch.full_like(targets, -1),
+                                    torch.full(shape, value, device=gpu), reduction)
+            assert not dx.any() and not dtable.any(), (tokens, reduction)

@@ -5,14 +5,16 @@ Tensors are float32, float16 or bfloat16 in any mixture, on one device; entries 
 order.
 
 Calls are asynchronous on torch's current stream, read nothing back and may be captured in a
-graph.  There is no CPU fallback, and no gradient.
+graph.  There is no CPU fallback.  Neither has a gradient: a norm of tensors that require one
+refuses its backward pass, both refuse tangents of forward mode, and clipping is no part of a history.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
-from .blocks import _MOST_SCALE, _TYPES, _call, _device_of
+from .blocks import _MOST_SCALE, _TYPES, _call, _device_of, _has_derivatives
 
 
 def _list(tensors, name):
@@ -51,16 +53,36 @@ def _dense(t):
     return True
 
 
-def gpu_grad_norm(tensors) -> torch.Tensor:
-    """The root of the sum of the squares of all elements of a tensor or of many, float32, on the
-    device."""
-    tensors = _list(tensors, "tensors")
-    device = _device(tensors)
-    got = _call("grad_norm", device, tuple(t for t in tensors if t is not None))
+def _norm(device, held, tensors):
+    got = _call("grad_norm", device, held)
     if got is None:
         _check(tensors, "tensors", device)
         raise ValueError("gpu_grad_norm: refused operands")
     return got
+
+
+class _GradNorm(torch.autograd.Function):
+    """(Refuses tangents, as a function without jvp.)"""
+
+    @staticmethod
+    def forward(ctx, device, *held):
+        return _norm(device, held, held)
+
+    @staticmethod
+    def backward(ctx, dnorm):
+        raise RuntimeError("gpu_grad_norm has no gradient: detach the tensors or the norm")
+
+
+def gpu_grad_norm(tensors) -> torch.Tensor:
+    """The root of the sum of the squares of all elements of a tensor or of many, float32, on the
+    device.  Not differentiable: of tensors that require a gradient, its backward pass raises."""
+    tensors = _list(tensors, "tensors")
+    device = _device(tensors)
+    held = tuple(t for t in tensors if t is not None)
+    if _has_derivatives(*held):
+        _check(tensors, "tensors", device)
+        return _GradNorm.apply(device, *held)
+    return _norm(device, held, tensors)
 
 
 def gpu_clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
@@ -72,7 +94,8 @@ def gpu_clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
     float32 (as an optimiser's own copies are).  A tensor that is written has to have its elements
     next to each other, in any order of its dimensions, and share no memory with another's.  A norm
     of infinity makes finite elements 0 and infinite ones no numbers; one that is no number makes
-    all of them that.  max_norm may be infinity: nothing is scaled."""
+    all of them that.  max_norm may be infinity: nothing is scaled.  Not differentiable: what is
+    written has the history that it had, and the norm none."""
     tensors = _list(tensors, "tensors")
     device = _device(tensors)
     if not max_norm >= 0:
@@ -84,6 +107,10 @@ def gpu_clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
     if len(outs) != len(tensors) or any((a is None) != (b is None)
                                         for a, b in zip(tensors, outs)):
         raise ValueError(f"out: expected a tensor for each of the {len(tensors)}, got {len(outs)}")
+    if forward_ad._current_level >= 0:
+        for t in (*tensors, *outs):
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("gpu_clip_grad_norm has no jvp: tensors with tangents")
     got = _call("clip_grad_norm", device, tuple(t for t in tensors if t is not None),
                 tuple(t for t in outs if t is not None), limit)
     if got is None:

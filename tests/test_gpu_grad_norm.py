@@ -218,3 +218,37 @@ def test_refusals(gpu):
     f([a, b], 1.0, out=[a.clone(), b.clone()])
     both = [a, a]  # read twice, written apart
     assert abs(float(f(both, 1.0, out=[a.clone(), a.clone()])) - math.sqrt(200)) < 1e-5
+
+
+def test_a_norm_has_no_gradient(gpu):
+    """What would lose its gradient or its tangent without a word raises."""
+    a, b = torch.randn(50, device=gpu, requires_grad=True), torch.randn(7, 3, device=gpu)
+    norm = nacho_amd.gpu_grad_norm([None, 2.0 * a, b])
+    assert torch.equal(norm.detach(), nacho_amd.gpu_grad_norm([2.0 * a.detach(), b]))
+    with pytest.raises(RuntimeError, match="gpu_grad_norm has no gradient"):
+        (a.sum() + norm).backward()
+    with torch.no_grad():
+        assert not nacho_amd.gpu_grad_norm(a).requires_grad
+    assert not nacho_amd.gpu_grad_norm(a.detach()).requires_grad
+    with pytest.raises(TypeError, match=r"tensors\[2\]: expected dtype"):
+        nacho_amd.gpu_grad_norm([None, a, b.double()])
+
+
+def test_refuses_tangents(gpu):
+    from torch.autograd import forward_ad
+
+    a, b = torch.randn(50, device=gpu), torch.randn(7, 3, device=gpu)
+    want, before = nacho_amd.gpu_grad_norm([a, b]), b.clone()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(b, torch.ones_like(b))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            nacho_amd.gpu_grad_norm([a, dual])
+        with pytest.raises(NotImplementedError, match="jvp"):
+            nacho_amd.gpu_clip_grad_norm([a, dual], 0.1)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            nacho_amd.gpu_clip_grad_norm([b], 0.1, out=[dual])
+        assert torch.equal(b, before)
+        assert torch.equal(nacho_amd.gpu_grad_norm([a, b]), want)
+        assert torch.equal(nacho_amd.gpu_clip_grad_norm([a, None, b], 0.1), want)
+    with pytest.raises(TypeError, match="expected a torch.Tensor"):
+        nacho_amd.gpu_clip_grad_norm([a, 3.0], 0.1)

@@ -531,7 +531,7 @@ int nacho_grad_norm(const nacho_gradient *tensors, int64_t count, float *norm, v
 /* The same, and every tensor's elements times min(1, max_norm / (norm + 1e-6)), that factor rounded
  * to float32, into its `out` in `out_dtype`, the tensor's own or NACHO_F32.  A norm that is no
  * number makes all of them that.  max_norm: 0 or more; infinity copies.  No `out` may overlap
- * another tensor's data or `out`, nor its own data but for being it. */
+ * another tensor's data or `out`, nor its own data but for being it, in the same type. */
 int nacho_clip_grad_norm(const nacho_gradient *tensors, int64_t count, float max_norm,
                          float *norm, void *stream, const nacho_allocator *alloc);
 

@@ -296,6 +296,10 @@ int check(const nacho_gradient *tensors, int64_t count, bool clip, const float *
         if (t.size > 0 && (!t.data || !element_aligned(t.data, item_of(t.dtype)))) {
             return NACHO_ERR_INVALID_ARGUMENT;
         }
+        // (wider elements over narrower ones that are still to be read)
+        if (clip && t.size > 0 && t.out == t.data && t.out_dtype != t.dtype) {
+            return NACHO_ERR_INVALID_ARGUMENT;
+        }
         if (clip && ((t.out_dtype != t.dtype && t.out_dtype != NACHO_F32) ||
                      (t.size > 0 && (!t.out || !element_aligned(t.out, item_of(t.out_dtype)))))) {
             return NACHO_ERR_INVALID_ARGUMENT;

@@ -116,6 +116,15 @@ def test_clip_refuses(lib):
     assert norm(one(size=1 << 40), 1, X, None, None) == OVERFLOW
 
 
+def test_clip_refuses_wider_elements_in_place(lib):
+    """float32 written where 16-bit elements are still to be read, past the end of their memory."""
+    from nacho_amd import _lib
+
+    for dtype in (1, 2):
+        t = _lib.Gradient(0x10000, 0x10000, 100, dtype, 0)
+        assert lib.nacho_clip_grad_norm(ctypes.byref(t), 1, 1.0, X, None, None) == INVALID
+
+
 def test_arguments_that_are_refused_before_the_library():
     import nacho_amd
 

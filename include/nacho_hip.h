@@ -477,7 +477,7 @@ int nacho_embedding(int32_t dtype, int64_t tokens, int64_t words, int64_t width,
                     void *rows, void *stream);
 
 /* The gradient of nacho_embedding: dtable[words][width] = scale * the sum of dout[token] over the
- * tokens with the word's id, in their order; 0 for a word without.  stride: elements between
+ * tokens with the word's id, in a fixed order; 0 for a word without.  stride: elements between
  * dout's rows; dtable is contiguous. */
 int nacho_embedding_backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width,
                              float scale, const void *ids, int32_t id_bytes, const void *dout,

@@ -7,7 +7,9 @@
 // by word, in order of the token within one, which gives every sum a fixed order; runs of kChunk
 // sorted entries are summed by one workgroup each, whatever their words, so that a word that half
 // of a batch has costs no more than others.  A word whose entries lie in more than one run gets its
-// parts joined by a second launch, in their order.
+// parts joined by another launch, in their order, for which many runs' parts are first added up in
+// groups, by workgroups of their own (262144 tokens of 2048 bfloat16, none, half and all of them of one word:
+// 300, 293 and 271 us; without such groups 297, 632 and 954).
 //
 // Measured, bfloat16: the lookup of 65536 rows of 4096 124 us, 5.7 TB/s; the gradient of 16384 tokens
 // of 2048 and 65537 words 74 us traced, of which sorting them beside clearing the table 48 (5.6 TB/s of
@@ -487,9 +489,43 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restri
     }
 }
 
-// Words that begin in a run and go on behind it: their parts in the order of the runs.
+// Runs that a workgroup of fold_kernel adds up.
+constexpr int kFold = 64;
+
+// Groups of kFold runs, the first at a multiple of kFold, that begin with a word that the run before
+// ends with, all of them: their parts' sum takes the place of the first's.
+template <int N, int LANES>
+__global__ __launch_bounds__(kThreads) void fold_kernel(Sums a) {
+    constexpr int kStep = 16;
+    const Part<N, LANES> own(a);
+    // (the first group's first run has none before it)
+    const int64_t first = (own.run + 1) * static_cast<int64_t>(kFold), last = first + kFold - 1;
+    if (last >= a.chunks || !own.there) return;
+    const int key = a.keys[first * kChunk];
+    if (key >= a.words || a.keys[first * kChunk - 1] != key || a.keys[last * kChunk] != key) return;
+    float sum[N] = {};
+    float *const mine = a.parts + first * 2 * a.width + own.col;
+    for (int r0 = 0; r0 < kFold; r0 += kStep) {
+        float part[kStep][N];
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) part[s][j] = mine[(r0 + s) * 2 * a.width + j];
+        }
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[j] += part[s][j];
+        }
+    }
+    store_part<N>(mine, sum);
+}
+
+// Words that begin in a run and go on behind it: their parts in the order of the runs, groups of them
+// in one where they are folded.
 template <typename T, int N, int LANES>
-__global__ __launch_bounds__(kThreads) void join_kernel(Sums a, T *__restrict__ dtable) {
+__global__ __launch_bounds__(kThreads) void join_kernel(Sums a, bool folded,
+                                                        T *__restrict__ dtable) {
     constexpr int kStep = 8;
     const Part<N, LANES> own(a);
     if (own.run + 1 >= a.chunks) return;
@@ -513,20 +549,33 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, T *__restrict__ 
     const float *mine = a.parts + (own.run * 2ll + 1) * a.width + col;
 #pragma unroll
     for (int j = 0; j < N; ++j) sum[j] = mine[j];
-    for (int run = own.run + 1; run <= last; run += kStep) {
-        float part[kStep][N];
+    // Adds the parts of `n` runs, or of groups of `by` runs, from `first` on.
+    auto add = [&](int first, int n, int by) {
+        for (int i = 0; i < n; i += kStep) {
+            float part[kStep][N];
 #pragma unroll
-        for (int s = 0; s < kStep; ++s) {
-            const float *from = a.parts + min(run + s, last) * 2ll * a.width + col;
+            for (int s = 0; s < kStep; ++s) {
+                const int run = first + min(i + s, n - 1) * by;
+                const float *from = a.parts + run * 2ll * a.width + col;
 #pragma unroll
-            for (int j = 0; j < N; ++j) part[s][j] = from[j];
+                for (int j = 0; j < N; ++j) part[s][j] = from[j];
+            }
+#pragma unroll
+            for (int s = 0; s < kStep; ++s) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) sum[j] += i + s < n ? part[s][j] : 0.0f;
+            }
         }
-#pragma unroll
-        for (int s = 0; s < kStep; ++s) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) sum[j] += run + s <= last ? part[s][j] : 0.0f;
-        }
+    };
+    // Single runs before the first whole group, groups, and single runs behind the last.
+    int next = own.run + 1;
+    const int whole = (next + kFold - 1) / kFold * kFold, behind = (last + 1) / kFold * kFold;
+    if (folded && whole < behind) {
+        add(next, whole - next, 1);
+        add(whole, (behind - whole) / kFold, kFold);
+        next = behind;
     }
+    add(next, last + 1 - next, 1);
     store_sum<T, N>(dtable + static_cast<int64_t>(key) * a.width + col, sum, a.scale);
 }
 
@@ -666,6 +715,11 @@ int sort_tokens(Call &call, const Ids &ids, int tokens, const Cleared &all, int 
     return NACHO_OK;
 }
 
+// Runs from which on fold_kernel is launched.  (us with it and without it, half of the tokens of one word,
+// and none: 8192 tokens of 2048 bfloat16 49 and 49, 43 and 41; 16384 70 and 78, 61 and 59; 262144 293 and
+// 632, 300 and 297; 1048576 of 64 float32 166 and 1300, 160 and 158.)
+constexpr int64_t kFoldChunks = 512;
+
 int backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float scale,
              const void *ids, int32_t id_bytes, const void *dout, int64_t stride, void *dtable,
              void *stream, const nacho_allocator *alloc) {
@@ -701,8 +755,15 @@ int backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float 
             sum_kernel<T, n(), of()><<<groups, kThreads, 0, s>>>(a, static_cast<const T *>(dout),
                                                                  stride, table);
             NACHO_TRY_HIP(hipGetLastError());
+            const bool fold = chunks >= kFoldChunks;
+            if (fold) {
+                const int64_t folds = (chunks / kFold * of() + kThreads - 1) / kThreads;
+                fold_kernel<n(), of()><<<dim3(static_cast<unsigned>(folds), groups.y), kThreads, 0,
+                                         s>>>(a);
+                NACHO_TRY_HIP(hipGetLastError());
+            }
             if (chunks > 1) {
-                join_kernel<T, n(), of()><<<groups, kThreads, 0, s>>>(a, table);
+                join_kernel<T, n(), of()><<<groups, kThreads, 0, s>>>(a, fold, table);
                 NACHO_TRY_HIP(hipGetLastError());
             }
             return NACHO_OK;

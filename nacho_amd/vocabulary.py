@@ -90,7 +90,7 @@ def gpu_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
 def gpu_embedding_backward(dout: torch.Tensor, ids: torch.Tensor, words: int,
                            scale: float = 1.0) -> torch.Tensor:
     """The gradient of gpu_embedding's table, [words, width], from that of its result: a word's
-    row is scale times the sum of its tokens' rows of dout, in the tokens' order."""
+    row is scale times the sum of its tokens' rows of dout, in a fixed order."""
     device = _device_of(dout, "dout")
     scale = _factor(scale)
     _check_words(words)

@@ -225,3 +225,44 @@ def test_refusals(gpu):
             (lambda: b(dout, ids.short(), 9), TypeError, "ids: expected dtype")]:
         with pytest.raises(error, match=text):
             call()
+
+
+@pytest.mark.parametrize("tokens", (16383, 16384, 18500, 70001, 300_000))
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16), ids=str)
+def test_words_of_many_runs(gpu, tokens, dtype):
+    """Words that a share of a large batch has, wherever their sorted tokens begin: sums of whole numbers,
+    which are exact whatever their order."""
+    for width, words, hot, word in ((3, 90, 0.5, 45), (72, 7, 0.0, 0), (40, 1000, 1.0, 0),
+                                    (333, 50, 0.9, 49), (1040, 3, 0.3, 1)):
+        g = torch.Generator(device=gpu).manual_seed(tokens + width)
+        ids = torch.randint(0, words, (tokens,), generator=g, device=gpu)
+        ids[torch.rand(tokens, generator=g, device=gpu) < hot] = word
+        ids[5::4001] = -1
+        dout = torch.randint(-8, 9, (tokens, width), generator=g, device=gpu).to(dtype)
+        got = nacho_amd.gpu_embedding_backward(dout, ids, words)
+        there = (ids == torch.arange(words, device=gpu)[:, None]).float()
+        assert torch.equal(got, (there @ dout.float()).to(dtype)), (width, words, hot)
+
+
+def test_a_word_costs_what_the_batch_costs(gpu):
+    """Half of a batch of one word takes at most twice as long as none of it."""
+    tokens, words, width = 1 << 20, 32000, 64
+    g = torch.Generator(device=gpu).manual_seed(1)
+    dout = torch.randn(tokens, width, generator=g, device=gpu)
+
+    def time_of(ids):
+        best = float("inf")
+        for _ in range(5):
+            start, end = torch.cuda.Event(True), torch.cuda.Event(True)
+            start.record()
+            for _ in range(5):
+                nacho_amd.gpu_embedding_backward(dout, ids, words)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    even = torch.randint(0, words, (tokens,), generator=g, device=gpu)
+    hot = torch.where(torch.rand(tokens, generator=g, device=gpu) < 0.5, 7, even)
+    time_of(even)
+    assert time_of(hot) <= 2.0 * time_of(even)

@@ -126,3 +126,27 @@ def test_loss_of_more_tokens_than_a_launch_has_workgroups(gpu):
     size = (dz.abs() * times).T @ few.double().abs()
     off = ((1 << 20) + 1000) * 2.0 ** -24 * size + u * size + u * right.abs()
     assert ((dtable.double() - right).abs() <= off).all()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float16, torch.bfloat16), ids=str)
+def test_sums_over_many_tokens_are_summed_in_parts(gpu, dtype):
+    """dtable's sums over 1,000,003 tokens are 64 sums of at most 15,680 products, which are added: no more
+    than 15,680 + 64 roundings of their terms' magnitudes, 9.4e-4, where one sum has a million."""
+    tokens, words, width = 1_000_003, 40, 16
+    g = torch.Generator(device=gpu).manual_seed(4)
+    x = (1.0 + torch.rand(tokens, width, generator=g, device=gpu)).to(dtype)
+    table = (0.1 * torch.randn(words, width, generator=g, device=gpu)).to(dtype)
+    targets = torch.randint(-1, words, (tokens,), generator=g, device=gpu)
+    stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, reduction="sum",
+                                               return_stats=True)[1]
+    dloss = torch.tensor(1e-3, device=gpu)
+    got = nacho_amd.gpu_linear_cross_entropy_backward(dloss, x, table, targets, stats,
+                                                      reduction="sum")[1]
+    want = Loss(x, table, targets, reduction="sum", dloss=dloss)
+    held = (targets >= 0)[:, None]
+    dz = torch.softmax(x.double() @ table.double().T, -1)
+    dz.scatter_add_(1, targets.clamp(min=0)[:, None], torch.full((tokens, 1), -1.0, device=gpu).double())
+    size = (torch.where(held, dz, 0.0).abs() * float(dloss)).T @ x.double()
+    one_sum = (2 * int(held.sum()) + 4) * 2.0 ** -24
+    parts = (15_680 + 64 + 4) * 2.0 ** -24
+    near(got, want.dtable, want.dtable_off + (parts - one_sum) * size, "dtable")

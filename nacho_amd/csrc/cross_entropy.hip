@@ -23,10 +23,10 @@
 // their own, without these for dx, and with them, over the largest, for dtable, whose sums join the
 // tokens (both gradients of 1000 tokens of 1024 and 50,001 words take 472 us instead of 413 with one
 // dz, of 8192 of 2048 and 131,072 words 14.2 ms instead of 12.4).
-// Up to kPartsMost tokens with a target, of 16 bits, have dz in two parts, a row for what the first has
-// rounded away behind all first ones and the gathered rows a second time with it: with few tokens the
-// results have little else to average a rounding of dz with (a single token's gradient of its target's row
-// was up to 0.004 of it off in bfloat16, of which its own rounding is 0.0017).
+// A rounded dz of a token's target is what the gradients lose most by: bfloat16 ones are up to 0.0024 of
+// their norms off, of which rounding the results alone is 0.0017 (float16 0.0003 and 0.0002).  Up to
+// kPartsMost tokens with a target, of 16 bits, have dz in two parts and lose nothing: a row for what the
+// first has rounded away behind all first ones, and the gathered rows a second time with it.
 //
 // Bound by the matrix cores, and by the table's bytes for few tokens.  Measured, bfloat16: 8192 tokens
 // of 2048, 131072 words, loss and gradients 15.05 to 15.35 ms; traced, the forward product 1.27
@@ -85,7 +85,10 @@ struct Held {
 };
 
 // The parts of dz, of which a token's gathered row has as many copies, by the tokens that have a target;
-// and the rows that all of them take at most.
+// and the rows that all of them take at most.  The number decides what two parts cost, not what they
+// bring: both gradients of 100 tokens of 1024 and 32,000 words take 115 us with two and 90 with one, of
+// 129 139 and 111, of 512 250 and 177, of 2000 790 and 457; bfloat16 targets of probabilities of 0.13 on
+// average leave them 0.00166 and 0.0019 to 0.0020 of their norms off, at 100 tokens as at 2000.
 constexpr int kPartsMost = 128;
 template <typename T>
 __device__ __forceinline__ int copies_of(int held) {
@@ -1194,6 +1197,21 @@ struct Operands {
 // products of a few tokens would be of nothing.  Few tokens are bound by the table's bytes, of which
 // small tiles of a small vocabulary have more on their way; and tiles are smaller where there are
 // fewer than compute units.
+//
+// Measured, us of the loss / of both gradients (bfloat16 unless float32 is said), tokens x words x
+// width, the tile that is taken and the other:
+// - 16 tokens and 64.  8 x 5000 x 1024: 18 / 43 and 20 / 47; float32 25 / 58 and 49 / 90.
+//   24 x 131072 x 4096 (of 64, or the table read twice): 191 / 765 and 205 / 776.  Not so for float32,
+//   513 / 1772 and 430 / 1689, and small tables: 24 x 5000 x 1024 20 / 51 and 19 / 48.
+// - 64 words and 256, up to 16 tokens.  1 x 16384 x 2048: 26 / 69 and 32 / 76; 1 x 65536 x 2048 (of 256)
+//   49 / 241 and 50 / 239, 1 x 100000 x 2048 104 / 342 and 112 / 350.
+// - 64 tokens and 256.  100 x 32768 x 2048: 38 / 169 and 38 / 188; 192 (of 256) 43 / 180 and 46 / 163,
+//   float32 168 / 503 and 216 / 664; float32 of 100 is better off with 256, 149 / 465 and 134 / 384.
+// - 128 words and 256, of 64 tokens, by two rounds of tiles.  64 x 32768 x 1024: 24 / 104 and 28 / 110;
+//   128 x 65536 x 1024 (of 256) 34 / 193 and 40 / 206.
+// - 128 words and 256, of 256 tokens, by one round.  256 x 5000 x 1024: 23 / 54 and 26 / 59;
+//   256 x 65536 x 1024 (of 256) 44 / 205 and 52 / 215.  Just under a round 256 words are better: 256 x
+//   50000 x 1024 49 / 200 and 42 / 184.
 template <typename F>
 int with_shape(int64_t tokens, int64_t words, F f) {
     auto tiles = [&](int64_t bn) { return up(words, 256) / 256 * (up(tokens, bn) / bn); };

@@ -13,29 +13,40 @@ namespace nacho {
 namespace dense {
 
 // N elements that are read or written together: 16 bytes where rows allow it, one element where
-// a row starts between (odd widths and strides).
-template <typename T, int N>
-struct alignas(N * sizeof(T)) Piece {
+// a row starts between (odd widths and strides).  With the alignment of an element they lie wherever
+// it does: loads and stores of 16 bytes take any address.
+template <typename T, int N, int ALIGN = N * sizeof(T)>
+struct alignas(ALIGN) Piece {
     T v[N];
 };
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 // Rows are too many to be read again from a cache by what comes next: they go past it.
-template <typename T, int N>
-__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
+template <typename T, int N, int ALIGN = N * sizeof(T)>
+__device__ __forceinline__ Piece<T, N, ALIGN> load_piece(const T *p) {
     if constexpr (N * sizeof(T) == 16) {
-        return __builtin_bit_cast(Piece<T, N>, __builtin_nontemporal_load(
-                                                   reinterpret_cast<const u32x4 *>(p)));
+        u32x4 v;
+        if constexpr (ALIGN < 16) {
+            v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
+        } else {
+            v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+        }
+        return __builtin_bit_cast(Piece<T, N, ALIGN>, v);
     } else {
-        return *reinterpret_cast<const Piece<T, N> *>(p);
+        return *reinterpret_cast<const Piece<T, N, ALIGN> *>(p);
     }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
+template <typename T, int N, int ALIGN>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T, N, ALIGN> &v) {
     if constexpr (N * sizeof(T) == 16) {
-        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v),
-                                    reinterpret_cast<u32x4 *>(p));
+        if constexpr (ALIGN < 16) {
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v),
+                                        reinterpret_cast<u32x4_any *>(p));
+        } else {
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4 *>(p));
+        }
     } else {
-        *reinterpret_cast<Piece<T, N> *>(p) = v;
+        *reinterpret_cast<Piece<T, N, ALIGN> *>(p) = v;
     }
 }
 

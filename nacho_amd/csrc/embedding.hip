@@ -32,34 +32,9 @@ using dense::item_of;
 
 constexpr int kThreads = 256;
 
-// N elements that are read or written together, wherever they start: 16 bytes, or one element where
-// a row is shorter.  (Rows of odd widths start between 16-byte pieces; loads and stores of 16 bytes
-// take any address.)
+// Pieces of rows that start anywhere.
 template <typename T, int N>
-struct alignas(sizeof(T)) Piece {
-    T v[N];
-};
-typedef dense::u32x4 u32x4_any __attribute__((aligned(2)));
-
-// Rows are too many to be read again from a cache by what comes next: they go past it.
-template <typename T, int N>
-__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
-    if constexpr (N * sizeof(T) == 16) {
-        return __builtin_bit_cast(
-            Piece<T, N>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p)));
-    } else {
-        return *reinterpret_cast<const Piece<T, N> *>(p);
-    }
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &v) {
-    if constexpr (N * sizeof(T) == 16) {
-        __builtin_nontemporal_store(__builtin_bit_cast(dense::u32x4, v),
-                                    reinterpret_cast<u32x4_any *>(p));
-    } else {
-        *reinterpret_cast<Piece<T, N> *>(p) = v;
-    }
-}
+using Piece = dense::Piece<T, N, sizeof(T)>;
 
 // Where the piece that starts at col < width lies: a row's last piece ends with the row, over
 // elements that the one before has too (and both give them the same value).
@@ -120,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(Ids ids, int64_t token
                                 static_cast<T>(scale * static_cast<float>(piece[s].v[j]));
                         }
                     }
-                    store_piece<T, N>(to + within<N>(col, width), piece[s]);
+                    dense::store_piece(to + within<N>(col, width), piece[s]);
                 }
             }
         }
@@ -463,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restri
         for (int s = 0; s < kStep; ++s) {
             const int e = min(e0 + s, end - 1);
             key[s] = a.keys[e];
-            piece[s] = load_piece<T, N>(dout + a.order[e] * stride + col);
+            piece[s] = dense::load_piece<T, N, sizeof(T)>(dout + a.order[e] * stride + col);
         }
         key[kStep] = e0 + kStep < end ? a.keys[e0 + kStep] : behind;
 #pragma unroll

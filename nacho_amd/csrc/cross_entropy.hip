@@ -29,8 +29,8 @@
 // first has rounded away behind all first ones, and the gathered rows a second time with it.
 //
 // Bound by the matrix cores, and by the table's bytes for few tokens.  Measured, bfloat16: 8192 tokens
-// of 2048, 131072 words, loss and gradients 15.05 to 15.35 ms; traced, the forward product 1.27
-// PFLOP/s, dz 1.11, the gradients 1.07.  One token of 4096, its loss alone: 183 us, 5.9 TB/s.
+// of 2048, 131072 words, loss and gradients 15.05 to 15.35 ms; traced, the forward product 1.26
+// PFLOP/s, dz 1.11, the gradients 1.06.  One token of 4096, its loss alone: 183 to 185 us, 5.8 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <climits>

@@ -10,7 +10,7 @@
 // transposing LDS read.
 //
 // Measured, bfloat16, 8028 x 131072 by 2048, matrix cores' share of the time in brackets: both operands
-// along k 1.27 PFLOP/s (60%), across k 1.07 for a mix of the two (46%, 47% of it waits).
+// along k 1.26 PFLOP/s (60%), across k 1.06 for a mix of the two (46%, 47% of it waits).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -12,8 +12,8 @@
 // 300, 293 and 271 us; without such groups 297, 632 and 954).
 //
 // Measured, bfloat16: the lookup of 65536 rows of 4096 124 us, 5.7 TB/s; the gradient of 16384 tokens
-// of 2048 and 65537 words 74 us traced, of which sorting them beside clearing the table 48 (5.6 TB/s of
-// zeros), sums 21, joins 6.
+// of 2048 and 65537 words 78 us traced, of which sorting them beside clearing the table 47 (5.7 TB/s of
+// zeros), sums 21, groups of parts 5, joins 6.
 #include <hip/hip_runtime.h>
 
 #include <climits>

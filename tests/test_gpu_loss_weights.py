@@ -109,3 +109,53 @@ def test_no_target_has_no_gradient(gpu, dtype, value):
             dx, dtable = _gradients(x, table, torch.full_like(targets, -1),
                                     torch.full(shape, value, device=gpu), reduction)
             assert not dx.any() and not dtable.any(), (tokens, reduction)
+
+
+@pytest.mark.parametrize("tokens", (50, 300))
+def test_one_gradient_at_a_time(gpu, tokens):
+    """float16 tokens with weights: each gradient by itself, of two dz's for both."""
+    x, table, targets = _operands(gpu, 6, tokens, 700, 72, torch.float16)
+    targets[::7] = -1
+    c = 2.0 ** torch.linspace(-6, 6, tokens, device=gpu)
+    want = Loss(x, table, targets, reduction="none", dloss=c)
+    for wanted in ((True, False), (False, True), (True, True)):
+        ops = [t.detach().requires_grad_(w) for t, w in zip((x, table), wanted)]
+        loss = nacho_amd.gpu_linear_cross_entropy(*ops, targets, reduction="none")
+        loss.backward(c)
+        if wanted[0]:
+            near(ops[0].grad, want.dx, want.dx_off, "dx")
+        if wanted[1]:
+            near(ops[1].grad, want.dtable, want.dtable_off, "dtable")
+
+
+@pytest.mark.parametrize("tokens", (300, 2500))
+@pytest.mark.parametrize("dtype", HALVES, ids=str)
+def test_graph_replays(gpu, dtype, tokens):
+    """One graph of a step whose replays have no target, few, and many: dz in two parts and in one."""
+    x, table, targets = _operands(gpu, 7, tokens, 900, 72, dtype)
+    c = torch.rand(tokens, device=gpu)
+
+    def step():
+        loss, stats = nacho_amd.gpu_linear_cross_entropy(x, table, targets, reduction="none",
+                                                         return_stats=True)
+        return loss, *nacho_amd.gpu_linear_cross_entropy_backward(c, x, table, targets, stats,
+                                                                  reduction="none")
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i, held in enumerate((3, tokens, 0, 128, 129)):
+        new_x, new_table, new_targets = _operands(gpu, 8 + i, tokens, 900, 72, dtype)
+        new_targets[held:] = -1
+        c.uniform_(0.1, 1000.0)
+        for t, new in zip((x, table, targets), (new_x, new_table, new_targets)):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), held

@@ -468,7 +468,9 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(Sums a, const T *__restri
 constexpr int kFold = 64;
 
 // Groups of kFold runs, the first at a multiple of kFold, that begin with a word that the run before
-// ends with, all of them: their parts' sum takes the place of the first's.
+// ends with, all of them: their parts' sum goes into the first's second place.  (It has no second part,
+// as it has no other word.  Not into the first place, which is read: threads whose pieces share columns
+// would read each other's sums.)
 template <int N, int LANES>
 __global__ __launch_bounds__(kThreads) void fold_kernel(Sums a) {
     constexpr int kStep = 16;
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(kThreads) void fold_kernel(Sums a) {
     const int key = a.keys[first * kChunk];
     if (key >= a.words || a.keys[first * kChunk - 1] != key || a.keys[last * kChunk] != key) return;
     float sum[N] = {};
-    float *const mine = a.parts + first * 2 * a.width + own.col;
+    const float *const mine = a.parts + first * 2 * a.width + own.col;
     for (int r0 = 0; r0 < kFold; r0 += kStep) {
         float part[kStep][N];
 #pragma unroll
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(kThreads) void fold_kernel(Sums a) {
             for (int j = 0; j < N; ++j) sum[j] += part[s][j];
         }
     }
-    store_part<N>(mine, sum);
+    store_part<N>(a.parts + (first * 2 + 1) * a.width + own.col, sum);
 }
 
 // Words that begin in a run and go on behind it: their parts in the order of the runs, groups of them
@@ -524,14 +526,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, bool folded,
     const float *mine = a.parts + (own.run * 2ll + 1) * a.width + col;
 #pragma unroll
     for (int j = 0; j < N; ++j) sum[j] = mine[j];
-    // Adds the parts of `n` runs, or of groups of `by` runs, from `first` on.
-    auto add = [&](int first, int n, int by) {
+    // Adds n parts, of the runs `by` apart from `first` on, in the given place of theirs.
+    auto add = [&](int first, int n, int by, int place) {
         for (int i = 0; i < n; i += kStep) {
             float part[kStep][N];
 #pragma unroll
             for (int s = 0; s < kStep; ++s) {
                 const int run = first + min(i + s, n - 1) * by;
-                const float *from = a.parts + run * 2ll * a.width + col;
+                const float *from = a.parts + (run * 2ll + place) * a.width + col;
 #pragma unroll
                 for (int j = 0; j < N; ++j) part[s][j] = from[j];
             }
@@ -546,11 +548,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, bool folded,
     int next = own.run + 1;
     const int whole = (next + kFold - 1) / kFold * kFold, behind = (last + 1) / kFold * kFold;
     if (folded && whole < behind) {
-        add(next, whole - next, 1);
-        add(whole, (behind - whole) / kFold, kFold);
+        add(next, whole - next, 1, 0);
+        add(whole, (behind - whole) / kFold, kFold, 1);
         next = behind;
     }
-    add(next, last + 1 - next, 1);
+    add(next, last + 1 - next, 1, 0);
     store_sum<T, N>(dtable + static_cast<int64_t>(key) * a.width + col, sum, a.scale);
 }
 

@@ -266,3 +266,20 @@ def test_a_word_costs_what_the_batch_costs(gpu):
     hot = torch.where(torch.rand(tokens, generator=g, device=gpu) < 0.5, 7, even)
     time_of(even)
     assert time_of(hot) <= 2.0 * time_of(even)
+
+
+@pytest.mark.parametrize("dtype,width", ((torch.float32, 257), (torch.float32, 259), (torch.float32, 515),
+                                         (torch.float32, 1027), (torch.bfloat16, 513),
+                                         (torch.bfloat16, 1027), (torch.bfloat16, 2051)), ids=str)
+def test_words_of_many_runs_in_rows_whose_last_pieces_overlap(gpu, width, dtype):
+    """A row's last piece shares columns with the one before, which is another wavefront's or workgroup's
+    here: neither may read what the other has already summed."""
+    tokens = 100_000
+    g = torch.Generator(device=gpu).manual_seed(width)
+    ids = torch.zeros(tokens, dtype=torch.int64, device=gpu)
+    ids[torch.rand(tokens, generator=g, device=gpu) < 0.3] = 2
+    dout = torch.randint(-8, 9, (tokens, width), generator=g, device=gpu).to(dtype)
+    there = (ids == torch.arange(4, device=gpu)[:, None]).float()
+    want = (there @ dout.float()).to(dtype)
+    for _ in range(10):
+        assert torch.equal(nacho_amd.gpu_embedding_backward(dout, ids, 4), want)

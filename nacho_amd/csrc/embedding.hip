@@ -9,7 +9,7 @@
 // of a batch has costs no more than others.  A word whose entries lie in more than one run gets its
 // parts joined by another launch, in their order, for which many runs' parts are first added up in
 // groups, by workgroups of their own (262144 tokens of 2048 bfloat16, none, half and all of them of one word:
-// 300, 293 and 271 us; without such groups 297, 632 and 954).
+// 300, 291 and 266 us; without such groups 299, 617 and 931).
 //
 // Measured, bfloat16: the lookup of 65536 rows of 4096 124 us, 5.7 TB/s; the gradient of 16384 tokens
 // of 2048 and 65537 words 78 us traced, of which sorting them beside clearing the table 47 (5.7 TB/s of
@@ -526,16 +526,24 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, bool folded,
     const float *mine = a.parts + (own.run * 2ll + 1) * a.width + col;
 #pragma unroll
     for (int j = 0; j < N; ++j) sum[j] = mine[j];
-    // Adds n parts, of the runs `by` apart from `first` on, in the given place of theirs.
-    auto add = [&](int first, int n, int by, int place) {
+    // Single runs before the first whole group, groups, and single runs behind the last.
+    int next = own.run + 1;
+    const int whole = (next + kFold - 1) / kFold * kFold, behind = (last + 1) / kFold * kFold;
+    const bool groups = folded && whole < behind;
+#pragma unroll 1  // (one copy of the loop: three of them were a tenth slower)
+    while (next <= last) {
+        const bool group = groups && next == whole;
+        const int end = group ? behind : groups && next < whole ? whole : last + 1;
+        const int n = group ? (end - next) / kFold : end - next;
+        const float *from = a.parts + (next * 2ll + (group ? 1 : 0)) * a.width + col;
+        const int64_t step = (group ? kFold * 2ll : 2ll) * a.width;
         for (int i = 0; i < n; i += kStep) {
             float part[kStep][N];
 #pragma unroll
             for (int s = 0; s < kStep; ++s) {
-                const int run = first + min(i + s, n - 1) * by;
-                const float *from = a.parts + (run * 2ll + place) * a.width + col;
 #pragma unroll
                 for (int j = 0; j < N; ++j) part[s][j] = from[j];
+                from += i + s + 1 < n ? step : 0;
             }
 #pragma unroll
             for (int s = 0; s < kStep; ++s) {
@@ -543,16 +551,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Sums a, bool folded,
                 for (int j = 0; j < N; ++j) sum[j] += i + s < n ? part[s][j] : 0.0f;
             }
         }
-    };
-    // Single runs before the first whole group, groups, and single runs behind the last.
-    int next = own.run + 1;
-    const int whole = (next + kFold - 1) / kFold * kFold, behind = (last + 1) / kFold * kFold;
-    if (folded && whole < behind) {
-        add(next, whole - next, 1, 0);
-        add(whole, (behind - whole) / kFold, kFold, 1);
-        next = behind;
+        next = end;
     }
-    add(next, last + 1 - next, 1, 0);
     store_sum<T, N>(dtable + static_cast<int64_t>(key) * a.width + col, sum, a.scale);
 }
 
@@ -693,8 +693,8 @@ int sort_tokens(Call &call, const Ids &ids, int tokens, const Cleared &all, int 
 }
 
 // Runs from which on fold_kernel is launched.  (us with it and without it, half of the tokens of one word,
-// and none: 8192 tokens of 2048 bfloat16 49 and 49, 43 and 41; 16384 70 and 78, 61 and 59; 262144 293 and
-// 632, 300 and 297; 1048576 of 64 float32 166 and 1300, 160 and 158.)
+// and none: 8192 tokens of 2048 bfloat16 49 and 47, 42 and 41; 16384 68 and 77, 60 and 59; 262144 291 and
+// 617, 300 and 299; 1048576 of 64 float32 161 and 961, 160 and 158.)
 constexpr int64_t kFoldChunks = 512;
 
 int backward(int32_t dtype, int64_t tokens, int64_t words, int64_t width, float scale,
